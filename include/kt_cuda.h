@@ -421,6 +421,121 @@ kt_status kt_gather_rows(kt_ctx* ctx, const float* src_dev, const int32_t* rows_
 /* *value_dev += delta on `stream` (advances a captured step's position). */
 kt_status kt_increment(kt_ctx* ctx, int32_t* value_dev, int32_t delta, void* stream);
 
+/* ------------------------------------------------------------ key/value cache in 8 bits
+ * (no reference counterpart: KVCache.kt:3-59 holds fp32)  One layer's cache of
+ * `batch` sequences, each with lengths[b] tokens in slots 0..lengths[b]-1:
+ *   codes  int8 [batch][kv_heads][capacity][head_dim]
+ *   scales fp32 [batch][kv_heads][capacity / block], one per block of slots and head
+ *   tail   fp32 [batch][kv_heads][block][head_dim]: the original values of the
+ *          open block (slots from lengths[b] - lengths[b] % block on), from which
+ *          it is quantized again whenever a token joins it, so what a cache holds
+ *          does not depend on how its tokens were split into calls
+ *   weights fp32 [batch][kv_heads][capacity] (NULL: not kept): attention weight
+ *          each slot has received, summed over rows and the heads of its group
+ * A block with largest magnitude a has scale = a * (1/127) and codes
+ * round_half_even(x * (127 * (1/a))), each step rounded to fp32; a < 2^-100 gives
+ * scale 0, and a value that is not finite gives scale NaN and codes 0, so that
+ * what reads the block shows it.  The value held is code * scale.
+ * lengths is device memory read by the kernels (a captured step replays at any
+ * length); no call below but kt_kv8_advance changes it.  head_dim is a multiple of
+ * 16 up to 128, block 16, 32 or 64, capacity a multiple of block, batch at most
+ * 32767, kv_heads at most 65535, all buffers 16-byte aligned; else
+ * KT_ERR_INVALID_ARGUMENT. */
+typedef struct {
+    int8_t* k_codes;
+    int8_t* v_codes;
+    float* k_scales;
+    float* v_scales;
+    float* k_tail;
+    float* v_tail;
+    float* weights;
+    const int32_t* lengths;
+    int32_t batch, kv_heads, head_dim, capacity, block;
+} kt_kv8_cache;
+
+/* Stores rows_per_seq new tokens of every sequence (row b * rows_per_seq + t of k
+ * and v, kv_heads * head_dim floats each, rows k_stride / v_stride floats apart)
+ * in slots lengths[b] + t, quantizing every block they touch.  counts_dev [batch]
+ * (NULL: rows_per_seq everywhere): only the first counts[b] rows of a sequence are
+ * tokens.  New slots' weights become 0.  Tokens past the capacity are dropped and
+ * set KT_ERR_INVALID_ARGUMENT in *status_dev (NULL: not reported). */
+kt_status kt_kv8_store(kt_ctx* ctx, const kt_kv8_cache* cache, const float* k_dev, const float* v_dev,
+                       int64_t k_stride, int64_t v_stride, int32_t rows_per_seq, const int32_t* counts_dev,
+                       int32_t* status_dev, void* stream);
+
+/* Scratch of kt_kv8_attention and kt_kv8_evict for a cache of these sizes; it must
+ * be zero-filled before its first use (its front holds counters that every call
+ * leaves at zero), and calls that share it must be ordered. */
+size_t kt_kv8_scratch_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                            int32_t capacity);
+
+/* Attention of rows_per_seq query rows per sequence (row r of q: `heads` heads of
+ * head_dim floats, rows q_stride floats apart; heads / kv_heads query heads share a
+ * key/value head): row t of sequence b attends to slots 0..lengths[b] + t, which
+ * kt_kv8_store has filled,
+ *   context[row][head] = softmax(scale * q . k) . v
+ * into context_dev [batch * rows_per_seq][heads * head_dim].  Rows t >= counts[b]
+ * give zeros and no weights.  accumulate_weights != 0 adds the attention weights
+ * of the rows to cache->weights.  Products and sums are fp32 class: the codes are
+ * exact in the tensor cores' fp16, queries and probabilities enter as two fp16
+ * terms each. */
+kt_status kt_kv8_attention(kt_ctx* ctx, const kt_kv8_cache* cache, const float* q_dev, int64_t q_stride,
+                           float* context_dev, int32_t rows_per_seq, const int32_t* counts_dev, int32_t heads,
+                           float scale, int32_t accumulate_weights, void* scratch_dev, void* stream);
+
+/* lengths_dev[b] = min(lengths_dev[b] + (counts_dev ? counts_dev[b] : rows), limit). */
+kt_status kt_kv8_advance(kt_ctx* ctx, int32_t* lengths_dev, int32_t batch, int32_t rows, const int32_t* counts_dev,
+                         int32_t limit, void* stream);
+
+/* Prunes every sequence with lengths[b] > keep to `keep` tokens, each key/value
+ * head for itself: the last `recent` slots stay, and of the others the
+ * keep - recent with the largest accumulated weight (the lowest slots among equal
+ * weights; a NaN weight ranks above all).  The kept tokens move, in their order,
+ * to slots 0..keep-1; the values they held are quantized again in their new
+ * blocks, the new open block's tail receives them, and their weights move with
+ * them.  Needs cache->weights and 0 <= recent <= keep, 1 <= keep.  lengths is left
+ * as it is: after the last layer, kt_kv8_advance with rows 0 and limit `keep`. */
+kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int32_t recent, void* scratch_dev,
+                       void* stream);
+
+/* ------------------------------------------------------------ logits before the choice of a token
+ * (no reference counterpart; the choice is argmaxOfLastToken, Transformer.kt:255-266)
+ * For each row and token id i, in this order, each step rounded to fp32:
+ *   y = x > 0 ? x / repetition : x * repetition   if i is among the row's tokens
+ *   y = y - frequency * n, then y - presence       if i occurs n > 0 times from
+ *                                                  index prompt_lengths[row] on
+ *   y = y + value for every bias entry (i, value), in list order
+ *   y = -inf                                       if bit i of the row's mask is 0
+ * and next_token[row] = kt_argmax of the row.  Every pointer but logits and out may
+ * be NULL (tokens needs lengths; the penalties need tokens).  Token and bias ids
+ * outside 0..vocab-1 are ignored. */
+typedef struct {
+    const float* logits;           /* [rows][vocab], rows logits_stride floats apart */
+    float* out;                    /* the same shape, out_stride apart; may be `logits` itself */
+    int64_t logits_stride, out_stride;
+    int32_t rows, vocab;
+    const int32_t* tokens;         /* [rows][token_width], rows token_stride apart (0: shared);
+                                      the first lengths[row] count */
+    const int32_t* lengths;
+    const int32_t* prompt_lengths; /* NULL: 0 */
+    int64_t token_stride;
+    int32_t token_width;
+    const float* repetition;       /* [rows] */
+    const float* frequency;
+    const float* presence;
+    int32_t bias_width;
+    const int32_t* bias_ids;       /* [rows][bias_width], rows bias_stride apart (0: shared);
+                                      the first bias_counts[row] count */
+    const float* bias_values;
+    const int32_t* bias_counts;    /* NULL: bias_width everywhere */
+    int64_t bias_stride;
+    const uint32_t* allowed;       /* bit i % 32 of word i / 32; rows allowed_stride words apart (0: shared) */
+    int64_t allowed_stride;
+    int32_t* next_token;           /* [rows] */
+    void* scratch;                 /* 16 bytes a row, zero-filled before the first call (left so); for next_token */
+} kt_logits_args;
+kt_status kt_logits_process(kt_ctx* ctx, const kt_logits_args* args, void* stream);
+
 /* ------------------------------------------------------------ LoRA adapters over a quantized base
  * LoRALinear (LoRA.kt:7-57) with a QuantizedLinear base: lora_a fp32 [K x rank],
  * lora_b fp32 [rank x N], scaling = alpha / rank, all row-major on the device;

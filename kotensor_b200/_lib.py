@@ -56,6 +56,28 @@ class KtInfo(ctypes.Structure):
     ]
 
 
+class KtKv8Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p), ("k_tail", ctypes.c_void_p), ("v_tail", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("batch", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("capacity", ctypes.c_int32),
+        ("block", ctypes.c_int32),
+    ]
+
+
+class KtLogitsArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("logits_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64), ("rows", ctypes.c_int32), ("vocab", ctypes.c_int32),
+        ("tokens", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("prompt_lengths", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64), ("token_width", ctypes.c_int32), ("repetition", ctypes.c_void_p), ("frequency", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p), ("bias_width", ctypes.c_int32), ("bias_ids", ctypes.c_void_p), ("bias_values", ctypes.c_void_p),
+        ("bias_counts", ctypes.c_void_p), ("bias_stride", ctypes.c_int64), ("allowed", ctypes.c_void_p),
+        ("allowed_stride", ctypes.c_int64), ("next_token", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
+    ]
+
+
 # name -> (argtypes, restype); the single source of the Python-side signatures.
 P, I32, I64, F32, SZ = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 PP = ctypes.POINTER(ctypes.c_void_p)
@@ -126,6 +148,12 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "kt_lora_backward": ([P, P, P, P, P, P, P, I32, F32, I32, P, I32, P, P, P], I32),
     "kt_gather_rows": ([P, P, P, I32, I32, P, P], I32),
     "kt_fused_cross_entropy": ([P, P, P, P, I32, P, I32, P, P, P, P], I32),
+    "kt_kv8_store": ([P, ctypes.POINTER(KtKv8Cache), P, P, I64, I64, I32, P, P, P], I32),
+    "kt_kv8_scratch_bytes": ([I32, I32, I32, I32, I32, I32], SZ),
+    "kt_kv8_attention": ([P, ctypes.POINTER(KtKv8Cache), P, I64, P, I32, P, I32, F32, I32, P, P], I32),
+    "kt_kv8_advance": ([P, P, I32, I32, P, I32, P], I32),
+    "kt_kv8_evict": ([P, ctypes.POINTER(KtKv8Cache), I32, I32, P, P], I32),
+    "kt_logits_process": ([P, ctypes.POINTER(KtLogitsArgs), P], I32),
     "kt_st_open": ([ctypes.c_char_p, PP], I32),
     "kt_st_close": ([P], I32),
     "kt_st_tensor_count": ([P], I32),

@@ -1,0 +1,112 @@
+// kt_kv8.h -- the 8-bit key/value cache as its kernels see it, and the
+// launchers of kt_kv8.cu and kt_kv8_attention.cu.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <exception>
+#include <new>
+#include <string>
+
+#include "kt_device.cuh"
+#include "kt_internal.h"
+
+namespace kt {
+
+using Kv8 = kt_kv8_cache;  // passed to kernels by value
+
+constexpr int kKv8MaxHeadDim = 128;
+
+// Scratch layout (kt_kv8_scratch_bytes): merge counters of the attention, one
+// per (sequence, key/value head), then the region the kernels use freely.
+inline size_t kv8_counter_bytes(int64_t batch, int64_t kv_heads) {
+    return static_cast<size_t>((batch * kv_heads * 4 + 255) / 256 * 256);
+}
+
+// Runs a C entry's body: no C++ exception crosses the boundary, and the
+// context's device is current inside (the caller's is put back).
+template <typename Body>
+kt_status c_entry(kt_ctx* ctx, Body body) {
+    try {
+        int before = 0;
+        cudaError_t e = cudaGetDevice(&before);
+        if (e == cudaSuccess && before != ctx->device) e = cudaSetDevice(ctx->device);
+        if (e != cudaSuccess) {
+            set_error(std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+            return KT_ERR_CUDA;
+        }
+        const kt_status st = body();
+        if (before != ctx->device) cudaSetDevice(before);
+        return st;
+    } catch (const std::bad_alloc&) {
+        return KT_ERR_OUT_OF_MEMORY;
+    } catch (...) {
+        return KT_ERR_CUDA;
+    }
+}
+
+inline kt_status entry_fail(kt_status st, const char* msg) {
+    try {
+        set_error(msg);
+    } catch (...) {  // the status stands without its message
+    }
+    return st;
+}
+
+inline kt_status entry_launch(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return KT_OK;
+    set_error(std::string(what) + ": " + cudaGetErrorString(e));
+    return e == cudaErrorMemoryAllocation ? KT_ERR_OUT_OF_MEMORY : KT_ERR_CUDA;
+}
+
+// A launch that may start while the previous kernel of its stream ends
+// (programmatic dependent launch): every kernel launched by it waits
+// (griddepcontrol.wait) before it touches memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                             Args... args) {
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = grid;
+    lc.blockDim = block;
+    lc.dynamicSmemBytes = smem;
+    lc.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    return cudaLaunchKernelEx(&lc, kernel, static_cast<Params>(args)...);
+}
+
+// NULL when the cache can be used, else what is wrong with it (kt_kv8.cu).
+const char* kv8_check(const Kv8* c);
+
+struct Kv8Attention {
+    Kv8 cache;
+    const float* q;
+    int64_t q_stride;
+    float* context;
+    const int32_t* counts;
+    int32_t rows_per_seq, heads;
+    float scale;
+    int32_t accumulate;
+    void* scratch;
+};
+// Bytes behind the counters that the attention of these sizes uses (kt_kv8_attention.cu).
+size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                           int32_t capacity);
+cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, cudaStream_t s);
+
+#ifdef __CUDACC__
+// Tokens that sequence b holds, whatever the caller left in lengths.
+__device__ __forceinline__ int kv8_held(const Kv8& c, int b) {
+    return min(max(c.lengths[b], 0), c.capacity);
+}
+// Rows of this call that sequence b adds or asks with.
+__device__ __forceinline__ int kv8_rows(const int32_t* counts, int b, int rows_per_seq) {
+    return counts == nullptr ? rows_per_seq : min(max(counts[b], 0), rows_per_seq);
+}
+#endif
+
+}  // namespace kt
