@@ -299,11 +299,11 @@ kt_status kt_kv8_store(kt_ctx* ctx, const kt_kv8_cache* cache, const float* k, c
 }
 
 size_t kt_kv8_scratch_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                            int32_t capacity) {
+                            int32_t capacity, int32_t weights) {
     if (batch <= 0 || rows_per_seq <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || capacity <= 0) return 0;
-    const size_t order = static_cast<size_t>(batch) * kv_heads * capacity * sizeof(int32_t);
-    return kv8_counter_bytes(batch, kv_heads) +
-           std::max(order, kv8_attention_bytes(batch, rows_per_seq, heads, kv_heads, head_dim, capacity));
+    const size_t order = weights ? static_cast<size_t>(batch) * kv_heads * capacity * sizeof(int32_t) : 0;
+    return kKv8CounterBytes +
+           std::max(order, kv8_attention_bytes(batch, rows_per_seq, heads, kv_heads, head_dim, capacity, weights != 0));
 }
 
 kt_status kt_kv8_attention(kt_ctx* ctx, const kt_kv8_cache* cache, const float* q, int64_t q_stride, float* context,
@@ -351,8 +351,7 @@ kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int
     if (keep >= cache->capacity) return KT_OK;  // nothing can hold more
     return c_entry(ctx, [&] {
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
-        int32_t* order = reinterpret_cast<int32_t*>(static_cast<char*>(scratch) +
-                                                    kv8_counter_bytes(cache->batch, cache->kv_heads));
+        int32_t* order = reinterpret_cast<int32_t*>(static_cast<char*>(scratch) + kKv8CounterBytes);
         const dim3 heads(cache->kv_heads, cache->batch);
         cudaError_t e = launch_dependent(kv8_select_kernel, heads, dim3(kSelectThreads), 0, s, *cache, keep, recent,
                                          order);

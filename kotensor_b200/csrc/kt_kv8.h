@@ -18,11 +18,10 @@ using Kv8 = kt_kv8_cache;  // passed to kernels by value
 
 constexpr int kKv8MaxHeadDim = 128;
 
-// Scratch layout (kt_kv8_scratch_bytes): merge counters of the attention, one
-// per (sequence, key/value head), then the region the kernels use freely.
-inline size_t kv8_counter_bytes(int64_t batch, int64_t kv_heads) {
-    return static_cast<size_t>((batch * kv_heads * 4 + 255) / 256 * 256);
-}
+// Scratch layout (kt_kv8_scratch_bytes): the attention's merge counters at the
+// front, at the same place for every call, then what one call uses freely.
+constexpr size_t kKv8CounterBytes = 4096;
+constexpr int kKv8MaxCtas = static_cast<int>(kKv8CounterBytes / sizeof(int32_t));
 
 // Runs a C entry's body: no C++ exception crosses the boundary, and the
 // context's device is current inside (the caller's is put back).
@@ -95,7 +94,7 @@ struct Kv8Attention {
 };
 // Bytes behind the counters that the attention of these sizes uses (kt_kv8_attention.cu).
 size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                           int32_t capacity);
+                           int32_t capacity, bool weights);
 cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, cudaStream_t s);
 
 #ifdef __CUDACC__

@@ -3,13 +3,529 @@
 // Row t of sequence b with n = lengths[b]: for each query head, over slots
 // j <= n + t,  s_j = scale * (q . K_j),  out = sum_j softmax(s)_j V_j, with
 // K_j = code * scale of the slot's block.
+//
+// Codes are whole numbers of at most 128 and exact in fp16, so the products run on
+// fp16 tensor cores with fp32 sums once the fp32 operand, the query or the
+// probability, is written as two fp16 terms: x = hi + lo with hi = fp16(x) and
+// lo = fp16(x - hi), 22 bits.  The scales of the blocks multiply the fp32 sums.
+#include <cuda_fp16.h>
+
 #include "kt_kv8.h"
 
 namespace kt {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds
+constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in the row kernel
+
+// ------------------------------------------------------------ few query rows
+//
+// The query vectors that share a key/value head (rows_per_seq x heads / kv_heads
+// of them) go eight to a tile: an m16n8k16 product holds their hi terms in rows
+// 0..7 and their lo terms in rows 8..15, so a thread finds both sums of a score in
+// its own accumulators, and probabilities leave it in the layout the second product
+// reads.  Work is the list of all tiles of kKeys slots over (sequence, key/value
+// head, vector tile), cut into equal runs, one per CTA: ragged batches and single
+// long sequences load every SM alike.  A warp takes every kWarps-th tile of its
+// CTA's run through its own ring of asynchronous copies; nothing waits for another
+// warp until an item's last tile, where the warps merge their maxima, sums and
+// weighted sums.  Items cut between CTAs are merged by the last CTA to arrive, in
+// the order of the cuts: equal bits on every run.
+
+constexpr int kKeys = 32;
+constexpr int kVectors = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+// Probabilities are kept 2^12 times larger, so that the fp16 terms of small ones
+// stay clear of the subnormals; the factor cancels in the division by their sum.
+constexpr float kLift = 12.0f;
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float lds32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+// 16 bytes global -> shared; `bytes` of them are read, the rest are zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// Bytes of codes with their sign bit flipped (0..255) -> fp16 pairs: 0x64xx is
+// 1024 + xx, less 1152 is the code.  `sel` picks the two bytes.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t flipped) {
+    const uint32_t r = dev::prmt(flipped, 0x64646464u, kSel);
+    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480))));
+}
+// x0, x1 as their two fp16 terms, packed in pairs.
+__device__ __forceinline__ void two_terms(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    hi = h2_bits(h);
+    lo = h2_bits(__floats2half2_rn(x0 - f.x, x1 - f.y));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A place in the list of tiles: tile `tile` of item `item` (key/value head times
+// vector tile) of sequence b.
+struct Place {
+    int b, item, tile, tiles;  // tiles of each of the sequence's items
+};
+
+template <int HDP>
+struct DecodeShape {
+    static constexpr int kStages = 3;
+    static constexpr int kTileBytes = kKeys * HDP;               // one of keys, values
+    static constexpr int kStageBytes = 2 * kTileBytes + 16;      // and 2 + 2 scales
+    static constexpr int kRing = kStages * kStageBytes;
+    static constexpr int kPartFloats = kVectors * (HDP + 2);     // sums, then maxima, then denominators
+    static constexpr int kSmem = kWarps * (kRing + kPartFloats * 4);
+};
+
+// Swizzle of 16-byte pieces that makes both fragment reads conflict-free: in
+// 128-byte rows piece ^ ((row / 2 ^ (row & 1) * 2) % 4 * 2); 64-byte rows lie in
+// pairs, (row & 1) * 4 + piece ^ (row / 2) % 4 * 2.
+template <int HDP>
+__device__ __forceinline__ int piece_offset(int row, int piece) {
+    if (HDP == 128) return row * 128 + ((piece ^ ((((row >> 1) ^ ((row & 1) << 1)) & 3) << 1)) << 4);
+    return (row >> 1) * 128 + ((((row & 1) * 4 + piece) ^ (((row >> 1) & 3) << 1)) << 4);
+}
+
+template <int HDP, bool kFine>
+__global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention a, int vector_tiles, int aligned,
+                                                                    float* __restrict__ parts,
+                                                                    float* __restrict__ scores,
+                                                                    float* __restrict__ lse) {
+    using S = DecodeShape<HDP>;
+    constexpr int kSteps = HDP / 16;       // k-steps of the first product
+    constexpr int kPieces = HDP / 64;      // 16-byte pieces of a key a thread reads
+    constexpr int kTiles = HDP / 8;        // n-tiles of the second product
+    constexpr int kOwn = HDP / 4;          // dims of the output a thread holds
+    dev::pdl_wait();
+    dev::pdl_launch_dependents();
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int last_cta;
+    const Kv8& c = a.cache;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = lane % 4, n8 = lane / 4;
+    const int d = c.head_dim, pieces = d / 16, group = a.heads / c.kv_heads;
+    const int vectors = a.rows_per_seq * group, items = c.kv_heads * vector_tiles;
+    const uint32_t ring = dev::smem_u32(smem) + warp * S::kRing;
+    float* const part_smem = reinterpret_cast<float*>(smem + kWarps * S::kRing);
+
+    // Slots the rows of sequence b see, and tiles of one of its items.
+    auto seen_by = [&](int b, int& rows) {
+        rows = kv8_rows(a.counts, b, a.rows_per_seq);
+        return rows == 0 ? 0 : min(kv8_held(c, b) + rows, c.capacity);
+    };
+    auto tiles_of = [&](int b) {
+        int rows;
+        return (seen_by(b, rows) + kKeys - 1) / kKeys;
+    };
+    if (a.counts != nullptr)  // rows that are no tokens
+        for (int64_t r = blockIdx.x; r < static_cast<int64_t>(c.batch) * a.rows_per_seq; r += gridDim.x)
+            if (static_cast<int>(r % a.rows_per_seq) >= kv8_rows(a.counts, static_cast<int>(r / a.rows_per_seq), a.rows_per_seq))
+                for (int i = threadIdx.x; i < a.heads * d; i += blockDim.x) a.context[r * a.heads * d + i] = 0.0f;
+
+    // This CTA's run [begin, end) of the list.
+    int64_t total = 0;
+    for (int b = lane; b < c.batch; b += 32) total += tiles_of(b);
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= items;
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max(static_cast<int64_t>(1), total / kWarps));
+    auto run_begin = [&](int64_t cta) { return total * cta / ctas; };
+    const int64_t begin = blockIdx.x < ctas ? run_begin(blockIdx.x) : total;
+    const int64_t end = blockIdx.x < ctas ? run_begin(blockIdx.x + 1) : total;
+    if (begin >= end) return;
+    Place at{0, 0, 0, 0};
+    int64_t base = 0;  // list index of the sequence's first tile
+    for (int b0 = 0; b0 < c.batch; b0 += 32) {
+        const int mine = b0 + lane < c.batch ? tiles_of(b0 + lane) : 0;
+        int64_t upto = static_cast<int64_t>(mine) * items;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t after = __ballot_sync(0xffffffffu, base + upto > begin);
+        if (after != 0) {
+            const int l = __ffs(after) - 1;
+            at.b = b0 + l;
+            at.tiles = __shfl_sync(0xffffffffu, mine, l);
+            base += __shfl_sync(0xffffffffu, upto, l) - static_cast<int64_t>(at.tiles) * items;
+            break;
+        }
+        base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    at.item = static_cast<int>((begin - base) / at.tiles);
+    at.tile = static_cast<int>((begin - base) % at.tiles);
+
+    // The first item after `p`'s: moves p to its tile 0.
+    auto next_item = [&](Place& p) {
+        p.tile = 0;
+        if (++p.item < items) return;
+        p.item = 0;
+        do ++p.b;
+        while (p.b < c.batch && (p.tiles = tiles_of(p.b)) == 0);
+    };
+
+    // The warp's copies run ahead of its work over the same sequence of tiles: from
+    // `ahead` (the warp's tile in the segment that starts at list index ahead_base).
+    Place ahead = at;
+    int64_t ahead_left = end - begin;  // tiles of the run from the segment's start on
+    int ahead_first = at.tile;         // the segment's first tile
+    ahead.tile += warp;
+    int fill = 0;
+    auto issue = [&] {
+        // skip segments without a tile of this warp
+        while (ahead_left > 0) {
+            const int stop = static_cast<int>(min(static_cast<int64_t>(ahead.tiles), ahead_first + ahead_left));
+            if (ahead.tile < stop) break;
+            ahead_left -= stop - ahead_first;
+            if (ahead_left > 0) {
+                next_item(ahead);
+                ahead_first = 0;
+                ahead.tile = warp;
+            }
+        }
+        if (ahead_left > 0) {
+            int rows;
+            const int seen = seen_by(ahead.b, rows), first = ahead.tile * kKeys;
+            const int64_t head = static_cast<int64_t>(ahead.b) * c.kv_heads + ahead.item / vector_tiles;
+            const uint32_t stage = ring + fill * S::kStageBytes;
+            const int8_t* k = c.k_codes + (head * c.capacity + first) * d;
+            const int8_t* v = c.v_codes + (head * c.capacity + first) * d;
+#pragma unroll
+            for (int i = 0; i < kKeys * HDP / 16 / 32; ++i) {
+                const int e = i * 32 + lane, row = e / (HDP / 16), piece = e % (HDP / 16);
+                const bool real = piece < pieces && first + row < seen;
+                const int64_t from = real ? row * d + piece * 16 : 0;
+                const uint32_t to = stage + piece_offset<HDP>(row, piece);
+                copy16(to, k + from, real ? 16 : 0);
+                copy16(to + S::kTileBytes, v + from, real ? 16 : 0);
+            }
+            if (lane < 4) {  // scales of slots first.. and first + 16.., keys then values
+                const int slot = first + (lane & 1) * 16;
+                const float* s = (lane < 2 ? c.k_scales : c.v_scales) + head * (c.capacity / c.block);
+                const bool real = slot < seen;
+                copy4(stage + 2 * S::kTileBytes + lane * 4, s + (real ? slot / c.block : 0), real ? 4 : 0);
+            }
+            ahead.tile += kWarps;
+        }
+        copy_commit();
+        fill = fill + 1 == S::kStages ? 0 : fill + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < S::kStages; ++i) issue();
+
+    int use = 0;
+    int64_t left = end - begin;
+    while (left > 0) {  // one segment: the run's tiles of one item
+        const int stop = static_cast<int>(min(static_cast<int64_t>(at.tiles), at.tile + left));
+        int rows;
+        const int seen = seen_by(at.b, rows), held = kv8_held(c, at.b);
+        const int h = at.item / vector_tiles, vt = at.item - h * vector_tiles;
+        const int vector = vt * kVectors + n8, row = vector / group;  // of this thread's fragments
+        const bool real = vector < vectors && row < rows;
+        const int limit = real ? min(held + row + 1, seen) : 0;                  // slots the vector sees
+        const int64_t head = static_cast<int64_t>(at.b) * c.kv_heads + h;
+
+        uint32_t qa[kSteps][4];
+        float factor;
+        {
+            const float* q = a.q + (static_cast<int64_t>(at.b) * a.rows_per_seq + row) * a.q_stride +
+                             static_cast<int64_t>(h * group + vector % group) * d;
+            float x[kSteps][4];
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const int dim = 16 * (t + 4 * (s / 4)) + 4 * (s % 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[s][i] = 0.0f;
+                if (real && dim < d) {
+                    if (aligned) {
+                        const float4 f = *reinterpret_cast<const float4*>(q + dim);
+                        x[s][0] = f.x, x[s][1] = f.y, x[s][2] = f.z, x[s][3] = f.w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[s][i] = q[dim + i];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[s][i]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // a power of two that brings the largest component to 1/2 .. 1
+            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 126, -126), 126);
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            factor = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                two_terms(x[s][0] * down, x[s][1] * down, qa[s][0], qa[s][1]);
+                two_terms(x[s][2] * down, x[s][3] * down, qa[s][2], qa[s][3]);
+            }
+        }
+        float o[kOwn], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) o[i] = 0.0f;
+
+        for (int tile = at.tile + warp; tile < stop; tile += kWarps) {
+            copy_wait<S::kStages - 1>();
+            __syncwarp();
+            const uint32_t stage = ring + use * S::kStageBytes;
+            const int first = tile * kKeys;
+            float s[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int u = 0; u < kPieces; ++u) {
+                    const uint4 w = lds128(stage + piece_offset<HDP>(8 * j + n8, t + 4 * u));
+                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t f = words[i] ^ 0x80808080u;
+                        mma(acc, qa[4 * u + i], codes_to_half2<0x4140>(f), codes_to_half2<0x4342>(f));
+                    }
+                }
+                const float ks = lds32(stage + 2 * S::kTileBytes + (j >> 1) * 4) * factor;
+                s[j][0] = (acc[0] + acc[2]) * ks;
+                s[j][1] = (acc[1] + acc[3]) * ks;
+            }
+            if (first + kKeys > held + 1) {  // the first row's end, or the end of all, lies in this tile
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (first + 8 * j + 2 * t + i >= limit) s[j][i] = -INFINITY;
+            }
+            if (scores != nullptr && vector < vectors) {
+                float* to = scores + (head * vectors + vector) * c.capacity + first;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (first + 8 * j < c.capacity)
+                        *reinterpret_cast<float2*>(to + 8 * j + 2 * t) = make_float2(s[j][0], s[j][1]);
+            }
+            float top = m;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float from = (top == -INFINITY ? 0.0f : top) - kLift;
+            if (__any_sync(0xffffffffu, top > m)) {
+                const float fade = m == -INFINITY ? 0.0f : ex2((m - kLift) - from);
+                l *= fade;
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) o[i] *= fade;
+            }
+            m = top;
+            uint32_t pa[2][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p0 = ex2(s[j][0] - from), p1 = ex2(s[j][1] - from);
+                l += p0 + p1;
+                two_terms(p0, p1, pa[j >> 1][(j & 1) * 2], pa[j >> 1][(j & 1) * 2 + 1]);
+            }
+            const float vs0 = lds32(stage + 2 * S::kTileBytes + 8), vs1 = lds32(stage + 2 * S::kTileBytes + 12);
+            // values: thread (t, n8) reads dims n8 * kTiles .. of slots 2t, 2t + 1, 2t + 8, 2t + 9 of
+            // each 16; n-tile q of the product is dim n8 * kTiles + q
+            uint32_t v[2][4][HDP / 32];
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int slot = 16 * kk + 8 * (r >> 1) + 2 * t + (r & 1);
+                    if (HDP == 128) {
+                        const uint4 w = lds128(stage + S::kTileBytes + piece_offset<HDP>(slot, n8));
+                        v[kk][r][0] = w.x, v[kk][r][1] = w.y, v[kk][r][HDP / 32 - 2] = w.z, v[kk][r][HDP / 32 - 1] = w.w;
+                    } else {
+                        const uint2 w = lds64(stage + S::kTileBytes + piece_offset<HDP>(slot, n8 >> 1) + (n8 & 1) * 8);
+                        v[kk][r][0] = w.x, v[kk][r][1] = w.y;
+                    }
+                }
+#pragma unroll
+            for (int w = 0; w < HDP / 32; ++w) {
+                float acc[4][4] = {};  // four n-tiles: bytes 0..3 of the words
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    uint32_t lowp[2], highp[2];  // bytes 0, 1 and 2, 3 of two slots, interleaved
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        lowp[r] = dev::prmt(v[kk][2 * r][w], v[kk][2 * r + 1][w], 0x5140) ^ 0x80808080u;
+                        highp[r] = dev::prmt(v[kk][2 * r][w], v[kk][2 * r + 1][w], 0x7362) ^ 0x80808080u;
+                    }
+                    mma(acc[0], pa[kk], codes_to_half2<0x4140>(lowp[0]), codes_to_half2<0x4140>(lowp[1]));
+                    mma(acc[1], pa[kk], codes_to_half2<0x4342>(lowp[0]), codes_to_half2<0x4342>(lowp[1]));
+                    mma(acc[2], pa[kk], codes_to_half2<0x4140>(highp[0]), codes_to_half2<0x4140>(highp[1]));
+                    mma(acc[3], pa[kk], codes_to_half2<0x4342>(highp[0]), codes_to_half2<0x4342>(highp[1]));
+                    if (kFine || kk == 1) {  // blocks of 16 slots: each half has its own scale
+                        const float vs = kFine && kk == 0 ? vs0 : kFine ? vs1 : vs0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[4 * w + i] = fmaf(vs, acc[i][0] + acc[i][2], o[4 * w + i]);
+                            o[kTiles + 4 * w + i] = fmaf(vs, acc[i][1] + acc[i][3], o[kTiles + 4 * w + i]);
+                            if (kFine) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            issue();
+            use = use + 1 == S::kStages ? 0 : use + 1;
+        }
+
+        // The item's (or its cut's) end: the warps' parts meet in shared memory.
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        float* mine = part_smem + warp * S::kPartFloats;
+#pragma unroll
+        for (int i = 0; i < kOwn; i += 4)
+            *reinterpret_cast<float4*>(mine + n8 * HDP + t * kOwn + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        if (t == 0) {
+            mine[kVectors * HDP + n8] = m - kLift;  // what the sums are relative to
+            mine[kVectors * HDP + kVectors + n8] = l;
+        }
+        __syncthreads();
+        const bool whole = at.tile == 0 && stop == at.tiles;
+        const int slot = at.tile == 0 ? 1 : 0;
+        float* part = parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * S::kPartFloats;
+        // a part's weight relative to the largest maximum; a part without slots has none
+        auto weigh = [](float pm, float psum, float top) { return psum == 0.0f ? 0.0f : ex2(pm - top); };
+        auto finish = [&](int vec, int dim, float4 y, float top, float sum) {
+            const int idx = vt * kVectors + vec, r = idx / group;
+            if (idx >= vectors || r >= rows || dim >= d) return;
+            const float by = 1.0f / sum;
+            float* to = a.context + (static_cast<int64_t>(at.b) * a.rows_per_seq + r) * a.heads * d +
+                        static_cast<int64_t>(h * group + idx % group) * d + dim;
+            if (aligned & 2) {
+                *reinterpret_cast<float4*>(to) = make_float4(y.x * by, y.y * by, y.z * by, y.w * by);
+            } else {
+                to[0] = y.x * by, to[1] = y.y * by, to[2] = y.z * by, to[3] = y.w * by;
+            }
+            if (dim == 0 && lse != nullptr) lse[head * vectors + idx] = top + log2f(sum);
+        };
+        for (int e = threadIdx.x; e < kVectors * HDP / 4; e += kWarps * 32) {
+            const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
+            float top = -INFINITY, sum = 0.0f;
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part_smem[w * S::kPartFloats + kVectors * HDP + vec]);
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int w = 0; w < kWarps; ++w) {
+                const float* p = part_smem + w * S::kPartFloats;
+                const float psum = p[kVectors * HDP + kVectors + vec], by = weigh(p[kVectors * HDP + vec], psum, top);
+                const float4 f = *reinterpret_cast<const float4*>(p + vec * HDP + dim);
+                sum = fmaf(by, psum, sum);
+                y.x = fmaf(by, f.x, y.x), y.y = fmaf(by, f.y, y.y), y.z = fmaf(by, f.z, y.z), y.w = fmaf(by, f.w, y.w);
+            }
+            if (whole) {
+                finish(vec, dim, y, top, sum);
+            } else {
+                *reinterpret_cast<float4*>(part + vec * HDP + dim) = y;
+                if (dim == 0) {
+                    part[kVectors * HDP + vec] = top;
+                    part[kVectors * HDP + kVectors + vec] = sum;
+                }
+            }
+        }
+        if (!whole) {
+            // the CTAs that share the item: those whose runs hold its first .. last tile
+            const int64_t item_first = base + static_cast<int64_t>(at.item) * at.tiles;
+            auto cta_of = [&](int64_t i) {  // the CTA whose run holds list index i
+                int64_t x = i * ctas / total;
+                while (run_begin(x) > i) --x;
+                while (run_begin(x + 1) <= i) ++x;
+                return x;
+            };
+            const int64_t c0 = cta_of(item_first), c1 = cta_of(item_first + at.tiles - 1);
+            int32_t* counter = static_cast<int32_t*>(a.scratch) + c0;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) last_cta = dev::atomic_add_acq_rel(counter, 1) == static_cast<int>(c1 - c0);
+            __syncthreads();
+            if (last_cta) {
+                __threadfence();
+                for (int e = threadIdx.x; e < kVectors * HDP / 4; e += kWarps * 32) {
+                    const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
+                    if (vt * kVectors + vec >= vectors) continue;
+                    auto part_of = [&](int64_t x) { return parts + (x * 2 + (x == c0 ? 1 : 0)) * S::kPartFloats; };
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int64_t x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(part_of(x) + kVectors * HDP + vec));
+                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                    for (int64_t x = c0; x <= c1; ++x) {
+                        const float* p = part_of(x);
+                        const float psum = __ldcg(p + kVectors * HDP + kVectors + vec);
+                        const float by = weigh(__ldcg(p + kVectors * HDP + vec), psum, top);
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + vec * HDP + dim));
+                        sum = fmaf(by, psum, sum);
+                        y.x = fmaf(by, f.x, y.x), y.y = fmaf(by, f.y, y.y);
+                        y.z = fmaf(by, f.z, y.z), y.w = fmaf(by, f.w, y.w);
+                    }
+                    finish(vec, dim, y, top, sum);
+                }
+                if (threadIdx.x == 0) *counter = 0;
+            }
+        }
+        __syncthreads();  // the merge area and last_cta are free again
+
+        left -= stop - at.tile;
+        if (left > 0) {
+            const int b = at.b, tiles = at.tiles;
+            next_item(at);
+            if (at.b != b) base += static_cast<int64_t>(tiles) * items;
+        }
+    }
+}
+
+// The weight of each slot, from the scores and row sums that the attention left:
+// w_j += sum over vectors of 2^(s_j - lse).
+__global__ void __launch_bounds__(256) kv8_add_weights_kernel(Kv8Attention a, const float* __restrict__ scores,
+                                                              const float* __restrict__ lse) {
+    dev::pdl_wait();
+    dev::pdl_launch_dependents();
+    const Kv8& c = a.cache;
+    const int j = (blockIdx.x * 256 + threadIdx.x) * 4, h = blockIdx.y, b = blockIdx.z;
+    const int rows = kv8_rows(a.counts, b, a.rows_per_seq), group = a.heads / c.kv_heads;
+    const int held = kv8_held(c, b), n = rows == 0 ? 0 : min(held + rows, c.capacity);
+    if (j >= n) return;
+    const int64_t head = static_cast<int64_t>(b) * c.kv_heads + h;
+    const int vectors = a.rows_per_seq * group;
+    float w[4] = {};
+#pragma unroll 4
+    for (int i = 0; i < rows * group; ++i) {
+        const float4 s = *reinterpret_cast<const float4*>(scores + (head * vectors + i) * c.capacity + j);
+        const float z = lse[head * vectors + i];
+        w[0] += ex2(s.x - z), w[1] += ex2(s.y - z), w[2] += ex2(s.z - z), w[3] += ex2(s.w - z);
+    }
+    float* to = c.weights + head * c.capacity + j;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (j + i < n) to[i] += w[i];
+}
 
 // One CTA per (row, query head, sequence): warp w takes slots w, w + 8, ..., a lane
 // dims lane, lane + 32, ...; each warp keeps a running maximum, sum and weighted
@@ -99,18 +615,73 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_weights_kernel(Kv8Attention a
 
 }  // namespace
 
-size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t, int32_t, int32_t) {
-    return static_cast<size_t>(batch) * rows_per_seq * heads * sizeof(float);
+namespace {
+// Blocks of query vectors that one row kernel launch would repeat the cache for.
+bool use_tiles(int32_t rows_per_seq, int32_t heads, int32_t kv_heads) {
+    return static_cast<int64_t>(rows_per_seq) * (heads / kv_heads) <= 64;
+}
+int tiles_of_vectors(int32_t rows_per_seq, int32_t heads, int32_t kv_heads) {
+    return (rows_per_seq * (heads / kv_heads) + kVectors - 1) / kVectors;
+}
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t part_bytes(int32_t head_dim) {
+    const size_t hdp = head_dim <= 64 ? 64 : 128;
+    return round256(static_cast<size_t>(kKv8MaxCtas) * 2 * kVectors * (hdp + 2) * sizeof(float));
+}
+size_t lse_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads) {
+    return round256(static_cast<size_t>(batch) * rows_per_seq * heads * sizeof(float));
 }
 
-cudaError_t launch_kv8_attention(const Kv8Attention& a, int, cudaStream_t s) {
+template <int HDP, bool kFine>
+cudaError_t launch_tiles(const Kv8Attention& a, int sm_count, int aligned, float* parts, float* scores, float* lse,
+                         cudaStream_t s) {
+    using S = DecodeShape<HDP>;
+    const auto kernel = kv8_attention_kernel<HDP, kFine>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return e;
     const Kv8& c = a.cache;
-    float* lse = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kv8_counter_bytes(c.batch, c.kv_heads));
+    const int vt = tiles_of_vectors(a.rows_per_seq, a.heads, c.kv_heads);
+    const int per_sm = HDP == 128 ? 1 : 2;  // what shared memory holds
+    const int64_t most = static_cast<int64_t>(c.batch) * c.kv_heads * vt * ((c.capacity + kKeys - 1) / kKeys);
+    const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count * per_sm, kKv8MaxCtas),
+                                                        std::max<int64_t>(1, most / kWarps)));
+    return launch_dependent(kernel, dim3(grid), dim3(kWarps * 32), S::kSmem, s, a, vt, aligned, parts, scores, lse);
+}
+}  // namespace
+
+size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                           int32_t capacity, bool weights) {
+    size_t n = part_bytes(head_dim) + lse_bytes(batch, rows_per_seq, heads);
+    if (weights && use_tiles(rows_per_seq, heads, kv_heads))
+        n += static_cast<size_t>(batch) * rows_per_seq * heads * capacity * sizeof(float);
+    return n;
+}
+
+cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, cudaStream_t s) {
+    const Kv8& c = a.cache;
+    char* free = static_cast<char*>(a.scratch) + kKv8CounterBytes;
+    float* parts = reinterpret_cast<float*>(free);
+    float* lse = reinterpret_cast<float*>(free + part_bytes(c.head_dim));
+    if (use_tiles(a.rows_per_seq, a.heads, c.kv_heads)) {
+        float* scores = reinterpret_cast<float*>(free + part_bytes(c.head_dim) + lse_bytes(c.batch, a.rows_per_seq, a.heads));
+        if (!a.accumulate) scores = nullptr;
+        const auto ok16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+        const int aligned = (ok16(a.q) && a.q_stride % 4 == 0 ? 1 : 0) | (ok16(a.context) ? 2 : 0);
+        const bool fine = c.block == 16, wide = c.head_dim > 64;
+        cudaError_t e = wide ? fine ? launch_tiles<128, true>(a, sm_count, aligned, parts, scores, lse, s)
+                                    : launch_tiles<128, false>(a, sm_count, aligned, parts, scores, lse, s)
+                        : fine ? launch_tiles<64, true>(a, sm_count, aligned, parts, scores, lse, s)
+                               : launch_tiles<64, false>(a, sm_count, aligned, parts, scores, lse, s);
+        if (e == cudaSuccess && a.accumulate)
+            e = launch_dependent(kv8_add_weights_kernel, dim3((c.capacity + 1023) / 1024, c.kv_heads, c.batch), dim3(256),
+                                 0, s, a, static_cast<const float*>(scores), static_cast<const float*>(lse));
+        return e;
+    }
     cudaError_t e = launch_dependent(kv8_attention_rows_kernel, dim3(a.rows_per_seq, a.heads, c.batch),
                                      dim3(kWarps * 32), 0, s, a, lse);
     if (e == cudaSuccess && a.accumulate)
         e = launch_dependent(kv8_weights_kernel, dim3((c.capacity + kWarps - 1) / kWarps, c.kv_heads, c.batch),
-                             dim3(kWarps * 32), 0, s, a, lse);
+                             dim3(kWarps * 32), 0, s, a, static_cast<const float*>(lse));
     return e;
 }
 

@@ -103,7 +103,7 @@ class KVCache8:
         """The shared scratch, grown to this call's sizes before its first call."""
         if (rows_per_seq, heads) not in self._scratch_for:
             need = self._lib.kt_kv8_scratch_bytes(self.batch, rows_per_seq, heads, self.kv_heads, self.head_dim,
-                                                  self.capacity)
+                                                  self.capacity, self.weights is not None)
             if need > self._scratch.numel():
                 self._scratch = torch.zeros(need, dtype=torch.uint8, device=self.device)
             self._scratch_for.add((rows_per_seq, heads))

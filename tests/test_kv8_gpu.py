@@ -467,4 +467,4 @@ def test_refusals(kt):
     assert lib.kt_kv8_store(h, ctypes.byref(s), None, None, 128, 128, 0, None, None, None) == 0
     assert lib.kt_kv8_store(h, ctypes.byref(s), x.data_ptr(), x.data_ptr(), 128, 128, -1, None, None, None) == 1
     assert lib.kt_kv8_attention(h, ctypes.byref(s), x.data_ptr(), 128, x.data_ptr(), 1, None, 2, 1.0, 0, None, None) == 1
-    assert lib.kt_kv8_scratch_bytes(0, 1, 1, 1, 64, 64) == 0
+    assert lib.kt_kv8_scratch_bytes(0, 1, 1, 1, 64, 64, 0) == 0
