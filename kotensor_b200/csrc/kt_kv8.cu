@@ -323,7 +323,7 @@ kt_status kt_kv8_attention(kt_ctx* ctx, const kt_kv8_cache* cache, const float* 
     if (!aligned16(scratch)) return entry_fail(KT_ERR_INVALID_ARGUMENT, "scratch must be 16-byte aligned");
     return c_entry(ctx, [&] {
         const Kv8Attention a{*cache, q, q_stride, context, counts, rows_per_seq, heads, scale, accumulate_weights, scratch};
-        return entry_launch(launch_kv8_attention(a, ctx->sm_count, static_cast<cudaStream_t>(stream)),
+        return entry_launch(launch_kv8_attention(a, ctx->sm_count, ctx->d_error, static_cast<cudaStream_t>(stream)),
                             "kv8 attention launch");
     });
 }

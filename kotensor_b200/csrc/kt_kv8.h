@@ -95,7 +95,11 @@ struct Kv8Attention {
 // Bytes behind the counters that the attention of these sizes uses (kt_kv8_attention.cu).
 size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
                            int32_t capacity, bool weights);
-cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, cudaStream_t s);
+cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, int32_t* err, cudaStream_t s);
+// Many query rows, on tcgen05 (kt_kv8_prompt.cu).  aligned: bit 0, q's rows lie on
+// 16-byte boundaries.  lse (NULL: not wanted): ln of the softmax's sum of every row
+// and head.
+cudaError_t launch_kv8_prompt(const Kv8Attention& a, int aligned, float* lse, int32_t* err, cudaStream_t s);
 
 #ifdef __CUDACC__
 // Tokens that sequence b holds, whatever the caller left in lengths.

@@ -16,7 +16,7 @@ namespace kt {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in the row kernel
+constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in kv8_weights_kernel
 
 // ------------------------------------------------------------ few query rows
 //
@@ -351,7 +351,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                 l += p0 + p1;
                 two_terms(p0, p1, pa[j >> 1][(j & 1) * 2], pa[j >> 1][(j & 1) * 2 + 1]);
             }
-            const float vs0 = lds32(stage + 2 * S::kTileBytes + 8), vs1 = lds32(stage + 2 * S::kTileBytes + 12);
+            // a block that the vector does not see has no scale, whatever is there
+            const float vs0 = first < limit ? lds32(stage + 2 * S::kTileBytes + 8) : 0.0f;
+            const float vs1 = first + 16 < limit ? lds32(stage + 2 * S::kTileBytes + 12) : 0.0f;
             // values: thread (t, n8) reads dims n8 * kTiles .. of slots 2t, 2t + 1, 2t + 8, 2t + 9 of
             // each 16; n-tile q of the product is dim n8 * kTiles + q
             uint32_t v[2][4][HDP / 32];
@@ -527,63 +529,6 @@ __global__ void __launch_bounds__(256) kv8_add_weights_kernel(Kv8Attention a, co
         if (j + i < n) to[i] += w[i];
 }
 
-// One CTA per (row, query head, sequence): warp w takes slots w, w + 8, ..., a lane
-// dims lane, lane + 32, ...; each warp keeps a running maximum, sum and weighted
-// sum of values, merged at the end.
-__global__ void __launch_bounds__(kWarps * 32) kv8_attention_rows_kernel(Kv8Attention a, float* __restrict__ lse) {
-    dev::pdl_wait();
-    dev::pdl_launch_dependents();
-    const Kv8& c = a.cache;
-    const int t = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, d = c.head_dim;
-    const int64_t row = static_cast<int64_t>(b) * a.rows_per_seq + t;
-    float* out = a.context + (row * a.heads + head) * d;
-    if (t >= kv8_rows(a.counts, b, a.rows_per_seq)) {
-        for (int i = threadIdx.x; i < d; i += blockDim.x) out[i] = 0.0f;
-        return;
-    }
-    const int n = min(kv8_held(c, b) + t + 1, c.capacity);
-    const int64_t kvh = static_cast<int64_t>(b) * c.kv_heads + head / (a.heads / c.kv_heads);
-    const int8_t* kc = c.k_codes + kvh * c.capacity * d;
-    const int8_t* vc = c.v_codes + kvh * c.capacity * d;
-    const float* ks = c.k_scales + kvh * (c.capacity / c.block);
-    const float* vs = c.v_scales + kvh * (c.capacity / c.block);
-    const float* q = a.q + row * a.q_stride + head * d;
-    float qr[kDims], o[kDims] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kDims; ++i) qr[i] = lane + 32 * i < d ? q[lane + 32 * i] : 0.0f;
-    for (int j = warp; j < n; j += kWarps) {
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kDims; ++i)
-            if (lane + 32 * i < d) s = fmaf(qr[i], kc[static_cast<int64_t>(j) * d + lane + 32 * i], s);
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s = s * ks[j / c.block] * a.scale;
-        const float top = fmaxf(m, s), keep = m == top ? 1.0f : expf(m - top), p = s == -INFINITY ? 0.0f : expf(s - top);
-        const float pv = p * vs[j / c.block];
-        l = l * keep + p;
-        m = top;
-#pragma unroll
-        for (int i = 0; i < kDims; ++i)
-            if (lane + 32 * i < d) o[i] = o[i] * keep + pv * vc[static_cast<int64_t>(j) * d + lane + 32 * i];
-    }
-    __shared__ float sm[kWarps], sl[kWarps], so[kWarps][kKv8MaxHeadDim];
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int i = 0; i < kDims; ++i) so[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float top = -INFINITY, sum = 0.0f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w]);
-    for (int w = 0; w < kWarps; ++w) sum += sl[w] > 0.0f || sl[w] != sl[w] ? sl[w] * expf(sm[w] - top) : 0.0f;
-    for (int i = threadIdx.x; i < d; i += blockDim.x) {
-        float y = 0.0f;
-        for (int w = 0; w < kWarps; ++w)
-            if (sl[w] > 0.0f || sl[w] != sl[w]) y += so[w][i] * expf(sm[w] - top);
-        out[i] = y / sum;
-    }
-    if (threadIdx.x == 0) lse[row * a.heads + head] = top + logf(sum);
-}
-
 // One warp per slot adds up its weight over the rows and heads of its group, in order.
 __global__ void __launch_bounds__(kWarps * 32) kv8_weights_kernel(Kv8Attention a, const float* __restrict__ lse) {
     dev::pdl_wait();
@@ -616,7 +561,6 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_weights_kernel(Kv8Attention a
 }  // namespace
 
 namespace {
-// Blocks of query vectors that one row kernel launch would repeat the cache for.
 bool use_tiles(int32_t rows_per_seq, int32_t heads, int32_t kv_heads) {
     return static_cast<int64_t>(rows_per_seq) * (heads / kv_heads) <= 64;
 }
@@ -657,16 +601,16 @@ size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, i
     return n;
 }
 
-cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, cudaStream_t s) {
+cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, int32_t* err, cudaStream_t s) {
     const Kv8& c = a.cache;
     char* free = static_cast<char*>(a.scratch) + kKv8CounterBytes;
     float* parts = reinterpret_cast<float*>(free);
     float* lse = reinterpret_cast<float*>(free + part_bytes(c.head_dim));
+    const auto ok16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const int aligned = (ok16(a.q) && a.q_stride % 4 == 0 ? 1 : 0) | (ok16(a.context) ? 2 : 0);
     if (use_tiles(a.rows_per_seq, a.heads, c.kv_heads)) {
         float* scores = reinterpret_cast<float*>(free + part_bytes(c.head_dim) + lse_bytes(c.batch, a.rows_per_seq, a.heads));
         if (!a.accumulate) scores = nullptr;
-        const auto ok16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-        const int aligned = (ok16(a.q) && a.q_stride % 4 == 0 ? 1 : 0) | (ok16(a.context) ? 2 : 0);
         const bool fine = c.block == 16, wide = c.head_dim > 64;
         cudaError_t e = wide ? fine ? launch_tiles<128, true>(a, sm_count, aligned, parts, scores, lse, s)
                                     : launch_tiles<128, false>(a, sm_count, aligned, parts, scores, lse, s)
@@ -677,8 +621,7 @@ cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, cudaStream
                                  0, s, a, static_cast<const float*>(scores), static_cast<const float*>(lse));
         return e;
     }
-    cudaError_t e = launch_dependent(kv8_attention_rows_kernel, dim3(a.rows_per_seq, a.heads, c.batch),
-                                     dim3(kWarps * 32), 0, s, a, lse);
+    cudaError_t e = launch_kv8_prompt(a, aligned, a.accumulate ? lse : nullptr, err, s);
     if (e == cudaSuccess && a.accumulate)
         e = launch_dependent(kv8_weights_kernel, dim3((c.capacity + kWarps - 1) / kWarps, c.kv_heads, c.batch),
                              dim3(kWarps * 32), 0, s, a, static_cast<const float*>(lse));

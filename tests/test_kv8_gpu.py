@@ -293,6 +293,24 @@ def test_attention_shows_values_that_are_not_finite(kt):
     assert bool(out[:, 256:320].isnan().all()) and bool(out[:, 320:].isfinite().all())
 
 
+@pytest.mark.parametrize("rows", [12, 60])
+def test_attention_of_rows_before_a_value_that_is_not_finite(kt, rows):
+    """A token of NaN poisons its block of 16 slots: rows before the block stay finite, rows from the
+    token on are NaN."""
+    from kotensor_b200.kv8 import KVCache8
+    for name in "kv":
+        cache = KVCache8(1, 1, 2, 64, 128, 16)
+        x = {n: torch.randn(rows, 128, device="cuda") for n in "kv"}
+        x[name][10, :64] = float("nan")   # slot 36 + 10 = 46 of head 0: the block 32..47
+        cache.store(0, torch.randn(36, 128, device="cuda"), torch.randn(36, 128, device="cuda"), 36)
+        cache.advance(36)
+        cache.store(0, x["k"], x["v"], rows)
+        cache.lengths.fill_(28)           # row t sees slots 0..28 + t
+        out = cache.attend(0, torch.randn(rows, 512, device="cuda"), 8, rows)
+        assert bool(out[:4].isfinite().all()), name
+        assert bool(out[4:, :256].isnan().all()) and bool(out[:, 256:].isfinite().all()), name
+
+
 def test_attention_is_the_same_on_every_run_and_in_a_graph(kt):
     """Equal bits from run to run, on another stream, and when a captured step replays at other lengths."""
     cache, ref, rng = make(kt, 3, 4, 128, 1024, 64, [5, 700, 300])
