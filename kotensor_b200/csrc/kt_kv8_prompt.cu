@@ -8,23 +8,27 @@
 // (kt_kv8_attention.cu), so each product is two tcgen05.mma chains into one fp32
 // accumulator: 4 x 128 x 128 x head_dim x 2 operations a tile.
 //
-// Even tiles and odd tiles are two streams with their own S, O, running maximum and
-// sum: while four warps turn one stream's S into P, the tensor cores work on the
-// other's products.  They meet once, at the end.  Tensor memory: S of stream x in
-// columns 128 x .., where P replaces it (a thread owns one vector, lane and row of
-// both: 32 scores read, 16 + 16 columns of hi and lo pairs written back in their
-// place); O of stream x in columns 256 + HDP x ...
-//   warps 0-3, 4-7  softmax of stream 0, 1, and their share of the epilogue
-//   warps 8-11      codes -> fp16, K and V tiles in 128-byte swizzled rows of 64 dims
+// Tensor memory holds Q (both terms, the first product's A), the scores of two
+// tiles, each replaced in place by its P (a thread owns one vector, a lane of all of
+// them; 32 scores read, 16 + 16 columns of hi and lo pairs written back), and one
+// O tile.  Only the B operands, K and V, pass through shared memory: with Q there
+// too, the first product alone would take its whole bandwidth.
+//   warps 0-3, 4-7  scores -> P of the even, the odd tiles; every tile has its own
+//                   references, so no tile waits for another's
+//   warps 8-11      add each O tile to sums in registers (the tensor cores' fp32
+//                   accumulation truncates: over a long run of tiles the error is
+//                   five times that of these rounded sums) and write the result;
+//                   lane 0 of warp 8 issues the products
+//   warps 12-15     codes -> fp16, K and V tiles in 128-byte swizzled rows of 64 dims
 //                   (K-major for the first product, MN-major for the second: the
 //                   same bytes, another descriptor)
-//   warp 12         issues the products
+// Order of the products: P V of tile i, then Q K^T of tile i + 2; while the second
+// runs, O of tile i is read, and tile i + 1 becomes P meanwhile.
 //
-// References.  The sum l is relative to the running maximum D of the scores.  The
-// numerators carry the values' scales, which may differ by any factor from block
-// to block, so they are relative to a reference R of their own, the maximum of
-// score + log2(value scale): both terms of P keep 22 bits of what matters to O.
-// R moves only when the maximum passes it by 2^kSlack, so O is seldom rescaled.
+// References.  A tile's sum l is relative to its largest score D.  The numerators
+// carry the values' scales, which may differ by any factor from block to block, so
+// they have a reference R of their own, the maximum of score + log2(value scale):
+// both terms of P keep 22 bits of what matters to O.
 #include <cuda_fp16.h>
 
 #include "kt_kv8.h"
@@ -34,23 +38,30 @@ namespace {
 
 constexpr int kVecTile = 128;   // query vectors of a CTA (the MMA's M)
 constexpr int kSlots = 128;     // slots of a tile (the first product's N, the second's K)
-constexpr int kSoftmaxWarps = 8;
-constexpr int kConvertWarps = 4;
-constexpr int kMmaWarp = kSoftmaxWarps + kConvertWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kSumWarp = 8;      // first of the four that add up O; before them the softmax warps
+constexpr int kConvertWarp = 12; // first of the four that convert
+constexpr int kThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLift = 7.0f;   // numerators are 2^kLift larger, up to 2^(kLift + kSlack) <= 2^15
-constexpr float kSlack = 8.0f;
+constexpr float kLift = 14.0f;   // numerators are 2^kLift larger: their lo terms stay clear of the subnormals
+constexpr float kSlack = 20.0f;  // the sums' reference moves when a tile's passes it by this much
+// Registers of each role's warps: 8 x 112 + 4 x 184 + 4 x 104 = 16 x 128 of the launch.
+constexpr int kSoftmaxRegs = 112, kSumRegs = 184, kConvertRegs = 104;
 
+// Tensor memory columns.
 template <int HDP>
 struct PromptShape {
     static constexpr int kBlocks = HDP / 64;              // blocks of 64 dims: 128-byte rows
     static constexpr int kTile = kBlocks * kSlots * 128;  // fp16 tile of 128 rows
-    static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile, kEnd = 6 * kTile;
-    static constexpr int kOutPitch = kVecTile + 1;        // epilogue: [dim][vector], over K and V
-    static constexpr int kSmem = 1024 + kEnd + kVecTile * 4 + 256;
-    static_assert(HDP * kOutPitch * 4 + 3 * kVecTile * 4 <= 4 * kTile + 4096, "epilogue area");
+    static constexpr int kK = 0, kV = 2 * kTile, kEnd = 4 * kTile;
+    static constexpr int kOutPitch = kVecTile + 1;        // at the end: [dim][vector], over K and V
+    // after the tiles: factor and largest component of each query, D, l, R of four tiles, barriers
+    static constexpr int kFactor = kEnd, kTop = kFactor + kVecTile * 4, kStats = kTop + 2 * kVecTile * 4;
+    static constexpr int kBars = kStats + 4 * 3 * kVecTile * 4;
+    static constexpr int kSmem = 1024 + kBars + 256;
+    static constexpr uint32_t kO = 2 * kSlots, kQ = kO + HDP;  // S of stream x at kSlots * x; Q hi, then lo
+    static_assert(HDP * kOutPitch * 4 <= kEnd, "epilogue area");
     static_assert(kSmem <= 232448, "shared memory per CTA");
+    static_assert(kQ + HDP <= 512, "tensor memory");
 };
 
 __device__ __forceinline__ uint64_t desc_base(uint32_t addr, uint32_t lead) {
@@ -58,13 +69,6 @@ __device__ __forceinline__ uint64_t desc_base(uint32_t addr, uint32_t lead) {
     return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
            (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
            (static_cast<uint64_t>(2) << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -111,6 +115,17 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -132,6 +147,67 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t flipped) {
 // Byte offset of 16-byte piece `piece` (of 64 dims: 8) of row `row` in a swizzled block.
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
     return static_cast<uint32_t>(row * 128 + ((piece ^ (row & 7)) << 4));
+}
+
+// Scores of one tile -> P in place, for the vector of this thread: first slot
+// `first`, S and P at tensor memory address s_tm.  Lane g of the warp has the scales
+// of slots first + 16 g .. in k_scale, v_scale.  kEdge: some vector of the warp does
+// not see all of the tile's slots; this one sees those below `limit`.
+template <bool kEdge>
+__device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit, float factor, float k_scale,
+                                            float v_scale, float& D, float& l, float& R) {
+    // a block the vector does not see has no scale, whatever is there
+    auto k_of = [&](int g) {
+        const float k = __shfl_sync(0xffffffffu, k_scale, g) * factor;
+        return kEdge && first + 16 * g >= limit ? 0.0f : k;
+    };
+    auto v_of = [&](int g) {
+        const float v = __shfl_sync(0xffffffffu, v_scale, g);
+        return kEdge && first + 16 * g >= limit ? 0.0f : v;
+    };
+    uint32_t s[32];
+    D = R = -INFINITY;
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+        ld32(s_tm + 32 * q, s);
+        float m[2] = {-INFINITY, -INFINITY};
+        const float k0 = k_of(2 * q), k1 = k_of(2 * q + 1), v0 = __log2f(v_of(2 * q)), v1 = __log2f(v_of(2 * q + 1));
+        wait_ld(s);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (!kEdge || first + 32 * q + j < limit) m[j / 16] = fmaxf(m[j / 16], __uint_as_float(s[j]));
+        m[0] = m[0] == -INFINITY ? m[0] : m[0] * k0;
+        m[1] = m[1] == -INFINITY ? m[1] : m[1] * k1;
+        D = fmaxf(D, fmaxf(m[0], m[1]));
+        R = fmaxf(R, fmaxf(m[0] + v0, m[1] + v1));
+    }
+    const float ref = D == -INFINITY ? 0.0f : D;
+    const float raise = R == -INFINITY ? 0.0f : ex2(fminf(ref - R + kLift, 126.0f));
+    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+        ld32(s_tm + 32 * q, s);
+        float k[2] = {k_of(2 * q), k_of(2 * q + 1)}, v[2] = {v_of(2 * q) * raise, v_of(2 * q + 1) * raise};
+        // where a product overflows its probabilities are 0
+        if (v[0] > 3e38f) v[0] = 3e38f;
+        if (v[1] > 3e38f) v[1] = 3e38f;
+        wait_ld(s);
+        uint32_t out[32];  // hi pairs of 32 slots, then lo pairs
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            float z0 = fmaf(__uint_as_float(s[j]), k[j / 16], -ref), z1 = fmaf(__uint_as_float(s[j + 1]), k[j / 16], -ref);
+            if (kEdge) {
+                if (first + 32 * q + j >= limit) z0 = -INFINITY;
+                if (first + 32 * q + j + 1 >= limit) z1 = -INFINITY;
+            }
+            const float p0 = ex2(z0), p1 = ex2(z1);
+            l0 += p0;
+            l1 += p1;
+            two_terms(p0 * v[j / 16], p1 * v[j / 16], out[j / 2], out[16 + j / 2]);
+        }
+        st32(s_tm + 32 * q, out);
+    }
+    l = l0 + l1;
 }
 
 template <int HDP>
@@ -165,29 +241,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = dev::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
-    float* const q_factor = reinterpret_cast<float*>(smem + S::kEnd);
-    const uint32_t bars = base + S::kEnd + kVecTile * 4;
+    float* const q_factor = reinterpret_cast<float*>(smem + S::kFactor);
+    float* const q_top = reinterpret_cast<float*>(smem + S::kTop);
+    float* const stats = reinterpret_cast<float*>(smem + S::kStats);  // [tile % 4][D, l, R][vector]
+    const uint32_t bars = base + S::kBars;
     auto k_full = [&](int x) { return bars + 8 * x; };
     auto k_free = [&](int x) { return bars + 16 + 8 * x; };
     auto v_full = [&](int x) { return bars + 32 + 8 * x; };
     auto v_free = [&](int x) { return bars + 48 + 8 * x; };
     auto s_full = [&](int x) { return bars + 64 + 8 * x; };
     auto p_full = [&](int x) { return bars + 80 + 8 * x; };
-    const uint32_t done = bars + 96;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kEnd + kVecTile * 4 + 104);
+    const uint32_t o_full = bars + 96, o_free = bars + 104;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kBars + 112);
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; ++x) {
-            dev::mbar_init(k_full(x), kConvertWarps);
+            dev::mbar_init(k_full(x), 4);
             dev::mbar_init(k_free(x), 1);
-            dev::mbar_init(v_full(x), kConvertWarps);
+            dev::mbar_init(v_full(x), 4);
             dev::mbar_init(v_free(x), 1);
             dev::mbar_init(s_full(x), 1);
             dev::mbar_init(p_full(x), 4);
         }
-        dev::mbar_init(done, 1);
+        dev::mbar_init(o_full, 1);
+        dev::mbar_init(o_free, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) {
+    if (warp == kSumWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dev::smem_u32(tmem_slot))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -210,148 +289,79 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
     auto wait_all = [&](uint32_t bar, uint32_t parity) {  // a warp: its lanes go on, or give up, together
         return __all_sync(0xffffffffu, wait(bar, parity));
     };
-    // The state of a softmax thread: vector v0 + row of stream x.
-    const int x = warp / 4, row = (warp % 4) * 32 + lane;
-    float D = -INFINITY, R = -INFINITY, l = 0.0f;
+    const int row = (warp % 4) * 32 + lane;  // the vector, and lane of tensor memory, of a thread
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp % 4) << 21);
 
-    if (warp < kSoftmaxWarps) {
-        // Queries, a warp to a vector, a lane to four dims: scaled by a power of two to
-        // at most 1 and split into two terms; a negative scale turns the query's sign.
-        for (int v = warp; v < kVecTile; v += kSoftmaxWarps) {
-            float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const int dim = 4 * lane;
-            if (v < real && dim < d) {
-                const float* q = a.q + place(v0 + v, a.q_stride) + dim;
-                if (aligned & 1) {
-                    const float4 t = *reinterpret_cast<const float4*>(q);
-                    f[0] = t.x, f[1] = t.y, f[2] = t.z, f[3] = t.w;
-                } else {
-                    f[0] = q[0], f[1] = q[1], f[2] = q[2], f[3] = q[3];
+    if (warp < kSumWarp) {
+        fewer_registers<kSoftmaxRegs>();
+        const int x = warp / 4;
+        {
+            // Queries: scaled by a power of two to at most 1, in two terms; a negative scale
+            // turns their sign.  Warps 0-3 take the first half of the dims, 4-7 the second.
+            constexpr int kHalf = HDP / 2;
+            const float* q = a.q + place(v0 + row, a.q_stride) + x * kHalf;
+            float f[kHalf];
+            uint32_t top = 0;  // the largest exponent, by the bits of |q|; NaN counts as infinity
+#pragma unroll
+            for (int i = 0; i < kHalf; i += 4) {
+                f[i] = f[i + 1] = f[i + 2] = f[i + 3] = 0.0f;
+                if (row < real && x * kHalf + i < d) {
+                    if (aligned & 1) {
+                        const float4 t = *reinterpret_cast<const float4*>(q + i);
+                        f[i] = t.x, f[i + 1] = t.y, f[i + 2] = t.z, f[i + 3] = t.w;
+                    } else {
+                        f[i] = q[i], f[i + 1] = q[i + 1], f[i + 2] = q[i + 2], f[i + 3] = q[i + 3];
+                    }
                 }
             }
-            uint32_t top = 0;  // the largest exponent, by the bits of |q|; NaN counts as infinity
-            for (int i = 0; i < 4; ++i) top = max(top, min(__float_as_uint(f[i]) & 0x7fffffffu, 0x7f800000u));
-            top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) top = max(top, min(__float_as_uint(f[i]) & 0x7fffffffu, 0x7f800000u));
+            q_top[x * kVecTile + row] = __uint_as_float(top);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            top = max(top, __float_as_uint(q_top[(1 - x) * kVecTile + row]));
             const int e = min(max(static_cast<int>(top >> 23) - 126, -126), 126);
             float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
             if (a.scale < 0.0f) down = -down;
-            if (lane == 0) q_factor[v] = fabsf(a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            if (dim < HDP) {
-                uint2 hi, lo;
-                two_terms(f[0] * down, f[1] * down, hi.x, lo.x);
-                two_terms(f[2] * down, f[3] * down, hi.y, lo.y);
-                const uint32_t at = S::kQ + (dim / 64) * (kVecTile * 128) + swizzled(v, dim % 64 / 8) + (lane & 1) * 8;
-                *reinterpret_cast<uint2*>(smem + at) = hi;
-                *reinterpret_cast<uint2*>(smem + at + S::kTile) = lo;
+            if (x == 0) q_factor[row] = fabsf(a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+            for (int q = 0; q < kHalf; q += 32) {
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) two_terms(f[q + 2 * i] * down, f[q + 2 * i + 1] * down, hi[i], lo[i]);
+                st16(lanes + S::kQ + (x * kHalf + q) / 2, hi);
+                st16(lanes + S::kQ + HDP / 2 + (x * kHalf + q) / 2, lo);
             }
+            wait_st();
+            tc_before();
+            asm volatile("bar.sync 2, 288;" ::: "memory");  // with warp 8: the queries are in place
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        asm volatile("bar.sync 1, %0;" ::"n"((kSoftmaxWarps + 1) * 32) : "memory");
-
-        const uint32_t s_tm = tmem + (static_cast<uint32_t>(row & ~31) << 16) + x * kSlots;
-        const uint32_t o_tm = tmem + (static_cast<uint32_t>(row & ~31) << 16) + 2 * kSlots + x * HDP;
+        const uint32_t s_tm = lanes + x * kSlots;
         const float factor = q_factor[row];
         const int limit = row < real ? min(held + (v0 + row) / group + 1, seen) : 0;
         const float* k_scales = c.k_scales + head * (c.capacity / c.block);
         const float* v_scales = c.v_scales + head * (c.capacity / c.block);
-        for (int i = x, it = 0; i < tiles; i += 2, ++it) {
-            const int first = i * kSlots;
-            float ks[8], vs[8];
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {  // a block the vector does not see has no scale, whatever is there
-                const bool in = first + 16 * g < limit;
-                const int at = in ? (first + 16 * g) / c.block : 0;
-                ks[g] = in ? k_scales[at] * factor : 0.0f;
-                vs[g] = in ? v_scales[at] : 0.0f;
-            }
-            if (!wait_all(s_full(x), it & 1)) break;
+        for (int i = x; i < tiles; i += 2) {
+            const int first = i * kSlots, at = first + 16 * (lane % 8);
+            const float ks = at < most ? k_scales[at / c.block] : 0.0f, vs = at < most ? v_scales[at / c.block] : 0.0f;
+            if (!wait_all(s_full(x), (i / 2) & 1)) break;
             tc_after();
-            const bool edge = __any_sync(0xffffffffu, first + kSlots > limit);
-            // the largest score of each 16 slots
-            float top[8];
-            uint32_t s[2][32];
-            ld32(s_tm, s[0]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                wait_ld(s[q & 1]);
-                if (q < 3) ld32(s_tm + 32 * (q + 1), s[(q + 1) & 1]);
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    float m = -INFINITY;
-                    if (edge) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (first + 32 * q + 16 * g + j < limit) m = fmaxf(m, __uint_as_float(s[q & 1][16 * g + j]));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) m = fmaxf(m, __uint_as_float(s[q & 1][16 * g + j]));
-                    }
-                    top[2 * q + g] = m == -INFINITY ? m : m * ks[2 * q + g];
-                }
-            }
-            ld32(s_tm, s[0]);
-            float new_d = D, most_w = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                new_d = fmaxf(new_d, top[g]);
-                most_w = fmaxf(most_w, top[g] + __log2f(vs[g]));
-            }
-            const float ref = new_d == -INFINITY ? 0.0f : new_d;
-            l = D == -INFINITY ? l : l * ex2(D - ref);
-            D = new_d;
-            const bool move = most_w > R + kSlack || (R == -INFINITY && most_w > R);
-            if (__any_sync(0xffffffffu, move)) {
-                const float fade = !move ? 1.0f : R == -INFINITY ? 0.0f : ex2(R - most_w);
-                if (move) R = most_w;
-                if (it > 0) {  // the stream's products are complete: its newest scores were issued after them
-                    wait_ld(s[0]);
-#pragma unroll
-                    for (int q = 0; q < HDP / 32; ++q) {
-                        ld32(o_tm + 32 * q, s[1]);
-                        wait_ld(s[1]);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) s[1][j] = __float_as_uint(__uint_as_float(s[1][j]) * fade);
-                        st32(o_tm + 32 * q, s[1]);
-                    }
-                }
-            }
-            const float raise = R == -INFINITY ? 0.0f : ex2(fminf(ref - R + kLift, 126.0f));
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                vs[g] *= raise;
-                if (vs[g] > 3e38f) vs[g] = 3e38f;  // its probabilities are 0 then
-            }
-            float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                wait_ld(s[q & 1]);
-                if (q < 3) ld32(s_tm + 32 * (q + 1), s[(q + 1) & 1]);
-                uint32_t out[32];  // hi pairs of 32 slots, then lo pairs
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    float z0 = fmaf(__uint_as_float(s[q & 1][j]), ks[2 * q + j / 16], -ref);
-                    float z1 = fmaf(__uint_as_float(s[q & 1][j + 1]), ks[2 * q + j / 16], -ref);
-                    if (edge) {
-                        if (first + 32 * q + j >= limit) z0 = -INFINITY;
-                        if (first + 32 * q + j + 1 >= limit) z1 = -INFINITY;
-                    }
-                    const float p0 = ex2(z0), p1 = ex2(z1);
-                    l0 += p0;
-                    l1 += p1;
-                    two_terms(p0 * vs[2 * q + j / 16], p1 * vs[2 * q + j / 16], out[j / 2], out[16 + j / 2]);
-                }
-                st32(s_tm + 32 * q, out);
-            }
-            l += l0 + l1;
+            float D, l, R;
+            if (__any_sync(0xffffffffu, first + kSlots > limit)) scores_to_p<true>(s_tm, first, limit, factor, ks, vs, D, l, R);
+            else scores_to_p<false>(s_tm, first, limit, factor, ks, vs, D, l, R);
+            float* mine = stats + (i % 4) * 3 * kVecTile + row;
+            mine[0] = D;
+            mine[kVecTile] = l;
+            mine[2 * kVecTile] = R;
             wait_st();
             tc_before();
             __syncwarp();
             if (lane == 0) dev::mbar_arrive(p_full(x));
         }
-    } else if (warp < kMmaWarp) {
+    } else if (warp >= kConvertWarp) {
+        fewer_registers<kConvertRegs>();
         // 128 threads: piece of 16 codes `piece` of rows r0, r0 + kStep, ...
         constexpr int kPieces = HDP / 16, kStep = 128 / kPieces, kLoads = kSlots / kStep;
-        const int tid = threadIdx.x - kSoftmaxWarps * 32, piece = tid % kPieces, r0 = tid / kPieces;
+        const int tid = threadIdx.x - kConvertWarp * 32, piece = tid % kPieces, r0 = tid / kPieces;
         const bool inside = piece * 16 < d;
         const int8_t* kc = c.k_codes + head * c.capacity * d + piece * 16;
         const int8_t* vc = c.v_codes + head * c.capacity * d + piece * 16;
@@ -395,105 +405,98 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             if (lane == 0) dev::mbar_arrive(v_full(y));
         }
     } else {
-        asm volatile("bar.sync 1, %0;" ::"n"((kSoftmaxWarps + 1) * 32) : "memory");  // the queries are in place
-        if (lane == 0) {
-            constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kSlots >> 3) << 17) | (static_cast<uint32_t>(kVecTile >> 4) << 24);
-            // the second product's B is MN-major (bit 16)
-            constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(HDP >> 3) << 17) |
-                                         (static_cast<uint32_t>(kVecTile >> 4) << 24);
-            auto scores = [&](int i) {
-                const int y = i & 1;
-                if (!wait(k_full(y), (i / 2) & 1)) return false;
-                tc_after();
+        more_registers<kSumRegs>();
+        constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kSlots >> 3) << 17) | (static_cast<uint32_t>(kVecTile >> 4) << 24);
+        // the second product's B is MN-major (bit 16)
+        constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(HDP >> 3) << 17) |
+                                     (static_cast<uint32_t>(kVecTile >> 4) << 24);
+        auto scores = [&](int i) {  // the small terms first: the accumulator's truncation is relative to its value
+            const int y = i & 1;
+            if (!wait(k_full(y), (i / 2) & 1)) return;
+            tc_after();
 #pragma unroll
-                for (int s = 0; s < HDP / 16; ++s) {
-                    const uint32_t at = (s / 4) * (128 * 128) + (s % 4) * 32;
-                    const uint64_t kd = desc_base(base + S::kK + y * S::kTile + at, 16);
-                    mma_ss(tmem + y * kSlots, desc_base(base + S::kQ + at, 16), kd, kIdescS, s > 0);
-                    mma_ss(tmem + y * kSlots, desc_base(base + S::kQ + S::kTile + at, 16), kd, kIdescS, 1);
-                }
-                mma_commit(s_full(y));
-                mma_commit(k_free(y));
-                return true;
-            };
-            bool go = true;
-            for (int i = 0; go && i < min(2, tiles); ++i) go = scores(i);
-            for (int i = 0; go && i < tiles; ++i) {
-                const int y = i & 1;
-                go = wait(v_full(y), (i / 2) & 1) && wait(p_full(y), (i / 2) & 1);
-                if (!go) break;
-                tc_after();
-#pragma unroll
-                for (int s = 0; s < kSlots / 16; ++s) {
-                    const uint64_t vd = desc_base(base + S::kV + y * S::kTile + s * 2048, kSlots * 128);
-                    const uint32_t p = tmem + y * kSlots + (s / 2) * 32 + (s % 2) * 8;
-                    mma_ts(tmem + 2 * kSlots + y * HDP, p, vd, kIdescO, i >= 2 || s > 0);
-                    mma_ts(tmem + 2 * kSlots + y * HDP, p + 16, vd, kIdescO, 1);
-                }
-                mma_commit(v_free(y));
-                if (i + 2 < tiles) go = scores(i + 2);
+            for (int s = 0; s < HDP / 8; ++s) {
+                const int k = s % (HDP / 16), term = s < HDP / 16 ? 1 : 0;
+                const uint64_t kd = desc_base(base + S::kK + y * S::kTile + (k / 4) * (128 * 128) + (k % 4) * 32, 16);
+                mma_ts(tmem + y * kSlots, tmem + S::kQ + term * (HDP / 2) + 8 * k, kd, kIdescS, s > 0);
             }
-            mma_commit(done);
-            ok = true;
-            wait(done, 0);  // no product is in flight past this point
+            mma_commit(s_full(y));
+            mma_commit(k_free(y));
+        };
+        if (warp == kSumWarp) {
+            asm volatile("bar.sync 2, 288;" ::: "memory");  // the queries are in place
+            tc_after();
+            if (lane == 0)
+                for (int i = 0; i < min(2, tiles); ++i) scores(i);
+            __syncwarp();
         }
-        __syncwarp();
-    }
-
-    // The streams meet: stream 1 leaves its numerators and references, stream 0 adds its own.
-    float* const area = reinterpret_cast<float*>(smem + S::kK);            // [dim][vector]
-    float* const other = area + HDP * S::kOutPitch;                        // D, l of stream 1
-    const uint32_t o_tm = tmem + (static_cast<uint32_t>(row & ~31) << 16) + 2 * kSlots + x * HDP;
-    tc_before();
-    __syncthreads();
-    tc_after();
-    if (warp >= 4 && warp < kSoftmaxWarps) {
-        other[row] = D;
-        other[kVecTile + row] = l;
-    }
-    __syncthreads();
-    float scale = 0.0f;
-    if (warp < 4) {
-        const float d1 = other[row], l1 = other[kVecTile + row], dm = fmaxf(D, d1);
-        const float sum = (l == 0.0f ? 0.0f : l * ex2(D - dm)) + (l1 == 0.0f ? 0.0f : l1 * ex2(d1 - dm));
-        other[row] = dm;
-        other[kVecTile + row] = 1.0f / sum;
-        if (lse != nullptr && row < real)
-            lse[(static_cast<int64_t>(b) * a.rows_per_seq + (v0 + row) / group) * a.heads + h * group + (v0 + row) % group] =
-                (dm + log2f(sum)) / kLog2e;
-    }
-    __syncthreads();
-    if (warp < kSoftmaxWarps) {
-        const float dm = other[row];
-        scale = R == -INFINITY ? 0.0f : ex2(R - kLift - dm) * other[kVecTile + row];
-        if (l != l) scale = l;
-    }
-    const bool second = tiles > 1;
+        float o[HDP], D = -INFINITY, l = 0.0f, R = -INFINITY;
 #pragma unroll
-    for (int turn = 1; turn >= 0; --turn) {
-        if (warp < kSoftmaxWarps && x == turn && (turn == 0 || second)) {
+        for (int j = 0; j < HDP; ++j) o[j] = 0.0f;
+        for (int i = 0; i < tiles; ++i) {
+            const int y = i & 1;
+            // Every warp has seen tile i's P before it gives up tile i - 1's O, and the next
+            // product into O waits for both: no barrier runs two phases ahead of a warp.
+            if (!wait_all(p_full(y), (i / 2) & 1)) break;
+            if (i > 0 && lane == 0) dev::mbar_arrive(o_free);
+            if (warp == kSumWarp && lane == 0) {
+                if (wait(v_full(y), (i / 2) & 1) && (i == 0 || wait(o_free, (i - 1) & 1))) {
+                    tc_after();
+#pragma unroll
+                    for (int s = 0; s < kSlots / 8; ++s) {
+                        const int k = s % (kSlots / 16), term = s < kSlots / 16 ? 1 : 0;
+                        const uint64_t vd = desc_base(base + S::kV + y * S::kTile + k * 2048, kSlots * 128);
+                        mma_ts(tmem + S::kO, tmem + y * kSlots + (k / 2) * 32 + (k % 2) * 8 + term * 16, vd, kIdescO, s > 0);
+                    }
+                    mma_commit(o_full);
+                    mma_commit(v_free(y));
+                    if (i + 2 < tiles) scores(i + 2);
+                }
+            }
+            __syncwarp();
+            if (!wait_all(o_full, i & 1)) break;
+            tc_after();
+            const float* tile = stats + (i % 4) * 3 * kVecTile + row;
+            const float tD = tile[0], tl = tile[kVecTile], tR = tile[2 * kVecTile];
+            const float top = fmaxf(D, tD);
+            l = (l == 0.0f ? 0.0f : l * ex2(D - top)) + (tl == 0.0f ? 0.0f : tl * ex2(tD - top));
+            D = top;
+            const bool move = tR > R + kSlack || (R == -INFINITY && tR > R);
+            if (__any_sync(0xffffffffu, move)) {
+                const float fade = !move ? 1.0f : R == -INFINITY ? 0.0f : ex2(R - tR);
+                if (move) R = tR;
+#pragma unroll
+                for (int j = 0; j < HDP; ++j) o[j] *= fade;
+            }
+            const float gain = tR == -INFINITY ? 0.0f : ex2(tR - R);
 #pragma unroll
             for (int q = 0; q < HDP / 32; ++q) {
-                uint32_t o[32];
-                ld32(o_tm + 32 * q, o);
-                wait_ld(o);
+                uint32_t part[32];
+                ld32(lanes + S::kO + 32 * q, part);
+                wait_ld(part);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float* to = area + (32 * q + j) * S::kOutPitch + row;
-                    const float y = __uint_as_float(o[j]) * scale;
-                    *to = turn == 0 && second ? *to + y : y;
-                }
+                for (int j = 0; j < 32; ++j) o[32 * q + j] = fmaf(__uint_as_float(part[j]), gain, o[32 * q + j]);
             }
+            tc_before();
+            __syncwarp();
         }
-        __syncthreads();
-    }
-    for (int v = warp; v < real; v += kThreads / 32) {
-        float* to = a.context + place(v0 + v, static_cast<int64_t>(a.heads) * d);
-        for (int i = lane; i < d; i += 32) to[i] = area[i * S::kOutPitch + v];
+        // every product is complete (the last o_full came after all of them): K and V are free
+        if (lse != nullptr && row < real)
+            lse[(static_cast<int64_t>(b) * a.rows_per_seq + (v0 + row) / group) * a.heads + h * group + (v0 + row) % group] =
+                (D + log2f(l)) / kLog2e;
+        const float scale = l != l ? l : R == -INFINITY ? 0.0f : ex2(R - kLift - D) / l;
+        float* const area = reinterpret_cast<float*>(smem);  // [dim][vector]
+#pragma unroll
+        for (int j = 0; j < HDP; ++j) area[j * S::kOutPitch + row] = o[j] * scale;
+        asm volatile("bar.sync 3, 128;" ::: "memory");
+        for (int v = warp - kSumWarp; v < real; v += 4) {
+            float* to = a.context + place(v0 + v, static_cast<int64_t>(a.heads) * d);
+            for (int i = lane; i < d; i += 32) to[i] = area[i * S::kOutPitch + v];
+        }
     }
     tc_before();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == kSumWarp) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
