@@ -10,11 +10,11 @@
 //
 // Tensor memory holds Q (both terms, the first product's A), the scores of two
 // tiles, each replaced in place by its P (a thread owns one vector, a lane of all of
-// them; 32 scores read, 16 + 16 columns of hi and lo pairs written back), and one
+// them; of 32 scores come 16 + 16 columns of hi and lo pairs), and one
 // O tile.  Only the B operands, K and V, pass through shared memory: with Q there
 // too, the first product alone would take its whole bandwidth.
-//   warps 0-3, 4-7  scores -> P of the even, the odd tiles; every tile has its own
-//                   references, so no tile waits for another's
+//   warps 0-3, 4-7  scores -> P of the first, the last 64 slots of a tile; every tile
+//                   has its own references, so no tile waits for another's
 //   warps 8-11      add each O tile to sums in registers (the tensor cores' fp32
 //                   accumulation truncates: over a long run of tiles the error is
 //                   five times that of these rounded sums) and write the result;
@@ -54,9 +54,11 @@ struct PromptShape {
     static constexpr int kTile = kBlocks * kSlots * 128;  // fp16 tile of 128 rows
     static constexpr int kK = 0, kV = 2 * kTile, kEnd = 4 * kTile;
     static constexpr int kOutPitch = kVecTile + 1;        // at the end: [dim][vector], over K and V
-    // after the tiles: factor and largest component of each query, D, l, R of four tiles, barriers
+    // after the tiles: factor and largest component of each query, D, R, l of both halves of
+    // four tiles, barriers
     static constexpr int kFactor = kEnd, kTop = kFactor + kVecTile * 4, kStats = kTop + 2 * kVecTile * 4;
-    static constexpr int kBars = kStats + 4 * 3 * kVecTile * 4;
+    static constexpr int kMeet = kStats + 4 * 4 * kVecTile * 4;         // largest scores of the halves of two tiles
+    static constexpr int kBars = kMeet + 4 * kVecTile * 8;
     static constexpr int kSmem = 1024 + kBars + 256;
     static constexpr uint32_t kO = 2 * kSlots, kQ = kO + HDP;  // S of stream x at kSlots * x; Q hi, then lo
     static_assert(HDP * kOutPitch * 4 <= kEnd, "epilogue area");
@@ -149,65 +151,110 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
     return static_cast<uint32_t>(row * 128 + ((piece ^ (row & 7)) << 4));
 }
 
-// Scores of one tile -> P in place, for the vector of this thread: first slot
-// `first`, S and P at tensor memory address s_tm.  Lane g of the warp has the scales
-// of slots first + 16 g .. in k_scale, v_scale.  kEdge: some vector of the warp does
-// not see all of the tile's slots; this one sees those below `limit`.
+// Two fp32 operations at a time.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// Scores of 64 slots of a tile -> their P in place, for the vector of this thread:
+// first slot `first`, S and P at tensor memory address s_tm.  Lane g of the warp has
+// the scales of slots first + 16 g .. in k_scale, v_scale.  The thread with the
+// vector's other 64 slots is in the warp that shares barrier `bar`; their largest
+// scores meet in mine, other.  kEdge: some vector of the warp does not see all of
+// the slots; this one sees those below `limit`.
 template <bool kEdge>
 __device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit, float factor, float k_scale,
-                                            float v_scale, float& D, float& l, float& R) {
-    // a block the vector does not see has no scale, whatever is there
-    auto k_of = [&](int g) {
-        const float k = __shfl_sync(0xffffffffu, k_scale, g) * factor;
-        return kEdge && first + 16 * g >= limit ? 0.0f : k;
-    };
-    auto v_of = [&](int g) {
-        const float v = __shfl_sync(0xffffffffu, v_scale, g);
-        return kEdge && first + 16 * g >= limit ? 0.0f : v;
-    };
-    uint32_t s[32];
-    D = R = -INFINITY;
-#pragma unroll 1
-    for (int q = 0; q < 4; ++q) {
-        ld32(s_tm + 32 * q, s);
-        float m[2] = {-INFINITY, -INFINITY};
-        const float k0 = k_of(2 * q), k1 = k_of(2 * q + 1), v0 = __log2f(v_of(2 * q)), v1 = __log2f(v_of(2 * q + 1));
-        wait_ld(s);
+                                            float v_scale, float2* mine, const float2* other, int bar, float& D,
+                                            float& l, float& R) {
+    uint32_t s[2][32];
+    ld32(s_tm, s[0]);
+    ld32(s_tm + 32, s[1]);
+    float k[4], v[4];
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (!kEdge || first + 32 * q + j < limit) m[j / 16] = fmaxf(m[j / 16], __uint_as_float(s[j]));
-        m[0] = m[0] == -INFINITY ? m[0] : m[0] * k0;
-        m[1] = m[1] == -INFINITY ? m[1] : m[1] * k1;
-        D = fmaxf(D, fmaxf(m[0], m[1]));
-        R = fmaxf(R, fmaxf(m[0] + v0, m[1] + v1));
+    for (int g = 0; g < 4; ++g) {  // a block the vector does not see has no scale, whatever is there
+        k[g] = __shfl_sync(0xffffffffu, k_scale, g) * factor;
+        v[g] = __shfl_sync(0xffffffffu, v_scale, g);
+        if (kEdge && first + 16 * g >= limit) k[g] = v[g] = 0.0f;
     }
+    wait_ld(s[0]);
+    wait_ld(s[1]);
+    D = R = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (kEdge && first + 16 * g + j >= limit) s[g / 2][g % 2 * 16 + j] = 0xff800000u;
+            m = fmaxf(m, __uint_as_float(s[g / 2][g % 2 * 16 + j]));
+        }
+        m = m == -INFINITY ? m : m * k[g];
+        D = fmaxf(D, m);
+        R = fmaxf(R, m + __log2f(v[g]));
+    }
+    *mine = make_float2(D, R);
+    asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+    const float2 there = *other;
+    D = fmaxf(D, there.x);
+    R = fmaxf(R, there.y);
     const float ref = D == -INFINITY ? 0.0f : D;
     const float raise = R == -INFINITY ? 0.0f : ex2(fminf(ref - R + kLift, 126.0f));
-    float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll 1
-    for (int q = 0; q < 4; ++q) {
-        ld32(s_tm + 32 * q, s);
-        float k[2] = {k_of(2 * q), k_of(2 * q + 1)}, v[2] = {v_of(2 * q) * raise, v_of(2 * q + 1) * raise};
-        // where a product overflows its probabilities are 0
-        if (v[0] > 3e38f) v[0] = 3e38f;
-        if (v[1] > 3e38f) v[1] = 3e38f;
-        wait_ld(s);
+    const uint64_t less = pair(-ref, -ref);
+    uint64_t sum = pair(0.0f, 0.0f);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
         uint32_t out[32];  // hi pairs of 32 slots, then lo pairs
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-            float z0 = fmaf(__uint_as_float(s[j]), k[j / 16], -ref), z1 = fmaf(__uint_as_float(s[j + 1]), k[j / 16], -ref);
-            if (kEdge) {
-                if (first + 32 * q + j >= limit) z0 = -INFINITY;
-                if (first + 32 * q + j + 1 >= limit) z1 = -INFINITY;
+        for (int g = 0; g < 2; ++g) {
+            const uint64_t kk = pair(k[2 * q + g], k[2 * q + g]);
+            float vg = v[2 * q + g] * raise;
+            if (vg > 3e38f) vg = 3e38f;  // its probabilities are 0 then
+            const uint64_t vv = pair(vg, vg);
+#pragma unroll
+            for (int j = 16 * g; j < 16 * g + 16; j += 2) {
+                float z0, z1;
+                unpair(fma2(pair(__uint_as_float(s[q][j]), __uint_as_float(s[q][j + 1])), kk, less), z0, z1);
+                if (kEdge) {  // (-infinity times a scale of 0 is not -infinity)
+                    if (s[q][j] == 0xff800000u) z0 = -INFINITY;
+                    if (s[q][j + 1] == 0xff800000u) z1 = -INFINITY;
+                }
+                const uint64_t p = pair(ex2(z0), ex2(z1));
+                sum = add2(sum, p);
+                const uint64_t n = mul2(p, vv);
+                float n0, n1;
+                unpair(n, n0, n1);
+                const __half2 hi = __floats2half2_rn(n0, n1);
+                const float2 back = __half22float2(hi);
+                float r0, r1;
+                unpair(add2(n, pair(-back.x, -back.y)), r0, r1);
+                out[j / 2] = h2_bits(hi);
+                out[16 + j / 2] = h2_bits(__floats2half2_rn(r0, r1));
             }
-            const float p0 = ex2(z0), p1 = ex2(z1);
-            l0 += p0;
-            l1 += p1;
-            two_terms(p0 * v[j / 16], p1 * v[j / 16], out[j / 2], out[16 + j / 2]);
         }
         st32(s_tm + 32 * q, out);
     }
-    l = l0 + l1;
+    float s0, s1;
+    unpair(sum, s0, s1);
+    l = s0 + s1;
 }
 
 template <int HDP>
@@ -243,7 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
     unsigned char* const smem = smem_raw + (base - raw);
     float* const q_factor = reinterpret_cast<float*>(smem + S::kFactor);
     float* const q_top = reinterpret_cast<float*>(smem + S::kTop);
-    float* const stats = reinterpret_cast<float*>(smem + S::kStats);  // [tile % 4][D, l, R][vector]
+    float* const stats = reinterpret_cast<float*>(smem + S::kStats);  // [tile % 4][D, R, l, l][vector]
+    float2* const meet = reinterpret_cast<float2*>(smem + S::kMeet);  // [tile % 2][half][vector]
     const uint32_t bars = base + S::kBars;
     auto k_full = [&](int x) { return bars + 8 * x; };
     auto k_free = [&](int x) { return bars + 16 + 8 * x; };
@@ -260,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             dev::mbar_init(v_full(x), 4);
             dev::mbar_init(v_free(x), 1);
             dev::mbar_init(s_full(x), 1);
-            dev::mbar_init(p_full(x), 4);
+            dev::mbar_init(p_full(x), 8);
         }
         dev::mbar_init(o_full, 1);
         dev::mbar_init(o_free, 4);
@@ -335,27 +383,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             tc_before();
             asm volatile("bar.sync 2, 288;" ::: "memory");  // with warp 8: the queries are in place
         }
-        const uint32_t s_tm = lanes + x * kSlots;
         const float factor = q_factor[row];
         const int limit = row < real ? min(held + (v0 + row) / group + 1, seen) : 0;
         const float* k_scales = c.k_scales + head * (c.capacity / c.block);
         const float* v_scales = c.v_scales + head * (c.capacity / c.block);
-        for (int i = x; i < tiles; i += 2) {
-            const int first = i * kSlots, at = first + 16 * (lane % 8);
+        for (int i = 0; i < tiles; ++i) {
+            const int y = i & 1, first = i * kSlots + 64 * x, at = first + 16 * (lane % 4);
             const float ks = at < most ? k_scales[at / c.block] : 0.0f, vs = at < most ? v_scales[at / c.block] : 0.0f;
-            if (!wait_all(s_full(x), (i / 2) & 1)) break;
+            if (!wait_all(s_full(y), (i / 2) & 1)) break;
             tc_after();
+            const uint32_t s_tm = lanes + y * kSlots + 64 * x;
+            float2* const mine = meet + (2 * y + x) * kVecTile + row;
+            const float2* const other = meet + (2 * y + 1 - x) * kVecTile + row;
+            const int bar = 4 + warp % 4;
             float D, l, R;
-            if (__any_sync(0xffffffffu, first + kSlots > limit)) scores_to_p<true>(s_tm, first, limit, factor, ks, vs, D, l, R);
-            else scores_to_p<false>(s_tm, first, limit, factor, ks, vs, D, l, R);
-            float* mine = stats + (i % 4) * 3 * kVecTile + row;
-            mine[0] = D;
-            mine[kVecTile] = l;
-            mine[2 * kVecTile] = R;
+            if (__any_sync(0xffffffffu, first + 64 > limit)) scores_to_p<true>(s_tm, first, limit, factor, ks, vs, mine, other, bar, D, l, R);
+            else scores_to_p<false>(s_tm, first, limit, factor, ks, vs, mine, other, bar, D, l, R);
+            float* const to = stats + (i % 4) * 4 * kVecTile + row;
+            if (x == 0) to[0] = D, to[kVecTile] = R;
+            to[(2 + x) * kVecTile] = l;
             wait_st();
             tc_before();
             __syncwarp();
-            if (lane == 0) dev::mbar_arrive(p_full(x));
+            if (lane == 0) dev::mbar_arrive(p_full(y));
         }
     } else if (warp >= kConvertWarp) {
         fewer_registers<kConvertRegs>();
@@ -430,9 +480,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
                 for (int i = 0; i < min(2, tiles); ++i) scores(i);
             __syncwarp();
         }
-        float o[HDP], D = -INFINITY, l = 0.0f, R = -INFINITY;
+        uint64_t o[HDP / 2];
+        float D = -INFINITY, l = 0.0f, R = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < HDP; ++j) o[j] = 0.0f;
+        for (int j = 0; j < HDP / 2; ++j) o[j] = 0;
         for (int i = 0; i < tiles; ++i) {
             const int y = i & 1;
             // Every warp has seen tile i's P before it gives up tile i - 1's O, and the next
@@ -456,8 +507,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             __syncwarp();
             if (!wait_all(o_full, i & 1)) break;
             tc_after();
-            const float* tile = stats + (i % 4) * 3 * kVecTile + row;
-            const float tD = tile[0], tl = tile[kVecTile], tR = tile[2 * kVecTile];
+            const float* tile = stats + (i % 4) * 4 * kVecTile + row;
+            const float tD = tile[0], tR = tile[kVecTile], tl = tile[2 * kVecTile] + tile[3 * kVecTile];
             const float top = fmaxf(D, tD);
             l = (l == 0.0f ? 0.0f : l * ex2(D - top)) + (tl == 0.0f ? 0.0f : tl * ex2(tD - top));
             D = top;
@@ -466,16 +517,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
                 const float fade = !move ? 1.0f : R == -INFINITY ? 0.0f : ex2(R - tR);
                 if (move) R = tR;
 #pragma unroll
-                for (int j = 0; j < HDP; ++j) o[j] *= fade;
+                for (int j = 0; j < HDP / 2; ++j) o[j] = mul2(o[j], pair(fade, fade));
             }
-            const float gain = tR == -INFINITY ? 0.0f : ex2(tR - R);
+            const float by = tR == -INFINITY ? 0.0f : ex2(tR - R);
+            const uint64_t gain = pair(by, by);
 #pragma unroll
             for (int q = 0; q < HDP / 32; ++q) {
                 uint32_t part[32];
                 ld32(lanes + S::kO + 32 * q, part);
                 wait_ld(part);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[32 * q + j] = fmaf(__uint_as_float(part[j]), gain, o[32 * q + j]);
+                for (int j = 0; j < 32; j += 2)
+                    o[16 * q + j / 2] = fma2(pair(__uint_as_float(part[j]), __uint_as_float(part[j + 1])), gain, o[16 * q + j / 2]);
             }
             tc_before();
             __syncwarp();
@@ -487,7 +540,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
         const float scale = l != l ? l : R == -INFINITY ? 0.0f : ex2(R - kLift - D) / l;
         float* const area = reinterpret_cast<float*>(smem);  // [dim][vector]
 #pragma unroll
-        for (int j = 0; j < HDP; ++j) area[j * S::kOutPitch + row] = o[j] * scale;
+        for (int j = 0; j < HDP; j += 2) {
+            float y0, y1;
+            unpair(o[j / 2], y0, y1);
+            area[j * S::kOutPitch + row] = y0 * scale;
+            area[(j + 1) * S::kOutPitch + row] = y1 * scale;
+        }
         asm volatile("bar.sync 3, 128;" ::: "memory");
         for (int v = warp - kSumWarp; v < real; v += 4) {
             float* to = a.context + place(v0 + v, static_cast<int64_t>(a.heads) * d);
