@@ -17,11 +17,13 @@
 //                   has its own references, so no tile waits for another's
 //   warps 8-11      add each O tile to sums in registers (the tensor cores' fp32
 //                   accumulation truncates: over a long run of tiles the error is
-//                   five times that of these rounded sums) and write the result;
-//                   lane 0 of warp 8 issues the products
+//                   five times that of these rounded sums) and write the result
 //   warps 12-15     codes -> fp16, K and V tiles in 128-byte swizzled rows of 64 dims
 //                   (K-major for the first product, MN-major for the second: the
 //                   same bytes, another descriptor)
+//   warp 16         issues the products; a warp of its own, since issuing takes as
+//                   long as the tensor cores do
+//   warp 17         bulk copies of the codes into shared memory, two tiles ahead
 // Order of the products: P V of tile i, then Q K^T of tile i + 2; while the second
 // runs, O of tile i is read, and tile i + 1 becomes P meanwhile.
 //
@@ -40,19 +42,26 @@ constexpr int kVecTile = 128;   // query vectors of a CTA (the MMA's M)
 constexpr int kSlots = 128;     // slots of a tile (the first product's N, the second's K)
 constexpr int kSumWarp = 8;      // first of the four that add up O; before them the softmax warps
 constexpr int kConvertWarp = 12; // first of the four that convert
-constexpr int kThreads = 512;
+constexpr int kIssueWarp = 16;   // issues the products
+constexpr int kCopyWarp = 17;    // copies codes; the two after it do nothing
+constexpr int kThreads = 640;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLift = 14.0f;   // numerators are 2^kLift larger: their lo terms stay clear of the subnormals
 constexpr float kSlack = 20.0f;  // the sums' reference moves when a tile's passes it by this much
-// Registers of each role's warps: 8 x 112 + 4 x 184 + 4 x 104 = 16 x 128 of the launch.
-constexpr int kSoftmaxRegs = 112, kSumRegs = 184, kConvertRegs = 104;
+// Registers of a thread at the launch, and of each role's warps, which raise or lower
+// theirs (a raise waits for the others' to be freed, so the sum must not grow).
+constexpr int kLaunchRegs = 96;
+constexpr int kSoftmaxRegs = 120, kSumRegs = 168, kConvertRegs = 48, kIssueRegs = 24;
+static_assert(8 * kSoftmaxRegs + 4 * kSumRegs + 4 * kConvertRegs + 4 * kIssueRegs <= 20 * kLaunchRegs, "registers");
 
 // Tensor memory columns.
 template <int HDP>
 struct PromptShape {
     static constexpr int kBlocks = HDP / 64;              // blocks of 64 dims: 128-byte rows
     static constexpr int kTile = kBlocks * kSlots * 128;  // fp16 tile of 128 rows
-    static constexpr int kK = 0, kV = 2 * kTile, kEnd = 4 * kTile;
+    static constexpr int kK = 0, kV = 2 * kTile;
+    static constexpr int kRaw = 4 * kTile, kRawTile = kSlots * HDP;  // codes of two K and two V tiles
+    static constexpr int kEnd = kRaw + 4 * kRawTile;
     static constexpr int kOutPitch = kVecTile + 1;        // at the end: [dim][vector], over K and V
     // after the tiles: factor and largest component of each query, D, R, l of both halves of
     // four tiles, barriers
@@ -61,7 +70,7 @@ struct PromptShape {
     static constexpr int kBars = kMeet + 4 * kVecTile * 8;
     static constexpr int kSmem = 1024 + kBars + 256;
     static constexpr uint32_t kO = 2 * kSlots, kQ = kO + HDP;  // S of stream x at kSlots * x; Q hi, then lo
-    static_assert(HDP * kOutPitch * 4 <= kEnd, "epilogue area");
+    static_assert(HDP * kOutPitch * 4 <= kRaw, "epilogue area");
     static_assert(kSmem <= 232448, "shared memory per CTA");
     static_assert(kQ + HDP <= 512, "tensor memory");
 };
@@ -107,15 +116,20 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
+// The same for 16 columns, complete on return.
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -125,9 +139,15 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
         : "memory");
 }
 template <int N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void fewer_registers() {
+    static_assert(N <= kLaunchRegs && N % 8 == 0 && N >= 24, "can only lower");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 template <int N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void more_registers() {
+    static_assert(N >= kLaunchRegs && N % 8 == 0 && N <= 256, "can only raise");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -140,17 +160,39 @@ __device__ __forceinline__ void two_terms(float x0, float x1, uint32_t& hi, uint
     hi = h2_bits(h);
     lo = h2_bits(__floats2half2_rn(x0 - f.x, x1 - f.y));
 }
-// Two of four codes as fp16: flipped sign bits, 0x64xx = 1024 + xx, less 1152.
-template <uint32_t kSel>
-__device__ __forceinline__ uint32_t codes_to_half2(uint32_t flipped) {
-    const uint32_t r = dev::prmt(flipped, 0x64646464u, kSel);
-    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480))));
+// Four codes as fp16 pairs {0, 2} and {1, 3}: a mask leaves every other byte, an
+// exclusive or makes it 0x64xx with the sign bit flipped, 1024 + code + 128, and
+// 1152 is taken off.  (Masks run at twice the rate of byte permutations; the tiles'
+// dims are in the order 0, 2, 1, 3 of every four, and so are the queries'.)
+__device__ __forceinline__ uint2 codes_to_half(uint32_t w) {
+    const __half2 offset = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t even = (w & 0x00ff00ffu) ^ 0x64806480u, odd = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    return make_uint2(h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&even), offset)),
+                      h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&odd), offset)));
 }
 // Byte offset of 16-byte piece `piece` (of 64 dims: 8) of row `row` in a swizzled block.
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
     return static_cast<uint32_t>(row * 128 + ((piece ^ (row & 7)) << 4));
 }
 
+// Waits for phase `parity` of `bar`; false after about kWaitLimitNs.  Each try lets
+// the hardware suspend the warp for up to kSuspendNs: a loop that polls and reads a
+// clock took a third of the SM's issue slots from the warps that work.
+__device__ __forceinline__ bool wait_suspended(uint32_t bar, uint32_t parity) {
+    constexpr uint32_t kSuspendNs = 20000;
+    for (uint32_t i = 0; i < dev::kWaitLimitNs / kSuspendNs; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity), "r"(kSuspendNs)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
 // Two fp32 operations at a time.
 __device__ __forceinline__ uint64_t pair(float x, float y) {
     uint64_t r;
@@ -176,40 +218,56 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     return r;
 }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
 // Scores of 64 slots of a tile -> their P in place, for the vector of this thread:
-// first slot `first`, S and P at tensor memory address s_tm.  Lane g of the warp has
+// first slot `first`, S at tensor memory address s_tm; P's hi terms of 32 slots lie in
+// the first 16 columns of theirs, the lo terms in the last.  Lane g of the warp has
 // the scales of slots first + 16 g .. in k_scale, v_scale.  The thread with the
 // vector's other 64 slots is in the warp that shares barrier `bar`; their largest
 // scores meet in mine, other.  kEdge: some vector of the warp does not see all of
-// the slots; this one sees those below `limit`.
+// the slots; this one sees those below `limit`.  The loops stay rolled and the scores
+// are read twice: unrolled, the roles' code did not fit the instruction caches, and
+// waiting for instructions was the longest of all stalls.
 template <bool kEdge>
 __device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit, float factor, float k_scale,
                                             float v_scale, float2* mine, const float2* other, int bar, float& D,
                                             float& l, float& R) {
-    uint32_t s[2][32];
-    ld32(s_tm, s[0]);
-    ld32(s_tm + 32, s[1]);
-    float k[4], v[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {  // a block the vector does not see has no scale, whatever is there
-        k[g] = __shfl_sync(0xffffffffu, k_scale, g) * factor;
-        v[g] = __shfl_sync(0xffffffffu, v_scale, g);
-        if (kEdge && first + 16 * g >= limit) k[g] = v[g] = 0.0f;
-    }
-    wait_ld(s[0]);
-    wait_ld(s[1]);
+    // a block the vector does not see has no scale, whatever is there
+    auto k_of = [&](int g) {
+        const float k = __shfl_sync(0xffffffffu, k_scale, g) * factor;
+        return kEdge && first + 16 * g >= limit ? 0.0f : k;
+    };
+    auto v_of = [&](int g) {
+        const float v = __shfl_sync(0xffffffffu, v_scale, g);
+        return kEdge && first + 16 * g >= limit ? 0.0f : v;
+    };
     D = R = -INFINITY;
-#pragma unroll
+#pragma unroll 1
     for (int g = 0; g < 4; ++g) {
-        float m = -INFINITY;
+        uint32_t s[16];
+        const float k = k_of(g), v = __log2f(v_of(g));
+        ld16(s_tm + 16 * g, s);
+        float m[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            if (kEdge && first + 16 * g + j >= limit) s[g / 2][g % 2 * 16 + j] = 0xff800000u;
-            m = fmaxf(m, __uint_as_float(s[g / 2][g % 2 * 16 + j]));
+        for (int j = 0; j < 16; j += 4) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = __uint_as_float(s[j + i]);
+                if (kEdge && first + 16 * g + j + i >= limit) x[i] = -INFINITY;
+            }
+            m[0] = max3(m[0], x[0], x[1]);
+            m[1] = max3(m[1], x[2], x[3]);
         }
-        m = m == -INFINITY ? m : m * k[g];
-        D = fmaxf(D, m);
-        R = fmaxf(R, m + __log2f(v[g]));
+        float top = fmaxf(m[0], m[1]);
+        top = top == -INFINITY ? top : top * k;
+        D = fmaxf(D, top);
+        R = fmaxf(R, top + v);
     }
     *mine = make_float2(D, R);
     asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
@@ -220,37 +278,43 @@ __device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit,
     const float raise = R == -INFINITY ? 0.0f : ex2(fminf(ref - R + kLift, 126.0f));
     const uint64_t less = pair(-ref, -ref);
     uint64_t sum = pair(0.0f, 0.0f);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        uint32_t out[32];  // hi pairs of 32 slots, then lo pairs
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        uint32_t lo[2][8];  // kept until both halves of these 32 scores have been read
+        uint32_t hi[2][8];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const uint64_t kk = pair(k[2 * q + g], k[2 * q + g]);
-            float vg = v[2 * q + g] * raise;
-            if (vg > 3e38f) vg = 3e38f;  // its probabilities are 0 then
-            const uint64_t vv = pair(vg, vg);
+            uint32_t s[16];
+            ld16(s_tm + 32 * h + 16 * g, s);
+            const float k = k_of(2 * h + g);
+            float v = v_of(2 * h + g) * raise;
+            if (v > 3e38f) v = 3e38f;  // its probabilities are 0 then
+            const uint64_t kk = pair(k, k), vv = pair(v, v);
 #pragma unroll
-            for (int j = 16 * g; j < 16 * g + 16; j += 2) {
+            for (int j = 0; j < 16; j += 2) {
                 float z0, z1;
-                unpair(fma2(pair(__uint_as_float(s[q][j]), __uint_as_float(s[q][j + 1])), kk, less), z0, z1);
-                if (kEdge) {  // (-infinity times a scale of 0 is not -infinity)
-                    if (s[q][j] == 0xff800000u) z0 = -INFINITY;
-                    if (s[q][j + 1] == 0xff800000u) z1 = -INFINITY;
+                unpair(fma2(pair(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), kk, less), z0, z1);
+                if (kEdge) {
+                    if (first + 32 * h + 16 * g + j >= limit) z0 = -INFINITY;
+                    if (first + 32 * h + 16 * g + j + 1 >= limit) z1 = -INFINITY;
                 }
                 const uint64_t p = pair(ex2(z0), ex2(z1));
                 sum = add2(sum, p);
                 const uint64_t n = mul2(p, vv);
-                float n0, n1;
+                float n0, n1, r0, r1;
                 unpair(n, n0, n1);
-                const __half2 hi = __floats2half2_rn(n0, n1);
-                const float2 back = __half22float2(hi);
-                float r0, r1;
+                const __half2 high = __floats2half2_rn(n0, n1);
+                const float2 back = __half22float2(high);
                 unpair(add2(n, pair(-back.x, -back.y)), r0, r1);
-                out[j / 2] = h2_bits(hi);
-                out[16 + j / 2] = h2_bits(__floats2half2_rn(r0, r1));
+                hi[g][j / 2] = h2_bits(high);
+                lo[g][j / 2] = h2_bits(__floats2half2_rn(r0, r1));
             }
         }
-        st32(s_tm + 32 * q, out);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            st8(s_tm + 32 * h + 8 * g, hi[g]);
+            st8(s_tm + 32 * h + 16 + 8 * g, lo[g]);
+        }
     }
     float s0, s1;
     unpair(sum, s0, s1);
@@ -300,7 +364,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
     auto s_full = [&](int x) { return bars + 64 + 8 * x; };
     auto p_full = [&](int x) { return bars + 80 + 8 * x; };
     const uint32_t o_full = bars + 96, o_free = bars + 104;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kBars + 112);
+    auto raw_full = [&](int v, int x) { return bars + 112 + 16 * v + 8 * x; };  // v: 0 keys, 1 values
+    auto raw_free = [&](int v, int x) { return bars + 144 + 16 * v + 8 * x; };
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kBars + 176);
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; ++x) {
             dev::mbar_init(k_full(x), 4);
@@ -309,12 +375,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             dev::mbar_init(v_free(x), 1);
             dev::mbar_init(s_full(x), 1);
             dev::mbar_init(p_full(x), 8);
+            dev::mbar_init(raw_full(0, x), 1);
+            dev::mbar_init(raw_full(1, x), 1);
+            dev::mbar_init(raw_free(0, x), 4);
+            dev::mbar_init(raw_free(1, x), 4);
         }
         dev::mbar_init(o_full, 1);
         dev::mbar_init(o_free, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kSumWarp) {
+    if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dev::smem_u32(tmem_slot))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -328,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
 
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {  // one lane
-        if (!dev::mbar_wait_bounded(bar, parity)) {
+        if (!wait_suspended(bar, parity)) {
             ok = false;
             atomicOr(err, 1);
         }
@@ -341,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp % 4) << 21);
 
     if (warp < kSumWarp) {
-        fewer_registers<kSoftmaxRegs>();
+        more_registers<kSoftmaxRegs>();
         const int x = warp / 4;
         {
             // Queries: scaled by a power of two to at most 1, in two terms; a negative scale
@@ -375,16 +445,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             for (int q = 0; q < kHalf; q += 32) {
                 uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) two_terms(f[q + 2 * i] * down, f[q + 2 * i + 1] * down, hi[i], lo[i]);
+                for (int i = 0; i < 16; i += 2) {  // the tiles' order of dims
+                    two_terms(f[q + 2 * i] * down, f[q + 2 * i + 2] * down, hi[i], lo[i]);
+                    two_terms(f[q + 2 * i + 1] * down, f[q + 2 * i + 3] * down, hi[i + 1], lo[i + 1]);
+                }
                 st16(lanes + S::kQ + (x * kHalf + q) / 2, hi);
                 st16(lanes + S::kQ + HDP / 2 + (x * kHalf + q) / 2, lo);
             }
             wait_st();
             tc_before();
-            asm volatile("bar.sync 2, 288;" ::: "memory");  // with warp 8: the queries are in place
+            asm volatile("bar.sync 2, 288;" ::: "memory");  // with the issuing warp: the queries are in place
         }
         const float factor = q_factor[row];
-        const int limit = row < real ? min(held + (v0 + row) / group + 1, seen) : 0;
+        // (lanes without a vector compute something that nobody reads)
+        const int limit = row < real ? min(held + (v0 + row) / group + 1, seen) : most;
         const float* k_scales = c.k_scales + head * (c.capacity / c.block);
         const float* v_scales = c.v_scales + head * (c.capacity / c.block);
         for (int i = 0; i < tiles; ++i) {
@@ -407,55 +481,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             __syncwarp();
             if (lane == 0) dev::mbar_arrive(p_full(y));
         }
-    } else if (warp >= kConvertWarp) {
-        fewer_registers<kConvertRegs>();
-        // 128 threads: piece of 16 codes `piece` of rows r0, r0 + kStep, ...
-        constexpr int kPieces = HDP / 16, kStep = 128 / kPieces, kLoads = kSlots / kStep;
-        const int tid = threadIdx.x - kConvertWarp * 32, piece = tid % kPieces, r0 = tid / kPieces;
-        const bool inside = piece * 16 < d;
-        const int8_t* kc = c.k_codes + head * c.capacity * d + piece * 16;
-        const int8_t* vc = c.v_codes + head * c.capacity * d + piece * 16;
-        auto load = [&](const int8_t* from, int tile, uint4 (&w)[kLoads]) {
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j) {
-                const int slot = tile * kSlots + r0 + j * kStep;
-                w[j] = inside && slot < most ? __ldg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(slot) * d))
-                                             : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto store = [&](uint32_t tile_at, const uint4 (&w)[kLoads]) {
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j) {
-                const int r = r0 + j * kStep;
-                uint4 o[2];
-                const uint32_t f0 = w[j].x ^ 0x80808080u, f1 = w[j].y ^ 0x80808080u, f2 = w[j].z ^ 0x80808080u, f3 = w[j].w ^ 0x80808080u;
-                o[0] = make_uint4(codes_to_half2<0x4140>(f0), codes_to_half2<0x4342>(f0), codes_to_half2<0x4140>(f1),
-                                  codes_to_half2<0x4342>(f1));
-                o[1] = make_uint4(codes_to_half2<0x4140>(f2), codes_to_half2<0x4342>(f2), codes_to_half2<0x4140>(f3),
-                                  codes_to_half2<0x4342>(f3));
-                unsigned char* to = smem + tile_at + (piece / 4) * (kSlots * 128);
-                const int p2 = piece % 4 * 2, odd = (piece / 4) & 1;  // the two halves of a row in opposite order: no bank conflict
-                *reinterpret_cast<uint4*>(to + swizzled(r, p2 + odd)) = odd ? o[1] : o[0];
-                *reinterpret_cast<uint4*>(to + swizzled(r, p2 + 1 - odd)) = odd ? o[0] : o[1];
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-        };
-        uint4 kw[kLoads], vw[kLoads];
-        load(kc, 0, kw);
-        for (int i = 0; i < tiles; ++i) {
-            const int y = i & 1;
-            load(vc, i, vw);
-            if (i >= 2 && !wait_all(k_free(y), (i / 2 - 1) & 1)) break;
-            store(S::kK + y * S::kTile, kw);
-            if (lane == 0) dev::mbar_arrive(k_full(y));
-            if (i + 1 < tiles) load(kc, i + 1, kw);
-            if (i >= 2 && !wait_all(v_free(y), (i / 2 - 1) & 1)) break;
-            store(S::kV + y * S::kTile, vw);
-            if (lane == 0) dev::mbar_arrive(v_full(y));
-        }
-    } else {
-        more_registers<kSumRegs>();
+    } else if (warp >= kIssueWarp) {
+        fewer_registers<kIssueRegs>();
         constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(kSlots >> 3) << 17) | (static_cast<uint32_t>(kVecTile >> 4) << 24);
         // the second product's B is MN-major (bit 16)
         constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(HDP >> 3) << 17) |
@@ -464,22 +491,103 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             const int y = i & 1;
             if (!wait(k_full(y), (i / 2) & 1)) return;
             tc_after();
+            const uint64_t kd = desc_base(base + S::kK + y * S::kTile, 16);
 #pragma unroll
             for (int s = 0; s < HDP / 8; ++s) {
                 const int k = s % (HDP / 16), term = s < HDP / 16 ? 1 : 0;
-                const uint64_t kd = desc_base(base + S::kK + y * S::kTile + (k / 4) * (128 * 128) + (k % 4) * 32, 16);
-                mma_ts(tmem + y * kSlots, tmem + S::kQ + term * (HDP / 2) + 8 * k, kd, kIdescS, s > 0);
+                mma_ts(tmem + y * kSlots, tmem + S::kQ + term * (HDP / 2) + 8 * k, kd + ((k / 4) * (128 * 128) + (k % 4) * 32) / 16,
+                       kIdescS, s > 0);
             }
             mma_commit(s_full(y));
             mma_commit(k_free(y));
         };
-        if (warp == kSumWarp) {
+        if (warp == kIssueWarp) {
             asm volatile("bar.sync 2, 288;" ::: "memory");  // the queries are in place
             tc_after();
-            if (lane == 0)
+            if (lane == 0) {
                 for (int i = 0; i < min(2, tiles); ++i) scores(i);
+                for (int i = 0; ok && i < tiles; ++i) {
+                    const int y = i & 1;
+                    if (!wait(v_full(y), (i / 2) & 1) || !wait(p_full(y), (i / 2) & 1) || (i > 0 && !wait(o_free, (i - 1) & 1))) break;
+                    tc_after();
+                    const uint64_t vd = desc_base(base + S::kV + y * S::kTile, kSlots * 128);
+#pragma unroll
+                    for (int s = 0; s < kSlots / 8; ++s) {
+                        const int k = s % (kSlots / 16), term = s < kSlots / 16 ? 1 : 0;
+                        mma_ts(tmem + S::kO, tmem + y * kSlots + (k / 2) * 32 + (k % 2) * 8 + term * 16, vd + k * 2048 / 16,
+                               kIdescO, s > 0);
+                    }
+                    mma_commit(o_full);
+                    mma_commit(v_free(y));
+                    if (i + 2 < tiles) scores(i + 2);
+                }
+            }
+            __syncwarp();
+        } else if (warp == kCopyWarp) {
+            if (lane == 0) {
+                auto copy = [&](int v, int i) {
+                    const int y = i & 1;
+                    if (i >= 2 && !wait(raw_free(v, y), (i / 2 - 1) & 1)) return;
+                    // (slots past the last one seen have some code: their scores are masked, their P is 0)
+                    const uint32_t bytes = static_cast<uint32_t>(min(kSlots, c.capacity - i * kSlots) * d);
+                    const int8_t* from = (v ? c.v_codes : c.k_codes) + (head * c.capacity + static_cast<int64_t>(i) * kSlots) * d;
+                    dev::mbar_expect_tx(raw_full(v, y), bytes);
+                    dev::bulk_load(base + S::kRaw + (2 * v + y) * S::kRawTile, from, bytes, raw_full(v, y));
+                };
+                copy(0, 0);
+                if (tiles > 1) copy(0, 1);
+                for (int i = 0; ok && i < tiles; ++i) {
+                    copy(1, i);
+                    if (ok && i + 2 < tiles) copy(0, i + 2);
+                }
+                // no copy is in flight past this point
+                for (int i = max(0, tiles - 2); ok && i < tiles; ++i)
+                    if (wait(raw_full(0, i & 1), (i / 2) & 1)) wait(raw_full(1, i & 1), (i / 2) & 1);
+            }
             __syncwarp();
         }
+    } else if (warp >= kConvertWarp) {
+        fewer_registers<kConvertRegs>();
+        // 128 threads: piece of 16 codes `piece` of rows r0, r0 + kStep, ...; eight
+        // neighbours have four pieces of two adjacent rows, whose 16-byte stores fall in
+        // different banks
+        constexpr int kPieces = HDP / 16, kStep = 128 / kPieces, kLoads = kSlots / kStep;
+        const int tid = threadIdx.x - kConvertWarp * 32, piece = tid % 4 + tid / 8 % (kPieces / 4) * 4;
+        const int r0 = tid / 4 % 2 + tid / (2 * kPieces) * 2;
+        auto convert = [&](int v, int i, uint32_t tile_at) {  // keys or values of tile i; false: gave up
+            const int y = i & 1;
+            if (!wait_all(raw_full(v, y), (i / 2) & 1)) return false;
+            const unsigned char* from = smem + S::kRaw + (2 * v + y) * S::kRawTile + piece * 16;
+#pragma unroll 2
+            for (int j = 0; j < kLoads; ++j) {
+                const int r = r0 + j * kStep;
+                const uint4 c4 = piece * 16 < d ? *reinterpret_cast<const uint4*>(from + r * d) : make_uint4(0, 0, 0, 0);
+                const uint2 h0 = codes_to_half(c4.x), h1 = codes_to_half(c4.y), h2 = codes_to_half(c4.z), h3 = codes_to_half(c4.w);
+                unsigned char* to = smem + tile_at + y * S::kTile + (piece / 4) * (kSlots * 128);
+                *reinterpret_cast<uint4*>(to + swizzled(r, piece % 4 * 2)) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+                *reinterpret_cast<uint4*>(to + swizzled(r, piece % 4 * 2 + 1)) = make_uint4(h2.x, h2.y, h3.x, h3.y);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                dev::mbar_arrive(raw_free(v, y));
+                dev::mbar_arrive(v == 0 ? k_full(y) : v_full(y));
+            }
+            return true;
+        };
+        // K(0), K(1), V(0), K(2), V(1), ...: the products need K(i + 2) right after V(i)
+        bool go = convert(0, 0, S::kK);
+        if (go && tiles > 1) go = convert(0, 1, S::kK);
+        for (int i = 0; go && i < tiles; ++i) {
+            const int y = i & 1;
+            if (i >= 2 && !wait_all(v_free(y), (i / 2 - 1) & 1)) break;
+            if (!convert(1, i, S::kV)) break;
+            if (i + 2 >= tiles) continue;
+            if (!wait_all(k_free(y), (i / 2) & 1)) break;
+            go = convert(0, i + 2, S::kK);
+        }
+    } else {
+        more_registers<kSumRegs>();
         uint64_t o[HDP / 2];
         float D = -INFINITY, l = 0.0f, R = -INFINITY;
 #pragma unroll
@@ -490,21 +598,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             // product into O waits for both: no barrier runs two phases ahead of a warp.
             if (!wait_all(p_full(y), (i / 2) & 1)) break;
             if (i > 0 && lane == 0) dev::mbar_arrive(o_free);
-            if (warp == kSumWarp && lane == 0) {
-                if (wait(v_full(y), (i / 2) & 1) && (i == 0 || wait(o_free, (i - 1) & 1))) {
-                    tc_after();
-#pragma unroll
-                    for (int s = 0; s < kSlots / 8; ++s) {
-                        const int k = s % (kSlots / 16), term = s < kSlots / 16 ? 1 : 0;
-                        const uint64_t vd = desc_base(base + S::kV + y * S::kTile + k * 2048, kSlots * 128);
-                        mma_ts(tmem + S::kO, tmem + y * kSlots + (k / 2) * 32 + (k % 2) * 8 + term * 16, vd, kIdescO, s > 0);
-                    }
-                    mma_commit(o_full);
-                    mma_commit(v_free(y));
-                    if (i + 2 < tiles) scores(i + 2);
-                }
-            }
-            __syncwarp();
             if (!wait_all(o_full, i & 1)) break;
             tc_after();
             const float* tile = stats + (i % 4) * 4 * kVecTile + row;
@@ -543,8 +636,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
         for (int j = 0; j < HDP; j += 2) {
             float y0, y1;
             unpair(o[j / 2], y0, y1);
-            area[j * S::kOutPitch + row] = y0 * scale;
-            area[(j + 1) * S::kOutPitch + row] = y1 * scale;
+            const int dim = j / 4 * 4 + j / 2 % 2;  // columns j, j + 1 are dims dim, dim + 2
+            area[dim * S::kOutPitch + row] = y0 * scale;
+            area[(dim + 2) * S::kOutPitch + row] = y1 * scale;
         }
         asm volatile("bar.sync 3, 128;" ::: "memory");
         for (int v = warp - kSumWarp; v < real; v += 4) {
@@ -554,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
     }
     tc_before();
     __syncthreads();
-    if (warp == kSumWarp) {
+    if (warp == kIssueWarp) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
@@ -563,8 +657,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
 template <int HDP>
 cudaError_t launch(const Kv8Attention& a, int aligned, float* lse, int32_t* err, cudaStream_t s) {
     using S = PromptShape<HDP>;
-    const cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
+    static const int regs = [] {  // what the compiler gave the kernel has to be what the roles share out
+        cudaFuncAttributes f{};
+        return cudaFuncGetAttributes(&f, kv8_prompt_kernel<HDP>) == cudaSuccess ? f.numRegs : -1;
+    }();
+    if (regs != kLaunchRegs) return cudaErrorInvalidConfiguration;
     const int64_t vectors = static_cast<int64_t>(a.rows_per_seq) * (a.heads / a.cache.kv_heads);
     const dim3 grid(static_cast<unsigned>((vectors + kVecTile - 1) / kVecTile), a.cache.kv_heads, a.cache.batch);
     return launch_dependent(kv8_prompt_kernel<HDP>, grid, dim3(kThreads), S::kSmem, s, a, aligned, lse, err);
