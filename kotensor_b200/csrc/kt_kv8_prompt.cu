@@ -175,22 +175,14 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
     return static_cast<uint32_t>(row * 128 + ((piece ^ (row & 7)) << 4));
 }
 
-// Waits for phase `parity` of `bar`; false after about kWaitLimitNs.  Each try lets
-// the hardware suspend the warp for up to kSuspendNs: a loop that polls and reads a
-// clock took a third of the SM's issue slots from the warps that work.
-__device__ __forceinline__ bool wait_suspended(uint32_t bar, uint32_t parity) {
-    constexpr uint32_t kSuspendNs = 20000;
-    for (uint32_t i = 0; i < dev::kWaitLimitNs / kSuspendNs; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity), "r"(kSuspendNs)
-            : "memory");
-        if (done) return true;
-    }
+// Waits for phase `parity` of `bar`; false after some seconds.  The hardware holds a
+// try for about a hundred cycles; reading a clock between tries, as the bounded wait
+// of kt_device.cuh does, or giving the try a longer time (which becomes a loop of
+// sleeps) took a third of the SM's issue slots from the warps that work.
+__device__ __forceinline__ bool wait_counted(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 25); ++i)
+        if (dev::mbar_try_wait(bar, parity)) return true;
     return false;
 }
 // Two fp32 operations at a time.
@@ -398,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
 
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {  // one lane
-        if (!wait_suspended(bar, parity)) {
+        if (!wait_counted(bar, parity)) {
             ok = false;
             atomicOr(err, 1);
         }
