@@ -4,10 +4,13 @@
 // j <= n + t,  s_j = scale * (q . K_j),  out = sum_j softmax(s)_j V_j, with
 // K_j = code * scale of the slot's block.
 //
-// Codes are whole numbers of at most 128 and exact in fp16, so the products run on
-// fp16 tensor cores with fp32 sums once the fp32 operand, the query or the
-// probability, is written as two fp16 terms: x = hi + lo with hi = fp16(x) and
-// lo = fp16(x - hi), 22 bits.  The scales of the blocks multiply the fp32 sums.
+// Codes are whole numbers of at most 128, so the products run on tensor cores at
+// fp32 accuracy once the fp32 operand is cut into terms that they take exactly.  The
+// query becomes three signed bytes, 24 bits relative to its largest component, and its
+// products with the keys' codes are integers, exact, with no conversion of the codes.
+// The probabilities become two fp16 terms, x = hi + lo with hi = fp16(x) and
+// lo = fp16(x - hi), 22 bits of each, and the values' codes are exact in fp16.  The
+// scales of the blocks multiply the sums in fp32.
 #include <cuda_fp16.h>
 
 #include "kt_kv8.h"
@@ -21,10 +24,11 @@ constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in kv8_weights_
 // ------------------------------------------------------------ few query rows
 //
 // The query vectors that share a key/value head (rows_per_seq x heads / kv_heads
-// of them) go eight to a tile: an m16n8k16 product holds their hi terms in rows
-// 0..7 and their lo terms in rows 8..15, so a thread finds both sums of a score in
-// its own accumulators, and probabilities leave it in the layout the second product
-// reads.  Work is the list of all tiles of kKeys slots over (sequence, key/value
+// of them) go eight to a tile: one m16n8k32 integer product holds their high bytes
+// in rows 0..7 and their middle bytes in rows 8..15, a second their low bytes; the
+// fp16 product of the probabilities holds hi terms in rows 0..7, lo terms in 8..15.
+// So a thread finds all sums of a score in its own accumulators, and probabilities
+// leave it in the layout the second product reads.  Work is the list of all tiles of kKeys slots over (sequence, key/value
 // head, vector tile), cut into equal runs, one per CTA: ragged batches and single
 // long sequences load every SM alike.  A warp takes every kWarps-th tile of its
 // CTA's run through its own ring of asynchronous copies; nothing waits for another
@@ -34,6 +38,8 @@ constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in kv8_weights_
 
 constexpr int kKeys = 32;
 constexpr int kVectors = 8;
+constexpr int kMostCtas = 400;  // of a launch
+static_assert(kMostCtas <= kKv8MaxCtas, "a counter each");
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are kept 2^12 times larger, so that the fp16 terms of small ones
 // stay clear of the subnormals; the factor cancels in the division by their sum.
@@ -43,6 +49,12 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
@@ -59,12 +71,12 @@ __device__ __forceinline__ float lds32(uint32_t a) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
     return v;
 }
-// 16 bytes global -> shared; `bytes` of them are read, the rest are zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Asynchronous copies global -> shared.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -72,12 +84,26 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// Bytes of codes with their sign bit flipped (0..255) -> fp16 pairs: 0x64xx is
-// 1024 + xx, less 1152 is the code.  `sel` picks the two bytes.
-template <uint32_t kSel>
-__device__ __forceinline__ uint32_t codes_to_half2(uint32_t flipped) {
-    const uint32_t r = dev::prmt(flipped, 0x64646464u, kSel);
+// Bytes 0 and 2 of w, two codes, as an fp16 pair: with its sign bit flipped a code is
+// 0x64xx = 1024 + 128 + code, less 1152 is the code.  (A mask and an exclusive or run
+// at twice the rate of a byte permutation.)
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t w) {
+    const uint32_t r = (w & 0x00ff00ffu) ^ 0x64806480u;
     return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480))));
+}
+// Four floats of magnitude <= kQueryMax -> their nearest integers' signed digits to
+// base 256, four to a word: high, middle, low.
+constexpr float kQueryMax = 127.0f * 65536.0f + 127.0f * 256.0f + 127.0f;
+__device__ __forceinline__ void three_bytes(const float (&x)[4], uint32_t& high, uint32_t& middle, uint32_t& low) {
+    high = middle = low = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = __float2int_rn(x[i]);
+        const int l = static_cast<int8_t>(n), rest = (n - l) >> 8, m = static_cast<int8_t>(rest), h = (rest - m) >> 8;
+        low |= static_cast<uint32_t>(l & 255) << (8 * i);
+        middle |= static_cast<uint32_t>(m & 255) << (8 * i);
+        high |= static_cast<uint32_t>(h & 255) << (8 * i);
+    }
 }
 // x0, x1 as their two fp16 terms, packed in pairs.
 __device__ __forceinline__ void two_terms(float x0, float x1, uint32_t& hi, uint32_t& lo) {
@@ -106,6 +132,7 @@ struct DecodeShape {
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kPartFloats = kVectors * (HDP + 2);     // sums, then maxima, then denominators
     static constexpr int kSmem = kWarps * (kRing + kPartFloats * 4);
+    static_assert(kWarps * kPartFloats >= kMostCtas * kVectors + 2 * kVectors, "weights of the parts");
 };
 
 // Swizzle of 16-byte pieces that makes both fragment reads conflict-free: in
@@ -123,7 +150,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                                                                     float* __restrict__ scores,
                                                                     float* __restrict__ lse) {
     using S = DecodeShape<HDP>;
-    constexpr int kSteps = HDP / 16;       // k-steps of the first product
+    constexpr int kSteps = HDP / 32;       // k-steps of the first product
     constexpr int kPieces = HDP / 64;      // 16-byte pieces of a key a thread reads
     constexpr int kTiles = HDP / 8;        // n-tiles of the second product
     constexpr int kOwn = HDP / 4;          // dims of the output a thread holds
@@ -200,6 +227,25 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
     int ahead_first = at.tile;         // the segment's first tile
     ahead.tile += warp;
     int fill = 0;
+    // A lane copies piece `lane % kPieceCount` of every kCopyRows-th row.  Slots past the
+    // last one seen come along (their scores are masked, their probabilities 0, and codes
+    // are finite whatever they are); pieces past head_dim are left out, and what lies in
+    // their place meets zeros of the query, or dims that nobody writes.
+    constexpr int kPieceCount = HDP / 16, kCopyRows = 32 / kPieceCount, kCopies = kKeys / kCopyRows;
+    const bool copies = lane % kPieceCount < pieces;
+    const int64_t lane_from = static_cast<int64_t>(lane / kPieceCount) * d + lane % kPieceCount * 16;
+    const uint32_t lane_to[2] = {static_cast<uint32_t>(piece_offset<HDP>(lane / kPieceCount, lane % kPieceCount)),
+                                 static_cast<uint32_t>(piece_offset<HDP>(kCopyRows + lane / kPieceCount, lane % kPieceCount))};
+    const int8_t *ahead_k, *ahead_v;  // of the lane, at slot 0 of the item
+    const float* ahead_s;             // lanes 0, 1: the keys' scales, 2, 3: the values'
+    auto enter = [&] {
+        const int64_t head = static_cast<int64_t>(ahead.b) * c.kv_heads + ahead.item / vector_tiles;
+        ahead_k = c.k_codes + head * c.capacity * d + lane_from;
+        ahead_v = c.v_codes + head * c.capacity * d + lane_from;
+        ahead_s = (lane < 2 ? c.k_scales : c.v_scales) + head * (c.capacity / c.block);
+    };
+    enter();
+    const int block_shift = 31 - __clz(c.block);
     auto issue = [&] {
         // skip segments without a tile of this warp
         while (ahead_left > 0) {
@@ -210,30 +256,26 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                 next_item(ahead);
                 ahead_first = 0;
                 ahead.tile = warp;
+                enter();
             }
         }
         if (ahead_left > 0) {
-            int rows;
-            const int seen = seen_by(ahead.b, rows), first = ahead.tile * kKeys;
-            const int64_t head = static_cast<int64_t>(ahead.b) * c.kv_heads + ahead.item / vector_tiles;
+            const int first = ahead.tile * kKeys;
             const uint32_t stage = ring + fill * S::kStageBytes;
-            const int8_t* k = c.k_codes + (head * c.capacity + first) * d;
-            const int8_t* v = c.v_codes + (head * c.capacity + first) * d;
+            const int8_t* k = ahead_k + static_cast<int64_t>(first) * d;
+            const int8_t* v = ahead_v + static_cast<int64_t>(first) * d;
+            const bool all = first + kKeys <= c.capacity;  // else the first half of the tile
+            if (copies) {
 #pragma unroll
-            for (int i = 0; i < kKeys * HDP / 16 / 32; ++i) {
-                const int e = i * 32 + lane, row = e / (HDP / 16), piece = e % (HDP / 16);
-                const bool real = piece < pieces && first + row < seen;
-                const int64_t from = real ? row * d + piece * 16 : 0;
-                const uint32_t to = stage + piece_offset<HDP>(row, piece);
-                copy16(to, k + from, real ? 16 : 0);
-                copy16(to + S::kTileBytes, v + from, real ? 16 : 0);
+                for (int i = 0; i < kCopies; ++i) {
+                    if (i >= kCopies / 2 && !all) break;
+                    const uint32_t to = stage + lane_to[i & 1] + (i & ~1) * (kCopyRows * HDP);
+                    copy16(to, k + i * kCopyRows * d);
+                    copy16(to + S::kTileBytes, v + i * kCopyRows * d);
+                }
             }
-            if (lane < 4) {  // scales of slots first.. and first + 16.., keys then values
-                const int slot = first + (lane & 1) * 16;
-                const float* s = (lane < 2 ? c.k_scales : c.v_scales) + head * (c.capacity / c.block);
-                const bool real = slot < seen;
-                copy4(stage + 2 * S::kTileBytes + lane * 4, s + (real ? slot / c.block : 0), real ? 4 : 0);
-            }
+            if (lane < 4 && (all || !(lane & 1)))  // scales of slots first.. and first + 16..
+                copy4(stage + 2 * S::kTileBytes + lane * 4, ahead_s + ((first + (lane & 1) * 16) >> block_shift));
             ahead.tile += kWarps;
         }
         copy_commit();
@@ -254,20 +296,22 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
         const int limit = real ? min(held + row + 1, seen) : 0;                  // slots the vector sees
         const int64_t head = static_cast<int64_t>(at.b) * c.kv_heads + h;
 
-        uint32_t qa[kSteps][4];
+        // Step s of the first product contracts the dims 16 (t + 4 (s / 2)) + 8 (s % 2) .. + 7 of
+        // thread t: the words its 16-byte pieces of a key hold.
+        uint32_t qa[kSteps][6];  // high, middle of the first four, of the last four; low of both
         float factor;
         {
             const float* q = a.q + (static_cast<int64_t>(at.b) * a.rows_per_seq + row) * a.q_stride +
                              static_cast<int64_t>(h * group + vector % group) * d;
-            float x[kSteps][4];
-            float top = 0.0f;
+            float x[2 * kSteps][4];
+            uint32_t top = 0;  // the largest magnitude, by its bits: NaN above infinity
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < 2 * kSteps; ++s) {
                 const int dim = 16 * (t + 4 * (s / 4)) + 4 * (s % 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[s][i] = 0.0f;
                 if (real && dim < d) {
-                    if (aligned) {
+                    if (aligned & 1) {
                         const float4 f = *reinterpret_cast<const float4*>(q + dim);
                         x[s][0] = f.x, x[s][1] = f.y, x[s][2] = f.z, x[s][3] = f.w;
                     } else {
@@ -276,19 +320,22 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[s][i]));
+                for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
             }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // a power of two that brings the largest component to 1/2 .. 1
-            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 126, -126), 126);
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-            factor = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float largest = __uint_as_float(top);
+            // below 2^-100 the query counts as 0; where it is not finite every score is NaN
+            const float up = top < 0x0d800000u ? 0.0f : kQueryMax / largest;
+            factor = a.scale * kLog2e * (top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : largest / kQueryMax);
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                two_terms(x[s][0] * down, x[s][1] * down, qa[s][0], qa[s][1]);
-                two_terms(x[s][2] * down, x[s][3] * down, qa[s][2], qa[s][3]);
-            }
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[2 * s + i][j] = fminf(fmaxf(x[2 * s + i][j] * up, -kQueryMax), kQueryMax);
+                    three_bytes(x[2 * s + i], qa[s][2 * i], qa[s][2 * i + 1], qa[s][4 + i]);
+                }
         }
         float o[kOwn], m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -302,20 +349,22 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
             float s[4][2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                int upper[4] = {0, 0, 0, 0}, lower[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int u = 0; u < kPieces; ++u) {
                     const uint4 w = lds128(stage + piece_offset<HDP>(8 * j + n8, t + 4 * u));
-                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t f = words[i] ^ 0x80808080u;
-                        mma(acc, qa[4 * u + i], codes_to_half2<0x4140>(f), codes_to_half2<0x4342>(f));
-                    }
+                    const uint32_t* const q0 = qa[2 * u];
+                    const uint32_t* const q1 = qa[2 * u + 1];
+                    mma(upper, q0[0], q0[1], q0[2], q0[3], w.x, w.y);
+                    mma(lower, q0[4], 0, q0[5], 0, w.x, w.y);
+                    mma(upper, q1[0], q1[1], q1[2], q1[3], w.z, w.w);
+                    mma(lower, q1[4], 0, q1[5], 0, w.z, w.w);
                 }
+                // |middle sums| <= 128 x 128 x 128: 256 of them and a low sum stay below 2^30
                 const float ks = lds32(stage + 2 * S::kTileBytes + (j >> 1) * 4) * factor;
-                s[j][0] = (acc[0] + acc[2]) * ks;
-                s[j][1] = (acc[1] + acc[3]) * ks;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    s[j][i] = fmaf(static_cast<float>(upper[i]), 65536.0f, static_cast<float>(upper[2 + i] * 256 + lower[i])) * ks;
             }
             if (first + kKeys > held + 1) {  // the first row's end, or the end of all, lies in this tile
 #pragma unroll
@@ -375,16 +424,16 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                 float acc[4][4] = {};  // four n-tiles: bytes 0..3 of the words
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
-                    uint32_t lowp[2], highp[2];  // bytes 0, 1 and 2, 3 of two slots, interleaved
+                    uint32_t x[2], y[2];  // bytes 0, 1 and 2, 3 of two slots side by side
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        lowp[r] = dev::prmt(v[kk][2 * r][w], v[kk][2 * r + 1][w], 0x5140) ^ 0x80808080u;
-                        highp[r] = dev::prmt(v[kk][2 * r][w], v[kk][2 * r + 1][w], 0x7362) ^ 0x80808080u;
+                        x[r] = dev::prmt(v[kk][2 * r][w], v[kk][2 * r + 1][w], 0x5410);
+                        y[r] = dev::prmt(v[kk][2 * r][w], v[kk][2 * r + 1][w], 0x7632);
                     }
-                    mma(acc[0], pa[kk], codes_to_half2<0x4140>(lowp[0]), codes_to_half2<0x4140>(lowp[1]));
-                    mma(acc[1], pa[kk], codes_to_half2<0x4342>(lowp[0]), codes_to_half2<0x4342>(lowp[1]));
-                    mma(acc[2], pa[kk], codes_to_half2<0x4140>(highp[0]), codes_to_half2<0x4140>(highp[1]));
-                    mma(acc[3], pa[kk], codes_to_half2<0x4342>(highp[0]), codes_to_half2<0x4342>(highp[1]));
+                    mma(acc[0], pa[kk], codes_to_half2(x[0]), codes_to_half2(x[1]));
+                    mma(acc[1], pa[kk], codes_to_half2(x[0] >> 8), codes_to_half2(x[1] >> 8));
+                    mma(acc[2], pa[kk], codes_to_half2(y[0]), codes_to_half2(y[1]));
+                    mma(acc[3], pa[kk], codes_to_half2(y[0] >> 8), codes_to_half2(y[1] >> 8));
                     if (kFine || kk == 1) {  // blocks of 16 slots: each half has its own scale
                         const float vs = kFine && kk == 0 ? vs0 : kFine ? vs1 : vs0;
 #pragma unroll
@@ -470,24 +519,37 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
             __syncthreads();
             if (last_cta) {
                 __threadfence();
+                const int n = static_cast<int>(c1 - c0) + 1;
+                auto part_of = [&](int x) { return parts + ((c0 + x) * 2 + (x == 0 ? 1 : 0)) * S::kPartFloats; };
+                // every part's weight, in shared memory; a warp to a vector for the largest reference
+                float* const weight = part_smem;                       // [part][vector]
+                float* const totals = weight + kMostCtas * kVectors;  // largest, sum of each vector
+                for (int v = warp; v < kVectors; v += kWarps) {
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int x = lane; x < n; x += 32) top = fmaxf(top, __ldcg(part_of(x) + kVectors * HDP + v));
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    for (int x = lane; x < n; x += 32) {
+                        const float psum = __ldcg(part_of(x) + kVectors * HDP + kVectors + v);
+                        const float by = weigh(__ldcg(part_of(x) + kVectors * HDP + v), psum, top);
+                        weight[x * kVectors + v] = by;
+                        sum = fmaf(by, psum, sum);
+                    }
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) totals[2 * v] = top, totals[2 * v + 1] = sum;
+                }
+                __syncthreads();
                 for (int e = threadIdx.x; e < kVectors * HDP / 4; e += kWarps * 32) {
                     const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
                     if (vt * kVectors + vec >= vectors) continue;
-                    auto part_of = [&](int64_t x) { return parts + (x * 2 + (x == c0 ? 1 : 0)) * S::kPartFloats; };
-                    float top = -INFINITY, sum = 0.0f;
-                    for (int64_t x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(part_of(x) + kVectors * HDP + vec));
                     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int64_t x = c0; x <= c1; ++x) {
-                        const float* p = part_of(x);
-                        const float psum = __ldcg(p + kVectors * HDP + kVectors + vec);
-                        const float by = weigh(__ldcg(p + kVectors * HDP + vec), psum, top);
-                        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + vec * HDP + dim));
-                        sum = fmaf(by, psum, sum);
+#pragma unroll 8
+                    for (int x = 0; x < n; ++x) {
+                        const float by = weight[x * kVectors + vec];
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(part_of(x) + vec * HDP + dim));
                         y.x = fmaf(by, f.x, y.x), y.y = fmaf(by, f.y, y.y);
                         y.z = fmaf(by, f.z, y.z), y.w = fmaf(by, f.w, y.w);
                     }
-                    finish(vec, dim, y, top, sum);
+                    finish(vec, dim, y, totals[2 * vec], totals[2 * vec + 1]);
                 }
                 if (threadIdx.x == 0) *counter = 0;
             }
@@ -587,7 +649,7 @@ cudaError_t launch_tiles(const Kv8Attention& a, int sm_count, int aligned, float
     const int vt = tiles_of_vectors(a.rows_per_seq, a.heads, c.kv_heads);
     const int per_sm = HDP == 128 ? 1 : 2;  // what shared memory holds
     const int64_t most = static_cast<int64_t>(c.batch) * c.kv_heads * vt * ((c.capacity + kKeys - 1) / kKeys);
-    const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count * per_sm, kKv8MaxCtas),
+    const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count * per_sm, kMostCtas),
                                                         std::max<int64_t>(1, most / kWarps)));
     return launch_dependent(kernel, dim3(grid), dim3(kWarps * 32), S::kSmem, s, a, vt, aligned, parts, scores, lse);
 }
