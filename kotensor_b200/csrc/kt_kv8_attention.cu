@@ -18,7 +18,7 @@
 namespace kt {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in kv8_weights_kernel
 
 // ------------------------------------------------------------ few query rows
@@ -38,7 +38,7 @@ constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in kv8_weights_
 
 constexpr int kKeys = 32;
 constexpr int kVectors = 8;
-constexpr int kMostCtas = 400;  // of a launch
+constexpr int kMostCtas = 1024;  // of a launch
 static_assert(kMostCtas <= kKv8MaxCtas, "a counter each");
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are kept 2^12 times larger, so that the fp16 terms of small ones
@@ -118,21 +118,29 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// A place in the list of tiles: tile `tile` of item `item` (key/value head times
-// vector tile) of sequence b.
+// A place in the list of work: tile `tile` of item `item` (key/value head times vector
+// tile) of sequence b, whose items have `tiles` tiles each; the item starts at list
+// index `base`.  An item counts as kStart tiles more than it has, ahead of its first:
+// what a CTA spends on entering and leaving it.
 struct Place {
-    int b, item, tile, tiles;  // tiles of each of the sequence's items
+    int64_t base;
+    int b, item, tile, tiles;
 };
+// Quotients whose operands mostly fit 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
 
 template <int HDP>
 struct DecodeShape {
     static constexpr int kStages = 3;
+    static constexpr int kStart = HDP == 128 ? 12 : 24;
     static constexpr int kTileBytes = kKeys * HDP;               // one of keys, values
     static constexpr int kStageBytes = 2 * kTileBytes + 16;      // and 2 + 2 scales
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kPartFloats = kVectors * (HDP + 2);     // sums, then maxima, then denominators
     static constexpr int kSmem = kWarps * (kRing + kPartFloats * 4);
-    static_assert(kWarps * kPartFloats >= kMostCtas * kVectors + 2 * kVectors, "weights of the parts");
 };
 
 // Swizzle of 16-byte pieces that makes both fragment reads conflict-free: in
@@ -180,39 +188,57 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                 for (int i = threadIdx.x; i < a.heads * d; i += blockDim.x) a.context[r * a.heads * d + i] = 0.0f;
 
     // This CTA's run [begin, end) of the list.
-    int64_t total = 0;
-    for (int b = lane; b < c.batch; b += 32) total += tiles_of(b);
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= items;
-    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max(static_cast<int64_t>(1), total / kWarps));
-    auto run_begin = [&](int64_t cta) { return total * cta / ctas; };
-    const int64_t begin = blockIdx.x < ctas ? run_begin(blockIdx.x) : total;
-    const int64_t end = blockIdx.x < ctas ? run_begin(blockIdx.x + 1) : total;
-    if (begin >= end) return;
-    Place at{0, 0, 0, 0};
-    int64_t base = 0;  // list index of the sequence's first tile
+    int64_t real_tiles = 0, sequences = 0;
+    for (int b = lane; b < c.batch; b += 32) {
+        const int n = tiles_of(b);
+        real_tiles += n;
+        sequences += n > 0;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        real_tiles += __shfl_xor_sync(0xffffffffu, real_tiles, o);
+        sequences += __shfl_xor_sync(0xffffffffu, sequences, o);
+    }
+    real_tiles *= items;
+    const int64_t total = real_tiles + sequences * items * S::kStart;
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max(static_cast<int64_t>(1), real_tiles / (2 * kWarps)));
+    if (blockIdx.x >= ctas) return;
+    const int64_t share = quotient(total, ctas), spare = total - share * ctas;  // the first `spare` runs are one longer
+    auto run_begin = [&](int64_t cta) { return cta * share + min(cta, spare); };
+    auto cta_of = [&](int64_t i) {  // the CTA whose run holds list index i
+        const int64_t longer = spare * (share + 1);
+        return i < longer ? quotient(i, share + 1) : spare + quotient(i - longer, share);
+    };
+    const int64_t begin = run_begin(blockIdx.x), end = run_begin(blockIdx.x + 1);
+    Place at{0, 0, 0, 0, 0};
     for (int b0 = 0; b0 < c.batch; b0 += 32) {
         const int mine = b0 + lane < c.batch ? tiles_of(b0 + lane) : 0;
-        int64_t upto = static_cast<int64_t>(mine) * items;
+        int64_t upto = mine > 0 ? static_cast<int64_t>(mine + S::kStart) * items : 0;
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
         }
-        const uint32_t after = __ballot_sync(0xffffffffu, base + upto > begin);
+        const uint32_t after = __ballot_sync(0xffffffffu, at.base + upto > begin);
         if (after != 0) {
             const int l = __ffs(after) - 1;
             at.b = b0 + l;
             at.tiles = __shfl_sync(0xffffffffu, mine, l);
-            base += __shfl_sync(0xffffffffu, upto, l) - static_cast<int64_t>(at.tiles) * items;
+            at.base += __shfl_sync(0xffffffffu, upto, l) - static_cast<int64_t>(at.tiles + S::kStart) * items;
             break;
         }
-        base += __shfl_sync(0xffffffffu, upto, 31);
+        at.base += __shfl_sync(0xffffffffu, upto, 31);
     }
-    at.item = static_cast<int>((begin - base) / at.tiles);
-    at.tile = static_cast<int>((begin - base) % at.tiles);
+    at.item = static_cast<int>(quotient(begin - at.base, at.tiles + S::kStart));
+    at.base += static_cast<int64_t>(at.item) * (at.tiles + S::kStart);
+    at.tile = static_cast<int>(max(static_cast<int64_t>(0), begin - at.base - S::kStart));
 
+    // Where the run's tiles of p's item end, and whether the run goes on after the item.
+    auto stop_of = [&](const Place& p) {
+        return static_cast<int>(min(static_cast<int64_t>(p.tiles), max(static_cast<int64_t>(0), end - p.base - S::kStart)));
+    };
+    auto goes_on = [&](const Place& p) { return p.base + p.tiles + S::kStart < end; };
     // The first item after `p`'s: moves p to its tile 0.
     auto next_item = [&](Place& p) {
+        p.base += p.tiles + S::kStart;
         p.tile = 0;
         if (++p.item < items) return;
         p.item = 0;
@@ -220,11 +246,35 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
         while (p.b < c.batch && (p.tiles = tiles_of(p.b)) == 0);
     };
 
-    // The warp's copies run ahead of its work over the same sequence of tiles: from
-    // `ahead` (the warp's tile in the segment that starts at list index ahead_base).
+    // The query of this thread's fragments at place p, ahead of its use and of the copies
+    // that would delay it: dims 16 (t + 4 (s / 4)) + 4 (s % 4) ..
+    float x[2 * kSteps][4];
+    auto load_query = [&](const Place& p) {
+        const int h = p.item / vector_tiles, vector = (p.item - h * vector_tiles) * kVectors + n8, row = vector / group;
+        const bool real = vector < vectors && row < kv8_rows(a.counts, p.b, a.rows_per_seq);
+        const float* q = a.q + (static_cast<int64_t>(p.b) * a.rows_per_seq + row) * a.q_stride +
+                         static_cast<int64_t>(h * group + vector % group) * d;
+#pragma unroll
+        for (int s = 0; s < 2 * kSteps; ++s) {
+            const int dim = 16 * (t + 4 * (s / 4)) + 4 * (s % 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[s][i] = 0.0f;
+            if (real && dim < d) {
+                if (aligned & 1) {
+                    const float4 f = *reinterpret_cast<const float4*>(q + dim);
+                    x[s][0] = f.x, x[s][1] = f.y, x[s][2] = f.z, x[s][3] = f.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[s][i] = q[dim + i];
+                }
+            }
+        }
+    };
+    if (at.tile < stop_of(at)) load_query(at);
+
+    // The warp's copies run ahead of its work over the same sequence of tiles.
     Place ahead = at;
-    int64_t ahead_left = end - begin;  // tiles of the run from the segment's start on
-    int ahead_first = at.tile;         // the segment's first tile
+    bool ahead_on = true;
     ahead.tile += warp;
     int fill = 0;
     // A lane copies piece `lane % kPieceCount` of every kCopyRows-th row.  Slots past the
@@ -247,19 +297,14 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
     enter();
     const int block_shift = 31 - __clz(c.block);
     auto issue = [&] {
-        // skip segments without a tile of this warp
-        while (ahead_left > 0) {
-            const int stop = static_cast<int>(min(static_cast<int64_t>(ahead.tiles), ahead_first + ahead_left));
-            if (ahead.tile < stop) break;
-            ahead_left -= stop - ahead_first;
-            if (ahead_left > 0) {
+        while (ahead_on && ahead.tile >= stop_of(ahead)) {  // past items without a tile of this warp
+            if ((ahead_on = goes_on(ahead))) {
                 next_item(ahead);
-                ahead_first = 0;
                 ahead.tile = warp;
                 enter();
             }
         }
-        if (ahead_left > 0) {
+        if (ahead_on) {
             const int first = ahead.tile * kKeys;
             const uint32_t stage = ring + fill * S::kStageBytes;
             const int8_t* k = ahead_k + static_cast<int64_t>(first) * d;
@@ -285,9 +330,10 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
     for (int i = 0; i < S::kStages; ++i) issue();
 
     int use = 0;
-    int64_t left = end - begin;
-    while (left > 0) {  // one segment: the run's tiles of one item
-        const int stop = static_cast<int>(min(static_cast<int64_t>(at.tiles), at.tile + left));
+    for (bool more = true; more;) {  // one segment: the run's tiles of one item
+        const int stop = stop_of(at);
+        more = goes_on(at);
+        if (at.tile >= stop) break;  // the run ends ahead of the item's first tile
         int rows;
         const int seen = seen_by(at.b, rows), held = kv8_held(c, at.b);
         const int h = at.item / vector_tiles, vt = at.item - h * vector_tiles;
@@ -301,27 +347,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
         uint32_t qa[kSteps][6];  // high, middle of the first four, of the last four; low of both
         float factor;
         {
-            const float* q = a.q + (static_cast<int64_t>(at.b) * a.rows_per_seq + row) * a.q_stride +
-                             static_cast<int64_t>(h * group + vector % group) * d;
-            float x[2 * kSteps][4];
             uint32_t top = 0;  // the largest magnitude, by its bits: NaN above infinity
 #pragma unroll
-            for (int s = 0; s < 2 * kSteps; ++s) {
-                const int dim = 16 * (t + 4 * (s / 4)) + 4 * (s % 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[s][i] = 0.0f;
-                if (real && dim < d) {
-                    if (aligned & 1) {
-                        const float4 f = *reinterpret_cast<const float4*>(q + dim);
-                        x[s][0] = f.x, x[s][1] = f.y, x[s][2] = f.z, x[s][3] = f.w;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[s][i] = q[dim + i];
-                    }
-                }
+            for (int s = 0; s < 2 * kSteps; ++s)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
-            }
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float largest = __uint_as_float(top);
@@ -461,6 +491,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
             mine[kVectors * HDP + n8] = m - kLift;  // what the sums are relative to
             mine[kVectors * HDP + kVectors + n8] = l;
         }
+        Place next = at;
+        if (more) {
+            next_item(next);
+            if (stop_of(next) > 0) load_query(next);
+        }
         __syncthreads();
         const bool whole = at.tile == 0 && stop == at.tiles;
         const int slot = at.tile == 0 ? 1 : 0;
@@ -504,14 +539,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
         }
         if (!whole) {
             // the CTAs that share the item: those whose runs hold its first .. last tile
-            const int64_t item_first = base + static_cast<int64_t>(at.item) * at.tiles;
-            auto cta_of = [&](int64_t i) {  // the CTA whose run holds list index i
-                int64_t x = i * ctas / total;
-                while (run_begin(x) > i) --x;
-                while (run_begin(x + 1) <= i) ++x;
-                return x;
-            };
-            const int64_t c0 = cta_of(item_first), c1 = cta_of(item_first + at.tiles - 1);
+            const int64_t c0 = cta_of(at.base + S::kStart), c1 = cta_of(at.base + S::kStart + at.tiles - 1);
             int32_t* counter = static_cast<int32_t*>(a.scratch) + c0;
             __threadfence();
             __syncthreads();
@@ -521,18 +549,15 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                 __threadfence();
                 const int n = static_cast<int>(c1 - c0) + 1;
                 auto part_of = [&](int x) { return parts + ((c0 + x) * 2 + (x == 0 ? 1 : 0)) * S::kPartFloats; };
-                // every part's weight, in shared memory; a warp to a vector for the largest reference
-                float* const weight = part_smem;                       // [part][vector]
-                float* const totals = weight + kMostCtas * kVectors;  // largest, sum of each vector
+                // a warp to a vector for the largest reference and the sum
+                float* const totals = part_smem;
                 for (int v = warp; v < kVectors; v += kWarps) {
                     float top = -INFINITY, sum = 0.0f;
                     for (int x = lane; x < n; x += 32) top = fmaxf(top, __ldcg(part_of(x) + kVectors * HDP + v));
                     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                     for (int x = lane; x < n; x += 32) {
                         const float psum = __ldcg(part_of(x) + kVectors * HDP + kVectors + v);
-                        const float by = weigh(__ldcg(part_of(x) + kVectors * HDP + v), psum, top);
-                        weight[x * kVectors + v] = by;
-                        sum = fmaf(by, psum, sum);
+                        sum = fmaf(weigh(__ldcg(part_of(x) + kVectors * HDP + v), psum, top), psum, sum);
                     }
                     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     if (lane == 0) totals[2 * v] = top, totals[2 * v + 1] = sum;
@@ -544,8 +569,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
                     for (int x = 0; x < n; ++x) {
-                        const float by = weight[x * kVectors + vec];
-                        const float4 f = __ldcg(reinterpret_cast<const float4*>(part_of(x) + vec * HDP + dim));
+                        const float* p = part_of(x);
+                        const float by = weigh(__ldcg(p + kVectors * HDP + vec), __ldcg(p + kVectors * HDP + kVectors + vec), totals[2 * vec]);
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + vec * HDP + dim));
                         y.x = fmaf(by, f.x, y.x), y.y = fmaf(by, f.y, y.y);
                         y.z = fmaf(by, f.z, y.z), y.w = fmaf(by, f.w, y.w);
                     }
@@ -556,12 +582,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
         }
         __syncthreads();  // the merge area and last_cta are free again
 
-        left -= stop - at.tile;
-        if (left > 0) {
-            const int b = at.b, tiles = at.tiles;
-            next_item(at);
-            if (at.b != b) base += static_cast<int64_t>(tiles) * items;
-        }
+        at = next;
     }
 }
 
@@ -647,10 +668,10 @@ cudaError_t launch_tiles(const Kv8Attention& a, int sm_count, int aligned, float
     if (e != cudaSuccess) return e;
     const Kv8& c = a.cache;
     const int vt = tiles_of_vectors(a.rows_per_seq, a.heads, c.kv_heads);
-    const int per_sm = HDP == 128 ? 1 : 2;  // what shared memory holds
+    const int per_sm = 233472 / (S::kSmem + 1152);  // what shared memory holds
     const int64_t most = static_cast<int64_t>(c.batch) * c.kv_heads * vt * ((c.capacity + kKeys - 1) / kKeys);
     const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count * per_sm, kMostCtas),
-                                                        std::max<int64_t>(1, most / kWarps)));
+                                                        std::max<int64_t>(1, most / (2 * kWarps))));
     return launch_dependent(kernel, dim3(grid), dim3(kWarps * 32), S::kSmem, s, a, vt, aligned, parts, scores, lse);
 }
 }  // namespace
