@@ -38,7 +38,7 @@ constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in kv8_weights_
 
 constexpr int kKeys = 32;
 constexpr int kVectors = 8;
-constexpr int kMostCtas = 1024;  // of a launch
+constexpr int kMostCtas = 456;  // of a launch
 static_assert(kMostCtas <= kKv8MaxCtas, "a counter each");
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are kept 2^12 times larger, so that the fp16 terms of small ones
@@ -140,7 +140,8 @@ struct DecodeShape {
     static constexpr int kStageBytes = 2 * kTileBytes + 16;      // and 2 + 2 scales
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kPartFloats = kVectors * (HDP + 2);     // sums, then maxima, then denominators
-    static constexpr int kSmem = kWarps * (kRing + kPartFloats * 4);
+    static constexpr int kMeet = kWarps * kPartFloats > (kMostCtas + 2) * kVectors ? kWarps * kPartFloats : (kMostCtas + 2) * kVectors;
+    static constexpr int kSmem = kWarps * kRing + kMeet * 4;
 };
 
 // Swizzle of 16-byte pieces that makes both fragment reads conflict-free: in
@@ -515,7 +516,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
             }
             if (dim == 0 && lse != nullptr) lse[head * vectors + idx] = top + log2f(sum);
         };
-        for (int e = threadIdx.x; e < kVectors * HDP / 4; e += kWarps * 32) {
+        const int valid = min(kVectors, vectors - vt * kVectors);
+        for (int e = threadIdx.x; e < valid * (HDP / 4); e += kWarps * 32) {
             const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
             float top = -INFINITY, sum = 0.0f;
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part_smem[w * S::kPartFloats + kVectors * HDP + vec]);
@@ -549,33 +551,38 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
                 __threadfence();
                 const int n = static_cast<int>(c1 - c0) + 1;
                 auto part_of = [&](int x) { return parts + ((c0 + x) * 2 + (x == 0 ? 1 : 0)) * S::kPartFloats; };
-                // a warp to a vector for the largest reference and the sum
-                float* const totals = part_smem;
-                for (int v = warp; v < kVectors; v += kWarps) {
+                // every part's weight in shared memory, a warp to a vector
+                float* const totals = part_smem;               // largest reference, sum of each vector
+                float* const weight = part_smem + 2 * kVectors;  // [part][vector]
+                for (int v = warp; v < valid; v += kWarps) {
                     float top = -INFINITY, sum = 0.0f;
-                    for (int x = lane; x < n; x += 32) top = fmaxf(top, __ldcg(part_of(x) + kVectors * HDP + v));
-                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                     for (int x = lane; x < n; x += 32) {
-                        const float psum = __ldcg(part_of(x) + kVectors * HDP + kVectors + v);
-                        sum = fmaf(weigh(__ldcg(part_of(x) + kVectors * HDP + v), psum, top), psum, sum);
+                        const float m = __ldcg(part_of(x) + kVectors * HDP + v), psum = __ldcg(part_of(x) + kVectors * HDP + kVectors + v);
+                        const float now = fmaxf(top, m);
+                        sum = (sum == 0.0f ? 0.0f : sum * ex2(top - now)) + weigh(m, psum, now) * psum;
+                        top = now;
+                        weight[x * kVectors + v] = psum == 0.0f ? -INFINITY : m;
                     }
+                    float all = top;
+                    for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+                    sum = sum == 0.0f ? 0.0f : sum * ex2(top - all);
                     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (lane == 0) totals[2 * v] = top, totals[2 * v + 1] = sum;
+                    if (lane == 0) totals[2 * v] = all, totals[2 * v + 1] = sum;
                 }
                 __syncthreads();
-                for (int e = threadIdx.x; e < kVectors * HDP / 4; e += kWarps * 32) {
+                for (int e = threadIdx.x; e < valid * (HDP / 4); e += kWarps * 32) {
                     const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
-                    if (vt * kVectors + vec >= vectors) continue;
+                    const float top = totals[2 * vec];
+                    const float* from = parts + c0 * 2 * S::kPartFloats + vec * HDP + dim;  // the first CTA's slot 1, the others' 0
                     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
+#pragma unroll 16
                     for (int x = 0; x < n; ++x) {
-                        const float* p = part_of(x);
-                        const float by = weigh(__ldcg(p + kVectors * HDP + vec), __ldcg(p + kVectors * HDP + kVectors + vec), totals[2 * vec]);
-                        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + vec * HDP + dim));
+                        const float m = weight[x * kVectors + vec], by = m == -INFINITY ? 0.0f : ex2(m - top);
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(from + (x == 0 ? 1 : 2 * x) * S::kPartFloats));
                         y.x = fmaf(by, f.x, y.x), y.y = fmaf(by, f.y, y.y);
                         y.z = fmaf(by, f.z, y.z), y.w = fmaf(by, f.w, y.w);
                     }
-                    finish(vec, dim, y, totals[2 * vec], totals[2 * vec + 1]);
+                    finish(vec, dim, y, top, totals[2 * vec + 1]);
                 }
                 if (threadIdx.x == 0) *counter = 0;
             }
