@@ -14,8 +14,7 @@ namespace kt {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kVecs = 64 * kKv8MaxHeadDim / 4 / kThreads;  // four-value pieces of a block a thread holds
-constexpr uint32_t kTiny = 0x0d800000u;                     // bits of 2^-100
+constexpr uint32_t kTiny = 0x0d800000u;  // bits of 2^-100
 constexpr uint32_t kInf = 0x7f800000u;
 
 struct BlockScale {
@@ -27,12 +26,17 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t top) {
     const float a = __uint_as_float(top);
     return {__fmul_rn(a, 1.0f / 127.0f), __fmul_rn(__frcp_rn(a), 127.0f)};
 }
-__device__ __forceinline__ int8_t code_of(float x, float inverse) {
-    if (inverse == 0.0f) return 0;  // NaN and infinity times 0 are not 0
-    return static_cast<int8_t>(fminf(fmaxf(rintf(__fmul_rn(x, inverse)), -127.0f), 127.0f));
+// The code in the low byte.  Adding 1.5 x 2^23 rounds to the nearest integer, ties to
+// even, and leaves it in the low bits; |x * inverse| < 127.5, since the rounding
+// errors of the three steps are 2^-24 each.
+__device__ __forceinline__ uint32_t code_bits(float x, float inverse) {
+    return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.0f));
 }
-__device__ __forceinline__ char4 codes_of(float4 x, float inverse) {
-    return make_char4(code_of(x.x, inverse), code_of(x.y, inverse), code_of(x.z, inverse), code_of(x.w, inverse));
+__device__ __forceinline__ uint32_t codes_of(float4 x, float inverse) {
+    if (inverse == 0.0f) return 0;  // NaN and infinity times 0 are not 0
+    const uint32_t lo = dev::prmt(code_bits(x.x, inverse), code_bits(x.y, inverse), 0x0040);
+    const uint32_t hi = dev::prmt(code_bits(x.z, inverse), code_bits(x.w, inverse), 0x0040);
+    return dev::prmt(lo, hi, 0x5410);
 }
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t magnitude(float4 x) {
@@ -49,19 +53,23 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v) {
 }
 // Four floats at p, by one load where the address allows it.
 __device__ __forceinline__ float4 load4(const float* p, bool aligned) {
-    if (aligned) return *reinterpret_cast<const float4*>(p);
+    if (aligned) return __ldg(reinterpret_cast<const float4*>(p));
     return make_float4(p[0], p[1], p[2], p[3]);
 }
 
 // One CTA per (block that the new tokens touch, head, sequence, key or value).
-// The block's values stay in registers between the search for the largest and
-// their rounding: each is read once.  The CTA of a sequence's first touched block
-// is the only one that reads the old tail and writes the new one.
+// kColumns threads (a power of two, head_dim / 4 or more) share a slot, four values
+// each, so no index needs a division; a block's values stay in registers between the
+// search for the largest and their rounding, each read once.  The CTA of a sequence's
+// first touched block is the only one that reads the old tail and writes the new one.
+// Bound by memory: every value is read as it is, in fp32, and leaves as a byte.
+template <int kColumns>
 __global__ void __launch_bounds__(kThreads) kv8_store_kernel(Kv8 c, const float* __restrict__ k,
                                                              const float* __restrict__ v, int64_t k_stride,
                                                              int64_t v_stride, int aligned, int rows_per_seq,
                                                              const int32_t* __restrict__ counts,
                                                              int32_t* __restrict__ status) {
+    constexpr int kSlots = kThreads / kColumns, kVecs = 64 / kSlots;  // slots a pass, passes of the largest block
     dev::pdl_wait();
     dev::pdl_launch_dependents();
     const int b = blockIdx.z >> 1, h = blockIdx.y, x = blockIdx.x;
@@ -72,52 +80,49 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(Kv8 c, const float*
         n = c.capacity - held;
         if (status != nullptr && threadIdx.x == 0 && x == 0 && h == 0 && !value) atomicOr(status, KT_ERR_INVALID_ARGUMENT);
     }
-    if (n == 0) return;
-    const int inside = held % c.block, first = held / c.block;
-    if (x * c.block >= inside + n) return;
-    const int d4 = c.head_dim / 4;
+    const int shift = 31 - __clz(c.block), first = held >> shift, inside = held - (first << shift);
+    if (n == 0 || (x << shift) >= inside + n) return;
     const int64_t head = static_cast<int64_t>(b) * c.kv_heads + h;
-    int8_t* codes = (value ? c.v_codes : c.k_codes) + (head * c.capacity + (first + x) * c.block) * c.head_dim;
-    float* tail = (value ? c.v_tail : c.k_tail) + head * c.block * c.head_dim;
+    const int col = threadIdx.x % kColumns * 4, slot0 = threadIdx.x / kColumns;
+    const bool has = col < c.head_dim;
+    int8_t* codes = (value ? c.v_codes : c.k_codes) +
+                    (head * c.capacity + (static_cast<int64_t>(first + x) << shift)) * c.head_dim + col;
+    float* tail = (value ? c.v_tail : c.k_tail) + (head << shift) * c.head_dim + col;
     const int64_t stride = value ? v_stride : k_stride;
-    const float* rows = (value ? v : k) + static_cast<int64_t>(b) * rows_per_seq * stride + h * c.head_dim;
+    const float* rows = (value ? v : k) + static_cast<int64_t>(b) * rows_per_seq * stride + h * c.head_dim + col;
+    const int row0 = (x << shift) - inside + slot0;  // negative: a slot that was held before (x == 0)
 
     float4 r[kVecs];
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-        const int e = i * kThreads + threadIdx.x, slot = e / d4, col = (e - slot * d4) * 4;
-        const int row = x * c.block + slot - inside;  // negative: a slot that was held before (x == 0)
+        const int slot = slot0 + i * kSlots, row = row0 + i * kSlots;
         r[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (slot < c.block && row < n)
-            r[i] = row < 0 ? *reinterpret_cast<const float4*>(tail + slot * c.head_dim + col)
-                           : load4(rows + row * stride + col, aligned);
-        top = max(top, magnitude(r[i]));
+        if (has && slot < c.block && row < n)
+            r[i] = row < 0 ? *reinterpret_cast<const float4*>(tail + slot * c.head_dim) : load4(rows + row * stride, aligned);
     }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) top = max(top, magnitude(r[i]));
     const BlockScale s = block_scale(block_max(top));
-    if (threadIdx.x == 0) (value ? c.v_scales : c.k_scales)[head * (c.capacity / c.block) + first + x] = s.scale;
-    const int last = (held + n) / c.block;  // the new open block
+    if (threadIdx.x == 0) (value ? c.v_scales : c.k_scales)[head * (c.capacity >> shift) + first + x] = s.scale;
+    const int last = (held + n) >> shift;  // the new open block
+    const bool grows = x == 0 && last == first;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-        const int e = i * kThreads + threadIdx.x, slot = e / d4, col = (e - slot * d4) * 4;
-        const int row = x * c.block + slot - inside;
-        if (slot >= c.block || row >= n) continue;
-        *reinterpret_cast<char4*>(codes + slot * c.head_dim + col) = codes_of(r[i], s.inverse);
-        if (x == 0 && last == first && row >= 0) *reinterpret_cast<float4*>(tail + slot * c.head_dim + col) = r[i];
+        const int slot = slot0 + i * kSlots, row = row0 + i * kSlots;
+        if (!has || slot >= c.block || row >= n) continue;
+        *reinterpret_cast<uint32_t*>(codes + slot * c.head_dim) = codes_of(r[i], s.inverse);
+        if (grows && row >= 0) *reinterpret_cast<float4*>(tail + slot * c.head_dim) = r[i];
     }
-    if (x == 0 && last != first) {  // the rows left over after the last full block
-        const int left = (held + n) % c.block;
-        for (int e = threadIdx.x; e < left * d4; e += kThreads) {
-            const int slot = e / d4, col = (e - slot * d4) * 4;
-            *reinterpret_cast<float4*>(tail + slot * c.head_dim + col) =
-                load4(rows + (n - left + slot) * stride + col, aligned);
-        }
+    if (x == 0 && last != first && has) {  // the rows left over after the last full block
+        const int left = held + n - (last << shift);
+        for (int slot = slot0; slot < left; slot += kSlots)
+            *reinterpret_cast<float4*>(tail + slot * c.head_dim) = load4(rows + (n - left + slot) * stride, aligned);
     }
-    if (c.weights != nullptr && !value)
-        for (int slot = threadIdx.x; slot < c.block; slot += kThreads) {
-            const int row = x * c.block + slot - inside;
-            if (row >= 0 && row < n) c.weights[head * c.capacity + held + row] = 0.0f;
-        }
+    if (c.weights != nullptr && !value && threadIdx.x < c.block) {
+        const int row = (x << shift) - inside + threadIdx.x;
+        if (row >= 0 && row < n) c.weights[head * c.capacity + held + row] = 0.0f;
+    }
 }
 
 __global__ void kv8_advance_kernel(int32_t* __restrict__ lengths, int batch, int rows,
@@ -131,6 +136,8 @@ __global__ void kv8_advance_kernel(int32_t* __restrict__ lengths, int batch, int
 // ------------------------------------------------------------ eviction
 
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectEach = 8;  // slots of a chunk a thread holds
+constexpr int kBins = 2048;
 
 // Weights ordered as unsigned integers: negative ones reversed below the others,
 // -0 as 0, NaN above all.
@@ -139,117 +146,205 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     const uint32_t u = __float_as_uint(w + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// Sum of v over the block; also a barrier on both sides.
-__device__ __forceinline__ int block_sum(int v) {
+// Exclusive prefix sum of v over the block's threads, and the sum of all; barriers on both sides.
+__device__ __forceinline__ int block_prefix(int v, int& all) {
     __shared__ int part[kSelectThreads / 32];
-    v = __reduce_add_sync(0xffffffffu, v);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    int upto = v;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+    }
     __syncthreads();
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
+    if (lane == 31) part[warp] = upto;
     __syncthreads();
-    return __reduce_add_sync(0xffffffffu, part[threadIdx.x % 32]);
+    int before = part[lane];
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += u;
+    }
+    all = __shfl_sync(0xffffffffu, before, 31);
+    before = __shfl_sync(0xffffffffu, before, max(warp - 1, 0));
+    return upto - v + (warp > 0 ? before : 0);
 }
 
-// One CTA per (head, sequence): the smallest key of the kept candidates, found bit
-// by bit from the top, then the kept slots in order into `order` and their weights
-// to the front.
+// One CTA per (head, sequence).  The smallest key that is kept comes from three
+// counting passes over its digits of 11, 11 and 10 bits (integer counts: any order of
+// the atomics gives the same), then the kept slots go in order into `order` and their
+// weights to the front.  Latency-bound: the weights are read from L1 after the first
+// pass; 16 sequences x 8 heads of 8k slots took 58 us bit by bit.
 __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(Kv8 c, int keep, int recent,
                                                                     int32_t* __restrict__ order) {
     dev::pdl_wait();
     dev::pdl_launch_dependents();
+    __shared__ int bins[kBins];
+    __shared__ uint32_t found;  // the digit, and how many above it
+    __shared__ int above_found;
     const int b = blockIdx.y, h = blockIdx.x, held = kv8_held(c, b);
     if (held <= keep) return;
     const int64_t head = static_cast<int64_t>(b) * c.kv_heads + h;
     float* w = c.weights + head * c.capacity;
     order += head * c.capacity;
-    const int candidates = held - recent, want = keep - recent;
-    uint32_t bound = 0;  // the largest key that at least `want` candidates reach
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t trial = bound | (1u << bit);
-        int n = 0;
-        for (int i = threadIdx.x; i < candidates; i += kSelectThreads) n += order_key(w[i]) >= trial;
-        if (block_sum(n) >= want) bound = trial;
+    const int candidates = held - recent;
+    uint32_t bound = 0;         // the key's digits found so far
+    int want = keep - recent;   // how many to keep among the candidates that share them
+    if (want > 0) {
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
+            const uint32_t digits = (1u << width) - 1, above_mask = pass == 0 ? 0u : ~0u << (low + width);
+            for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < candidates; i += kSelectThreads) {
+                const uint32_t key = order_key(w[i]);
+                if ((key & above_mask) == bound) atomicAdd(bins + (key >> low & digits), 1);
+            }
+            __syncthreads();
+            // from the top: thread i has bins kBins - 2 - 2 i and the one above it
+            const int hi = kBins - 1 - 2 * threadIdx.x, n1 = bins[hi], n0 = bins[hi - 1];
+            int all;
+            const int before = block_prefix(n1 + n0, all);
+            if (before < want && before + n1 + n0 >= want) {
+                const bool upper = before + n1 >= want;
+                found = upper ? hi : hi - 1;
+                above_found = upper ? before : before + n1;
+            }
+            __syncthreads();
+            bound |= found << low;
+            want -= above_found;
+            __syncthreads();
+        }
+    } else {
+        bound = 0xffffffffu;  // none; a NaN's key is not above it, and no tie is wanted
     }
-    int above = 0;
-    for (int i = threadIdx.x; i < candidates; i += kSelectThreads) above += order_key(w[i]) > bound;
-    const int ties = want - block_sum(above);  // how many of those equal to the bound are kept, lowest slots first
-    __shared__ int kept_of[32], tied_of[32];
+    // `want` is now how many of those equal to the bound are kept, lowest slots first
     int kept_before = 0, tied_before = 0;
-    for (int base = 0; base < held; base += kSelectThreads) {
-        const int i = base + threadIdx.x;
-        const float x = i < held ? w[i] : 0.0f;
-        const bool late = i >= candidates && i < held;
-        const uint32_t key = i < candidates ? order_key(x) : 0;
-        const bool tied = i < candidates && key == bound;
-        const uint32_t tied_lanes = __ballot_sync(0xffffffffu, tied);
-        const uint32_t before = (1u << (threadIdx.x % 32)) - 1;
-        if (threadIdx.x % 32 == 0) tied_of[threadIdx.x / 32] = __popc(tied_lanes);
-        __syncthreads();
-        int rank = tied_before + __popc(tied_lanes & before), all_tied = 0;
-        for (int o = 0; o < 32; ++o) {
-            if (o < threadIdx.x / 32) rank += tied_of[o];
-            all_tied += tied_of[o];
+    for (int base = 0; base < held; base += kSelectThreads * kSelectEach) {
+        const int i0 = base + threadIdx.x * kSelectEach;
+        float x[kSelectEach];
+        int tied = 0;
+#pragma unroll
+        for (int j = 0; j < kSelectEach; ++j) {
+            x[j] = i0 + j < held ? w[i0 + j] : 0.0f;
+            tied += i0 + j < candidates && order_key(x[j]) == bound;
         }
-        const bool keep_it = late || (i < candidates && (key > bound || (tied && rank < ties)));
-        const uint32_t kept_lanes = __ballot_sync(0xffffffffu, keep_it);
-        if (threadIdx.x % 32 == 0) kept_of[threadIdx.x / 32] = __popc(kept_lanes);
-        __syncthreads();
-        int place = kept_before + __popc(kept_lanes & before), all_kept = 0;
-        for (int o = 0; o < 32; ++o) {
-            if (o < threadIdx.x / 32) place += kept_of[o];
-            all_kept += kept_of[o];
+        int all;
+        int rank = tied_before + block_prefix(tied, all);  // (every weight of the chunk has been read)
+        tied_before += all;
+        uint32_t keeps = 0;
+#pragma unroll
+        for (int j = 0; j < kSelectEach; ++j) {
+            const int i = i0 + j;
+            if (i >= held) continue;
+            if (i >= candidates) {
+                keeps |= 1u << j;
+            } else {
+                const uint32_t key = order_key(x[j]);
+                if (key > bound || (key == bound && rank < want)) keeps |= 1u << j;
+                rank += key == bound;
+            }
         }
-        if (keep_it) {  // place <= i, and every weight up to this chunk's end has been read
-            order[place] = i;
-            w[place] = x;
-        }
-        kept_before += all_kept;
-        tied_before += all_tied;
+        int place = kept_before + block_prefix(__popc(keeps), all);
+        kept_before += all;
+#pragma unroll
+        for (int j = 0; j < kSelectEach; ++j)
+            if (keeps >> j & 1) {  // place <= i0 + j: later chunks lose nothing
+                order[place] = i0 + j;
+                w[place++] = x[j];
+            }
         __syncthreads();
     }
 }
 
-// One CTA per (head, sequence, key or value) walks the new blocks in order: the
-// token that moves to slot i comes from a slot >= i, so what a block overwrites no
-// later block still needs, and its own values are all in registers at the barrier.
-__global__ void __launch_bounds__(kThreads) kv8_move_kernel(Kv8 c, int keep, const int32_t* __restrict__ order) {
+// A warp moves a unit of 64 tokens: lane l has piece l % kPieces (16 codes) of every
+// (32 / kPieces)-th token, all in registers at once.  A cluster of CTAs walks the
+// units of one (head, sequence, key or value) in rounds, a unit to each of its warps:
+// the token that moves to slot i comes from a slot >= i, so what a round overwrites no
+// later round still needs, and a round's own values are in registers at the barrier
+// ahead of its writes.  Bound by memory when there are heads enough; where there are
+// few, a cluster of up to 8 CTAs shares each.
+constexpr int kUnit = 64;
+constexpr int kMoveWarps = 4;
+template <int kPieces>
+__global__ void __launch_bounds__(kMoveWarps * 32, 3) kv8_move_kernel(Kv8 c, int keep, const int32_t* __restrict__ order) {
+    constexpr int kTokens = 32 / kPieces, kLoads = kUnit / kTokens, kPer16 = 16 / kTokens;
     dev::pdl_wait();
     dev::pdl_launch_dependents();
-    const int b = blockIdx.z >> 1, h = blockIdx.y;
+    const int b = blockIdx.z >> 1, h = blockIdx.y, lane = threadIdx.x % 32;
     const bool value = blockIdx.z & 1;
     if (kv8_held(c, b) <= keep) return;
     const int64_t head = static_cast<int64_t>(b) * c.kv_heads + h;
     order += head * c.capacity;
-    int8_t* codes = (value ? c.v_codes : c.k_codes) + head * c.capacity * c.head_dim;
-    float* scales = (value ? c.v_scales : c.k_scales) + head * (c.capacity / c.block);
-    float* tail = (value ? c.v_tail : c.k_tail) + head * c.block * c.head_dim;
-    const int d4 = c.head_dim / 4;
-    for (int base = 0; base < keep; base += c.block) {
-        float4 r[kVecs];
-        uint32_t top = 0;
+    const int shift = 31 - __clz(c.block), d = c.head_dim, col = lane % kPieces * 16, token0 = lane / kPieces;
+    const bool has = col < d;
+    int8_t* codes = (value ? c.v_codes : c.k_codes) + head * c.capacity * d + col;
+    float* scales = (value ? c.v_scales : c.k_scales) + head * (c.capacity >> shift);
+    float* tail = (value ? c.v_tail : c.k_tail) + (head << shift) * d + col;
+    const int full = keep >> shift << shift;  // slots of whole blocks
+    for (int base = (blockIdx.x * kMoveWarps + threadIdx.x / 32) * kUnit, left = (keep + kUnit - 1) / kUnit; left > 0;
+         left -= gridDim.x * kMoveWarps, base += gridDim.x * kMoveWarps * kUnit) {
+        uint4 r[kLoads];
+        float s[kLoads];
+        int from[kLoads];
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int e = i * kThreads + threadIdx.x, slot = e / d4, col = (e - slot * d4) * 4;
-            r[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (slot < c.block && base + slot < keep) {
-                const int from = order[base + slot];
-                const char4 q = *reinterpret_cast<const char4*>(codes + static_cast<int64_t>(from) * c.head_dim + col);
-                const float s = scales[from / c.block];
-                r[i] = make_float4(__fmul_rn(s, q.x), __fmul_rn(s, q.y), __fmul_rn(s, q.z), __fmul_rn(s, q.w));
+        for (int i = 0; i < kLoads; ++i) {
+            const int slot = base + token0 + i * kTokens;
+            from[i] = slot < keep ? order[slot] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            r[i] = make_uint4(0, 0, 0, 0);
+            s[i] = 0.0f;
+            if (from[i] >= 0) {
+                if (has) r[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(from[i]) * d);
+                s[i] = scales[from[i] >> shift];
             }
-            top = max(top, magnitude(r[i]));
         }
-        const BlockScale s = block_scale(block_max(top));
-        if (threadIdx.x == 0) scales[base / c.block] = s.scale;
-        const bool open = keep - base < c.block;
+        // the largest value of each 16 tokens: scale x largest code, exactly the largest product
+        uint32_t top[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int e = i * kThreads + threadIdx.x, slot = e / d4, col = (e - slot * d4) * 4;
-            if (slot >= c.block || base + slot >= keep) continue;
-            *reinterpret_cast<char4*>(codes + static_cast<int64_t>(base + slot) * c.head_dim + col) =
-                codes_of(r[i], s.inverse);
-            if (open) *reinterpret_cast<float4*>(tail + slot * c.head_dim + col) = r[i];
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t words[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) m = fmaxf(m, fabsf(static_cast<float>(static_cast<int8_t>(words[j] >> (8 * n)))));
+            top[i / kPer16] = max(top[i / kPer16], magnitude(__fmul_rn(s[i], m)));
         }
-        __syncthreads();  // block_max's shared words are free again
+#pragma unroll
+        for (int g = 0; g < 4; ++g) top[g] = __reduce_max_sync(0xffffffffu, top[g]);
+        if (shift >= 5) top[0] = top[1] = max(top[0], top[1]), top[2] = top[3] = max(top[2], top[3]);
+        if (shift >= 6) top[0] = top[1] = top[2] = top[3] = max(top[0], top[2]);
+        dev::cluster_sync();
+        float inverse[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const BlockScale bs = block_scale(top[g]);
+            inverse[g] = bs.inverse;
+            const int slot = base + 16 * g;
+            if (lane == 0 && slot < keep && (slot & (c.block - 1)) == 0) scales[slot >> shift] = bs.scale;
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int slot = base + token0 + i * kTokens;
+            if (!has || slot >= keep) continue;
+            uint32_t words[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+            // converted again: kept from the search, the floats would not fit the registers
+            asm volatile("" : "+r"(words[0]), "+r"(words[1]), "+r"(words[2]), "+r"(words[3]));
+            uint32_t out[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float4 x;
+                x.x = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j])));
+                x.y = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j] >> 8)));
+                x.z = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j] >> 16)));
+                x.w = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j] >> 24)));
+                out[j] = codes_of(x, inverse[i / kPer16]);
+                if (slot >= full) *reinterpret_cast<float4*>(tail + static_cast<int64_t>(slot - full) * d + 4 * j) = x;
+            }
+            *reinterpret_cast<uint4*>(codes + static_cast<int64_t>(slot) * d) = make_uint4(out[0], out[1], out[2], out[3]);
+        }
     }
 }
 
@@ -290,10 +385,11 @@ kt_status kt_kv8_store(kt_ctx* ctx, const kt_kv8_cache* cache, const float* k, c
     return c_entry(ctx, [&] {
         const int aligned = aligned16(k) && aligned16(v) && k_stride % 4 == 0 && v_stride % 4 == 0;
         const int rows = std::min(rows_per_seq, cache->capacity);  // more would be dropped
-        const dim3 grid((rows + cache->block - 1) / cache->block + 1, cache->kv_heads, 2 * cache->batch);
-        return entry_launch(launch_dependent(kv8_store_kernel, grid, dim3(kThreads), 0,
-                                             static_cast<cudaStream_t>(stream), *cache, k, v, k_stride, v_stride,
-                                             aligned, rows_per_seq, counts, status),
+        // blocks that rows can touch from any place in the first
+        const dim3 grid((rows + cache->block - 2) / cache->block + 1, cache->kv_heads, 2 * cache->batch);
+        const auto kernel = cache->head_dim > 64 ? kv8_store_kernel<32> : cache->head_dim > 32 ? kv8_store_kernel<16> : kv8_store_kernel<8>;
+        return entry_launch(launch_dependent(kernel, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(stream), *cache, k, v,
+                                             k_stride, v_stride, aligned, rows_per_seq, counts, status),
                             "kv8 store launch");
     });
 }
@@ -355,9 +451,28 @@ kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int
         const dim3 heads(cache->kv_heads, cache->batch);
         cudaError_t e = launch_dependent(kv8_select_kernel, heads, dim3(kSelectThreads), 0, s, *cache, keep, recent,
                                          order);
-        if (e == cudaSuccess)
-            e = launch_dependent(kv8_move_kernel, dim3(1, cache->kv_heads, 2 * cache->batch), dim3(kThreads), 0, s,
-                                 *cache, keep, order);
+        if (e == cudaSuccess) {
+            // CTAs that share a head's units: while one to a head leaves SMs idle and there
+            // are units for more
+            const int64_t alone = 2ll * cache->batch * cache->kv_heads;
+            const int units = (keep + kUnit - 1) / kUnit;
+            int share = 1;
+            while (share < 8 && alone * share * 2 <= 4ll * ctx->sm_count && units > share * kMoveWarps) share *= 2;
+            const auto kernel = cache->head_dim > 64 ? kv8_move_kernel<8> : cache->head_dim > 32 ? kv8_move_kernel<4> : kv8_move_kernel<2>;
+            cudaLaunchConfig_t lc = {};
+            lc.gridDim = dim3(share, cache->kv_heads, 2 * cache->batch);
+            lc.blockDim = dim3(kMoveWarps * 32);
+            lc.stream = s;
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = share;
+            attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+            lc.attrs = attr;
+            lc.numAttrs = 2;
+            e = cudaLaunchKernelEx(&lc, kernel, static_cast<Kv8>(*cache), keep, static_cast<const int32_t*>(order));
+        }
         return entry_launch(e, "kv8 evict launch");
     });
 }
