@@ -27,7 +27,8 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t top) {
     return {__fmul_rn(a, 1.0f / 127.0f), __fmul_rn(__frcp_rn(a), 127.0f)};
 }
 // The code in the low byte.  Adding 1.5 x 2^23 rounds to the nearest integer, ties to
-// even, and leaves it in the low bits; |x * inverse| < 127.5, since the rounding
+// even, and leaves it in the low bits (scalar operations: the assembler contracts
+// packed products and sums into one rounding); |x * inverse| < 127.5, since the rounding
 // errors of the three steps are 2^-24 each.
 __device__ __forceinline__ uint32_t code_bits(float x, float inverse) {
     return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.0f));
@@ -266,11 +267,13 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(Kv8 c, int k
 constexpr int kUnit = 64;
 constexpr int kMoveWarps = 4;
 template <int kPieces>
-__global__ void __launch_bounds__(kMoveWarps * 32, 3) kv8_move_kernel(Kv8 c, int keep, const int32_t* __restrict__ order) {
+__global__ void __launch_bounds__(kMoveWarps * 32, 5) kv8_move_kernel(Kv8 c, int keep, const int32_t* __restrict__ order) {
     constexpr int kTokens = 32 / kPieces, kLoads = kUnit / kTokens, kPer16 = 16 / kTokens;
+    __shared__ int from_of[kMoveWarps][kUnit];
+    __shared__ float scale_of[kMoveWarps][kUnit];
     dev::pdl_wait();
     dev::pdl_launch_dependents();
-    const int b = blockIdx.z >> 1, h = blockIdx.y, lane = threadIdx.x % 32;
+    const int b = blockIdx.z >> 1, h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const bool value = blockIdx.z & 1;
     if (kv8_held(c, b) <= keep) return;
     const int64_t head = static_cast<int64_t>(b) * c.kv_heads + h;
@@ -281,24 +284,24 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 3) kv8_move_kernel(Kv8 c, int
     float* scales = (value ? c.v_scales : c.k_scales) + head * (c.capacity >> shift);
     float* tail = (value ? c.v_tail : c.k_tail) + (head << shift) * d + col;
     const int full = keep >> shift << shift;  // slots of whole blocks
-    for (int base = (blockIdx.x * kMoveWarps + threadIdx.x / 32) * kUnit, left = (keep + kUnit - 1) / kUnit; left > 0;
+    int* const from = from_of[warp] + token0;
+    const float* const scale = scale_of[warp] + token0;
+    for (int base = (blockIdx.x * kMoveWarps + warp) * kUnit, left = (keep + kUnit - 1) / kUnit; left > 0;
          left -= gridDim.x * kMoveWarps, base += gridDim.x * kMoveWarps * kUnit) {
-        uint4 r[kLoads];
-        float s[kLoads];
-        int from[kLoads];
+        __syncwarp();  // the last unit's tokens and scales have been used
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int slot = base + token0 + i * kTokens;
-            from[i] = slot < keep ? order[slot] : -1;
+        for (int i = lane; i < kUnit; i += 32) {
+            const int f = base + i < keep ? order[base + i] : -1;
+            from_of[warp][i] = f;
+            scale_of[warp][i] = f >= 0 ? scales[f >> shift] : 0.0f;
         }
+        __syncwarp();
+        uint4 r[kLoads];
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
+            const int f = from[i * kTokens];
             r[i] = make_uint4(0, 0, 0, 0);
-            s[i] = 0.0f;
-            if (from[i] >= 0) {
-                if (has) r[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(from[i]) * d);
-                s[i] = scales[from[i] >> shift];
-            }
+            if (f >= 0 && has) r[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(f) * d);
         }
         // the largest value of each 16 tokens: scale x largest code, exactly the largest product
         uint32_t top[4] = {0, 0, 0, 0};
@@ -310,18 +313,17 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 3) kv8_move_kernel(Kv8 c, int
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int n = 0; n < 4; ++n) m = fmaxf(m, fabsf(static_cast<float>(static_cast<int8_t>(words[j] >> (8 * n)))));
-            top[i / kPer16] = max(top[i / kPer16], magnitude(__fmul_rn(s[i], m)));
+            top[i / kPer16] = max(top[i / kPer16], magnitude(__fmul_rn(scale[i * kTokens], m)));
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) top[g] = __reduce_max_sync(0xffffffffu, top[g]);
         if (shift >= 5) top[0] = top[1] = max(top[0], top[1]), top[2] = top[3] = max(top[2], top[3]);
         if (shift >= 6) top[0] = top[1] = top[2] = top[3] = max(top[0], top[2]);
         dev::cluster_sync();
-        float inverse[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const BlockScale bs = block_scale(top[g]);
-            inverse[g] = bs.inverse;
+            top[g] = __float_as_uint(bs.inverse);
             const int slot = base + 16 * g;
             if (lane == 0 && slot < keep && (slot & (c.block - 1)) == 0) scales[slot >> shift] = bs.scale;
         }
@@ -332,15 +334,16 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 3) kv8_move_kernel(Kv8 c, int
             uint32_t words[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
             // converted again: kept from the search, the floats would not fit the registers
             asm volatile("" : "+r"(words[0]), "+r"(words[1]), "+r"(words[2]), "+r"(words[3]));
+            const float inverse = __uint_as_float(top[i / kPer16]), s = scale[i * kTokens];
             uint32_t out[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float4 x;
-                x.x = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j])));
-                x.y = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j] >> 8)));
-                x.z = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j] >> 16)));
-                x.w = __fmul_rn(s[i], static_cast<float>(static_cast<int8_t>(words[j] >> 24)));
-                out[j] = codes_of(x, inverse[i / kPer16]);
+                x.x = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j])));
+                x.y = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j] >> 8)));
+                x.z = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j] >> 16)));
+                x.w = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j] >> 24)));
+                out[j] = codes_of(x, inverse);
                 if (slot >= full) *reinterpret_cast<float4*>(tail + static_cast<int64_t>(slot - full) * d + 4 * j) = x;
             }
             *reinterpret_cast<uint4*>(codes + static_cast<int64_t>(slot) * d) = make_uint4(out[0], out[1], out[2], out[3]);
