@@ -26,18 +26,32 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t top) {
     const float a = __uint_as_float(top);
     return {__fmul_rn(a, 1.0f / 127.0f), __fmul_rn(__frcp_rn(a), 127.0f)};
 }
-// The code in the low byte.  Adding 1.5 x 2^23 rounds to the nearest integer, ties to
-// even, and leaves it in the low bits (scalar operations: the assembler contracts
-// packed products and sums into one rounding); |x * inverse| < 127.5, since the rounding
-// errors of the three steps are 2^-24 each.
-__device__ __forceinline__ uint32_t code_bits(float x, float inverse) {
-    return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.0f));
-}
+// The nearest integer to y, ties to even, in the low bits: adding 1.5 x 2^23 rounds.
+// (A scalar operation: the assembler contracts packed products and sums into one
+// rounding.)  A code's y stays below 127.5: its three roundings are 2^-24 each.
+__device__ __forceinline__ uint32_t nearest_bits(float y) { return __float_as_uint(__fadd_rn(y, 12582912.0f)); }
+__device__ __forceinline__ uint32_t code_bits(float x, float inverse) { return nearest_bits(__fmul_rn(x, inverse)); }
 __device__ __forceinline__ uint32_t codes_of(float4 x, float inverse) {
     if (inverse == 0.0f) return 0;  // NaN and infinity times 0 are not 0
     const uint32_t lo = dev::prmt(code_bits(x.x, inverse), code_bits(x.y, inverse), 0x0040);
     const uint32_t hi = dev::prmt(code_bits(x.z, inverse), code_bits(x.w, inverse), 0x0040);
     return dev::prmt(lo, hi, 0x5410);
+}
+// Two products at a time.
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
 }
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t magnitude(float4 x) {
@@ -308,11 +322,16 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 5) kv8_move_kernel(Kv8 c, int
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t words[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-            float m = 0.0f;
+            uint32_t most = 0, least = 0x00ff00ffu;  // of code + 128, in two 16-bit lanes
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) m = fmaxf(m, fabsf(static_cast<float>(static_cast<int8_t>(words[j] >> (8 * n)))));
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t even = (words[j] & 0x00ff00ffu) ^ 0x00800080u, odd = ((words[j] >> 8) & 0x00ff00ffu) ^ 0x00800080u;
+                most = __vmaxu2(most, __vmaxu2(even, odd));
+                least = __vminu2(least, __vminu2(even, odd));
+            }
+            const int hi = max(static_cast<int>(most >> 16), static_cast<int>(most & 0xffffu)) - 128;
+            const int lo = 128 - min(static_cast<int>(least >> 16), static_cast<int>(least & 0xffffu));
+            const float m = static_cast<float>(max(hi, lo));
             top[i / kPer16] = max(top[i / kPer16], magnitude(__fmul_rn(scale[i * kTokens], m)));
         }
 #pragma unroll
@@ -336,16 +355,23 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 5) kv8_move_kernel(Kv8 c, int
             asm volatile("" : "+r"(words[0]), "+r"(words[1]), "+r"(words[2]), "+r"(words[3]));
             const float inverse = __uint_as_float(top[i / kPer16]), s = scale[i * kTokens];
             uint32_t out[4];
+            const uint64_t ss = pair(s, s), ii = pair(inverse, inverse);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float4 x;
-                x.x = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j])));
-                x.y = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j] >> 8)));
-                x.z = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j] >> 16)));
-                x.w = __fmul_rn(s, static_cast<float>(static_cast<int8_t>(words[j] >> 24)));
-                out[j] = codes_of(x, inverse);
-                if (slot >= full) *reinterpret_cast<float4*>(tail + static_cast<int64_t>(slot - full) * d + 4 * j) = x;
+                const uint64_t x0 = mul2(ss, pair(static_cast<float>(static_cast<int8_t>(words[j])),
+                                                  static_cast<float>(static_cast<int8_t>(words[j] >> 8))));
+                const uint64_t x1 = mul2(ss, pair(static_cast<float>(static_cast<int8_t>(words[j] >> 16)),
+                                                  static_cast<float>(static_cast<int8_t>(words[j] >> 24))));
+                const float2 y0 = unpair(mul2(x0, ii)), y1 = unpair(mul2(x1, ii));
+                const uint32_t lo = dev::prmt(nearest_bits(y0.x), nearest_bits(y0.y), 0x0040);
+                const uint32_t hi = dev::prmt(nearest_bits(y1.x), nearest_bits(y1.y), 0x0040);
+                out[j] = dev::prmt(lo, hi, 0x5410);
+                if (slot >= full) {
+                    const float2 a = unpair(x0), e = unpair(x1);
+                    *reinterpret_cast<float4*>(tail + static_cast<int64_t>(slot - full) * d + 4 * j) = make_float4(a.x, a.y, e.x, e.y);
+                }
             }
+            if (inverse == 0.0f) out[0] = out[1] = out[2] = out[3] = 0;
             *reinterpret_cast<uint4*>(codes + static_cast<int64_t>(slot) * d) = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
@@ -460,7 +486,7 @@ kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int
             const int64_t alone = 2ll * cache->batch * cache->kv_heads;
             const int units = (keep + kUnit - 1) / kUnit;
             int share = 1;
-            while (share < 8 && alone * share * 2 <= 4ll * ctx->sm_count && units > share * kMoveWarps) share *= 2;
+            while (share < 8 && alone * share * 2 <= 8ll * ctx->sm_count && units > share * kMoveWarps) share *= 2;
             const auto kernel = cache->head_dim > 64 ? kv8_move_kernel<8> : cache->head_dim > 32 ? kv8_move_kernel<4> : kv8_move_kernel<2>;
             cudaLaunchConfig_t lc = {};
             lc.gridDim = dim3(share, cache->kv_heads, 2 * cache->batch);
