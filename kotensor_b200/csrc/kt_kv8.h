@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <exception>
 #include <new>
@@ -76,6 +77,20 @@ cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, s
     lc.attrs = attr;
     lc.numAttrs = 1;
     return cudaLaunchKernelEx(&lc, kernel, static_cast<Params>(args)...);
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory; asked of the runtime once a
+// device for each place of use (`done`, a static of the caller, has a bit for each).
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // NULL when the cache can be used, else what is wrong with it (kt_kv8.cu).

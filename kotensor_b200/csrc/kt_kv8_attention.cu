@@ -671,7 +671,8 @@ cudaError_t launch_tiles(const Kv8Attention& a, int sm_count, int aligned, float
                          cudaStream_t s) {
     using S = DecodeShape<HDP>;
     const auto kernel = kv8_attention_kernel<HDP, kFine>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = allow_shared(kernel, S::kSmem, allowed);
     if (e != cudaSuccess) return e;
     const Kv8& c = a.cache;
     const int vt = tiles_of_vectors(a.rows_per_seq, a.heads, c.kv_heads);

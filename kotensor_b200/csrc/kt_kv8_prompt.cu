@@ -649,7 +649,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
 template <int HDP>
 cudaError_t launch(const Kv8Attention& a, int aligned, float* lse, int32_t* err, cudaStream_t s) {
     using S = PromptShape<HDP>;
-    cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = allow_shared(kv8_prompt_kernel<HDP>, S::kSmem, allowed);
     if (e != cudaSuccess) return e;
     static const int regs = [] {  // what the compiler gave the kernel has to be what the roles share out
         cudaFuncAttributes f{};

@@ -5,9 +5,10 @@
 // that fall in its slice in shared memory (integer counts: any order of the atomics
 // gives the same; bit 31 marks a token seen anywhere, the low bits its occurrences in
 // the answer) while its logits are on their way, then each logit is changed in
-// registers and written once: bound by the two streams of logits, 8 bytes each.  What
-// is rare, a counted token, a bias, a new largest value, is found by one test for four
-// logits.  The row's largest logit is merged over its CTAs by a 64-bit maximum of
+// registers and written once: bound by the two streams of logits, 8 bytes each.  Few
+// ids are counted or have a bias: a bit for every four ids says where, so that the
+// tables behind it are neither cleared nor read elsewhere, and one test finds a new
+// largest value among four.  The row's largest logit is merged over its CTAs by a 64-bit maximum of
 // {ordered value, ~index}: any order gives the same winner, the lowest index among
 // equal values.
 #include "kt_kv8.h"
@@ -15,11 +16,13 @@
 namespace kt {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kVecs = 8;
+constexpr int kThreads = 512;
+constexpr int kVecs = 4;
 constexpr int kSlice = kThreads * kVecs * 4;
 constexpr uint32_t kSeen = 0x80000000u;
 constexpr uint32_t kNoBias = 0xffffffffu;
+constexpr int kEarly = 2;   // tokens of a thread that are loaded ahead
+constexpr int kList = 512;  // tokens, biases of a slice that are listed
 
 // Larger floats give larger keys; -0 counts as 0.
 __device__ __forceinline__ uint32_t float_key(float x) {
@@ -33,14 +36,21 @@ struct RowScratch {
 };
 
 template <bool kPenal, bool kBiased>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant__ kt_logits_args a) {
+__global__ void __launch_bounds__(kThreads, 3) logits_kernel(const __grid_constant__ kt_logits_args a) {
     dev::pdl_wait();
     dev::pdl_launch_dependents();
-    // occurrences of each id of the slice, then the list index of its first bias
+    // tables of the slice, set where `touched` has the bit of their four ids: occurrences
+    // of each id, and the list index of its first bias
     extern __shared__ __align__(16) uint32_t counts[];
     uint32_t* const first_bias = counts + (kPenal ? kSlice : 0);
+    __shared__ uint32_t touched[kSlice / 128];
     __shared__ int repeated;  // an id of the slice has several biases
-    __shared__ unsigned long long part[kThreads / 32];
+    __shared__ float penalty[3];  // repetition, frequency, presence
+    __shared__ int listed, listed_biases;
+    __shared__ uint32_t list[kPenal ? kList : 1];  // tokens of the slice, kSeen: of the answer
+    __shared__ int bias_list[kBiased ? kList : 1], bias_index[kBiased ? kList : 1];
+    __shared__ float early_value[kBiased ? kThreads : 1];
+    __shared__ uint32_t part[kThreads / 32], part_id[kThreads / 32];
     const int row = blockIdx.y;
     const float* x = a.logits + row * a.logits_stride;
     float* y = a.out + row * a.out_stride;
@@ -64,91 +74,148 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
             v[i].w = at + 3 >= 0 && at + 3 < a.vocab ? x[at + 3] : -INFINITY;
         }
     }
-    if (kPenal || kBiased) {
+    // what else the row needs is asked for now, to arrive with the logits: the mask's words
+    // of each four ids, lengths and penalties
+    const uint32_t* allowed = a.allowed != nullptr ? a.allowed + row * a.allowed_stride : nullptr;
+    uint32_t mask[kVecs];
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int at = (i * kThreads + threadIdx.x) * 4;
-            if (kPenal) *reinterpret_cast<uint4*>(counts + at) = make_uint4(0, 0, 0, 0);
-            if (kBiased) *reinterpret_cast<uint4*>(first_bias + at) = make_uint4(kNoBias, kNoBias, kNoBias, kNoBias);
-        }
-        if (threadIdx.x == 0) repeated = 0;
-        __syncthreads();
+    for (int i = 0; i < kVecs; ++i) {
+        const int at = begin + (i * kThreads + threadIdx.x) * 4, word = max(at, 0) >> 5;
+        mask[i] = allowed != nullptr && at < a.vocab ? allowed[word] : 0;
     }
-    // ids of this slice, and of the row
-    const int low = max(begin, 0), high = min(begin + kSlice, a.vocab);
-    if (kPenal) {
-        const int32_t* tokens = a.tokens + row * a.token_stride;
-        const int n = min(a.lengths[row], a.token_width), prompt = a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
-#pragma unroll 8
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const int id = tokens[i];
-            if (id < low || id >= high) continue;
-            if (i >= prompt) atomicAdd(counts + id - begin, 1u);
-            atomicOr(counts + id - begin, kSeen);
-        }
-    }
+    // and the first tokens and biases of each thread, whatever the lists' lengths are
+    const int32_t* tokens = a.tokens + row * a.token_stride;
     const int32_t* bias_ids = a.bias_ids + row * a.bias_stride;
     const float* bias_values = a.bias_values + row * a.bias_stride;
-    const int biases = !kBiased ? 0 : a.bias_counts != nullptr ? min(a.bias_counts[row], a.bias_width) : a.bias_width;
-    if (kBiased) {
-        for (int i = threadIdx.x; i < biases; i += kThreads) {
-            const int id = bias_ids[i];
-            if (id < low || id >= high) continue;
-            if (atomicMin(first_bias + id - begin, static_cast<uint32_t>(i)) != kNoBias) repeated = 1;
+    int early[kEarly], early_id = -1;
+    float early_bias = 0.0f;
+    if (kPenal) {
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i) {
+            const int k = i * kThreads + static_cast<int>(threadIdx.x);
+            early[i] = k < a.token_width ? tokens[k] : -1;
         }
     }
-    if (kPenal || kBiased) __syncthreads();
+    if (kBiased && threadIdx.x < a.bias_width) {
+        early_id = bias_ids[threadIdx.x];
+        early_bias = bias_values[threadIdx.x];
+    }
+    const int biases = !kBiased ? 0 : a.bias_counts != nullptr ? min(a.bias_counts[row], a.bias_width) : a.bias_width;
+    const int length = kPenal ? min(a.lengths[row], a.token_width) : 0;
+    const int prompt = kPenal && a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
+    if (kPenal || kBiased) {
+        const int low = max(begin, 0), high = min(begin + kSlice, a.vocab);  // ids of this slice, and of the row
+        auto each_token = [&](auto f) {
+#pragma unroll
+            for (int i = 0; i < kEarly; ++i) {
+                const int k = i * kThreads + static_cast<int>(threadIdx.x);
+                if (k < length && early[i] >= low && early[i] < high) f(k, early[i] - begin);
+            }
+#pragma unroll 4
+            for (int k = kEarly * kThreads + threadIdx.x; k < length; k += kThreads) {
+                const int id = tokens[k];
+                if (id >= low && id < high) f(k, id - begin);
+            }
+        };
+        auto each_bias = [&](auto f) {
+            for (int k = threadIdx.x; k < biases; k += kThreads) {
+                const int id = k < kThreads ? early_id : bias_ids[k];
+                if (id >= low && id < high) f(k, id - begin);
+            }
+        };
+        if (threadIdx.x < kSlice / 128) touched[threadIdx.x] = 0;
+        if (threadIdx.x == 0) repeated = listed = listed_biases = 0;
+        if (kPenal && threadIdx.x < 3) {
+            const float* from = threadIdx.x == 0 ? a.repetition : threadIdx.x == 1 ? a.frequency : a.presence;
+            penalty[threadIdx.x] = from != nullptr ? from[row] : threadIdx.x == 0 ? 1.0f : 0.0f;
+        }
+        __syncthreads();
+        auto touch = [&](int at) {
+            atomicOr(touched + at / 128, 1u << (at / 4 % 32));
+            if (kPenal) *reinterpret_cast<uint4*>(counts + (at & ~3)) = make_uint4(0, 0, 0, 0);
+            if (kBiased) *reinterpret_cast<uint4*>(first_bias + (at & ~3)) = make_uint4(kNoBias, kNoBias, kNoBias, kNoBias);
+        };
+        // what falls in the slice is listed, so that the lists are read from memory once
+        if (kPenal)
+            each_token([&](int k, int at) {
+                touch(at);
+                const int place = atomicAdd(&listed, 1);
+                if (place < kList) list[place] = k >= prompt ? at | kSeen : at;
+            });
+        if (kBiased) {
+            each_bias([&](int k, int at) {
+                touch(at);
+                const int place = atomicAdd(&listed_biases, 1);
+                if (place < kList) {
+                    bias_list[place] = at;
+                    bias_index[place] = k;
+                }
+            });
+            early_value[threadIdx.x] = early_bias;
+        }
+        __syncthreads();
+        if (kPenal) {
+            auto count = [&](int at, bool answer) {
+                if (answer) atomicAdd(counts + at, 1u);
+                atomicOr(counts + at, kSeen);
+            };
+            if (listed <= kList) {
+                for (int i = threadIdx.x; i < listed; i += kThreads) count(list[i] & ~kSeen, list[i] & kSeen);
+            } else {
+                each_token([&](int k, int at) { count(at, k >= prompt); });
+            }
+        }
+        if (kBiased) {
+            auto claim = [&](int k, int at) {
+                if (atomicMin(first_bias + at, static_cast<uint32_t>(k)) != kNoBias) repeated = 1;
+            };
+            if (listed_biases <= kList) {
+                for (int i = threadIdx.x; i < listed_biases; i += kThreads) claim(bias_index[i], bias_list[i]);
+            } else {
+                each_bias(claim);
+            }
+        }
+        __syncthreads();
+    }
 
-    const float repetition = kPenal && a.repetition != nullptr ? a.repetition[row] : 1.0f;
-    const float frequency = kPenal && a.frequency != nullptr ? a.frequency[row] : 0.0f;
-    const float presence = kPenal && a.presence != nullptr ? a.presence[row] : 0.0f;
-    const uint32_t* allowed = a.allowed != nullptr ? a.allowed + row * a.allowed_stride : nullptr;
     float best = -1e9f;
     int best_id = 0;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
         const int local = (i * kThreads + threadIdx.x) * 4, at = begin + local;
         float w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        if (kPenal) {
-            const uint4 c = *reinterpret_cast<const uint4*>(counts + local);
-            if ((c.x | c.y | c.z | c.w) != 0) {
+        if ((kPenal || kBiased) && touched[local / 128] >> (local / 4 % 32) & 1) {
+            if (kPenal) {
+                const uint4 c = *reinterpret_cast<const uint4*>(counts + local);
                 const uint32_t n[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (n[j] == 0) continue;
-                    w[j] = w[j] > 0.0f ? __fdiv_rn(w[j], repetition) : __fmul_rn(w[j], repetition);
+                    w[j] = w[j] > 0.0f ? __fdiv_rn(w[j], penalty[0]) : __fmul_rn(w[j], penalty[0]);
                     const uint32_t made = n[j] & ~kSeen;
                     if (made != 0) {
-                        w[j] = __fsub_rn(w[j], __fmul_rn(frequency, static_cast<float>(made)));
-                        w[j] = __fsub_rn(w[j], presence);
+                        w[j] = __fsub_rn(w[j], __fmul_rn(penalty[1], static_cast<float>(made)));
+                        w[j] = __fsub_rn(w[j], penalty[2]);
                     }
                 }
             }
-        }
-        if (kBiased) {
-            const uint4 c = *reinterpret_cast<const uint4*>(first_bias + local);
-            if ((c.x & c.y & c.z & c.w) != kNoBias) {
+            if (kBiased) {
+                const uint4 c = *reinterpret_cast<const uint4*>(first_bias + local);
                 const uint32_t first[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (first[j] == kNoBias) continue;
-                    w[j] = __fadd_rn(w[j], bias_values[first[j]]);
+                    w[j] = __fadd_rn(w[j], first[j] < kThreads ? early_value[first[j]] : bias_values[first[j]]);
                     if (repeated)  // the id's other entries, in list order
                         for (int k = static_cast<int>(first[j]) + 1; k < biases; ++k)
                             if (bias_ids[k] == at + j) w[j] = __fadd_rn(w[j], bias_values[k]);
                 }
             }
         }
-        if (allowed != nullptr && at + 3 >= 0 && at < a.vocab) {
-            uint32_t bits;
-            if (at >= 0) {
-                const int word = at >> 5, last = (a.vocab - 1) >> 5;
-                const uint32_t w0 = allowed[word];
-                bits = w0 >> (at & 31);
-                if ((at & 31) > 28 && word < last) bits = __funnelshift_r(w0, allowed[word + 1], at & 31);
-            } else {
-                bits = allowed[0] << -at;
-            }
+        if (allowed != nullptr) {
+            uint32_t bits = at < 0 ? mask[i] << (-at & 31) : mask[i] >> (at & 31);
+            if (at >= 0 && (at & 31) > 28 && at >> 5 < (a.vocab - 1) >> 5)  // four ids over two words: rows off the boundary only
+                bits |= allowed[(at >> 5) + 1] << (32 - (at & 31));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (!(bits >> j & 1)) w[j] = -INFINITY;
@@ -167,15 +234,25 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
         }
     }
     if (a.next_token == nullptr) return;
-    unsigned long long key = best > -1e9f ? static_cast<unsigned long long>(float_key(best)) << 32 | (0xffffffffu - best_id) : 0;
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-        key = key > other ? key : other;
+    // the CTA's largest value, then the lowest of its ids
+    auto reduce = [](uint32_t& value, uint32_t& id) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, value);
+        id = __reduce_min_sync(0xffffffffu, value == top ? id : 0xffffffffu);
+        value = top;
+    };
+    uint32_t value = best > -1e9f ? float_key(best) : 0, id = best_id;
+    reduce(value, id);
+    if (threadIdx.x % 32 == 0) {
+        part[threadIdx.x / 32] = value;
+        part_id[threadIdx.x / 32] = id;
     }
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = key;
     __syncthreads();
+    if (threadIdx.x >= 32) return;
+    value = threadIdx.x < kThreads / 32 ? part[threadIdx.x] : 0;
+    id = threadIdx.x < kThreads / 32 ? part_id[threadIdx.x] : 0xffffffffu;
+    reduce(value, id);
     if (threadIdx.x != 0) return;
-    for (int i = 1; i < kThreads / 32; ++i) key = key > part[i] ? key : part[i];
+    const unsigned long long key = value == 0 ? 0 : static_cast<unsigned long long>(value) << 32 | (0xffffffffu - id);
     RowScratch* r = static_cast<RowScratch*>(a.scratch) + row;
     atomicMax(&r->best, key);
     const int slices = (a.vocab + skew + kSlice - 1) / kSlice;
@@ -190,7 +267,8 @@ cudaError_t launch_logits(const kt_logits_args& a, cudaStream_t s) {
     constexpr size_t smem = static_cast<size_t>(kSlice) * 4 * (kPenal + kBiased);
     const auto kernel = logits_kernel<kPenal, kBiased>;
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        static std::atomic<uint64_t> allowed{0};
+        const cudaError_t e = allow_shared(kernel, smem, allowed);
         if (e != cudaSuccess) return e;
     }
     return launch_dependent(kernel, dim3((a.vocab + 3 + kSlice - 1) / kSlice, a.rows), dim3(kThreads), smem, s, a);

@@ -17,7 +17,7 @@ import math
 from typing import Optional
 
 from . import _lib
-from .quantized import Context, _stream_of
+from .quantized import Context, raw_stream
 
 try:
     import torch
@@ -28,12 +28,13 @@ except ImportError:  # pragma: no cover
 def _rows(name: str, x, rows: int, width: int):
     """Pointer and row stride of float32 rows on the device (rows may lie apart, as
     in a fused q|k|v projection)."""
-    if not x.is_cuda or x.dtype != torch.float32 or x.dim() != 2 or x.shape[0] != rows or x.shape[1] != width:
+    if x.dtype is not torch.float32 or not x.is_cuda or x.shape != (rows, width):
         raise ValueError(f"{name} must be a float32 CUDA tensor of shape [{rows}, {width}], got "
                          f"{str(x.dtype).replace('torch.', '')} {list(x.shape)}")
-    if x.stride(1) != 1 or (rows > 1 and x.stride(0) < width):
+    stride, column = x.stride()
+    if column != 1 or (rows > 1 and stride < width):
         raise ValueError(f"{name} must have contiguous rows that do not overlap")
-    return x.data_ptr(), max(x.stride(0), width)
+    return x.data_ptr(), stride if stride > width else width
 
 
 class KVCache8:
@@ -77,9 +78,12 @@ class KVCache8:
         self.weights = torch.zeros(*shape, capacity, dtype=torch.float32, device=dev) if track_weights else None
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._status = self.status.data_ptr()
         self._scratch = torch.zeros(0, dtype=torch.uint8, device=dev)
         self._scratch_for = set()
-        self._lib = _lib.load()
+        lib = _lib.load()
+        self._lib, self._store, self._attention = lib, lib.kt_kv8_store, lib.kt_kv8_attention
+        self._scale = 1.0 / math.sqrt(head_dim)
         buffers = (self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.k_tail, self.v_tail, self.weights)
         self._layer = []
         for l in range(layers):
@@ -117,8 +121,8 @@ class KVCache8:
         rows, width = self.batch * rows_per_seq, self.kv_heads * self.head_dim
         kp, ks = _rows("k", k, rows, width)
         vp, vs = _rows("v", v, rows, width)
-        _lib.check(self._lib.kt_kv8_store(self.ctx.handle, self._cache(layer), kp, vp, ks, vs, rows_per_seq,
-                                          self._counts(counts), self.status.data_ptr(), _stream_of(k)))
+        _lib.check(self._store(self.ctx.handle, self._cache(layer), kp, vp, ks, vs, rows_per_seq, self._counts(counts),
+                               self._status, raw_stream(self.ctx.device)))
 
     def attend(self, layer: int, q, heads: int, rows_per_seq: int = 1, scale: Optional[float] = None, out=None,
                counts=None, accumulate: bool = False):
@@ -129,27 +133,27 @@ class KVCache8:
         rows, width = self.batch * rows_per_seq, heads * self.head_dim
         qp, qs = _rows("q", q, rows, width)
         if out is None:
-            out = torch.empty((rows, width), dtype=torch.float32, device=self.device)
+            out = q.new_empty((rows, width))
         elif not out.is_cuda or out.dtype != torch.float32 or tuple(out.shape) != (rows, width) or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous float32 CUDA tensor of shape [{rows}, {width}]")
         scratch = self._scratch_of(rows_per_seq, heads) if rows_per_seq > 0 and heads > 0 else None
-        _lib.check(self._lib.kt_kv8_attention(
-            self.ctx.handle, self._cache(layer), qp, qs, out.data_ptr(), rows_per_seq, self._counts(counts), heads,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, accumulate, scratch, _stream_of(q)))
+        _lib.check(self._attention(self.ctx.handle, self._cache(layer), qp, qs, out.data_ptr(), rows_per_seq,
+                                   self._counts(counts), heads, self._scale if scale is None else scale, accumulate,
+                                   scratch, raw_stream(self.ctx.device)))
         return out
 
     def advance(self, rows: int = 1, counts=None, limit: Optional[int] = None) -> None:
         """lengths[b] += rows (or counts[b]), at most ``limit`` (the capacity unless given)."""
         _lib.check(self._lib.kt_kv8_advance(self.ctx.handle, self.lengths.data_ptr(), self.batch, rows,
                                             self._counts(counts), self.capacity if limit is None else limit,
-                                            _stream_of(self.lengths)))
+                                            raw_stream(self.ctx.device)))
 
     def evict_layer(self, layer: int, keep: int, recent: int) -> None:
         """Prunes one layer's sequences of more than ``keep`` tokens to the ``recent`` last
         ones and the others of largest accumulated weight, each head for itself;
         ``lengths`` stays (see ``evict``)."""
         _lib.check(self._lib.kt_kv8_evict(self.ctx.handle, self._cache(layer), keep, recent, self._scratch_of(1, self.kv_heads),
-                                          _stream_of(self.lengths)))
+                                          raw_stream(self.ctx.device)))
 
     def evict(self, keep: int, recent: int) -> None:
         """``evict_layer`` on every layer, then lengths[b] = min(lengths[b], keep)."""

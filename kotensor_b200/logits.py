@@ -7,7 +7,7 @@ from __future__ import annotations
 import ctypes
 
 from . import _lib
-from .quantized import Context, _stream_of
+from .quantized import Context, raw_stream
 
 try:
     import torch
@@ -15,18 +15,23 @@ except ImportError:  # pragma: no cover
     torch = None
 
 
-def _per_row(name: str, x, rows: int, dtype, width=None):
-    """Pointer of a per-request device array: [rows], or [rows, >= width] with contiguous rows."""
+def _one(name: str, x, rows: int, dtype):
+    """Pointer of a device array with one element for each row."""
     if x is None:
         return None
-    if not x.is_cuda or x.dtype != dtype:
-        raise ValueError(f"{name} must be a CUDA tensor of {str(dtype).replace('torch.', '')}")
-    if width is None:
-        if x.shape != (rows,) or not x.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous tensor of {rows} elements, got {list(x.shape)}")
-    elif x.dim() != 2 or x.shape[0] != rows or x.shape[1] < width or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise ValueError(f"{name} must be [{rows}, at least {width}] with contiguous rows, got {list(x.shape)}")
+    if x.dtype is not dtype or not x.is_cuda or x.shape != (rows,) or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous CUDA tensor of {rows} {str(dtype).replace('torch.', '')}, got "
+                         f"{str(x.dtype).replace('torch.', '')} {list(x.shape)}")
     return x.data_ptr()
+
+
+def _list(name: str, x, rows: int, dtype, least: int = 0):
+    """Pointer, row stride and width of a device array [rows, at least `least`] with contiguous rows."""
+    if x.dtype is not dtype or not x.is_cuda or x.dim() != 2 or x.shape[0] != rows or x.shape[1] < least or \
+            (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError(f"{name} must be a CUDA tensor of {str(dtype).replace('torch.', '')}, [{rows}, at least {least}] with "
+                         f"contiguous rows, got {str(x.dtype).replace('torch.', '')} {list(x.shape)}")
+    return x.data_ptr(), x.stride(0), x.shape[1]
 
 
 class LogitsProcessor:
@@ -41,7 +46,8 @@ class LogitsProcessor:
         dev = torch.device("cuda", self.ctx.device)
         self._scratch = torch.zeros(16 * rows, dtype=torch.uint8, device=dev)
         self.next_token = torch.zeros(rows, dtype=torch.int32, device=dev)
-        self._lib = _lib.load()
+        self._process = _lib.load().kt_logits_process
+        self._scratch_ptr = self._scratch.data_ptr()
 
     def __call__(self, logits, out=None, tokens=None, lengths=None, prompt_lengths=None, repetition=None,
                  frequency=None, presence=None, bias_ids=None, bias_values=None, bias_counts=None, allowed=None,
@@ -57,38 +63,39 @@ class LogitsProcessor:
         first bias_counts[row] count; ``allowed`` int32 words.  Writes ``out`` (the logits
         themselves unless given) and returns the greedy choice of each row (int32)."""
         rows, vocab = self.rows, self.vocab
-        if not logits.is_cuda or logits.dtype != torch.float32 or tuple(logits.shape) != (rows, vocab) or \
-                (vocab > 1 and logits.stride(1) != 1):
-            raise ValueError(f"logits must be a float32 CUDA tensor of shape [{rows}, {vocab}] with contiguous rows")
+        f32, i32 = torch.float32, torch.int32
+        a = _lib.KtLogitsArgs()
+        a.rows, a.vocab, a.scratch = rows, vocab, self._scratch_ptr
+        for name, x in (("logits", logits), ("out", out)):
+            if x is not None and (x.dtype is not f32 or not x.is_cuda or x.shape != (rows, vocab) or
+                                  (x.stride(1) != 1 and vocab > 1)):
+                raise ValueError(f"{name} must be a float32 CUDA tensor of shape [{rows}, {vocab}] with contiguous rows")
         if out is None:
             out = logits
-        elif not out.is_cuda or out.dtype != torch.float32 or tuple(out.shape) != (rows, vocab) or \
-                (vocab > 1 and out.stride(1) != 1):
-            raise ValueError(f"out must be a float32 CUDA tensor of shape [{rows}, {vocab}] with contiguous rows")
-        if tokens is not None and lengths is None:
-            raise ValueError("tokens need lengths")
-        if tokens is None and not (repetition is None and frequency is None and presence is None):
+        a.logits, a.logits_stride, a.out, a.out_stride = logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0)
+        if tokens is not None:
+            if lengths is None:
+                raise ValueError("tokens need lengths")
+            a.tokens, a.token_stride, a.token_width = _list("tokens", tokens, rows, i32)
+            a.lengths = _one("lengths", lengths, rows, i32)
+            a.prompt_lengths = _one("prompt_lengths", prompt_lengths, rows, i32)
+            a.repetition = _one("repetition", repetition, rows, f32)
+            a.frequency = _one("frequency", frequency, rows, f32)
+            a.presence = _one("presence", presence, rows, f32)
+        elif not (repetition is None and frequency is None and presence is None):
             raise ValueError("penalties need tokens")
         if (bias_ids is None) != (bias_values is None):
             raise ValueError("bias_ids and bias_values come together")
-        if bias_ids is not None and bias_ids.shape != bias_values.shape:
-            raise ValueError("bias_ids and bias_values must have the same shape")
+        if bias_ids is not None:
+            if bias_ids.shape != bias_values.shape or bias_ids.stride() != bias_values.stride():
+                raise ValueError("bias_ids and bias_values must have the same shape and strides")
+            a.bias_ids, a.bias_stride, a.bias_width = _list("bias_ids", bias_ids, rows, i32)
+            a.bias_values = _list("bias_values", bias_values, rows, f32)[0]
+            a.bias_counts = _one("bias_counts", bias_counts, rows, i32)
+        if allowed is not None:
+            a.allowed, a.allowed_stride, _ = _list("allowed", allowed, rows, i32, (vocab + 31) // 32)
         if next_token is None:
             next_token = self.next_token
-        i32, f32 = torch.int32, torch.float32
-        if bias_ids is not None and bias_ids.stride() != bias_values.stride():
-            raise ValueError("bias_ids and bias_values must have the same strides")
-        a = _lib.KtLogitsArgs(
-            logits.data_ptr(), out.data_ptr(), logits.stride(0), out.stride(0), rows, vocab,
-            _per_row("tokens", tokens, rows, i32, 0), _per_row("lengths", lengths, rows, i32),
-            _per_row("prompt_lengths", prompt_lengths, rows, i32), 0 if tokens is None else tokens.stride(0),
-            0 if tokens is None else tokens.shape[1],
-            _per_row("repetition", repetition, rows, f32), _per_row("frequency", frequency, rows, f32),
-            _per_row("presence", presence, rows, f32), 0 if bias_ids is None else bias_ids.shape[1],
-            _per_row("bias_ids", bias_ids, rows, i32, 0),
-            _per_row("bias_values", bias_values, rows, f32, 0), _per_row("bias_counts", bias_counts, rows, i32),
-            0 if bias_ids is None else bias_ids.stride(0), _per_row("allowed", allowed, rows, i32, (vocab + 31) // 32),
-            0 if allowed is None else allowed.stride(0), _per_row("next_token", next_token, rows, i32),
-            self._scratch.data_ptr())
-        _lib.check(self._lib.kt_logits_process(self.ctx.handle, ctypes.byref(a), _stream_of(logits)))
+        a.next_token = _one("next_token", next_token, rows, i32)
+        _lib.check(self._process(self.ctx.handle, ctypes.byref(a), raw_stream(self.ctx.device)))
         return next_token

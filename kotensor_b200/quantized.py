@@ -74,6 +74,11 @@ def _stream_of(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(device: int) -> int:
+    """The cudaStream_t of the device's current stream, without making a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def _is_device(t) -> bool:
     return torch is not None and isinstance(t, torch.Tensor) and t.is_cuda
 
