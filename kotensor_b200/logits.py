@@ -5,6 +5,7 @@ Engine/kotensor/src/main/kotlin/Transformer.kt:255-266)."""
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import _lib
 from .quantized import Context, raw_stream
@@ -15,11 +16,15 @@ except ImportError:  # pragma: no cover
     torch = None
 
 
+_PACK = struct.Struct("@PPqqiiPPPqiPPPiPPPqPqPP")
+assert _PACK.size == ctypes.sizeof(_lib.KtLogitsArgs)
+
+
 def _one(name: str, x, rows: int, dtype):
     """Pointer of a device array with one element for each row."""
     if x is None:
-        return None
-    if x.dtype is not dtype or not x.is_cuda or x.shape != (rows,) or not x.is_contiguous():
+        return 0
+    if x.dtype is not dtype or not x.is_cuda or x.dim() != 1 or x.numel() != rows or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous CUDA tensor of {rows} {str(dtype).replace('torch.', '')}, got "
                          f"{str(x.dtype).replace('torch.', '')} {list(x.shape)}")
     return x.data_ptr()
@@ -48,6 +53,8 @@ class LogitsProcessor:
         self.next_token = torch.zeros(rows, dtype=torch.int32, device=dev)
         self._process = _lib.load().kt_logits_process
         self._scratch_ptr = self._scratch.data_ptr()
+        self._args = _lib.KtLogitsArgs()  # filled anew by every call
+        self._args_ref = ctypes.byref(self._args)
 
     def __call__(self, logits, out=None, tokens=None, lengths=None, prompt_lengths=None, repetition=None,
                  frequency=None, presence=None, bias_ids=None, bias_values=None, bias_counts=None, allowed=None,
@@ -64,24 +71,23 @@ class LogitsProcessor:
         themselves unless given) and returns the greedy choice of each row (int32)."""
         rows, vocab = self.rows, self.vocab
         f32, i32 = torch.float32, torch.int32
-        a = _lib.KtLogitsArgs()
-        a.rows, a.vocab, a.scratch = rows, vocab, self._scratch_ptr
+        token_p = lengths_p = prompt_p = repetition_p = frequency_p = presence_p = 0
+        token_stride = token_width = bias_p = value_p = count_p = bias_stride = bias_width = allowed_p = allowed_stride = 0
         for name, x in (("logits", logits), ("out", out)):
             if x is not None and (x.dtype is not f32 or not x.is_cuda or x.shape != (rows, vocab) or
                                   (x.stride(1) != 1 and vocab > 1)):
                 raise ValueError(f"{name} must be a float32 CUDA tensor of shape [{rows}, {vocab}] with contiguous rows")
         if out is None:
             out = logits
-        a.logits, a.logits_stride, a.out, a.out_stride = logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0)
         if tokens is not None:
             if lengths is None:
                 raise ValueError("tokens need lengths")
-            a.tokens, a.token_stride, a.token_width = _list("tokens", tokens, rows, i32)
-            a.lengths = _one("lengths", lengths, rows, i32)
-            a.prompt_lengths = _one("prompt_lengths", prompt_lengths, rows, i32)
-            a.repetition = _one("repetition", repetition, rows, f32)
-            a.frequency = _one("frequency", frequency, rows, f32)
-            a.presence = _one("presence", presence, rows, f32)
+            token_p, token_stride, token_width = _list("tokens", tokens, rows, i32)
+            lengths_p = _one("lengths", lengths, rows, i32)
+            prompt_p = _one("prompt_lengths", prompt_lengths, rows, i32)
+            repetition_p = _one("repetition", repetition, rows, f32)
+            frequency_p = _one("frequency", frequency, rows, f32)
+            presence_p = _one("presence", presence, rows, f32)
         elif not (repetition is None and frequency is None and presence is None):
             raise ValueError("penalties need tokens")
         if (bias_ids is None) != (bias_values is None):
@@ -89,13 +95,17 @@ class LogitsProcessor:
         if bias_ids is not None:
             if bias_ids.shape != bias_values.shape or bias_ids.stride() != bias_values.stride():
                 raise ValueError("bias_ids and bias_values must have the same shape and strides")
-            a.bias_ids, a.bias_stride, a.bias_width = _list("bias_ids", bias_ids, rows, i32)
-            a.bias_values = _list("bias_values", bias_values, rows, f32)[0]
-            a.bias_counts = _one("bias_counts", bias_counts, rows, i32)
+            bias_p, bias_stride, bias_width = _list("bias_ids", bias_ids, rows, i32)
+            value_p = _list("bias_values", bias_values, rows, f32)[0]
+            count_p = _one("bias_counts", bias_counts, rows, i32)
         if allowed is not None:
-            a.allowed, a.allowed_stride, _ = _list("allowed", allowed, rows, i32, (vocab + 31) // 32)
+            allowed_p, allowed_stride, _ = _list("allowed", allowed, rows, i32, (vocab + 31) // 32)
         if next_token is None:
             next_token = self.next_token
-        a.next_token = _one("next_token", next_token, rows, i32)
-        _lib.check(self._process(self.ctx.handle, ctypes.byref(a), raw_stream(self.ctx.device)))
+        # kt_logits_args, field by field (a ctypes structure takes twice as long to fill)
+        _PACK.pack_into(self._args, 0, logits.data_ptr(), out.data_ptr(), logits.stride(0), out.stride(0), rows, vocab,
+                        token_p, lengths_p, prompt_p, token_stride, token_width, repetition_p, frequency_p, presence_p,
+                        bias_width, bias_p, value_p, count_p, bias_stride, allowed_p, allowed_stride,
+                        _one("next_token", next_token, rows, i32), self._scratch_ptr)
+        _lib.check(self._process(self.ctx.handle, self._args_ref, raw_stream(self.ctx.device)))
         return next_token
