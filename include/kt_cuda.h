@@ -439,7 +439,7 @@ kt_status kt_increment(kt_ctx* ctx, int32_t* value_dev, int32_t delta, void* str
  * lengths is device memory read by the kernels (a captured step replays at any
  * length); no call below but kt_kv8_advance changes it.  head_dim is a multiple of
  * 16 up to 128, block 16, 32 or 64, capacity a multiple of block, batch at most
- * 32767, kv_heads at most 65535, all buffers 16-byte aligned; else
+ * 32767, kv_heads at most 65535, codes and tails 16-byte aligned; else
  * KT_ERR_INVALID_ARGUMENT. */
 typedef struct {
     int8_t* k_codes;
@@ -452,6 +452,12 @@ typedef struct {
     const int32_t* lengths;
     int32_t batch, kv_heads, head_dim, capacity, block;
 } kt_kv8_cache;
+
+/* kt_rope_kv_seqs without the cache: RoPE of the q and k parts of fused q|k|v rows
+ * in place (row r at position *position_dev + r % rows_per_seq), ahead of
+ * kt_kv8_store. */
+kt_status kt_rope_seqs(kt_ctx* ctx, float* qkv_dev, int32_t rows, int32_t q_width, int32_t kv_heads, int32_t head_dim,
+                       const float* inv_freq_dev, const int32_t* position_dev, int32_t rows_per_seq, void* stream);
 
 /* Stores rows_per_seq new tokens of every sequence (row b * rows_per_seq + t of k
  * and v, kv_heads * head_dim floats each, rows k_stride / v_stride floats apart)

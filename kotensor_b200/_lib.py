@@ -148,6 +148,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "kt_lora_backward": ([P, P, P, P, P, P, P, I32, F32, I32, P, I32, P, P, P], I32),
     "kt_gather_rows": ([P, P, P, I32, I32, P, P], I32),
     "kt_fused_cross_entropy": ([P, P, P, P, I32, P, I32, P, P, P, P], I32),
+    "kt_rope_seqs": ([P, P, I32, I32, I32, I32, P, P, I32, P], I32),
     "kt_kv8_store": ([P, ctypes.POINTER(KtKv8Cache), P, P, I64, I64, I32, P, P, P], I32),
     "kt_kv8_scratch_bytes": ([I32, I32, I32, I32, I32, I32, I32], SZ),
     "kt_kv8_attention": ([P, ctypes.POINTER(KtKv8Cache), P, I64, P, I32, P, I32, F32, I32, P, P], I32),

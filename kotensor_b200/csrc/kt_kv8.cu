@@ -140,6 +140,26 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(Kv8 c, const float*
     }
 }
 
+// RoPE (RoPE.kt:117-155) of the query and key heads of fused q|k|v rows in place: a
+// thread has a pair (i, i + half) of one head.
+__global__ void __launch_bounds__(kThreads) rope_seqs_kernel(float* __restrict__ qkv, int heads, int head_dim, int64_t stride,
+                                                             const float* __restrict__ inv_freq,
+                                                             const int32_t* __restrict__ position, int rows_per_seq) {
+    dev::pdl_wait();
+    dev::pdl_launch_dependents();
+    const int half = head_dim / 2, r = blockIdx.y, at = *position + r % rows_per_seq;
+    float* row = qkv + r * stride;
+    for (int e = blockIdx.x * kThreads + threadIdx.x; e < heads * half; e += gridDim.x * kThreads) {
+        const int head = e / half, i = e - head * half;
+        float* v = row + head * head_dim;
+        float sn, cs;
+        sincosf(static_cast<float>(at) * inv_freq[i], &sn, &cs);
+        const float x1 = v[i], x2 = v[i + half];
+        v[i] = x1 * cs - x2 * sn;
+        v[i + half] = x1 * sn + x2 * cs;
+    }
+}
+
 __global__ void kv8_advance_kernel(int32_t* __restrict__ lengths, int batch, int rows,
                                    const int32_t* __restrict__ counts, int limit) {
     dev::pdl_wait();
@@ -391,15 +411,29 @@ const char* kv8_check(const Kv8* c) {
         return "head_dim must be a multiple of 16 in 16..128";
     if (c->block != 16 && c->block != 32 && c->block != 64) return "block must be 16, 32 or 64";
     if (c->capacity < c->block || c->capacity % c->block != 0) return "capacity must be a positive multiple of block";
-    if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_scales) || !aligned16(c->v_scales) ||
-        !aligned16(c->k_tail) || !aligned16(c->v_tail) || !aligned16(c->weights))
-        return "cache buffers must be 16-byte aligned";
+    if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_tail) || !aligned16(c->v_tail))
+        return "codes and tails must be 16-byte aligned";
     return nullptr;
 }
 
 }  // namespace kt
 
 using namespace kt;
+
+kt_status kt_rope_seqs(kt_ctx* ctx, float* qkv, int32_t rows, int32_t q_width, int32_t kv_heads, int32_t head_dim,
+                       const float* inv_freq, const int32_t* position, int32_t rows_per_seq, void* stream) {
+    if (!ctx || !qkv || !inv_freq || !position || rows <= 0 || rows > 65535 || head_dim <= 0 || head_dim % 2 != 0 ||
+        q_width % head_dim != 0 || kv_heads <= 0 || rows_per_seq <= 0 || rows % rows_per_seq != 0)
+        return entry_fail(KT_ERR_INVALID_ARGUMENT, "bad rope_seqs arguments");
+    return c_entry(ctx, [&] {
+        const int heads = q_width / head_dim + kv_heads;
+        const dim3 grid((heads * (head_dim / 2) + kThreads - 1) / kThreads, rows);
+        return entry_launch(launch_dependent(rope_seqs_kernel, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(stream), qkv,
+                                             heads, head_dim, static_cast<int64_t>(q_width) + 2ll * kv_heads * head_dim,
+                                             inv_freq, position, rows_per_seq),
+                            "rope_seqs launch");
+    });
+}
 
 kt_status kt_kv8_store(kt_ctx* ctx, const kt_kv8_cache* cache, const float* k, const float* v, int64_t k_stride,
                        int64_t v_stride, int32_t rows_per_seq, const int32_t* counts, int32_t* status, void* stream) {

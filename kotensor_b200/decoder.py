@@ -134,12 +134,23 @@ class DeviceDecoder:
     The two row-parallel products of a layer end in the only exchange: an
     all-reduce of [batch x dim] partial sums (fused into the m = 1 GEMV over
     peer memory, else NCCL), after which every rank holds the whole residual
-    stream."""
+    stream.
+
+    ``kv_bits`` 8: keys and values in a KVCache8 (``cache``) with a scale for every
+    ``kv_block`` positions of a head, a quarter of the fp32 cache's memory and of the
+    bytes a step's attention reads.  ``kv_weights`` also accumulates the attention
+    weight every slot receives, by which ``evict`` prunes the cache.  ``penalize``
+    puts penalties, biases and a grammar mask between the logits and the greedy
+    choice."""
 
     max_block_rows = 65535
 
     def __init__(self, cfg: DecoderConfig, weights, max_seq: int, device: Optional[int] = None, batch: int = 1,
-                 comm=None):
+                 comm=None, kv_bits: int = 32, kv_block: int = 64, kv_weights: bool = False):
+        if kv_bits not in (8, 32):
+            raise ValueError(f"kv_bits must be 8 or 32, got {kv_bits}")
+        if kv_weights and kv_bits != 8:
+            raise ValueError("attention weights are kept by the 8-bit cache only")
         self.cfg = cfg
         self.max_seq = max_seq
         self.ctx = Context.get(device)
@@ -195,8 +206,14 @@ class DeviceDecoder:
         self.batch = batch
         # one KV cache per sequence, each in the reference's layout [L][kvH][maxSeq][hd]
         # (this rank's key/value heads under tensor parallelism)
-        self.keys = torch.zeros((batch, cfg.layers, self.kv_local, max_seq, cfg.head_dim), **f32)
-        self.values = torch.zeros_like(self.keys)
+        self.cache = self.keys = self.values = None
+        if kv_bits == 8:
+            from .kv8 import KVCache8
+            self.cache = KVCache8(cfg.layers, batch, self.kv_local, cfg.head_dim, max_seq, kv_block, kv_weights, self.ctx.device)
+            self.cache._scratch_of(1, self.heads_local)  # what a captured step needs
+        else:
+            self.keys = torch.zeros((batch, cfg.layers, self.kv_local, max_seq, cfg.head_dim), **f32)
+            self.values = torch.zeros_like(self.keys)
         self.cache_stride = cfg.layers * self.kv_local * max_seq * cfg.head_dim
         self.inv_freq = vec(rope_inv_freq(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling))
         self.token = torch.zeros(batch, dtype=torch.int32, device=dev)
@@ -209,7 +226,9 @@ class DeviceDecoder:
         self._last_rows = torch.empty(batch, dtype=torch.int32, device=dev)
         self._step_bufs = self._buffers(batch, tokens=self.token)
         self._prefill_bufs = None  # prefill buffers, allocated on first use
-        self.length = 0
+        self.length = 0  # tokens processed
+        self.held = 0    # positions in the cache (fewer after an eviction)
+        self._penal = None
         self.scale = float(np.float32(1.0) / np.float32(math.sqrt(float(cfg.head_dim))))
         self._graph = None
         g_ = self.heads_local // self.kv_local
@@ -226,8 +245,13 @@ class DeviceDecoder:
         return ctypes.c_void_p(torch.cuda.current_stream(self.ctx.device).cuda_stream)
 
     def reset(self) -> None:
-        self.length = 0
+        self.length = self.held = 0
         self.position.zero_()
+        if self.cache is not None:
+            self.cache.reset()
+        if self._penal is not None:
+            self._history_lengths.zero_()
+            self._prompt_lengths.zero_()
 
     def _buffers(self, rows: int, tokens=None) -> "_Rows":
         cfg = self.cfg
@@ -244,8 +268,9 @@ class DeviceDecoder:
         b.act = torch.empty((rows, self.hidden_local), **f32)
         b.tokens = tokens if tokens is not None else torch.empty(rows, dtype=torch.int32, device=dev)
         # attention scratch; zero-filled: its tail holds the fused kernel's merge counters
-        b.scores = torch.zeros(_lib.load().kt_attention_scratch_floats(rows, self.heads_local, cfg.head_dim,
-                                                                       self.max_seq), **f32)
+        # (the 8-bit cache has its own)
+        b.scores = None if self.cache is not None else torch.zeros(
+            _lib.load().kt_attention_scratch_floats(rows, self.heads_local, cfg.head_dim, self.max_seq), **f32)
         return b
 
     def _row_parallel(self, x, w, out, rows: int, bias, accumulate: bool = True) -> None:
@@ -303,8 +328,12 @@ class DeviceDecoder:
         L_ = _lib.load()
         cfg, h = self.cfg, self.ctx.handle
         s, p = self._stream(), self._p
-        keys = ctypes.c_void_p(self.keys.data_ptr() + seq0 * self.cache_stride * self.keys.element_size())
-        values = ctypes.c_void_p(self.values.data_ptr() + seq0 * self.cache_stride * self.values.element_size())
+        if self.cache is None:
+            keys = ctypes.c_void_p(self.keys.data_ptr() + seq0 * self.cache_stride * self.keys.element_size())
+            values = ctypes.c_void_p(self.values.data_ptr() + seq0 * self.cache_stride * self.values.element_size())
+        else:
+            n = rows // rows_per_seq
+            cache = self.cache if n == self.batch else self.cache.sequences(seq0, seq0 + n)
         hd, kvh = cfg.head_dim, self.kv_local
         kv = self.kv_width
         if cfg.tied:
@@ -315,7 +344,14 @@ class DeviceDecoder:
         for l, L in enumerate(self.layers):
             _lib.check(L_.kt_rmsnorm_qmatmul(h, L["wqkv"].handle, p(b.x), p(L["norm1"]), cfg.eps, p(b.normed),
                                              p(b.qkv), rows, 0, p(L["bqkv"]), s))
-            if rows_per_seq == 1 and self._fused_attention and rows <= (16 if cfg.head_dim == 128 else 8):
+            if self.cache is not None:
+                _lib.check(L_.kt_rope_seqs(h, p(b.qkv), rows, self.q_width, kvh, hd, p(self.inv_freq), p(self.position),
+                                           rows_per_seq, s))
+                q, k, v = b.qkv[:rows].split([self.q_width, kv, kv], 1)
+                cache.store(l, k, v, rows_per_seq)
+                cache.attend(l, q, self.heads_local, rows_per_seq, self.scale, out=b.ctx[:rows],
+                             accumulate=cache.weights is not None)
+            elif rows_per_seq == 1 and self._fused_attention and rows <= (16 if cfg.head_dim == 128 else 8):
                 # one token per sequence: RoPE, cache store, attention and merge in one launch
                 # (measured slower than the separate kernels once more sequences share a
                 # step: beyond 16 at head_dim 128, beyond 8 at 64)
@@ -342,12 +378,17 @@ class DeviceDecoder:
         h, s, p = self.ctx.handle, self._stream(), self._p
         _lib.check(L_.kt_rmsnorm_qmatmul(h, self.head.handle, p(x_rows), p(self.final_norm), self.cfg.eps,
                                          p(self._head_xn), p(self.logits), self.batch, 0, p(self.head_bias), s))
-        if self.comm is None:
+        if self._penal is not None:  # penalties, biases, mask and the choice in one pass
+            self._processor(self.logits, tokens=self._history, lengths=self._history_lengths,
+                            prompt_lengths=self._prompt_lengths, next_token=self.next_token, **self._penal)
+        elif self.comm is None:
             _lib.check(L_.kt_argmax(h, p(self.logits), self.batch, self.cfg.vocab, p(self.next_token), s))
         else:  # every rank's best column, merged across ranks: the same token everywhere
             from .parallel import argmax_column_parallel
             argmax_column_parallel(self.comm, self.logits, self.vocab_begin, self.next_token)
         _lib.check(L_.kt_increment(h, p(self.position), advance, s))
+        if self.cache is not None:
+            self.cache.advance(advance)
         self.token.copy_(self.next_token)
 
     def _launch_step(self) -> None:
@@ -355,6 +396,10 @@ class DeviceDecoder:
         self.position, writes self.logits and self.next_token, advances
         the position and feeds the next tokens back."""
         b = self._step_bufs
+        if self._penal is not None:  # the step's tokens join the history
+            room = self._history.shape[1]
+            self._history.scatter_(1, self._history_lengths.clamp(max=room - 1).long()[:, None], self.token[:, None])
+            self._history_lengths.add_(1).clamp_(max=room)
         self._layers(b, self.batch, 1)
         self._head(b.x, 1)
 
@@ -379,8 +424,8 @@ class DeviceDecoder:
             raise ValueError("prompts of one batch must have equal lengths")
         if any(not 0 <= t < self.cfg.vocab for pr in prompts for t in pr):
             raise ValueError("token out of vocab bounds")
-        if self.length + T > self.max_seq:
-            raise ValueError(f"KV cache full: {self.length} + {T} positions exceed maxSequenceLength {self.max_seq}")
+        if self.held + T > self.max_seq:
+            raise ValueError(f"KV cache full: {self.held} + {T} positions exceed maxSequenceLength {self.max_seq}")
         if T > self.max_block_rows:
             raise ValueError(f"{T} prompt tokens exceed {self.max_block_rows} rows of one prefill block")
         # whole sequences per block: a block holds at most max_block_rows rows (the
@@ -392,6 +437,8 @@ class DeviceDecoder:
             # a larger block may replace the communicator's scratch that a
             # captured step refers to: capture again before the next replay
             self._graph = None
+        if self._penal is not None:
+            self._append_prompt(prompts, T)
         b = self._prefill_bufs
         flat = torch.tensor([t for pr in prompts for t in pr], dtype=torch.int32)
         L_ = _lib.load()
@@ -407,6 +454,7 @@ class DeviceDecoder:
                                          self.cfg.dim, dst, self._stream()))
         self._head(self._head_in, T)
         self.length += T
+        self.held += T
         return self._result()
 
     def step(self, tokens):
@@ -418,11 +466,12 @@ class DeviceDecoder:
         for t in tokens:
             if not 0 <= t < self.cfg.vocab:
                 raise ValueError(f"{t} out of vocab bounds {self.cfg.vocab}")
-        if self.length >= self.max_seq:
+        if self.held >= self.max_seq:
             raise ValueError(f"KV cache full: maxSequenceLength {self.max_seq}")
         self.token.copy_(torch.tensor(tokens, dtype=torch.int32))
         self._launch_step()
         self.length += 1
+        self.held += 1
         return self._result()
 
     def capture(self) -> None:
@@ -440,6 +489,8 @@ class DeviceDecoder:
         if len(prompt) + max_tokens > self.max_seq:
             raise ValueError("prompt + max_tokens exceed max_seq")
         for t in prompt:
+            if self._penal is not None:  # a token of the prompt
+                self._prompt_lengths.copy_(self._history_lengths + 1)
             self.step(t)
         out = [int(self.next_token[0].item())]
         if self._graph is None:
@@ -447,23 +498,90 @@ class DeviceDecoder:
         for _ in range(max_tokens - 1):
             self._graph.replay()
             self.length += 1
+            self.held += 1
             out.append(int(self.next_token[0].item()))
         return out
 
-    def generate_batch(self, prompts, max_tokens: int) -> list:
+    def generate_batch(self, prompts, max_tokens: int, keep: Optional[int] = None, recent: int = 0) -> list:
         """Greedy continuation of every sequence: the prompts prefilled as blocks,
-        then ``max_tokens`` - 1 replays of the captured batched step."""
-        if len(prompts[0]) + max_tokens > self.max_seq:
+        then ``max_tokens`` - 1 replays of the captured batched step.  With ``keep``
+        the cache is pruned to ``keep`` positions (``evict``) after the prompts and
+        whenever it is full, so the text may outgrow it."""
+        if keep is not None:
+            self._check_evict(keep, recent)
+            if not keep < self.max_seq:
+                raise ValueError(f"keep must be below max_seq {self.max_seq}, got {keep}")
+        elif len(prompts[0]) + max_tokens > self.max_seq:
             raise ValueError("prompt + max_tokens exceed max_seq")
         self.prefill(prompts)
         out = [self.next_token.cpu().tolist()]
+        if keep is not None:
+            self.evict(keep, recent)
         if self._graph is None:
             self.capture()
         for _ in range(max_tokens - 1):
+            if keep is not None and self.held >= self.max_seq:
+                self.evict(keep, recent)
             self._graph.replay()
             self.length += 1
+            self.held += 1
             out.append(self.next_token.cpu().tolist())
         return [[row[q] for row in out] for q in range(self.batch)]
+
+    # -- the 8-bit cache and the choice of tokens
+    def _check_evict(self, keep: int, recent: int) -> None:
+        if self.cache is None or self.cache.weights is None:
+            raise ValueError("eviction needs kv_bits 8 and kv_weights")
+        if keep < 1 or not 0 <= recent <= keep:
+            raise ValueError(f"eviction needs 0 <= recent <= keep and 1 <= keep, got {recent} and {keep}")
+
+    def evict(self, keep: int, recent: int) -> None:
+        """Prunes the cache to ``keep`` positions: in every layer each key/value head keeps
+        its ``recent`` last ones and those of the others that received most attention
+        (KVCache8.evict).  Positions of later tokens go on from ``length``."""
+        self._check_evict(keep, recent)
+        if self.held > keep:
+            self.cache.evict(keep, recent)
+            self.held = keep
+
+    def penalize(self, repetition=None, frequency=None, presence=None, bias_ids=None, bias_values=None, bias_counts=None,
+                 allowed=None, history: Optional[int] = None) -> None:
+        """From the next step on the logits go through a LogitsProcessor: penalties (a
+        number, or one for each sequence) for the tokens of prompt and answer, sparse
+        biases and a mask of allowed tokens (device tensors as LogitsProcessor takes
+        them; the mask's contents may change between steps).  ``history`` bounds the
+        tokens remembered (max_seq unless given).  No arguments: plain argmax again."""
+        self._graph = None  # a captured step has the old choice
+        given = dict(repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
+                     bias_values=bias_values, bias_counts=bias_counts, allowed=allowed)
+        given = {k: v for k, v in given.items() if v is not None}
+        if not given:
+            self._penal = None
+            return
+        if self.comm is not None:
+            raise ValueError("penalties need the whole logits: not under tensor parallelism")
+        from .logits import LogitsProcessor
+        dev = self.position.device
+        for k in ("repetition", "frequency", "presence"):
+            if k in given:
+                x = torch.as_tensor(given[k], dtype=torch.float32, device=dev)
+                if x.numel() not in (1, self.batch):
+                    raise ValueError(f"{k} must be a number or one for each of {self.batch} sequences")
+                given[k] = x.reshape(-1).expand(self.batch).contiguous()
+        self._processor = LogitsProcessor(self.batch, self.cfg.vocab, self.ctx.device)
+        self._history = torch.zeros((self.batch, history or self.max_seq), dtype=torch.int32, device=dev)
+        self._history_lengths = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        self._prompt_lengths = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        self._penal = given
+
+    def _append_prompt(self, prompts, T: int) -> None:
+        """Prompt tokens into the history; what is there so far counts as prompt."""
+        n = int(self._history_lengths[0].item())
+        room = max(0, min(T, self._history.shape[1] - n))
+        if room:
+            self._history[:, n:n + room] = torch.tensor([list(p)[:room] for p in prompts], dtype=torch.int32)
+        self._history_lengths.fill_(n + room)
+        self._prompt_lengths.fill_(n + room)
 
     # -- files (Transformer.saveQuantized / loadQuantized, Transformer.kt:402-471)
     def save_quantized(self, path) -> None:
@@ -508,11 +626,11 @@ class DeviceDecoder:
         save_entries(path, entries, meta)
 
     @staticmethod
-    def load_quantized(path, max_seq: int, device: Optional[int] = None) -> "DeviceDecoder":
+    def load_quantized(path, max_seq: int, device: Optional[int] = None, **options) -> "DeviceDecoder":
         """Transformer.loadQuantized: a decoder whose weights go from the file
-        straight into HBM."""
+        straight into HBM; ``options`` are the constructor's (batch, kv_bits, ...)."""
         cfg, weights = load_quantized_weights(path, device)
-        return DeviceDecoder(cfg, weights, max_seq, device)
+        return DeviceDecoder(cfg, weights, max_seq, device, **options)
 
 
 # (file name suffix, decoder weight key) in Transformer.namedProjections order (Transformer.kt:268-282)

@@ -12,6 +12,7 @@ numbers of tokens (``lengths``, on the device).
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
 from typing import Optional
@@ -81,15 +82,33 @@ class KVCache8:
         self._status = self.status.data_ptr()
         self._scratch = torch.zeros(0, dtype=torch.uint8, device=dev)
         self._scratch_for = set()
+        self._retired = []  # scratch that a captured graph may still use
         lib = _lib.load()
         self._lib, self._store, self._attention = lib, lib.kt_kv8_store, lib.kt_kv8_attention
         self._scale = 1.0 / math.sqrt(head_dim)
+        self._describe()
+
+    def _describe(self) -> None:
+        """The C descriptor of every layer."""
         buffers = (self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.k_tail, self.v_tail, self.weights)
         self._layer = []
-        for l in range(layers):
+        for l in range(self.layers):
             s = _lib.KtKv8Cache(*(None if t is None else t[l].data_ptr() for t in buffers), self.lengths.data_ptr(),
-                                batch, kv_heads, head_dim, capacity, block)
+                                self.batch, self.kv_heads, self.head_dim, self.capacity, self.block)
             self._layer.append((s, ctypes.byref(s)))
+
+    def sequences(self, begin: int, end: int) -> "KVCache8":
+        """A view of sequences begin..end-1: the same buffers, its own scratch."""
+        if not 0 <= begin < end <= self.batch:
+            raise ValueError(f"sequences {begin}..{end} of {self.batch}")
+        view = copy.copy(self)
+        view.batch, view.lengths = end - begin, self.lengths[begin:end]
+        for name in ("k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail", "weights"):
+            t = getattr(self, name)
+            setattr(view, name, None if t is None else t[:, begin:end])
+        view._scratch, view._scratch_for, view._retired = self._scratch[:0], set(), []
+        view._describe()
+        return view
 
     def _cache(self, layer: int):
         if not 0 <= layer < self.layers:
@@ -109,6 +128,7 @@ class KVCache8:
             need = self._lib.kt_kv8_scratch_bytes(self.batch, rows_per_seq, heads, self.kv_heads, self.head_dim,
                                                   self.capacity, self.weights is not None)
             if need > self._scratch.numel():
+                self._retired.append(self._scratch)
                 self._scratch = torch.zeros(need, dtype=torch.uint8, device=self.device)
             self._scratch_for.add((rows_per_seq, heads))
         return self._scratch.data_ptr()

@@ -68,7 +68,8 @@ class LogitsProcessor:
         ``tokens`` int32 [rows, n] of which the first lengths[row] count; the penalties
         float32 [rows]; ``bias_ids`` int32 / ``bias_values`` float32 [rows, e] of which the
         first bias_counts[row] count; ``allowed`` int32 words.  Writes ``out`` (the logits
-        themselves unless given) and returns the greedy choice of each row (int32)."""
+        themselves unless given) and returns the greedy choice of each row: ``next_token``
+        (int32 [rows]), or a buffer of this object that its next call overwrites."""
         rows, vocab = self.rows, self.vocab
         f32, i32 = torch.float32, torch.int32
         token_p = lengths_p = prompt_p = repetition_p = frequency_p = presence_p = 0
