@@ -113,8 +113,12 @@ size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, i
 cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, int32_t* err, cudaStream_t s);
 // Many query rows, on tcgen05 (kt_kv8_prompt.cu).  aligned: bit 0, q's rows lie on
 // 16-byte boundaries.  lse (NULL: not wanted): ln of the softmax's sum of every row
-// and head.
-cudaError_t launch_kv8_prompt(const Kv8Attention& a, int aligned, float* lse, int32_t* err, cudaStream_t s);
+// and head.  parts: kv8_prompt_bytes of scratch, used where a launch of fewer CTAs than
+// SMs splits the slots into kv8_prompt_splits parts.
+constexpr int kPromptCtas = 148;
+int kv8_prompt_splits(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t capacity);
+size_t kv8_prompt_bytes(int32_t head_dim);
+cudaError_t launch_kv8_prompt(const Kv8Attention& a, int aligned, float* parts, float* lse, int32_t* err, cudaStream_t s);
 
 #ifdef __CUDACC__
 // Tokens that sequence b holds, whatever the caller left in lengths.

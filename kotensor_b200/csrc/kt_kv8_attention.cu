@@ -651,8 +651,19 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_weights_kernel(Kv8Attention a
 }  // namespace
 
 namespace {
-bool use_tiles(int32_t rows_per_seq, int32_t heads, int32_t kv_heads) {
-    return static_cast<int64_t>(rows_per_seq) * (heads / kv_heads) <= 64;
+// Which kernel is the faster.  The one of this file reads the cache for every eight
+// query vectors and spreads all tiles of 32 slots over the card: 1.3 ns a tile, with
+// head_dim 128 and the codes in L2.  The one on tcgen05 gives 128 vectors to a CTA: 2 us
+// for 128 slots of a wave of 148, or of their part where fewer share the slots out.
+// Both grow with the lengths, which only the device knows and which drop out:
+//   sequences x kv_heads x eights x 4 x 1.3 ns  against  waves x 2 us.
+// (The choice must not ask whether weights are accumulated: a context has the same bits
+// either way.)
+bool use_tiles(int64_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads) {
+    const int64_t vectors = static_cast<int64_t>(rows_per_seq) * (heads / kv_heads);
+    const int64_t eights = (vectors + 7) / 8, ctas = batch * kv_heads * ((vectors + 127) / 128);
+    const double waves = ctas < kPromptCtas ? static_cast<double>(ctas) / kPromptCtas : static_cast<double>((ctas + kPromptCtas - 1) / kPromptCtas);
+    return eights == 1 || static_cast<double>(batch * kv_heads * eights) * 5.2 < 2000.0 * waves;
 }
 int tiles_of_vectors(int32_t rows_per_seq, int32_t heads, int32_t kv_heads) {
     return (rows_per_seq * (heads / kv_heads) + kVectors - 1) / kVectors;
@@ -686,8 +697,8 @@ cudaError_t launch_tiles(const Kv8Attention& a, int sm_count, int aligned, float
 
 size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
                            int32_t capacity, bool weights) {
-    size_t n = part_bytes(head_dim) + lse_bytes(batch, rows_per_seq, heads);
-    if (weights && use_tiles(rows_per_seq, heads, kv_heads))
+    size_t n = std::max(part_bytes(head_dim), round256(kv8_prompt_bytes(head_dim))) + lse_bytes(batch, rows_per_seq, heads);
+    if (weights && use_tiles(batch, rows_per_seq, heads, kv_heads))
         n += static_cast<size_t>(batch) * rows_per_seq * heads * capacity * sizeof(float);
     return n;
 }
@@ -696,11 +707,12 @@ cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, int32_t* e
     const Kv8& c = a.cache;
     char* free = static_cast<char*>(a.scratch) + kKv8CounterBytes;
     float* parts = reinterpret_cast<float*>(free);
-    float* lse = reinterpret_cast<float*>(free + part_bytes(c.head_dim));
+    const size_t lse_at = std::max(part_bytes(c.head_dim), round256(kv8_prompt_bytes(c.head_dim)));
+    float* lse = reinterpret_cast<float*>(free + lse_at);
     const auto ok16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const int aligned = (ok16(a.q) && a.q_stride % 4 == 0 ? 1 : 0) | (ok16(a.context) ? 2 : 0);
-    if (use_tiles(a.rows_per_seq, a.heads, c.kv_heads)) {
-        float* scores = reinterpret_cast<float*>(free + part_bytes(c.head_dim) + lse_bytes(c.batch, a.rows_per_seq, a.heads));
+    if (use_tiles(c.batch, a.rows_per_seq, a.heads, c.kv_heads)) {
+        float* scores = reinterpret_cast<float*>(free + lse_at + lse_bytes(c.batch, a.rows_per_seq, a.heads));
         if (!a.accumulate) scores = nullptr;
         const bool fine = c.block == 16, wide = c.head_dim > 64;
         cudaError_t e = wide ? fine ? launch_tiles<128, true>(a, sm_count, aligned, parts, scores, lse, s)
@@ -712,7 +724,7 @@ cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, int32_t* e
                                  0, s, a, static_cast<const float*>(scores), static_cast<const float*>(lse));
         return e;
     }
-    cudaError_t e = launch_kv8_prompt(a, aligned, a.accumulate ? lse : nullptr, err, s);
+    cudaError_t e = launch_kv8_prompt(a, aligned, parts, a.accumulate ? lse : nullptr, err, s);
     if (e == cudaSuccess && a.accumulate)
         e = launch_dependent(kv8_weights_kernel, dim3((c.capacity + kWarps - 1) / kWarps, c.kv_heads, c.batch),
                              dim3(kWarps * 32), 0, s, a, static_cast<const float*>(lse));

@@ -33,6 +33,8 @@
 // both terms of P keep 22 bits of what matters to O.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "kt_kv8.h"
 
 namespace kt {
@@ -69,6 +71,7 @@ struct PromptShape {
     static constexpr int kMeet = kStats + 4 * 4 * kVecTile * 4;         // largest scores of the halves of two tiles
     static constexpr int kBars = kMeet + 4 * kVecTile * 8;
     static constexpr int kSmem = 1024 + kBars + 256;
+    static constexpr int kPart = kVecTile * (HDP + 1);    // floats of a split: its results, then logarithms
     static constexpr uint32_t kO = 2 * kSlots, kQ = kO + HDP;  // S of stream x at kSlots * x; Q hi, then lo
     static_assert(HDP * kOutPitch * 4 <= kRaw, "epilogue area");
     static_assert(kSmem <= 232448, "shared memory per CTA");
@@ -314,14 +317,15 @@ __device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit,
 }
 
 template <int HDP>
-__global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a, int aligned, float* __restrict__ lse,
+__global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a, int aligned, int splits,
+                                                                 float* __restrict__ parts, float* __restrict__ lse,
                                                                  int32_t* __restrict__ err) {
     using S = PromptShape<HDP>;
     dev::pdl_wait();
     const Kv8& c = a.cache;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, d = c.head_dim;
     const int b = blockIdx.z, h = blockIdx.y;
-    const int vt = gridDim.x - 1 - blockIdx.x;  // the rows that see most first
+    const int vt = gridDim.x / splits - 1 - blockIdx.x / splits;  // the rows that see most first
     const int group = a.heads / c.kv_heads, vectors = a.rows_per_seq * group, v0 = vt * kVecTile;
     const int rows = kv8_rows(a.counts, b, a.rows_per_seq), held = kv8_held(c, b);
     const int seen = min(held + rows, c.capacity);
@@ -339,7 +343,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
         return;
     }
     const int most = min(held + (v0 + real - 1) / group + 1, seen);  // slots its last vector sees
-    const int tiles = (most + kSlots - 1) / kSlots;
+    // the CTA's tiles: part `split` of those its vectors see, numbered from `from`
+    const int all_tiles = (most + kSlots - 1) / kSlots, split = blockIdx.x % splits;
+    const int from = split * all_tiles / splits, tiles = (split + 1) * all_tiles / splits - from;
+    // with splits, each leaves its result and the logarithms of its sums in its place
+    float* const part = parts + ((static_cast<int64_t>(b) * c.kv_heads + h) * (gridDim.x / splits) + vt) * splits * S::kPart +
+                        static_cast<int64_t>(split) * S::kPart;
+    if (tiles == 0) {
+        for (int v = threadIdx.x; v < kVecTile; v += kThreads) part[kVecTile * HDP + v] = -INFINITY;
+        dev::pdl_launch_dependents();
+        return;
+    }
 
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = dev::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -454,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
         const float* k_scales = c.k_scales + head * (c.capacity / c.block);
         const float* v_scales = c.v_scales + head * (c.capacity / c.block);
         for (int i = 0; i < tiles; ++i) {
-            const int y = i & 1, first = i * kSlots + 64 * x, at = first + 16 * (lane % 4);
+            const int y = i & 1, first = (from + i) * kSlots + 64 * x, at = first + 16 * (lane % 4);
             const float ks = at < most ? k_scales[at / c.block] : 0.0f, vs = at < most ? v_scales[at / c.block] : 0.0f;
             if (!wait_all(s_full(y), (i / 2) & 1)) break;
             tc_after();
@@ -521,10 +535,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
                     const int y = i & 1;
                     if (i >= 2 && !wait(raw_free(v, y), (i / 2 - 1) & 1)) return;
                     // (slots past the last one seen have some code: their scores are masked, their P is 0)
-                    const uint32_t bytes = static_cast<uint32_t>(min(kSlots, c.capacity - i * kSlots) * d);
-                    const int8_t* from = (v ? c.v_codes : c.k_codes) + (head * c.capacity + static_cast<int64_t>(i) * kSlots) * d;
+                    const int slot = (from + i) * kSlots;
+                    const uint32_t bytes = static_cast<uint32_t>(min(kSlots, c.capacity - slot) * d);
+                    const int8_t* codes = (v ? c.v_codes : c.k_codes) + (head * c.capacity + slot) * d;
                     dev::mbar_expect_tx(raw_full(v, y), bytes);
-                    dev::bulk_load(base + S::kRaw + (2 * v + y) * S::kRawTile, from, bytes, raw_full(v, y));
+                    dev::bulk_load(base + S::kRaw + (2 * v + y) * S::kRawTile, codes, bytes, raw_full(v, y));
                 };
                 copy(0, 0);
                 if (tiles > 1) copy(0, 1);
@@ -619,7 +634,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             __syncwarp();
         }
         // every product is complete (the last o_full came after all of them): K and V are free
-        if (lse != nullptr && row < real)
+        if (splits > 1) part[kVecTile * HDP + row] = D + log2f(l);
+        else if (lse != nullptr && row < real)
             lse[(static_cast<int64_t>(b) * a.rows_per_seq + (v0 + row) / group) * a.heads + h * group + (v0 + row) % group] =
                 (D + log2f(l)) / kLog2e;
         const float scale = l != l ? l : R == -INFINITY ? 0.0f : ex2(R - kLift - D) / l;
@@ -634,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
         }
         asm volatile("bar.sync 3, 128;" ::: "memory");
         for (int v = warp - kSumWarp; v < real; v += 4) {
-            float* to = a.context + place(v0 + v, static_cast<int64_t>(a.heads) * d);
+            float* to = splits > 1 ? part + v * HDP : a.context + place(v0 + v, static_cast<int64_t>(a.heads) * d);
             for (int i = lane; i < d; i += 32) to[i] = area[i * S::kOutPitch + v];
         }
     }
@@ -646,8 +662,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
     }
 }
 
+// The splits of a vector's slots: a warp to a vector, results weighted by their sums.
 template <int HDP>
-cudaError_t launch(const Kv8Attention& a, int aligned, float* lse, int32_t* err, cudaStream_t s) {
+__global__ void __launch_bounds__(256) kv8_prompt_merge_kernel(Kv8Attention a, int splits, const float* __restrict__ parts,
+                                                               float* __restrict__ lse) {
+    using S = PromptShape<HDP>;
+    dev::pdl_wait();
+    dev::pdl_launch_dependents();
+    const Kv8& c = a.cache;
+    const int b = blockIdx.z, h = blockIdx.y, v = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32, d = c.head_dim;
+    const int group = a.heads / c.kv_heads, rows = kv8_rows(a.counts, b, a.rows_per_seq);
+    if (v >= rows * group) return;
+    const int tiles = (a.rows_per_seq * group + kVecTile - 1) / kVecTile;
+    const float* part = parts + ((static_cast<int64_t>(b) * c.kv_heads + h) * tiles + v / kVecTile) * splits * S::kPart;
+    const int at = v % kVecTile;
+    float top = -INFINITY, sum = 0.0f, y[HDP / 32] = {};
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, part[s * S::kPart + kVecTile * HDP + at]);
+    for (int s = 0; s < splits; ++s) {
+        const float z = part[s * S::kPart + kVecTile * HDP + at];
+        if (z == -INFINITY) continue;
+        const float by = ex2(z - top);
+        sum += by;
+#pragma unroll
+        for (int i = 0; i < HDP / 32; ++i)
+            if (lane + 32 * i < d) y[i] = fmaf(by, part[s * S::kPart + at * HDP + lane + 32 * i], y[i]);
+    }
+    const int64_t row = static_cast<int64_t>(b) * a.rows_per_seq + v / group;
+    const int head = h * group + v % group;
+#pragma unroll
+    for (int i = 0; i < HDP / 32; ++i)
+        if (lane + 32 * i < d) a.context[row * a.heads * d + static_cast<int64_t>(head) * d + lane + 32 * i] = y[i] / sum;
+    if (lse != nullptr && lane == 0) lse[row * a.heads + head] = (top + log2f(sum)) / kLog2e;
+}
+
+template <int HDP>
+cudaError_t launch(const Kv8Attention& a, int aligned, float* parts, float* lse, int32_t* err, cudaStream_t s) {
     using S = PromptShape<HDP>;
     static std::atomic<uint64_t> allowed{0};
     cudaError_t e = allow_shared(kv8_prompt_kernel<HDP>, S::kSmem, allowed);
@@ -658,14 +707,32 @@ cudaError_t launch(const Kv8Attention& a, int aligned, float* lse, int32_t* err,
     }();
     if (regs != kLaunchRegs) return cudaErrorInvalidConfiguration;
     const int64_t vectors = static_cast<int64_t>(a.rows_per_seq) * (a.heads / a.cache.kv_heads);
-    const dim3 grid(static_cast<unsigned>((vectors + kVecTile - 1) / kVecTile), a.cache.kv_heads, a.cache.batch);
-    return launch_dependent(kv8_prompt_kernel<HDP>, grid, dim3(kThreads), S::kSmem, s, a, aligned, lse, err);
+    const int64_t tiles = (vectors + kVecTile - 1) / kVecTile;
+    // Too few CTAs for the card: each vector tile's slots in parts.  (4 sequences of 8 key/value
+    // heads, 60 rows of 4 heads each, 4000 slots: 64 CTAs 80 us, 128 of half the slots KT_SPLIT us.)
+    const int splits = kv8_prompt_splits(a.cache.batch, a.rows_per_seq, a.heads, a.cache.kv_heads, a.cache.capacity);
+    const dim3 grid(static_cast<unsigned>(tiles * splits), a.cache.kv_heads, a.cache.batch);
+    e = launch_dependent(kv8_prompt_kernel<HDP>, grid, dim3(kThreads), S::kSmem, s, a, aligned, splits, parts, lse, err);
+    if (e == cudaSuccess && splits > 1)
+        e = launch_dependent(kv8_prompt_merge_kernel<HDP>, dim3(static_cast<unsigned>((vectors + 7) / 8), a.cache.kv_heads, a.cache.batch),
+                             dim3(256), 0, s, a, splits, static_cast<const float*>(parts), lse);
+    return e;
 }
 
 }  // namespace
 
-cudaError_t launch_kv8_prompt(const Kv8Attention& a, int aligned, float* lse, int32_t* err, cudaStream_t s) {
-    return a.cache.head_dim <= 64 ? launch<64>(a, aligned, lse, err, s) : launch<128>(a, aligned, lse, err, s);
+int kv8_prompt_splits(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t capacity) {
+    const int64_t vectors = static_cast<int64_t>(rows_per_seq) * (heads / kv_heads);
+    const int64_t ctas = static_cast<int64_t>(batch) * kv_heads * ((vectors + kVecTile - 1) / kVecTile);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kPromptCtas / ctas, 16, (capacity + kSlots - 1) / kSlots})));
+}
+
+size_t kv8_prompt_bytes(int32_t head_dim) {
+    return static_cast<size_t>(kPromptCtas) * (head_dim <= 64 ? PromptShape<64>::kPart : PromptShape<128>::kPart) * sizeof(float);
+}
+
+cudaError_t launch_kv8_prompt(const Kv8Attention& a, int aligned, float* parts, float* lse, int32_t* err, cudaStream_t s) {
+    return a.cache.head_dim <= 64 ? launch<64>(a, aligned, parts, lse, err, s) : launch<128>(a, aligned, parts, lse, err, s);
 }
 
 }  // namespace kt

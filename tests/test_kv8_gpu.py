@@ -218,12 +218,15 @@ def test_attention_of_one_row(kt, b, heads, h, d, block, lengths):
     (3, 12, 1, 96, 64, [64, 7, 0], 31),
     (1, 8, 2, 128, 64, [1000], 200),
     (2, 6, 6, 112, 32, [3, 90], 130),
+    (2, 8, 2, 128, 64, [5000, 3], 70),            # slots split between CTAs, one sequence with fewer than splits
+    (1, 14, 2, 64, 16, [3000], 90),
+    (3, 32, 8, 64, 32, [700, 0, 64], 33),
 ])
 def test_attention_of_several_rows(kt, b, heads, h, d, block, lengths, rows):
     attention_case(kt, b, heads, h, d, block, lengths, rows, seed=rows)
 
 
-@pytest.mark.parametrize("rows", [1, 5, 70])
+@pytest.mark.parametrize("rows", [1, 5, 20, 70])
 def test_attention_counts(kt, rows):
     """Rows past counts[b] give zeros and no weights; a sequence may have none at all."""
     lengths, counts = [0, 9, 120, 33], [0, rows, rows - 1, 1]
