@@ -136,6 +136,10 @@ template <int HDP>
 struct DecodeShape {
     static constexpr int kStages = 3;
     static constexpr int kStart = HDP == 128 ? 12 : 24;
+    // Items up to this many tiles stay whole where there are CTAs enough: 4 tiles take 0.35 us of
+    // head_dim 64, 0.8 of 128, joining the parts of an item 3.5 us (700 slots, 22 tiles, of
+    // 2 heads x 64: whole 9.3 us, cut 10.7; of 8 heads x 128: whole 13.0, cut 11.9).
+    static constexpr int kUncut = HDP == 128 ? 16 : 32;
     static constexpr int kTileBytes = kKeys * HDP;               // one of keys, values
     static constexpr int kStageBytes = 2 * kTileBytes + 16;      // and 2 + 2 scales
     static constexpr int kRing = kStages * kStageBytes;
@@ -190,18 +194,25 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
 
     // This CTA's run [begin, end) of the list.
     int64_t real_tiles = 0, sequences = 0;
+    int longest = 0;
     for (int b = lane; b < c.batch; b += 32) {
         const int n = tiles_of(b);
         real_tiles += n;
+        longest = max(longest, n);
         sequences += n > 0;
     }
     for (int o = 16; o > 0; o >>= 1) {
         real_tiles += __shfl_xor_sync(0xffffffffu, real_tiles, o);
         sequences += __shfl_xor_sync(0xffffffffu, sequences, o);
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
     }
     real_tiles *= items;
     const int64_t total = real_tiles + sequences * items * S::kStart;
-    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max(static_cast<int64_t>(1), real_tiles / (2 * kWarps)));
+    // A CTA an item, or one for each kWarps tiles of long ones, as far as the grid goes.  (One for
+    // each 2 kWarps tiles left 15 items of one tile to one CTA: 65 us, now 6.8.)
+    const int64_t whole = max(static_cast<int64_t>(1), sequences * items);
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x),
+                             longest <= S::kUncut ? whole : whole * max(static_cast<int64_t>(1), quotient(real_tiles, whole * kWarps)));
     if (blockIdx.x >= ctas) return;
     const int64_t share = quotient(total, ctas), spare = total - share * ctas;  // the first `spare` runs are one longer
     auto run_begin = [&](int64_t cta) { return cta * share + min(cta, spare); };
@@ -688,9 +699,10 @@ cudaError_t launch_tiles(const Kv8Attention& a, int sm_count, int aligned, float
     const Kv8& c = a.cache;
     const int vt = tiles_of_vectors(a.rows_per_seq, a.heads, c.kv_heads);
     const int per_sm = 233472 / (S::kSmem + 1152);  // what shared memory holds
-    const int64_t most = static_cast<int64_t>(c.batch) * c.kv_heads * vt * ((c.capacity + kKeys - 1) / kKeys);
+    // A CTA an item, or one for each kWarps tiles.
+    const int64_t items = static_cast<int64_t>(c.batch) * c.kv_heads * vt, most = items * ((c.capacity + kKeys - 1) / kKeys);
     const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count * per_sm, kMostCtas),
-                                                        std::max<int64_t>(1, most / (2 * kWarps))));
+                                                        std::max(items, most / kWarps)));
     return launch_dependent(kernel, dim3(grid), dim3(kWarps * 32), S::kSmem, s, a, vt, aligned, parts, scores, lse);
 }
 }  // namespace
