@@ -48,6 +48,11 @@ __device__ __forceinline__ uint64_t pair(float x, float y) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
     return r;
 }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
 __device__ __forceinline__ float2 unpair(uint64_t p) {
     float2 r;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
@@ -207,7 +212,8 @@ __device__ __forceinline__ int block_prefix(int v, int& all) {
 // counting passes over its digits of 11, 11 and 10 bits (integer counts: any order of
 // the atomics gives the same), then the kept slots go in order into `order` and their
 // weights to the front.  Latency-bound: the weights are read from L1 after the first
-// pass; 16 sequences x 8 heads of 8k slots took 58 us bit by bit.
+// pass.  A head of 6401 slots takes 10.5 us, 3.9 of them the first pass and 3.1 the
+// last; one of 62 slots 6 us.  (Bit by bit, 16 sequences x 8 heads of 8k took 58 us.)
 __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(Kv8 c, int keep, int recent,
                                                                     int32_t* __restrict__ order) {
     dev::pdl_wait();
@@ -252,59 +258,84 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(Kv8 c, int k
     } else {
         bound = 0xffffffffu;  // none; a NaN's key is not above it, and no tie is wanted
     }
-    // `want` is now how many of those equal to the bound are kept, lowest slots first
+    // `want` is now how many of those equal to the bound are kept, lowest slots first.  A warp
+    // has 32 kSelectEach slots of a chunk, a lane every 32nd, so loads and stores run along the
+    // slots; slots kept for certain and ties before a slot are counted together, in halves of a word.
+    const int lane = threadIdx.x % 32, first = threadIdx.x / 32 * (32 * kSelectEach) + lane;
     int kept_before = 0, tied_before = 0;
     for (int base = 0; base < held; base += kSelectThreads * kSelectEach) {
-        const int i0 = base + threadIdx.x * kSelectEach;
         float x[kSelectEach];
-        int tied = 0;
+        uint32_t certain[kSelectEach], tied[kSelectEach];  // the warp's slots
+        int counts = 0;
 #pragma unroll
         for (int j = 0; j < kSelectEach; ++j) {
-            x[j] = i0 + j < held ? w[i0 + j] : 0.0f;
-            tied += i0 + j < candidates && order_key(x[j]) == bound;
+            const int i = base + first + 32 * j;
+            certain[j] = tied[j] = 0;
+            if (i - lane >= held) continue;
+            x[j] = i < held ? w[i] : 0.0f;
+            const uint32_t key = order_key(x[j]);
+            certain[j] = __ballot_sync(0xffffffffu, i < held && (i >= candidates || key > bound));
+            tied[j] = __ballot_sync(0xffffffffu, i < candidates && key == bound);
+            counts += __popc(certain[j]) + (__popc(tied[j]) << 16);
         }
         int all;
-        int rank = tied_before + block_prefix(tied, all);  // (every weight of the chunk has been read)
-        tied_before += all;
-        uint32_t keeps = 0;
+        const int before = block_prefix(lane == 0 ? counts : 0, all);  // (every weight of the chunk has been read)
+        const int warp_before = __shfl_sync(0xffffffffu, before, 0);
+        int sure = kept_before + (warp_before & 0xffff), ties = tied_before + (warp_before >> 16);
 #pragma unroll
         for (int j = 0; j < kSelectEach; ++j) {
-            const int i = i0 + j;
-            if (i >= held) continue;
-            if (i >= candidates) {
-                keeps |= 1u << j;
-            } else {
-                const uint32_t key = order_key(x[j]);
-                if (key > bound || (key == bound && rank < want)) keeps |= 1u << j;
-                rank += key == bound;
+            if ((certain[j] | tied[j]) == 0) continue;
+            const uint32_t below = (1u << lane) - 1;
+            const int rank = ties + __popc(tied[j] & below);
+            if ((certain[j] >> lane & 1) || ((tied[j] >> lane & 1) && rank < want)) {
+                // at most the slot itself: later chunks lose nothing
+                const int place = sure + __popc(certain[j] & below) + min(rank, want);
+                order[place] = base + first + 32 * j;
+                w[place] = x[j];
             }
+            sure += __popc(certain[j]);
+            ties += __popc(tied[j]);
         }
-        int place = kept_before + block_prefix(__popc(keeps), all);
-        kept_before += all;
-#pragma unroll
-        for (int j = 0; j < kSelectEach; ++j)
-            if (keeps >> j & 1) {  // place <= i0 + j: later chunks lose nothing
-                order[place] = i0 + j;
-                w[place++] = x[j];
-            }
-        __syncthreads();
+        kept_before += all & 0xffff;
+        tied_before += all >> 16;
     }
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+// 16 bytes global -> shared, asynchronously; zeros unless `real`.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
 // A warp moves a unit of 64 tokens: lane l has piece l % kPieces (16 codes) of every
 // (32 / kPieces)-th token, all in registers at once.  A cluster of CTAs walks the
 // units of one (head, sequence, key or value) in rounds, a unit to each of its warps:
 // the token that moves to slot i comes from a slot >= i, so what a round overwrites no
-// later round still needs, and a round's own values are in registers at the barrier
-// ahead of its writes.  Bound by memory when there are heads enough; where there are
-// few, a cluster of up to 8 CTAs shares each.
+// later round still needs, and a round's own codes have been read at the barrier ahead
+// of its writes.  For the same reason the next unit's codes may come by asynchronous
+// copies while this one is quantised.  The barrier orders reads before writes only, so
+// its arrival need not wait for this warp's writes.  Where there are few heads, a cluster
+// of up to 8 CTAs shares each.  16 sequences x 8 heads of 128, 4000 of 8k slots kept:
+// 65 us for 262 MB, 4.0 TB/s; 8 operations a code issue over half of the cycles.
+// (Without the copies ahead 84 us, with five CTAs on an SM, whose registers spill, 77.)
 constexpr int kUnit = 64;
 constexpr int kMoveWarps = 4;
 template <int kPieces>
-__global__ void __launch_bounds__(kMoveWarps * 32, 5) kv8_move_kernel(Kv8 c, int keep, const int32_t* __restrict__ order) {
-    constexpr int kTokens = 32 / kPieces, kLoads = kUnit / kTokens, kPer16 = 16 / kTokens;
+struct MoveShape {
+    static constexpr int kTokens = 32 / kPieces, kLoads = kUnit / kTokens, kPer16 = 16 / kTokens;
+    static constexpr int kBuffer = kLoads * 32 * 16;  // bytes of a warp: [load][lane]
+    static constexpr int kSmem = kMoveWarps * kBuffer;
+};
+template <int kPieces>
+__global__ void __launch_bounds__(kMoveWarps * 32, 4) kv8_move_kernel(Kv8 c, int keep, const int32_t* __restrict__ order) {
+    using S = MoveShape<kPieces>;
+    constexpr int kTokens = S::kTokens, kLoads = S::kLoads, kPer16 = S::kPer16;
+    extern __shared__ __align__(16) unsigned char move_smem[];
     __shared__ int from_of[kMoveWarps][kUnit];
-    __shared__ float scale_of[kMoveWarps][kUnit];
+    __shared__ float scale_of[2][kMoveWarps][kUnit];
     dev::pdl_wait();
     dev::pdl_launch_dependents();
     const int b = blockIdx.z >> 1, h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -318,47 +349,71 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 5) kv8_move_kernel(Kv8 c, int
     float* scales = (value ? c.v_scales : c.k_scales) + head * (c.capacity >> shift);
     float* tail = (value ? c.v_tail : c.k_tail) + (head << shift) * d + col;
     const int full = keep >> shift << shift;  // slots of whole blocks
-    int* const from = from_of[warp] + token0;
-    const float* const scale = scale_of[warp] + token0;
-    for (int base = (blockIdx.x * kMoveWarps + warp) * kUnit, left = (keep + kUnit - 1) / kUnit; left > 0;
-         left -= gridDim.x * kMoveWarps, base += gridDim.x * kMoveWarps * kUnit) {
-        __syncwarp();  // the last unit's tokens and scales have been used
+    const uint32_t buffer = dev::smem_u32(move_smem) + warp * S::kBuffer + lane * 16;
+    const int stride = gridDim.x * kMoveWarps * kUnit;
+    int next[2];  // the slots that move to lane and lane + 32 of the unit after
+    auto look = [&](int base) {
 #pragma unroll
-        for (int i = lane; i < kUnit; i += 32) {
-            const int f = base + i < keep ? order[base + i] : -1;
-            from_of[warp][i] = f;
-            scale_of[warp][i] = f >= 0 ? scales[f >> shift] : 0.0f;
+        for (int i = 0; i < 2; ++i) next[i] = base + 32 * i + lane < keep ? order[base + 32 * i + lane] : -1;
+    };
+    // Asynchronous copies of the unit whose slots are in `next`; its scales to half y of scale_of.
+    auto fetch = [&](int y) {
+        __syncwarp();  // the last unit's tokens have been used
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            from_of[warp][32 * i + lane] = next[i];
+            scale_of[y][warp][32 * i + lane] = next[i] >= 0 ? scales[next[i] >> shift] : 0.0f;
         }
         __syncwarp();
-        uint4 r[kLoads];
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int f = from[i * kTokens];
-            r[i] = make_uint4(0, 0, 0, 0);
-            if (f >= 0 && has) r[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(f) * d);
+            const int f = from_of[warp][token0 + i * kTokens];
+            const bool real = f >= 0 && has;
+            copy16(buffer + i * 512, codes + (real ? static_cast<int64_t>(f) * d : 0), real);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // A packed sum, of a product by a one that the assembler does not know: it would join
+    // a packed sum with the product before it, in one rounding.
+    float one = 1.0f;
+    asm volatile("" : "+f"(one));
+    const uint64_t ones = pair(one, one), magic = pair(12582912.0f, 12582912.0f);
+    int base = (blockIdx.x * kMoveWarps + warp) * kUnit, y = 0;
+    look(base);
+    fetch(0);
+    look(base + stride);
+    for (int left = (keep + kUnit - 1) / kUnit; left > 0; left -= gridDim.x * kMoveWarps, base += stride, y ^= 1) {
+        const float* const scale = scale_of[y][warp] + token0;
+        uint4 r[kLoads];
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) r[i] = lds128(buffer + i * 512);
         // the largest value of each 16 tokens: scale x largest code, exactly the largest product
         uint32_t top[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t words[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-            uint32_t most = 0, least = 0x00ff00ffu;  // of code + 128, in two 16-bit lanes
+            uint32_t most = 0, least = 0;  // signed 16-bit lanes; a code is a lane's high byte, what is below it does not matter
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t even = (words[j] & 0x00ff00ffu) ^ 0x00800080u, odd = ((words[j] >> 8) & 0x00ff00ffu) ^ 0x00800080u;
-                most = __vmaxu2(most, __vmaxu2(even, odd));
-                least = __vminu2(least, __vminu2(even, odd));
+                most = __vimax3_s16x2(most, words[j], words[j] << 8);
+                least = __vimin3_s16x2(least, words[j], words[j] << 8);
             }
-            const int hi = max(static_cast<int>(most >> 16), static_cast<int>(most & 0xffffu)) - 128;
-            const int lo = 128 - min(static_cast<int>(least >> 16), static_cast<int>(least & 0xffffu));
+            const int hi = max(static_cast<int>(most) >> 24, static_cast<int8_t>(most >> 8));
+            const int lo = -min(static_cast<int>(least) >> 24, static_cast<int8_t>(least >> 8));
             const float m = static_cast<float>(max(hi, lo));
             top[i / kPer16] = max(top[i / kPer16], magnitude(__fmul_rn(scale[i * kTokens], m)));
+        }
+        if (left > gridDim.x * kMoveWarps) {  // the codes are in registers
+            fetch(y ^ 1);
+            look(base + 2 * stride);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) top[g] = __reduce_max_sync(0xffffffffu, top[g]);
         if (shift >= 5) top[0] = top[1] = max(top[0], top[1]), top[2] = top[3] = max(top[2], top[3]);
         if (shift >= 6) top[0] = top[1] = top[2] = top[3] = max(top[0], top[2]);
-        dev::cluster_sync();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const BlockScale bs = block_scale(top[g]);
@@ -382,9 +437,9 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 5) kv8_move_kernel(Kv8 c, int
                                                   static_cast<float>(static_cast<int8_t>(words[j] >> 8))));
                 const uint64_t x1 = mul2(ss, pair(static_cast<float>(static_cast<int8_t>(words[j] >> 16)),
                                                   static_cast<float>(static_cast<int8_t>(words[j] >> 24))));
-                const float2 y0 = unpair(mul2(x0, ii)), y1 = unpair(mul2(x1, ii));
-                const uint32_t lo = dev::prmt(nearest_bits(y0.x), nearest_bits(y0.y), 0x0040);
-                const uint32_t hi = dev::prmt(nearest_bits(y1.x), nearest_bits(y1.y), 0x0040);
+                const float2 y0 = unpair(fma2(mul2(x0, ii), ones, magic)), y1 = unpair(fma2(mul2(x1, ii), ones, magic));
+                const uint32_t lo = dev::prmt(__float_as_uint(y0.x), __float_as_uint(y0.y), 0x0040);
+                const uint32_t hi = dev::prmt(__float_as_uint(y1.x), __float_as_uint(y1.y), 0x0040);
                 out[j] = dev::prmt(lo, hi, 0x5410);
                 if (slot >= full) {
                     const float2 a = unpair(x0), e = unpair(x1);
@@ -525,6 +580,7 @@ kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int
             cudaLaunchConfig_t lc = {};
             lc.gridDim = dim3(share, cache->kv_heads, 2 * cache->batch);
             lc.blockDim = dim3(kMoveWarps * 32);
+            lc.dynamicSmemBytes = cache->head_dim > 64 ? MoveShape<8>::kSmem : cache->head_dim > 32 ? MoveShape<4>::kSmem : MoveShape<2>::kSmem;
             lc.stream = s;
             cudaLaunchAttribute attr[2];
             attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
