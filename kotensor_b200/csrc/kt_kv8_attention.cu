@@ -19,7 +19,6 @@ namespace kt {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kDims = kKv8MaxHeadDim / 32;  // dims a lane holds in kv8_weights_kernel
 
 // ------------------------------------------------------------ few query rows
 //
@@ -104,6 +103,30 @@ __device__ __forceinline__ void three_bytes(const float (&x)[4], uint32_t& high,
         middle |= static_cast<uint32_t>(m & 255) << (8 * i);
         high |= static_cast<uint32_t>(h & 255) << (8 * i);
     }
+}
+// A thread's part of a query vector (four threads share one) as signed bytes in the
+// layout of the first product; returns what a unit of the whole numbers is worth.
+// Below 2^-100 a query counts as 0; where it is not finite every score is NaN.
+template <int kSteps>
+__device__ __forceinline__ float cut_query(float (&x)[2 * kSteps][4], uint32_t (&qa)[kSteps][6]) {
+    uint32_t top = 0;  // the largest magnitude, by its bits: NaN above infinity
+#pragma unroll
+    for (int s = 0; s < 2 * kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float largest = __uint_as_float(top);
+    const float up = top < 0x0d800000u ? 0.0f : kQueryMax / largest;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[2 * s + i][j] = fminf(fmaxf(x[2 * s + i][j] * up, -kQueryMax), kQueryMax);
+            three_bytes(x[2 * s + i], qa[s][2 * i], qa[s][2 * i + 1], qa[s][4 + i]);
+        }
+    return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : largest / kQueryMax;
 }
 // x0, x1 as their two fp16 terms, packed in pairs.
 __device__ __forceinline__ void two_terms(float x0, float x1, uint32_t& hi, uint32_t& lo) {
@@ -357,28 +380,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
         // Step s of the first product contracts the dims 16 (t + 4 (s / 2)) + 8 (s % 2) .. + 7 of
         // thread t: the words its 16-byte pieces of a key hold.
         uint32_t qa[kSteps][6];  // high, middle of the first four, of the last four; low of both
-        float factor;
-        {
-            uint32_t top = 0;  // the largest magnitude, by its bits: NaN above infinity
-#pragma unroll
-            for (int s = 0; s < 2 * kSteps; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[s][i]) & 0x7fffffffu);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float largest = __uint_as_float(top);
-            // below 2^-100 the query counts as 0; where it is not finite every score is NaN
-            const float up = top < 0x0d800000u ? 0.0f : kQueryMax / largest;
-            factor = a.scale * kLog2e * (top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : largest / kQueryMax);
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[2 * s + i][j] = fminf(fmaxf(x[2 * s + i][j] * up, -kQueryMax), kQueryMax);
-                    three_bytes(x[2 * s + i], qa[s][2 * i], qa[s][2 * i + 1], qa[s][4 + i]);
-                }
-        }
+        const float factor = a.scale * kLog2e * cut_query<kSteps>(x, qa);
         float o[kOwn], m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) o[i] = 0.0f;
@@ -630,33 +632,204 @@ __global__ void __launch_bounds__(256) kv8_add_weights_kernel(Kv8Attention a, co
         if (j + i < n) to[i] += w[i];
 }
 
-// One warp per slot adds up its weight over the rows and heads of its group, in order.
-__global__ void __launch_bounds__(kWarps * 32) kv8_weights_kernel(Kv8Attention a, const float* __restrict__ lse) {
+// The weight of each slot where the rows are many: w_j += sum over rows and heads of
+// 2^(s_j - lse), the scores formed again from the codes, as in the first product above.
+// First every query vector is cut into bytes, once, as the products read them, eight
+// vectors to a tile: kCutWords x 512 bytes and an int4 a vector, {what a unit of its
+// whole numbers is worth, its lse, the slots it sees}.
+template <int HDP>
+constexpr int kCutWords = 6 * HDP / 128;  // 16-byte words of a lane
+size_t cut_bytes(int32_t head_dim) { return (head_dim > 64 ? kCutWords<128> : kCutWords<64>) * 512 + 8 * sizeof(int4); }
+template <int HDP>
+__global__ void __launch_bounds__(kWarps * 32) kv8_cut_kernel(Kv8Attention a, int aligned, const float* __restrict__ lse,
+                                                              uint4* __restrict__ cut, int4* __restrict__ facts) {
+    constexpr int kSteps = HDP / 32;
     dev::pdl_wait();
     dev::pdl_launch_dependents();
     const Kv8& c = a.cache;
-    const int j = blockIdx.x * kWarps + threadIdx.x / 32, h = blockIdx.y, b = blockIdx.z;
-    const int lane = threadIdx.x % 32, d = c.head_dim, group = a.heads / c.kv_heads;
-    const int rows = kv8_rows(a.counts, b, a.rows_per_seq), held = kv8_held(c, b);
-    if (j >= min(held + rows, c.capacity)) return;
-    const int64_t kvh = static_cast<int64_t>(b) * c.kv_heads + h;
-    float k[kDims], sum = 0.0f;
+    const int lane = threadIdx.x % 32, t = lane % 4, n8 = lane / 4, h = blockIdx.y, b = blockIdx.z;
+    const int d = c.head_dim, group = a.heads / c.kv_heads, tiles = (a.rows_per_seq * group + 7) / 8;
+    const int rows = kv8_rows(a.counts, b, a.rows_per_seq), vectors = rows * group;
+    const int tile = blockIdx.x * kWarps + threadIdx.x / 32;
+    if (tile * 8 >= vectors) return;
+    const int v = tile * 8 + n8, row = v / group, of = h * group + v - row * group;
+    const int64_t r = static_cast<int64_t>(b) * a.rows_per_seq + row;
+    const float* q = a.q + r * a.q_stride + static_cast<int64_t>(of) * d;
+    float x[2 * kSteps][4];
 #pragma unroll
-    for (int i = 0; i < kDims; ++i)
-        k[i] = lane + 32 * i < d ? c.k_codes[(kvh * c.capacity + j) * d + lane + 32 * i] : 0.0f;
-    const float ks = c.k_scales[kvh * (c.capacity / c.block) + j / c.block];
-    for (int t = max(0, j - held); t < rows; ++t)
-        for (int g = 0; g < group; ++g) {
-            const int64_t row = static_cast<int64_t>(b) * a.rows_per_seq + t;
-            const int head = h * group + g;
-            float s = 0.0f;
+    for (int s = 0; s < 2 * kSteps; ++s) {
+        const int dim = 16 * (t + 4 * (s / 4)) + 4 * (s % 4);
 #pragma unroll
-            for (int i = 0; i < kDims; ++i)
-                if (lane + 32 * i < d) s = fmaf(a.q[row * a.q_stride + head * d + lane + 32 * i], k[i], s);
-            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            sum += expf(s * ks * a.scale - lse[row * a.heads + head]);
+        for (int i = 0; i < 4; ++i) x[s][i] = 0.0f;
+        if (v < vectors && dim < d) {
+            if (aligned & 1) {
+                const float4 f = *reinterpret_cast<const float4*>(q + dim);
+                x[s][0] = f.x, x[s][1] = f.y, x[s][2] = f.z, x[s][3] = f.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[s][i] = q[dim + i];
+            }
         }
-    if (lane == 0) c.weights[kvh * c.capacity + j] += sum;
+    }
+    uint32_t qa[kSteps][6];
+    const float unit = a.scale * kLog2e * cut_query<kSteps>(x, qa);
+    const int64_t at = (static_cast<int64_t>(b) * c.kv_heads + h) * tiles + tile;
+#pragma unroll
+    for (int i = 0; i < kCutWords<HDP>; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = qa[(4 * i + e) / 6][(4 * i + e) % 6];
+        cut[(at * kCutWords<HDP> + i) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (t == 0) {
+        const int held = kv8_held(c, b);
+        const float less = v < vectors ? lse[r * a.heads + of] * kLog2e : 0.0f;
+        facts[at * 8 + n8] = make_int4(__float_as_int(unit), __float_as_int(less),
+                                       v < vectors ? min(held + row + 1, min(held + rows, c.capacity)) : 0, 0);
+    }
+}
+// A CTA has kWeightSlots slots of one key/value head, 64 to a warp, whose codes stay in
+// registers, and runs over the tiles of vectors that see them, the next one's bytes on
+// their way; a cluster shares the tiles where there are few slots, and its first CTA adds
+// up.  Sums are in a fixed order: equal bits on every run.  Bound by the integer
+// products, 512 clocks of a scheduler's tensor core for 512 scores, which are under way
+// in 63% of the cycles: 2 sequences x 509 rows x 32 heads over 3500 slots of 128 dims
+// 171 us, 6000 rows over themselves 1.2 ms.  (A warp to a slot on the fp32 units took 30
+// times as long; queries cut again by each CTA 486 us; three CTAs on an SM, whose
+// registers spill, 189; two or eight n-tiles together 180.)
+constexpr int kWeightSlots = 64 * kWarps;
+template <int HDP>
+__global__ void __launch_bounds__(kWarps * 32, 2) kv8_weights_kernel(Kv8Attention a, const uint4* __restrict__ cut,
+                                                                     const int4* __restrict__ facts, int splits) {
+    constexpr int kSteps = HDP / 32, kPieces = HDP / 64, kTogether = 4;  // n-tiles whose products do not wait for one another
+    __shared__ float sums[kWeightSlots];
+    dev::pdl_wait();
+    dev::pdl_launch_dependents();
+    const Kv8& c = a.cache;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = lane % 4, n8 = lane / 4;
+    const int split = blockIdx.x % splits, h = blockIdx.y, b = blockIdx.z;  // (`splits` CTAs are a cluster)
+    const int d = c.head_dim, group = a.heads / c.kv_heads, tiles = (a.rows_per_seq * group + 7) / 8;
+    const int rows = kv8_rows(a.counts, b, a.rows_per_seq), held = kv8_held(c, b);
+    const int seen = rows == 0 ? 0 : min(held + rows, c.capacity);
+    const int block_first = static_cast<int>(blockIdx.x / splits) * kWeightSlots, first = block_first + 64 * warp;
+    if (block_first >= seen) return;  // as the whole cluster does
+    const int64_t head = static_cast<int64_t>(b) * c.kv_heads + h;
+    const int8_t* codes = c.k_codes + head * c.capacity * d;
+    uint4 k[8][kPieces];
+    float ks[4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+            const int slot = first + 8 * j + n8, dim = 16 * (t + 4 * u);
+            k[j][u] = make_uint4(0, 0, 0, 0);
+            if (slot < seen && dim < d) k[j][u] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(slot) * d + dim);
+        }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        ks[j] = first + 16 * j < seen ? c.k_scales[head * (c.capacity / c.block) + (first + 16 * j) / c.block] : 0.0f;
+
+    // vector v belongs to row v / group; the first that sees a slot of the CTA
+    const int end = (rows * group + 7) / 8;
+    int tile = max(0, block_first - held) * group / 8 + split;
+    cut += head * tiles * kCutWords<HDP> * 32 + lane;
+    facts += head * tiles * 8 + n8;
+    uint4 next[kCutWords<HDP>];
+    int4 next_facts = make_int4(0, 0, 0, 0);
+    auto load = [&](int x) {
+#pragma unroll
+        for (int i = 0; i < kCutWords<HDP>; ++i) next[i] = cut[(static_cast<int64_t>(x) * kCutWords<HDP> + i) * 32];
+        next_facts = facts[static_cast<int64_t>(x) * 8];
+    };
+    float sum[8][2] = {};
+    if (tile < end) load(tile);
+#pragma unroll 1
+    for (; tile < end; tile += splits) {
+        uint32_t qa[kSteps][6];
+#pragma unroll
+        for (int i = 0; i < kCutWords<HDP>; ++i) {
+            const uint32_t words[4] = {next[i].x, next[i].y, next[i].z, next[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qa[(4 * i + e) / 6][(4 * i + e) % 6] = words[e];
+        }
+        const float unit = __int_as_float(next_facts.x), less = __int_as_float(next_facts.y);
+        const int limit = next_facts.z;
+        if (tile + splits < end) load(tile + splits);
+        const bool part = __any_sync(0xffffffffu, limit < first + 64);  // some vector does not see all of the slots
+#pragma unroll
+        for (int j0 = 0; j0 < 8; j0 += kTogether) {
+            int upper[kTogether][4] = {}, lower[kTogether][4] = {};
+#pragma unroll
+            for (int u = 0; u < 2 * kPieces; ++u)
+#pragma unroll
+                for (int j = 0; j < kTogether; ++j) {
+                    const uint32_t* const q = qa[u];
+                    const uint4 w4 = k[j0 + j][u / 2];
+                    mma(upper[j], q[0], q[1], q[2], q[3], u % 2 ? w4.z : w4.x, u % 2 ? w4.w : w4.y);
+                    mma(lower[j], q[4], 0, q[5], 0, u % 2 ? w4.z : w4.x, u % 2 ? w4.w : w4.y);
+                }
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) {
+                const float by = ks[(j0 + j) / 2] * unit;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float dot = fmaf(static_cast<float>(upper[j][i]), 65536.0f,
+                                           static_cast<float>(upper[j][2 + i] * 256 + lower[j][i]));
+                    float p = ex2(dot * by - less);
+                    if (part && first + 8 * (j0 + j) + 2 * t + i >= limit) p = 0.0f;
+                    sum[j0 + j][i] += p;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            for (int o = 4; o < 32; o <<= 1) sum[j][i] += __shfl_xor_sync(0xffffffffu, sum[j][i], o);
+            if (n8 == 0) sums[64 * warp + 8 * j + 2 * t + i] = sum[j][i];
+        }
+    dev::cluster_sync();
+    if (split == 0)
+        for (int i = threadIdx.x; i < min(kWeightSlots, seen - block_first); i += kWarps * 32) {
+            float all = 0.0f;
+            for (int x = 0; x < splits; ++x) {
+                uint32_t at;
+                float f;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(dev::smem_u32(sums + i)), "r"(x));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at));
+                all += f;
+            }
+            c.weights[head * c.capacity + block_first + i] += all;
+        }
+    dev::cluster_sync();  // nobody leaves while its sums are read
+}
+
+template <int HDP>
+cudaError_t launch_weights(const Kv8Attention& a, int sm_count, int aligned, const float* lse, void* room, cudaStream_t s) {
+    const Kv8& c = a.cache;
+    const int tiles = (a.rows_per_seq * (a.heads / c.kv_heads) + 7) / 8;
+    int4* facts = static_cast<int4*>(room);
+    uint4* cut = reinterpret_cast<uint4*>(facts + static_cast<int64_t>(c.batch) * c.kv_heads * tiles * 8);
+    cudaError_t e = launch_dependent(kv8_cut_kernel<HDP>, dim3((tiles + kWarps - 1) / kWarps, c.kv_heads, c.batch),
+                                     dim3(kWarps * 32), 0, s, a, aligned, lse, cut, facts);
+    if (e != cudaSuccess) return e;
+    const int64_t blocks = (c.capacity + kWeightSlots - 1) / kWeightSlots, alone = blocks * c.kv_heads * c.batch;
+    int splits = 1;  // while SMs lack a second CTA and there are tiles for more
+    while (splits < 8 && alone * splits < 2 * sm_count && splits * 8 < tiles) splits *= 2;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(static_cast<unsigned>(blocks * splits), c.kv_heads, c.batch);
+    lc.blockDim = dim3(kWarps * 32);
+    lc.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 2;
+    return cudaLaunchKernelEx(&lc, kv8_weights_kernel<HDP>, a, static_cast<const uint4*>(cut), static_cast<const int4*>(facts), splits);
 }
 
 }  // namespace
@@ -712,6 +885,8 @@ size_t kv8_attention_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, i
     size_t n = std::max(part_bytes(head_dim), round256(kv8_prompt_bytes(head_dim))) + lse_bytes(batch, rows_per_seq, heads);
     if (weights && use_tiles(batch, rows_per_seq, heads, kv_heads))
         n += static_cast<size_t>(batch) * rows_per_seq * heads * capacity * sizeof(float);
+    else if (weights)
+        n += static_cast<size_t>(batch) * kv_heads * tiles_of_vectors(rows_per_seq, heads, kv_heads) * cut_bytes(head_dim);
     return n;
 }
 
@@ -737,9 +912,11 @@ cudaError_t launch_kv8_attention(const Kv8Attention& a, int sm_count, int32_t* e
         return e;
     }
     cudaError_t e = launch_kv8_prompt(a, aligned, parts, a.accumulate ? lse : nullptr, err, s);
-    if (e == cudaSuccess && a.accumulate)
-        e = launch_dependent(kv8_weights_kernel, dim3((c.capacity + kWarps - 1) / kWarps, c.kv_heads, c.batch),
-                             dim3(kWarps * 32), 0, s, a, static_cast<const float*>(lse));
+    if (e == cudaSuccess && a.accumulate) {
+        void* room = free + lse_at + lse_bytes(c.batch, a.rows_per_seq, a.heads);
+        e = c.head_dim > 64 ? launch_weights<128>(a, sm_count, aligned, lse, room, s)
+                            : launch_weights<64>(a, sm_count, aligned, lse, room, s);
+    }
     return e;
 }
 

@@ -226,6 +226,28 @@ def test_attention_of_several_rows(kt, b, heads, h, d, block, lengths, rows):
     attention_case(kt, b, heads, h, d, block, lengths, rows, seed=rows)
 
 
+@pytest.mark.parametrize("b,heads,h,d,block,lengths,rows", [
+    (2, 28, 4, 80, 16, [700, 3], 150),            # a group of 7, slots of several CTAs, vectors shared by a cluster
+    (1, 7, 1, 128, 64, [20], 600),                # slots that only later rows see
+    (1, 16, 16, 48, 32, [300], 140),
+])
+def test_weights_of_many_rows(kt, b, heads, h, d, block, lengths, rows):
+    """Weights of prompts, twice with equal bits, and from queries at any address."""
+    cache, ref = attention_case(kt, b, heads, h, d, block, lengths, rows, seed=d)
+    room = torch.randn(b * rows * (heads * d + 3) + 1, device="cuda")
+    shifted = room[1:].reshape(b * rows, heads * d + 3)[:, :heads * d]
+    results = []
+    for q in (shifted, shifted.contiguous(), shifted):
+        cache.weights.zero_()
+        context = cache.attend(0, q, heads, rows, accumulate=True)
+        results.append((context, cache.weights.clone()))
+    for context, weights in results[1:]:
+        assert torch.equal(context, results[0][0]) and torch.equal(weights, results[0][1])
+    # every row hands out one unit of weight per query head; each exponential's relative error is below 2^-16
+    given = results[0][1].double().sum() / (b * rows * heads)
+    assert abs(float(given) - 1.0) < 2.0 ** -16
+
+
 @pytest.mark.parametrize("rows", [1, 5, 20, 70])
 def test_attention_counts(kt, rows):
     """Rows past counts[b] give zeros and no weights; a sequence may have none at all."""
