@@ -484,8 +484,9 @@ size_t kt_kv8_scratch_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, 
  * into context_dev [batch * rows_per_seq][heads * head_dim].  Rows t >= counts[b]
  * give zeros and no weights.  accumulate_weights != 0 adds the attention weights
  * of the rows to cache->weights.  Products and sums are fp32 class: the codes are
- * exact in the tensor cores' fp16, queries and probabilities enter as two fp16
- * terms each. */
+ * exact in the tensor cores' integers and fp16, a query enters as three signed bytes
+ * (24 bits relative to its largest component; few rows) or two fp16 terms (many
+ * rows), a probability as two fp16 terms. */
 kt_status kt_kv8_attention(kt_ctx* ctx, const kt_kv8_cache* cache, const float* q_dev, int64_t q_stride,
                            float* context_dev, int32_t rows_per_seq, const int32_t* counts_dev, int32_t heads,
                            float scale, int32_t accumulate_weights, void* scratch_dev, void* stream);

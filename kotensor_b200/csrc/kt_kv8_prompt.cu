@@ -31,6 +31,12 @@
 // carry the values' scales, which may differ by any factor from block to block, so
 // they have a reference R of their own, the maximum of score + log2(value scale):
 // both terms of P keep 22 bits of what matters to O.
+//
+// Bound by turns by the products and by the exponentials with the cut of P into terms: a
+// tile takes about 3700 clocks, its products 2048.  2 sequences x 509 rows x 32 heads
+// of 128 over 1500 to 3508 slots: 102 us, 37.6 GFLOP as fp32 counts them, 369 TFLOP/s, or
+// 740 with both terms.  (Sixteen softmax warps and two issuing ones 112 us where these
+// took 109.)  A CTA spends about 7 us on entering and 3 on leaving.
 #include <cuda_fp16.h>
 
 #include <algorithm>
