@@ -36,8 +36,8 @@ constexpr int kWarps = 4;
 // arrive, in the order of the cuts: equal bits on every run.
 // Bound by memory at full batches, 64 sequences of 16k slots, 8 heads of 128: 445 us for
 // 2.09 GB, 4.7 TB/s; one of 120001 slots 64 us, 3.9 TB/s; by latency when short: 301 slots of
-// 2 heads of 64 6.7 us.  (Queries as two fp16 terms, which need the keys' codes converted:
-// 507, 75 and 12 us.)
+// 2 heads of 64 6.7 us.  (With queries as two fp16 terms, which need the keys' codes
+// converted, and one CTA of eight warps an SM: 507, 75 and 12 us.)
 
 constexpr int kKeys = 32;
 constexpr int kVectors = 8;

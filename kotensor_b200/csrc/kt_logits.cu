@@ -13,8 +13,9 @@
 // among equal values.
 // 256 rows of 151936: 50 us (6.3 TB/s) with nothing on, 51 with a mask, 63 with penalties
 // over 1025 tokens, 59 with 300 biases, 103 with all: then a CTA's three phases over
-// the lists, not memory, are what its SM waits for.  (Slices of 4096 to 16384 ids, 256 to
-// 1024 threads: 91 to 107 with all, and slower without.)  One row 6.5 us.
+// the lists, not memory, are what its SM waits for.  (256 threads to a CTA, slices of 4096
+// ids: 120 to 126 with all, 48 to 61 with nothing; the touched logits computed by a
+// phase of their own, once each: 105 with all, 68 with penalties.)  One row 6.5 us.
 #include "kt_kv8.h"
 
 namespace kt {
