@@ -491,7 +491,10 @@ kt_status kt_kv8_attention(kt_ctx* ctx, const kt_kv8_cache* cache, const float* 
                            float* context_dev, int32_t rows_per_seq, const int32_t* counts_dev, int32_t heads,
                            float scale, int32_t accumulate_weights, void* scratch_dev, void* stream);
 
-/* lengths_dev[b] = min(lengths_dev[b] + (counts_dev ? counts_dev[b] : rows), limit). */
+/* Moves on by what kt_kv8_store of the same rows and counts added:
+ * lengths_dev[b] = min(lengths_dev[b] + n, limit), not below 0, with n = rows, or with
+ * counts_dev min(max(counts_dev[b], 0), rows).  A negative `rows` takes tokens back, which
+ * leaves a cache that can be stored to only within the open block. */
 kt_status kt_kv8_advance(kt_ctx* ctx, int32_t* lengths_dev, int32_t batch, int32_t rows, const int32_t* counts_dev,
                          int32_t limit, void* stream);
 

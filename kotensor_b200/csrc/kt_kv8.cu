@@ -172,8 +172,11 @@ __global__ void kv8_advance_kernel(int32_t* __restrict__ lengths, int batch, int
                                    const int32_t* __restrict__ counts, int limit) {
     dev::pdl_wait();
     dev::pdl_launch_dependents();
-    for (int b = threadIdx.x; b < batch; b += blockDim.x)
-        lengths[b] = min(lengths[b] + (counts == nullptr ? rows : counts[b]), limit);
+    for (int b = threadIdx.x; b < batch; b += blockDim.x) {
+        // what the store of these rows added
+        const int64_t to = static_cast<int64_t>(lengths[b]) + kv8_rows(counts, b, rows);
+        lengths[b] = static_cast<int32_t>(min(max(to, static_cast<int64_t>(0)), static_cast<int64_t>(limit)));
+    }
 }
 
 // ------------------------------------------------------------ eviction
@@ -548,7 +551,7 @@ kt_status kt_kv8_attention(kt_ctx* ctx, const kt_kv8_cache* cache, const float* 
 kt_status kt_kv8_advance(kt_ctx* ctx, int32_t* lengths, int32_t batch, int32_t rows, const int32_t* counts,
                          int32_t limit, void* stream) {
     if (!ctx || !lengths) return entry_fail(KT_ERR_INVALID_ARGUMENT, "NULL argument");
-    if (batch < 1 || limit < 0) return entry_fail(KT_ERR_INVALID_ARGUMENT, "bad advance arguments");
+    if (batch < 1 || limit < 0 || (counts && rows < 0)) return entry_fail(KT_ERR_INVALID_ARGUMENT, "bad advance arguments");
     return c_entry(ctx, [&] {
         return entry_launch(launch_dependent(kv8_advance_kernel, dim3(1), dim3(256), 0,
                                              static_cast<cudaStream_t>(stream), lengths, batch, rows, counts, limit),

@@ -162,8 +162,12 @@ class KVCache8:
                                    scratch, raw_stream(self.ctx.device)))
         return out
 
-    def advance(self, rows: int = 1, counts=None, limit: Optional[int] = None) -> None:
-        """lengths[b] += rows (or counts[b]), at most ``limit`` (the capacity unless given)."""
+    def advance(self, rows: Optional[int] = None, counts=None, limit: Optional[int] = None) -> None:
+        """lengths[b] += what ``store`` of the same ``rows`` (1 unless given) and ``counts`` added:
+        rows, or counts[b] between 0 and rows (the capacity unless given); at most ``limit``
+        (the capacity unless given)."""
+        if rows is None:
+            rows = 1 if counts is None else self.capacity
         _lib.check(self._lib.kt_kv8_advance(self.ctx.handle, self.lengths.data_ptr(), self.batch, rows,
                                             self._counts(counts), self.capacity if limit is None else limit,
                                             raw_stream(self.ctx.device)))

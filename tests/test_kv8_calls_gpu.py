@@ -1,0 +1,54 @@
+"""Calls of the 8-bit key/value cache one after another: lengths that follow the
+counts of a store."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+
+def cuda(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+def test_advance_takes_counts_as_the_store_does(kt):
+    """Counts above the rows and below zero: lengths move by the tokens that were stored, over several calls, so
+    what is attended to is what the oracle holds (tolerance of the attention: test_kv8_gpu.py)."""
+    from test_kv8_gpu import assert_same, make
+    b, h, d, heads, rows = 4, 2, 64, 8, 7
+    cache, ref, rng = make(kt, b, h, d, 128, 16, [0, 10, 33, 60])
+    for counts in ([40, -2, 3, 0], [7, 8, -100, 2 ** 31 - 1], [-2 ** 31, 5, 7, 6]):
+        k, v = (rng.standard_normal((b * rows, h * d), dtype=np.float32) for _ in range(2))
+        dev = torch.tensor(counts, dtype=torch.int32, device="cuda")
+        cache.store(0, cuda(k), cuda(v), rows, counts=dev)
+        assert not ref.store(k, v, rows, counts)
+        q = rng.standard_normal((b * rows, heads * d), dtype=np.float32)
+        got = cache.attend(0, cuda(q), heads, rows, counts=dev).cpu().numpy()
+        want, _, size, top = ref.attend(q, heads, rows, d ** -0.5, counts)
+        assert np.abs(got - want).max() <= (4 * d ** 0.5 * 2.0 ** -24 * size + 2.0 ** -20) * top
+        cache.advance(rows, counts=dev)
+        ref.lengths += np.clip(counts, 0, rows).astype(np.int32)
+        assert cache.lengths.tolist() == ref.lengths.tolist()
+        assert_same(cache, ref)
+
+
+def test_advance_stays_between_zero_and_its_limit(kt):
+    from kotensor_b200.kv8 import KVCache8
+    cache = KVCache8(1, 4, 1, 16, 64, 16)
+    cache.lengths.copy_(torch.tensor([0, 5, 60, 64], dtype=torch.int32))
+    cache.advance(10)
+    assert cache.lengths.tolist() == [10, 15, 64, 64]
+    cache.advance(counts=torch.tensor([3, 70, -4, 1], dtype=torch.int32, device="cuda"))  # rows not given: as counted
+    assert cache.lengths.tolist() == [13, 64, 64, 64]
+    cache.advance(0, counts=torch.tensor([3, 3, 3, 3], dtype=torch.int32, device="cuda"))
+    assert cache.lengths.tolist() == [13, 64, 64, 64]
+    cache.advance(0, limit=20)
+    assert cache.lengths.tolist() == [13, 20, 20, 20]
+    cache.advance(2 ** 31 - 1)
+    assert cache.lengths.tolist() == [64] * 4
+    cache.lengths.fill_(5)
+    cache.advance(-9)
+    assert cache.lengths.tolist() == [0] * 4
+    with pytest.raises(ValueError):
+        cache.advance(-1, counts=torch.ones(4, dtype=torch.int32, device="cuda"))
