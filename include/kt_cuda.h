@@ -518,8 +518,9 @@ kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int
  *   y = y + value for every bias entry (i, value), in list order
  *   y = -inf                                       if bit i of the row's mask is 0
  * and next_token[row] = kt_argmax of the row.  Every pointer but logits and out may
- * be NULL (tokens needs lengths; the penalties need tokens).  Token and bias ids
- * outside 0..vocab-1 are ignored. */
+ * be NULL (tokens needs lengths; the penalties need lengths and tokens, which may be
+ * NULL only where token_width is 0).  Token and bias ids outside 0..vocab-1 are
+ * ignored. */
 typedef struct {
     const float* logits;           /* [rows][vocab], rows logits_stride floats apart */
     float* out;                    /* the same shape, out_stride apart; may be `logits` itself */

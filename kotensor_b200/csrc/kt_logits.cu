@@ -293,7 +293,8 @@ kt_status kt_logits_process(kt_ctx* ctx, const kt_logits_args* args, void* strea
     if (!a.logits || !a.out) return entry_fail(KT_ERR_INVALID_ARGUMENT, "NULL argument");
     if (a.logits_stride < a.vocab || a.out_stride < a.vocab)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "rows of the logits are shorter than vocab");
-    if (a.tokens ? !a.lengths : (a.repetition || a.frequency || a.presence))
+    const bool penalties = a.repetition || a.frequency || a.presence;
+    if (((a.tokens || penalties) && !a.lengths) || (penalties && !a.tokens && a.token_width != 0))  // (a list of width 0 may have no address)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "penalties need tokens and their lengths");
     if (!a.bias_ids != !a.bias_values)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "bias ids and values come together");
