@@ -30,13 +30,18 @@ def _one(name: str, x, rows: int, dtype):
     return x.data_ptr()
 
 
+def _stride(x):
+    """Elements from row to row; where there is one row its stride says nothing."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
 def _list(name: str, x, rows: int, dtype, least: int = 0):
     """Pointer, row stride and width of a device array [rows, at least `least`] with contiguous rows."""
     if x.dtype is not dtype or not x.is_cuda or x.dim() != 2 or x.shape[0] != rows or x.shape[1] < least or \
             (x.stride(1) != 1 and x.shape[1] > 1):
         raise ValueError(f"{name} must be a CUDA tensor of {str(dtype).replace('torch.', '')}, [{rows}, at least {least}] with "
                          f"contiguous rows, got {str(x.dtype).replace('torch.', '')} {list(x.shape)}")
-    return x.data_ptr(), x.stride(0), x.shape[1]
+    return x.data_ptr(), _stride(x), x.shape[1]
 
 
 class LogitsProcessor:
@@ -94,17 +99,17 @@ class LogitsProcessor:
         if (bias_ids is None) != (bias_values is None):
             raise ValueError("bias_ids and bias_values come together")
         if bias_ids is not None:
-            if bias_ids.shape != bias_values.shape or bias_ids.stride() != bias_values.stride():
-                raise ValueError("bias_ids and bias_values must have the same shape and strides")
             bias_p, bias_stride, bias_width = _list("bias_ids", bias_ids, rows, i32)
-            value_p = _list("bias_values", bias_values, rows, f32)[0]
+            value_p, *same = _list("bias_values", bias_values, rows, f32)
+            if same != [bias_stride, bias_width]:
+                raise ValueError("bias_ids and bias_values must have the same shape and strides")
             count_p = _one("bias_counts", bias_counts, rows, i32)
         if allowed is not None:
             allowed_p, allowed_stride, _ = _list("allowed", allowed, rows, i32, (vocab + 31) // 32)
         if next_token is None:
             next_token = self.next_token
         # kt_logits_args, field by field (a ctypes structure takes twice as long to fill)
-        _PACK.pack_into(self._args, 0, logits.data_ptr(), out.data_ptr(), logits.stride(0), out.stride(0), rows, vocab,
+        _PACK.pack_into(self._args, 0, logits.data_ptr(), out.data_ptr(), _stride(logits), _stride(out), rows, vocab,
                         token_p, lengths_p, prompt_p, token_stride, token_width, repetition_p, frequency_p, presence_p,
                         bias_width, bias_p, value_p, count_p, bias_stride, allowed_p, allowed_stride,
                         _one("next_token", next_token, rows, i32), self._scratch_ptr)

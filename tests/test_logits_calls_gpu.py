@@ -1,5 +1,5 @@
-"""kt_logits_process with lists that are empty: the same steps as with nothing in them
-(oracle/kv8_oracle.py)."""
+"""kt_logits_process with lists that are empty and with single rows of any stride:
+the same steps as with nothing in them (oracle/kv8_oracle.py)."""
 import numpy as np
 import pytest
 
@@ -42,3 +42,17 @@ def test_an_empty_history_at_the_c_entry(kt):
     assert lib.kt_logits_process(h, ctypes.byref(a), stream) == 1
     a.token_width, a.lengths = 0, None
     assert lib.kt_logits_process(h, ctypes.byref(a), stream) == 1
+
+
+def test_one_row_of_any_stride(kt):
+    """The stride between rows means nothing where there is one row: a column seen as a row."""
+    from test_logits_gpu import case, check
+    from kotensor_b200.logits import LogitsProcessor
+    a = case(1, 5000, 20, 3, True, seed=1)
+    dev = {k: torch.from_numpy(v).cuda() for k, v in a.items()}
+    for name in ("logits", "tokens", "bias_ids", "allowed"):
+        dev[name] = dev[name].reshape(-1, 1).t()
+        assert dev[name].stride() == (1, 1)
+    out = torch.empty(5000, 1, device="cuda").t()
+    token = LogitsProcessor(1, 5000)(out=out, **dev)
+    check(a, out, token)
