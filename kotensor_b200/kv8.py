@@ -26,12 +26,12 @@ except ImportError:  # pragma: no cover
     torch = None
 
 
-def _rows(name: str, x, rows: int, width: int):
+def _rows(name: str, x, rows: int, width: int, device: int):
     """Pointer and row stride of float32 rows on the device (rows may lie apart, as
     in a fused q|k|v projection)."""
-    if x.dtype is not torch.float32 or not x.is_cuda or x.shape != (rows, width):
-        raise ValueError(f"{name} must be a float32 CUDA tensor of shape [{rows}, {width}], got "
-                         f"{str(x.dtype).replace('torch.', '')} {list(x.shape)}")
+    if x.dtype is not torch.float32 or x.get_device() != device or x.shape != (rows, width):
+        raise ValueError(f"{name} must be a float32 tensor of shape [{rows}, {width}] on cuda:{device}, got "
+                         f"{str(x.dtype).replace('torch.', '')} {list(x.shape)} on {x.device}")
     stride, column = x.stride()
     if column != 1 or (rows > 1 and stride < width):
         raise ValueError(f"{name} must have contiguous rows that do not overlap")
@@ -118,8 +118,9 @@ class KVCache8:
     def _counts(self, counts):
         if counts is None:
             return None
-        if not counts.is_cuda or counts.dtype != torch.int32 or counts.shape != (self.batch,) or not counts.is_contiguous():
-            raise ValueError(f"counts must be a contiguous int32 CUDA tensor of {self.batch} elements")
+        if counts.get_device() != self.ctx.device or counts.dtype != torch.int32 or counts.shape != (self.batch,) or \
+                not counts.is_contiguous():
+            raise ValueError(f"counts must be a contiguous int32 tensor of {self.batch} elements on {self.device}")
         return counts.data_ptr()
 
     def _scratch_of(self, rows_per_seq: int, heads: int):
@@ -139,8 +140,8 @@ class KVCache8:
         [batch]): only the first counts[b] rows of a sequence are tokens.  Tokens past
         the capacity are dropped and set ``status``."""
         rows, width = self.batch * rows_per_seq, self.kv_heads * self.head_dim
-        kp, ks = _rows("k", k, rows, width)
-        vp, vs = _rows("v", v, rows, width)
+        kp, ks = _rows("k", k, rows, width, self.ctx.device)
+        vp, vs = _rows("v", v, rows, width, self.ctx.device)
         _lib.check(self._store(self.ctx.handle, self._cache(layer), kp, vp, ks, vs, rows_per_seq, self._counts(counts),
                                self._status, raw_stream(self.ctx.device)))
 
@@ -151,11 +152,12 @@ class KVCache8:
         heads * head_dim]; ``scale`` is 1 / sqrt(head_dim) unless given.
         ``accumulate`` adds the attention weights to ``weights``."""
         rows, width = self.batch * rows_per_seq, heads * self.head_dim
-        qp, qs = _rows("q", q, rows, width)
+        qp, qs = _rows("q", q, rows, width, self.ctx.device)
         if out is None:
             out = q.new_empty((rows, width))
-        elif not out.is_cuda or out.dtype != torch.float32 or tuple(out.shape) != (rows, width) or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous float32 CUDA tensor of shape [{rows}, {width}]")
+        elif out.get_device() != self.ctx.device or out.dtype != torch.float32 or tuple(out.shape) != (rows, width) or \
+                not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous float32 tensor of shape [{rows}, {width}] on {self.device}")
         scratch = self._scratch_of(rows_per_seq, heads) if rows_per_seq > 0 and heads > 0 else None
         _lib.check(self._attention(self.ctx.handle, self._cache(layer), qp, qs, out.data_ptr(), rows_per_seq,
                                    self._counts(counts), heads, self._scale if scale is None else scale, accumulate,

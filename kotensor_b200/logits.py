@@ -20,28 +20,25 @@ _PACK = struct.Struct("@PPqqiiPPPqiPPPiPPPqPqPP")
 assert _PACK.size == ctypes.sizeof(_lib.KtLogitsArgs)
 
 
-def _one(name: str, x, rows: int, dtype):
+def _one(name: str, x, rows: int, dtype, device: int):
     """Pointer of a device array with one element for each row."""
     if x is None:
         return 0
-    if x.dtype is not dtype or not x.is_cuda or x.dim() != 1 or x.numel() != rows or not x.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous CUDA tensor of {rows} {str(dtype).replace('torch.', '')}, got "
-                         f"{str(x.dtype).replace('torch.', '')} {list(x.shape)}")
+    if x.dtype is not dtype or x.get_device() != device or x.dim() != 1 or x.numel() != rows or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of {rows} {str(dtype).replace('torch.', '')} on cuda:{device}, got "
+                         f"{str(x.dtype).replace('torch.', '')} {list(x.shape)} on {x.device}")
     return x.data_ptr()
 
 
-def _stride(x):
-    """Elements from row to row; where there is one row its stride says nothing."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
-
-
-def _list(name: str, x, rows: int, dtype, least: int = 0):
-    """Pointer, row stride and width of a device array [rows, at least `least`] with contiguous rows."""
-    if x.dtype is not dtype or not x.is_cuda or x.dim() != 2 or x.shape[0] != rows or x.shape[1] < least or \
+def _list(name: str, x, rows: int, dtype, device: int, least: int = 0):
+    """Pointer, row stride and width of a device array [rows, at least `least`] with contiguous rows
+    (the stride of a single row says nothing: its width)."""
+    if x.dtype is not dtype or x.get_device() != device or x.dim() != 2 or x.shape[0] != rows or x.shape[1] < least or \
             (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ValueError(f"{name} must be a CUDA tensor of {str(dtype).replace('torch.', '')}, [{rows}, at least {least}] with "
-                         f"contiguous rows, got {str(x.dtype).replace('torch.', '')} {list(x.shape)}")
-    return x.data_ptr(), _stride(x), x.shape[1]
+        raise ValueError(f"{name} must be a tensor of {str(dtype).replace('torch.', '')}, [{rows}, at least {least}] with "
+                         f"contiguous rows, on cuda:{device}, got {str(x.dtype).replace('torch.', '')} {list(x.shape)} on {x.device}")
+    width = x.shape[1]
+    return x.data_ptr(), x.stride(0) if rows > 1 else width, width
 
 
 class LogitsProcessor:
@@ -75,43 +72,45 @@ class LogitsProcessor:
         first bias_counts[row] count; ``allowed`` int32 words.  Writes ``out`` (the logits
         themselves unless given) and returns the greedy choice of each row: ``next_token``
         (int32 [rows]), or a buffer of this object that its next call overwrites."""
-        rows, vocab = self.rows, self.vocab
+        rows, vocab, device = self.rows, self.vocab, self.ctx.device
         f32, i32 = torch.float32, torch.int32
         token_p = lengths_p = prompt_p = repetition_p = frequency_p = presence_p = 0
         token_stride = token_width = bias_p = value_p = count_p = bias_stride = bias_width = allowed_p = allowed_stride = 0
         for name, x in (("logits", logits), ("out", out)):
-            if x is not None and (x.dtype is not f32 or not x.is_cuda or x.shape != (rows, vocab) or
+            if x is not None and (x.dtype is not f32 or x.get_device() != device or x.shape != (rows, vocab) or
                                   (x.stride(1) != 1 and vocab > 1)):
-                raise ValueError(f"{name} must be a float32 CUDA tensor of shape [{rows}, {vocab}] with contiguous rows")
+                raise ValueError(f"{name} must be a float32 tensor of shape [{rows}, {vocab}] with contiguous rows on "
+                                 f"cuda:{device}")
         if out is None:
             out = logits
         if tokens is not None:
             if lengths is None:
                 raise ValueError("tokens need lengths")
-            token_p, token_stride, token_width = _list("tokens", tokens, rows, i32)
-            lengths_p = _one("lengths", lengths, rows, i32)
-            prompt_p = _one("prompt_lengths", prompt_lengths, rows, i32)
-            repetition_p = _one("repetition", repetition, rows, f32)
-            frequency_p = _one("frequency", frequency, rows, f32)
-            presence_p = _one("presence", presence, rows, f32)
+            token_p, token_stride, token_width = _list("tokens", tokens, rows, i32, device)
+            lengths_p = _one("lengths", lengths, rows, i32, device)
+            prompt_p = _one("prompt_lengths", prompt_lengths, rows, i32, device)
+            repetition_p = _one("repetition", repetition, rows, f32, device)
+            frequency_p = _one("frequency", frequency, rows, f32, device)
+            presence_p = _one("presence", presence, rows, f32, device)
         elif not (repetition is None and frequency is None and presence is None):
             raise ValueError("penalties need tokens")
         if (bias_ids is None) != (bias_values is None):
             raise ValueError("bias_ids and bias_values come together")
         if bias_ids is not None:
-            bias_p, bias_stride, bias_width = _list("bias_ids", bias_ids, rows, i32)
-            value_p, *same = _list("bias_values", bias_values, rows, f32)
+            bias_p, bias_stride, bias_width = _list("bias_ids", bias_ids, rows, i32, device)
+            value_p, *same = _list("bias_values", bias_values, rows, f32, device)
             if same != [bias_stride, bias_width]:
                 raise ValueError("bias_ids and bias_values must have the same shape and strides")
-            count_p = _one("bias_counts", bias_counts, rows, i32)
+            count_p = _one("bias_counts", bias_counts, rows, i32, device)
         if allowed is not None:
-            allowed_p, allowed_stride, _ = _list("allowed", allowed, rows, i32, (vocab + 31) // 32)
+            allowed_p, allowed_stride, _ = _list("allowed", allowed, rows, i32, device, (vocab + 31) // 32)
         if next_token is None:
             next_token = self.next_token
+        x_stride, y_stride = (logits.stride(0), out.stride(0)) if rows > 1 else (vocab, vocab)
         # kt_logits_args, field by field (a ctypes structure takes twice as long to fill)
-        _PACK.pack_into(self._args, 0, logits.data_ptr(), out.data_ptr(), _stride(logits), _stride(out), rows, vocab,
+        _PACK.pack_into(self._args, 0, logits.data_ptr(), out.data_ptr(), x_stride, y_stride, rows, vocab,
                         token_p, lengths_p, prompt_p, token_stride, token_width, repetition_p, frequency_p, presence_p,
                         bias_width, bias_p, value_p, count_p, bias_stride, allowed_p, allowed_stride,
-                        _one("next_token", next_token, rows, i32), self._scratch_ptr)
+                        _one("next_token", next_token, rows, i32, device), self._scratch_ptr)
         _lib.check(self._process(self.ctx.handle, self._args_ref, raw_stream(self.ctx.device)))
         return next_token
