@@ -21,7 +21,7 @@ constexpr int kKv8MaxHeadDim = 128;
 
 // Scratch layout (kt_kv8_scratch_bytes): the attention's merge counters at the
 // front, at the same place for every call, then what one call uses freely.
-constexpr size_t kKv8CounterBytes = 4096;
+constexpr size_t kKv8CounterBytes = 4096;  // (include/kt_cuda.h and kv8.py give this number)
 constexpr int kKv8MaxCtas = static_cast<int>(kKv8CounterBytes / sizeof(int32_t));
 
 // Runs a C entry's body: no C++ exception crosses the boundary, and the

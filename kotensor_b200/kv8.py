@@ -38,6 +38,33 @@ def _rows(name: str, x, rows: int, width: int, device: int):
     return x.data_ptr(), stride if stride > width else width
 
 
+def _zeroed(need: int, device):
+    """Scratch whose counters, at its front, are zero as its first use needs them."""
+    buffer = torch.empty(need, dtype=torch.uint8, device=device)
+    buffer[:4096].zero_()
+    return buffer
+
+
+class _Scratch:
+    """Scratch that grows with the calls that use it.  A buffer that is outgrown is freed
+    once the stream is past its last use, unless a captured graph refers to it."""
+
+    def __init__(self, device):
+        self.buffer = torch.empty(0, dtype=torch.uint8, device=device)
+        self.captured, self.kept = False, []
+
+    def of(self, need: int) -> int:
+        """Pointer to at least `need` bytes."""
+        if need > self.buffer.numel():
+            if self.captured:
+                self.kept.append(self.buffer)
+            elif self.buffer.numel():
+                self.buffer.record_stream(torch.cuda.current_stream(self.buffer.device))
+            self.buffer, self.captured = _zeroed(need, self.buffer.device), False
+        self.captured = self.captured or torch.cuda.is_current_stream_capturing()
+        return self.buffer.data_ptr()
+
+
 class KVCache8:
     """An 8-bit cache of ``layers`` layers, ``batch`` sequences and ``kv_heads``
     heads of ``head_dim`` (a multiple of 16 up to 128), ``capacity`` slots each
@@ -80,9 +107,7 @@ class KVCache8:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._status = self.status.data_ptr()
-        self._scratch = torch.zeros(0, dtype=torch.uint8, device=dev)
-        self._scratch_for = set()
-        self._retired = []  # scratch that a captured graph may still use
+        self._new_scratch()
         lib = _lib.load()
         self._lib, self._store, self._attention = lib, lib.kt_kv8_store, lib.kt_kv8_attention
         self._scale = 1.0 / math.sqrt(head_dim)
@@ -106,7 +131,7 @@ class KVCache8:
         for name in ("k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail", "weights"):
             t = getattr(self, name)
             setattr(view, name, None if t is None else t[:, begin:end])
-        view._scratch, view._scratch_for, view._retired = self._scratch[:0], set(), []
+        view._new_scratch()
         view._describe()
         return view
 
@@ -123,16 +148,25 @@ class KVCache8:
             raise ValueError(f"counts must be a contiguous int32 tensor of {self.batch} elements on {self.device}")
         return counts.data_ptr()
 
+    def _new_scratch(self) -> None:
+        self._prompt = _Scratch(self.device)
+        self._steps = {}  # heads: (pointer, buffer)
+
     def _scratch_of(self, rows_per_seq: int, heads: int):
-        """The shared scratch, grown to this call's sizes before its first call."""
-        if (rows_per_seq, heads) not in self._scratch_for:
-            need = self._lib.kt_kv8_scratch_bytes(self.batch, rows_per_seq, heads, self.kv_heads, self.head_dim,
-                                                  self.capacity, self.weights is not None)
-            if need > self._scratch.numel():
-                self._retired.append(self._scratch)
-                self._scratch = torch.zeros(need, dtype=torch.uint8, device=self.device)
-            self._scratch_for.add((rows_per_seq, heads))
-        return self._scratch.data_ptr()
+        """Scratch of this call's sizes.  Single-token steps, whose size only the heads
+        change, have their own: it stays where it is through prompts of any length."""
+        step = self._steps.get(heads) if rows_per_seq == 1 else None
+        if step is not None:
+            return step[0]
+        need = self._lib.kt_kv8_scratch_bytes(self.batch, rows_per_seq, heads, self.kv_heads, self.head_dim, self.capacity,
+                                              self.weights is not None)
+        if rows_per_seq != 1:
+            return self._prompt.of(need)
+        buffer = max((b for _, b in self._steps.values()), key=torch.Tensor.numel, default=None)
+        if buffer is None or buffer.numel() < need:
+            buffer = _zeroed(need, self.device)
+        self._steps[heads] = buffer.data_ptr(), buffer
+        return buffer.data_ptr()
 
     def store(self, layer: int, k, v, rows_per_seq: int = 1, counts=None) -> None:
         """Row b * rows_per_seq + t of ``k`` and ``v`` ([batch * rows_per_seq, kv_heads *

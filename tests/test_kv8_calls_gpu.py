@@ -1,5 +1,5 @@
 """Calls of the 8-bit key/value cache one after another: lengths that follow the
-counts of a store."""
+counts of a store, and scratch over prompts of many lengths."""
 import numpy as np
 import pytest
 
@@ -52,3 +52,42 @@ def test_advance_stays_between_zero_and_its_limit(kt):
     assert cache.lengths.tolist() == [0] * 4
     with pytest.raises(ValueError):
         cache.advance(-1, counts=torch.ones(4, dtype=torch.int32, device="cuda"))
+
+
+def test_scratch_does_not_pile_up_over_prompt_lengths(kt):
+    """Attention with weights over prompts of ever more rows: what the cache holds is bounded by the scratch of the
+    longest call and of a single-token step, whatever came before."""
+    import gc
+    from kotensor_b200 import _lib
+    from kotensor_b200.kv8 import KVCache8
+    b, h, d, heads, cap = 2, 8, 128, 32, 4096
+    cache = KVCache8(1, b, h, d, cap, 64, track_weights=True)
+    q = torch.randn(b * 3000, heads * d, device="cuda")
+    out = torch.empty_like(q)
+    gc.collect()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    lengths = [1] + list(range(200, 3001, 200))
+    for rows in lengths:
+        cache.attend(0, q[:b * rows], heads, rows, out=out[:b * rows], accumulate=True)
+        cache.lengths.zero_()
+    gc.collect()
+    torch.cuda.synchronize()
+    need = [_lib.load().kt_kv8_scratch_bytes(b, rows, heads, h, d, cap, 1) for rows in (1, max(lengths))]
+    assert torch.cuda.memory_allocated() - before <= sum(need) + 4096
+    # a step captured in a graph keeps its scratch through longer prompts
+    step = q[:b].contiguous()
+    held = torch.empty_like(step)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.attend(0, step, heads, out=held)
+    big = KVCache8(1, b, h, d, cap, 64, track_weights=True)
+    cache.attend(0, torch.randn(b * 3500, heads * d, device="cuda"), heads, 3500, accumulate=True)
+    cache.lengths.fill_(1234)
+    big.lengths.fill_(1234)
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+        x = getattr(cache, name)
+        x.copy_(torch.randint(-127, 128, x.shape, device="cuda") if x.dtype == torch.int8 else torch.rand(x.shape, device="cuda"))
+        getattr(big, name).copy_(x)
+    g.replay()
+    assert torch.equal(held, big.attend(0, step, heads))
