@@ -50,19 +50,33 @@ class _Scratch:
     once the stream is past its last use, unless a captured graph refers to it."""
 
     def __init__(self, device):
-        self.buffer = torch.empty(0, dtype=torch.uint8, device=device)
+        self.buffer = self.graphs = torch.empty(0, dtype=torch.uint8, device=device)
         self.captured, self.kept = False, []
 
     def of(self, need: int) -> int:
         """Pointer to at least `need` bytes."""
+        if torch.cuda.is_current_stream_capturing():
+            return self.of_graph(need)
         if need > self.buffer.numel():
             if self.captured:
                 self.kept.append(self.buffer)
             elif self.buffer.numel():
                 self.buffer.record_stream(torch.cuda.current_stream(self.buffer.device))
             self.buffer, self.captured = _zeroed(need, self.buffer.device), False
-        self.captured = self.captured or torch.cuda.is_current_stream_capturing()
         return self.buffer.data_ptr()
+
+    def of_graph(self, need: int) -> int:
+        """The same while a graph is captured.  A buffer made now would be zeroed by
+        replays, not for a call before them: it serves graphs alone, zeroed at each use."""
+        if need <= self.buffer.numel():
+            self.captured = True
+            return self.buffer.data_ptr()
+        if need > self.graphs.numel():
+            self.kept.append(self.graphs)
+            self.graphs = _zeroed(need, self.buffer.device)
+        else:
+            self.graphs[:4096].zero_()
+        return self.graphs.data_ptr()
 
 
 class KVCache8:
@@ -164,6 +178,8 @@ class KVCache8:
             return self._prompt.of(need)
         buffer = max((b for _, b in self._steps.values()), key=torch.Tensor.numel, default=None)
         if buffer is None or buffer.numel() < need:
+            if torch.cuda.is_current_stream_capturing():
+                return self._prompt.of_graph(need)
             buffer = _zeroed(need, self.device)
         self._steps[heads] = buffer.data_ptr(), buffer
         return buffer.data_ptr()

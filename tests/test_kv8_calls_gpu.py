@@ -1,5 +1,6 @@
 """Calls of the 8-bit key/value cache one after another: lengths that follow the
-counts of a store, and scratch over prompts of many lengths."""
+counts of a store, scratch over prompts of many lengths, a cache used first inside
+a captured graph, and views of some sequences."""
 import numpy as np
 import pytest
 
@@ -91,3 +92,65 @@ def test_scratch_does_not_pile_up_over_prompt_lengths(kt):
         getattr(big, name).copy_(x)
     g.replay()
     assert torch.equal(held, big.attend(0, step, heads))
+
+
+def test_a_graph_that_is_the_first_to_call_leaves_the_scratch_usable(kt):
+    """The first call of a cache is captured, in a pool whose free memory is full of ones; a call outside the graph
+    comes before the first replay."""
+    from kotensor_b200.kv8 import KVCache8
+    pool = torch.cuda.graph_pool_handle()
+    dirt = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(dirt, pool=pool):
+        x = torch.full((64 << 20,), -1, dtype=torch.int8, device="cuda")
+    dirt.replay()
+    torch.cuda.synchronize()
+    del x
+    one, two = (KVCache8(1, 1, 2, 64, 8192, 16) for _ in range(2))
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+        x = getattr(one, name)
+        x.copy_(torch.randint(-127, 128, x.shape, device="cuda") if x.dtype == torch.int8 else torch.rand(x.shape, device="cuda"))
+        getattr(two, name).copy_(x)
+    for c in (one, two):
+        c.lengths.fill_(8000)
+    q = torch.randn(1, 512, device="cuda")
+    held = torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, pool=pool):
+        one.attend(0, q, 8, out=held)
+    want = two.attend(0, q, 8)
+    assert torch.equal(one.attend(0, q, 8, out=torch.zeros_like(q)), want)
+    g.replay()
+    assert torch.equal(held, want)
+    assert torch.equal(one.attend(0, q, 8), want)
+
+
+def test_a_view_of_some_sequences(kt):
+    """`sequences` stores, attends, advances and evicts on its part of the buffers alone."""
+    from test_kv8_gpu import assert_same, make, push
+    cache, ref, rng = make(kt, 4, 2, 64, 256, 32, [3, 70, 33, 100])
+    part, part_ref, _ = make(kt, 2, 2, 64, 256, 32, [70, 33])
+    for name in ("codes", "scales", "tail"):
+        for n in "kv":
+            getattr(part_ref, name)[n][:] = getattr(ref, name)[n][1:3]
+    part_ref.weights[:] = np.abs(rng.standard_normal(part_ref.weights.shape)).astype(np.float32)
+    ref.weights[1:3] = part_ref.weights
+    push(cache, ref)
+    push(part, part_ref)
+    view = cache.sequences(1, 3)
+    k = cuda(rng.standard_normal((2 * 5, 128), dtype=np.float32))
+    q = cuda(rng.standard_normal((2 * 5, 512), dtype=np.float32))
+    results = []
+    for c in (view, part):
+        c.store(0, k, k, 5)
+        results.append(c.attend(0, q, 8, 5, accumulate=True))
+        c.advance(5)
+        c.evict(40, 8)
+    assert torch.equal(*results)
+    assert cache.lengths.tolist() == [3, 40, 38, 100] and part.lengths.tolist() == [40, 38]
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail", "weights"):
+        a, b = getattr(cache, name)[0], getattr(part, name)[0]
+        assert torch.equal(a[1:3].nan_to_num(), b.nan_to_num())
+    for n in "kv":  # the others are as they were
+        for name in ("codes", "scales", "tail"):
+            got = getattr(cache, f"{n}_{name}")[0].cpu().numpy()[[0, 3]]
+            assert np.array_equal(got, getattr(ref, name)[n][[0, 3]], equal_nan=name != "codes")
