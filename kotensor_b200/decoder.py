@@ -226,8 +226,8 @@ class DeviceDecoder:
         self._last_rows = torch.empty(batch, dtype=torch.int32, device=dev)
         self._step_bufs = self._buffers(batch, tokens=self.token)
         self._prefill_bufs = None  # prefill buffers, allocated on first use
-        self.length = 0  # tokens processed
-        self.held = 0    # positions in the cache (fewer after an eviction)
+        self.length = 0    # tokens processed
+        self._evicted = 0  # of them, no longer in the cache
         self._penal = None
         self.scale = float(np.float32(1.0) / np.float32(math.sqrt(float(cfg.head_dim))))
         self._graph = None
@@ -244,8 +244,13 @@ class DeviceDecoder:
     def _stream(self) -> ctypes.c_void_p:
         return ctypes.c_void_p(torch.cuda.current_stream(self.ctx.device).cuda_stream)
 
+    @property
+    def held(self) -> int:
+        """Positions in the cache (fewer than ``length`` after an eviction)."""
+        return self.length - self._evicted
+
     def reset(self) -> None:
-        self.length = self.held = 0
+        self.length = self._evicted = 0
         self.position.zero_()
         if self.cache is not None:
             self.cache.reset()
@@ -454,7 +459,6 @@ class DeviceDecoder:
                                          self.cfg.dim, dst, self._stream()))
         self._head(self._head_in, T)
         self.length += T
-        self.held += T
         return self._result()
 
     def step(self, tokens):
@@ -471,7 +475,6 @@ class DeviceDecoder:
         self.token.copy_(torch.tensor(tokens, dtype=torch.int32))
         self._launch_step()
         self.length += 1
-        self.held += 1
         return self._result()
 
     def capture(self) -> None:
@@ -498,7 +501,6 @@ class DeviceDecoder:
         for _ in range(max_tokens - 1):
             self._graph.replay()
             self.length += 1
-            self.held += 1
             out.append(int(self.next_token[0].item()))
         return out
 
@@ -524,7 +526,6 @@ class DeviceDecoder:
                 self.evict(keep, recent)
             self._graph.replay()
             self.length += 1
-            self.held += 1
             out.append(self.next_token.cpu().tolist())
         return [[row[q] for row in out] for q in range(self.batch)]
 
@@ -542,7 +543,7 @@ class DeviceDecoder:
         self._check_evict(keep, recent)
         if self.held > keep:
             self.cache.evict(keep, recent)
-            self.held = keep
+            self._evicted = self.length - keep
 
     def penalize(self, repetition=None, frequency=None, presence=None, bias_ids=None, bias_values=None, bias_counts=None,
                  allowed=None, history: Optional[int] = None) -> None:
