@@ -484,13 +484,21 @@ class DeviceDecoder:
         with torch.cuda.graph(self._graph):
             self._launch_step()
 
+    def _check_room(self, prompt: int, max_tokens: int) -> None:
+        """Refuses a generation that does not fit: nothing checks the replays of the
+        captured step, and the last token chosen is not processed."""
+        if prompt + max_tokens > self.max_seq:
+            raise ValueError("prompt + max_tokens exceed max_seq")
+        if self.held + prompt + max_tokens - 1 > self.max_seq:
+            raise ValueError(f"KV cache full: {self.held} + {prompt} + {max_tokens - 1} positions exceed maxSequenceLength "
+                             f"{self.max_seq}")
+
     def generate(self, prompt: list[int], max_tokens: int) -> list[int]:
         """Greedy continuation of one sequence (batch 1): the prompt fed step by
         step (eager), then ``max_tokens`` replays of the captured step."""
         if self.batch != 1:
             raise ValueError("generate is for batch 1; use generate_batch")
-        if len(prompt) + max_tokens > self.max_seq:
-            raise ValueError("prompt + max_tokens exceed max_seq")
+        self._check_room(len(prompt), max_tokens)
         for t in prompt:
             if self._penal is not None:  # a token of the prompt
                 self._prompt_lengths.copy_(self._history_lengths + 1)
@@ -513,8 +521,8 @@ class DeviceDecoder:
             self._check_evict(keep, recent)
             if not keep < self.max_seq:
                 raise ValueError(f"keep must be below max_seq {self.max_seq}, got {keep}")
-        elif len(prompts[0]) + max_tokens > self.max_seq:
-            raise ValueError("prompt + max_tokens exceed max_seq")
+        else:
+            self._check_room(len(prompts[0]), max_tokens)
         self.prefill(prompts)
         out = [self.next_token.cpu().tolist()]
         if keep is not None:
