@@ -493,6 +493,11 @@ class DeviceDecoder:
             raise ValueError(f"KV cache full: {self.held} + {prompt} + {max_tokens - 1} positions exceed maxSequenceLength "
                              f"{self.max_seq}")
 
+    def _check_dropped(self) -> None:
+        """An error if the 8-bit cache, until ``reset``, had no room for a token it was given."""
+        if self.cache is not None and int(self.cache.status.item()) != 0:
+            raise ValueError("KV cache full: tokens were dropped")
+
     def generate(self, prompt: list[int], max_tokens: int) -> list[int]:
         """Greedy continuation of one sequence (batch 1): the prompt fed step by
         step (eager), then ``max_tokens`` replays of the captured step."""
@@ -510,6 +515,7 @@ class DeviceDecoder:
             self._graph.replay()
             self.length += 1
             out.append(int(self.next_token[0].item()))
+        self._check_dropped()
         return out
 
     def generate_batch(self, prompts, max_tokens: int, keep: Optional[int] = None, recent: int = 0) -> list:
@@ -535,6 +541,7 @@ class DeviceDecoder:
             self._graph.replay()
             self.length += 1
             out.append(self.next_token.cpu().tolist())
+        self._check_dropped()
         return [[row[q] for row in out] for q in range(self.batch)]
 
     # -- the 8-bit cache and the choice of tokens

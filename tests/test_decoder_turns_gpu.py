@@ -59,3 +59,13 @@ def test_the_limit_counts_positions_that_a_caller_replayed(kt, oracle):
     assert d.held == 16
     d.reset()
     assert d.held == d.length == 0
+
+
+def test_dropped_tokens_are_an_error(kt, oracle):
+    """A cache that holds more than the decoder knows: the tokens it drops end the generation with an error."""
+    d = decoder(max_seq=32, batch=2, kv_bits=8)
+    d.cache.lengths.fill_(d.cache.capacity - 5)
+    with pytest.raises(ValueError):
+        d.generate_batch(prompts(2, 4), 10)
+    d.reset()
+    assert len(d.generate_batch(prompts(2, 4), 10)[0]) == 10
