@@ -255,8 +255,7 @@ class DeviceDecoder:
         if self.cache is not None:
             self.cache.reset()
         if self._penal is not None:
-            self._history_lengths.zero_()
-            self._prompt_lengths.zero_()
+            self._lay_out(self._history[:, :0], 0)
 
     def _buffers(self, rows: int, tokens=None) -> "_Rows":
         cfg = self.cfg
@@ -396,15 +395,17 @@ class DeviceDecoder:
             self.cache.advance(advance)
         self.token.copy_(self.next_token)
 
-    def _launch_step(self) -> None:
+    def _launch_step(self, remember: bool = True) -> None:
         """One decode step on the current stream: reads self.token and
         self.position, writes self.logits and self.next_token, advances
         the position and feeds the next tokens back."""
         b = self._step_bufs
-        if self._penal is not None:  # the step's tokens join the history
-            room = self._history.shape[1]
-            self._history.scatter_(1, self._history_lengths.clamp(max=room - 1).long()[:, None], self.token[:, None])
-            self._history_lengths.add_(1).clamp_(max=room)
+        if self._penal is not None and remember:  # the step's tokens join the history
+            column, forgotten, length, after = self._places.index_select(0, self._place)[0].split(1)
+            self._history.scatter_(1, forgotten.expand(self.batch, 1), -1)
+            self._history.scatter_(1, column.expand(self.batch, 1), self.token[:, None])
+            self._history_lengths.copy_(length.expand(self.batch))
+            self._place.copy_(after)
         self._layers(b, self.batch, 1)
         self._head(b.x, 1)
 
@@ -442,10 +443,10 @@ class DeviceDecoder:
             # a larger block may replace the communicator's scratch that a
             # captured step refers to: capture again before the next replay
             self._graph = None
-        if self._penal is not None:
-            self._append_prompt(prompts, T)
         b = self._prefill_bufs
         flat = torch.tensor([t for pr in prompts for t in pr], dtype=torch.int32)
+        if self._penal is not None:
+            self._append_prompt(flat.view(self.batch, T))
         L_ = _lib.load()
         for s0 in range(0, self.batch, per):
             s1 = min(self.batch, s0 + per)
@@ -464,6 +465,9 @@ class DeviceDecoder:
     def step(self, tokens):
         """Transformer.decode(token) for every sequence (an int when batch == 1):
         the logits of this step (device tensor)."""
+        return self._step(tokens)
+
+    def _step(self, tokens, remember: bool = True):
         tokens = [tokens] if isinstance(tokens, (int, np.integer)) else list(tokens)
         if len(tokens) != self.batch:
             raise ValueError(f"{len(tokens)} tokens for a batch of {self.batch}")
@@ -473,7 +477,7 @@ class DeviceDecoder:
         if self.held >= self.max_seq:
             raise ValueError(f"KV cache full: maxSequenceLength {self.max_seq}")
         self.token.copy_(torch.tensor(tokens, dtype=torch.int32))
-        self._launch_step()
+        self._launch_step(remember)
         self.length += 1
         return self._result()
 
@@ -504,10 +508,12 @@ class DeviceDecoder:
         if self.batch != 1:
             raise ValueError("generate is for batch 1; use generate_batch")
         self._check_room(len(prompt), max_tokens)
+        if any(not 0 <= t < self.cfg.vocab for t in prompt):
+            raise ValueError("token out of vocab bounds")
+        if self._penal is not None and len(prompt) > 0:
+            self._append_prompt(torch.tensor([list(prompt)], dtype=torch.int32))
         for t in prompt:
-            if self._penal is not None:  # a token of the prompt
-                self._prompt_lengths.copy_(self._history_lengths + 1)
-            self.step(t)
+            self._step(t, remember=False)
         out = [int(self.next_token[0].item())]
         if self._graph is None:
             self.capture()  # captures the position reached after the prompt
@@ -565,8 +571,9 @@ class DeviceDecoder:
         """From the next step on the logits go through a LogitsProcessor: penalties (a
         number, or one for each sequence) for the tokens of prompt and answer, sparse
         biases and a mask of allowed tokens (device tensors as LogitsProcessor takes
-        them; the mask's contents may change between steps).  ``history`` bounds the
-        tokens remembered (max_seq unless given).  No arguments: plain argmax again."""
+        them; the mask's contents may change between steps).  Of each text the last
+        ``history`` tokens are remembered (max_seq unless given).  No arguments: plain
+        argmax again."""
         self._graph = None  # a captured step has the old choice
         given = dict(repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
                      bias_values=bias_values, bias_counts=bias_counts, allowed=allowed)
@@ -585,19 +592,48 @@ class DeviceDecoder:
                     raise ValueError(f"{k} must be a number or one for each of {self.batch} sequences")
                 given[k] = x.reshape(-1).expand(self.batch).contiguous()
         self._processor = LogitsProcessor(self.batch, self.cfg.vocab, self.ctx.device)
-        self._history = torch.zeros((self.batch, history or self.max_seq), dtype=torch.int32, device=dev)
+        room = history or self.max_seq
+        i64 = dict(dtype=torch.int64, device=dev)
+        self._history = torch.empty((self.batch, 2 * room), dtype=torch.int32, device=dev)
         self._history_lengths = torch.zeros(self.batch, dtype=torch.int32, device=dev)
         self._prompt_lengths = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        self._place, self._places = torch.zeros(1, **i64), torch.zeros((2 * room, 4), **i64)
+        self._lay_out(self._history[:, :0], 0)
         self._penal = given
 
-    def _append_prompt(self, prompts, T: int) -> None:
-        """Prompt tokens into the history; what is there so far counts as prompt."""
-        n = int(self._history_lengths[0].item())
-        room = max(0, min(T, self._history.shape[1] - n))
-        if room:
-            self._history[:, n:n + room] = torch.tensor([list(p)[:room] for p in prompts], dtype=torch.int32)
-        self._history_lengths.fill_(n + room)
-        self._prompt_lengths.fill_(n + room)
+    # The tokens that penalties see: the last `room` of each text, in 2 * room columns.  Token m of a
+    # text is in column m until the columns 0..room-1 are full.  Then the columns are taken round and
+    # round, the oldest token first, but that an answer's token must not lie ahead of the prompt's end
+    # (_prompt_lengths): it takes column m + room where the prompt's token m is forgotten (-1: no token).
+    # _places has, for every place m in 0..2*room-1, its column, the one forgotten, the columns in use
+    # after it and the place after it, so that a captured step needs no host.
+    def _lay_out(self, text, prompt: int) -> None:
+        """The history is `text` [batch, at most room tokens], of which the first `prompt` are the prompt's."""
+        text = text.to(self._history.device, copy=True)
+        n, room = text.shape[1], self._history.shape[1] // 2
+        self._history.fill_(-1)
+        self._history[:, :n] = text
+        self._history_lengths.fill_(n)
+        self._prompt_lengths.fill_(prompt)
+        self._place.fill_(n)
+        m = torch.arange(2 * room, device=text.device)
+        full, again = m >= room, m - room
+        self._places.copy_(torch.stack([torch.where(full & (again >= prompt), again, m), torch.where(full, again, m),
+                                        torch.where(full, room + prompt, m + 1), torch.where(m + 1 < 2 * room, m + 1, room)], 1))
+
+    def _remembered(self):
+        """The history in the texts' order, and how many of its tokens are the prompt's."""
+        room, place = self._history.shape[1] // 2, int(self._place.item())
+        first, again = self._history[:, :room], self._history[:, room:]
+        prompt = int((first[0, :int(self._prompt_lengths[0].item())] >= 0).sum().item())
+        text = torch.where(first >= 0, first, again)
+        return (text[:, :place] if place < room else text.roll(room - place, 1)), prompt
+
+    def _append_prompt(self, prompts) -> None:
+        """Prompt tokens [batch, n] into the history; what is there so far counts as prompt."""
+        room = self._history.shape[1] // 2
+        text = torch.cat([self._remembered()[0], prompts.to(self._history.device)], 1)[:, -room:]
+        self._lay_out(text, text.shape[1])
 
     # -- files (Transformer.saveQuantized / loadQuantized, Transformer.kt:402-471)
     def save_quantized(self, path) -> None:

@@ -1,4 +1,5 @@
-"""DeviceDecoder over several turns: the limit of the cache."""
+"""DeviceDecoder over several turns: the limit of the cache and the tokens that
+penalties remember."""
 import numpy as np
 import pytest
 
@@ -69,3 +70,55 @@ def test_dropped_tokens_are_an_error(kt, oracle):
         d.generate_batch(prompts(2, 4), 10)
     d.reset()
     assert len(d.generate_batch(prompts(2, 4), 10)[0]) == 10
+
+
+def repeats(tokens, window):
+    return [i for i, t in enumerate(tokens) if t in tokens[max(0, i - window):i]]
+
+
+def test_penalties_hold_past_the_history(kt, oracle):
+    """With a history of n tokens, no token comes again within n: long past the cache's end, for texts whose
+    prompt is shorter and longer than the history, and over a second prompt."""
+    for history, n in ((None, 20), (16, 5), (16, 30), (7, 7), (1, 3)):
+        d = decoder(max_seq=48, batch=2, kv_bits=8, kv_block=16, kv_weights=True)
+        d.penalize(presence=1e6, repetition=None, history=history)
+        text = prompts(2, n, seed=n)
+        for turn in range(2):
+            out = d.generate_batch(text, 120, keep=24, recent=8)
+            for q in range(2):
+                assert repeats(out[q], history or 48) == [], (history, n, turn)
+            text = prompts(2, 4, seed=turn)
+            d.evict(24, 8)
+
+
+def remembered(text, split, room):
+    """What penalties see of `text`, of which the first `split` are the prompt: (tokens in any order, answer's)."""
+    last = text[-room:]
+    cut = max(0, split - (len(text) - len(last)))
+    return sorted(last), sorted(last[cut:])
+
+
+def seen(d, q=0):
+    n, p = int(d._history_lengths[q].item()), int(d._prompt_lengths[q].item())
+    line = [t for t in d._history[q, :n].tolist()]
+    return sorted(t for t in line if t >= 0), sorted(t for t in line[max(0, p):] if t >= 0)
+
+
+@pytest.mark.parametrize("room,first", [(5, 3), (5, 5), (5, 9), (1, 1), (8, 1), (40, 4)])
+def test_the_history_is_the_last_tokens(kt, oracle, room, first):
+    """Token by token against a list, over prompts, steps, a second prompt and more steps."""
+    d = decoder(max_seq=200, kv_bits=8)
+    d.penalize(frequency=0.5, history=room)
+    rng = np.random.default_rng(room)
+    text, split = [], 0
+    for n in (first, 4, 1):
+        part = rng.integers(0, 700, n).tolist()
+        d.prefill([part])
+        text += part
+        split = len(text)  # all that is there when a prompt comes counts as prompt
+        assert seen(d) == remembered(text, split, room)
+        for _ in range(3 * room + 2 if room < 10 else 12):
+            t = int(rng.integers(0, 700))
+            d.step(t)
+            text.append(t)
+            assert seen(d) == remembered(text, split, room)
