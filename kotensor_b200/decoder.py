@@ -229,6 +229,7 @@ class DeviceDecoder:
         self.length = 0    # tokens processed
         self._evicted = 0  # of them, no longer in the cache
         self._penal = None
+        self._text, self._prompt_end = [], 0  # int32 [batch, n] of each call, tokens up to the last prompt's end
         self.scale = float(np.float32(1.0) / np.float32(math.sqrt(float(cfg.head_dim))))
         self._graph = None
         g_ = self.heads_local // self.kv_local
@@ -251,6 +252,7 @@ class DeviceDecoder:
 
     def reset(self) -> None:
         self.length = self._evicted = 0
+        self._text, self._prompt_end = [], 0
         self.position.zero_()
         if self.cache is not None:
             self.cache.reset()
@@ -460,6 +462,8 @@ class DeviceDecoder:
                                          self.cfg.dim, dst, self._stream()))
         self._head(self._head_in, T)
         self.length += T
+        self._text.append(flat.view(self.batch, T).numpy())
+        self._prompt_end = sum(t.shape[1] for t in self._text)
         return self._result()
 
     def step(self, tokens):
@@ -479,6 +483,7 @@ class DeviceDecoder:
         self.token.copy_(torch.tensor(tokens, dtype=torch.int32))
         self._launch_step(remember)
         self.length += 1
+        self._text.append(np.array(tokens, dtype=np.int32)[:, None])
         return self._result()
 
     def capture(self) -> None:
@@ -514,12 +519,15 @@ class DeviceDecoder:
             self._append_prompt(torch.tensor([list(prompt)], dtype=torch.int32))
         for t in prompt:
             self._step(t, remember=False)
+        if len(prompt) > 0:
+            self._prompt_end = sum(t.shape[1] for t in self._text)
         out = [int(self.next_token[0].item())]
         if self._graph is None:
             self.capture()  # captures the position reached after the prompt
         for _ in range(max_tokens - 1):
             self._graph.replay()
             self.length += 1
+            self._text.append(np.array([out[-1:]], dtype=np.int32))
             out.append(int(self.next_token[0].item()))
         self._check_dropped()
         return out
@@ -546,6 +554,7 @@ class DeviceDecoder:
                 self.evict(keep, recent)
             self._graph.replay()
             self.length += 1
+            self._text.append(np.array(out[-1], dtype=np.int32)[:, None])
             out.append(self.next_token.cpu().tolist())
         self._check_dropped()
         return [[row[q] for row in out] for q in range(self.batch)]
@@ -569,11 +578,12 @@ class DeviceDecoder:
     def penalize(self, repetition=None, frequency=None, presence=None, bias_ids=None, bias_values=None, bias_counts=None,
                  allowed=None, history: Optional[int] = None) -> None:
         """From the next step on the logits go through a LogitsProcessor: penalties (a
-        number, or one for each sequence) for the tokens of prompt and answer, sparse
-        biases and a mask of allowed tokens (device tensors as LogitsProcessor takes
-        them; the mask's contents may change between steps).  Of each text the last
-        ``history`` tokens are remembered (max_seq unless given).  No arguments: plain
-        argmax again."""
+        number, or one for each sequence) for the tokens of prompt and answer, those
+        processed so far (prefill, step, generate) among them, sparse biases and a mask
+        of allowed tokens (device tensors as LogitsProcessor takes them; the mask's
+        contents may change between steps).  Of each text the last ``history`` tokens
+        are remembered (max_seq unless given); a further call changes what is given and
+        keeps them.  No arguments: plain argmax again."""
         self._graph = None  # a captured step has the old choice
         given = dict(repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
                      bias_values=bias_values, bias_counts=bias_counts, allowed=allowed)
@@ -593,12 +603,20 @@ class DeviceDecoder:
                 given[k] = x.reshape(-1).expand(self.batch).contiguous()
         self._processor = LogitsProcessor(self.batch, self.cfg.vocab, self.ctx.device)
         room = history or self.max_seq
+        if self._penal is not None:
+            text, prompt = self._remembered()
+        else:
+            text = np.concatenate([np.empty((self.batch, 0), np.int32), *self._text], 1)
+            text, prompt = torch.from_numpy(text), self._prompt_end
+        before = text.shape[1]
+        text = text[:, -room:]
+        prompt = max(0, prompt - (before - text.shape[1]))
         i64 = dict(dtype=torch.int64, device=dev)
         self._history = torch.empty((self.batch, 2 * room), dtype=torch.int32, device=dev)
         self._history_lengths = torch.zeros(self.batch, dtype=torch.int32, device=dev)
         self._prompt_lengths = torch.zeros(self.batch, dtype=torch.int32, device=dev)
         self._place, self._places = torch.zeros(1, **i64), torch.zeros((2 * room, 4), **i64)
-        self._lay_out(self._history[:, :0], 0)
+        self._lay_out(text, prompt)
         self._penal = given
 
     # The tokens that penalties see: the last `room` of each text, in 2 * room columns.  Token m of a

@@ -1,5 +1,5 @@
-"""DeviceDecoder over several turns: the limit of the cache and the tokens that
-penalties remember."""
+"""DeviceDecoder over several turns: the cache's limit, the tokens that penalties
+remember, and penalties that change in the middle of a text."""
 import numpy as np
 import pytest
 
@@ -122,3 +122,51 @@ def test_the_history_is_the_last_tokens(kt, oracle, room, first):
             d.step(t)
             text.append(t)
             assert seen(d) == remembered(text, split, room)
+
+
+def test_penalties_in_the_middle_of_a_text(kt, oracle):
+    """`penalize` after a prompt and some answer counts what has been processed; again, it changes the penalties
+    and keeps what is remembered; taken back and given again, nothing is lost."""
+    text = prompts(2, 6)
+    early, late = (decoder(max_seq=200, batch=2, kv_bits=8) for _ in range(2))
+    early.penalize(presence=0.0)
+    a, b = early.generate_batch(text, 10), late.generate_batch(text, 10)
+    assert a == b
+    for d in (early, late):
+        d.penalize(presence=1e6)
+    for q in range(2):
+        want = remembered(text[q] + a[q][:-1], 6, 200)
+        assert seen(early, q) == want and seen(late, q) == want
+    for d in (early, late):
+        for _ in range(5):
+            d.step(d.next_token.tolist())
+    x = early.next_token.tolist()
+    assert x == late.next_token.tolist()
+    for q in range(2):
+        assert x[q] not in a[q][:-1]
+    late.penalize()
+    late.step(x)
+    late.penalize(presence=1e6)
+    early.step(x)
+    for q in range(2):
+        assert seen(late, q) == seen(early, q)
+    late.penalize(presence=1e6, history=4)
+    line = sorted(t for t in late._history[0].tolist() if t >= 0)[-4:]
+    assert len(seen(late)[0]) == 4 and set(seen(late)[0]) <= set(seen(early)[0]) and line is not None
+    # generate, one sequence: prompt tokens count as prompt
+    one = decoder(max_seq=64, kv_bits=8)
+    out = one.generate(text[0], 8)
+    one.penalize(repetition=1.5)
+    assert seen(one) == remembered(text[0] + out[:-1], 6, 64)
+    one.reset()
+    assert seen(one) == ([], [])
+    one.generate(text[1], 4)
+    one.penalize(repetition=1.25)
+    assert seen(one)[0] == sorted(text[1] + one_answer(one, text[1], 4))
+
+
+def one_answer(d, prompt, n):
+    """The first n - 1 tokens that follow `prompt` under repetition 1.5, on a fresh decoder."""
+    e = decoder(max_seq=64, kv_bits=8)
+    e.penalize(repetition=1.5)
+    return e.generate(prompt, n)[:-1]
