@@ -322,9 +322,12 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool real)
 // the token that moves to slot i comes from a slot >= i, so what a round overwrites no
 // later round still needs, and a round's own codes have been read at the barrier ahead
 // of its writes.  For the same reason the next unit's codes may come by asynchronous
-// copies while this one is quantised.  The barrier orders reads before writes only, so
-// its arrival need not wait for this warp's writes.  Where there are few heads, a cluster
-// of up to 8 CTAs shares each.  16 sequences x 8 heads of 128, 4000 of 8k slots kept:
+// copies while this one is quantised.  The barrier's arrival is a release, so that every
+// code read before it is read before what others write after it; it comes once the last
+// round's writes, which it also waits for, are long under way (16 sequences x 8 heads
+// with selection: 87 us, ahead of the search for the largest 89, with a relaxed arrival,
+// which promises no order, 85).  Where there are few heads, a cluster of up to 8 CTAs
+// shares each.  16 sequences x 8 heads of 128, 4000 of 8k slots kept:
 // 65 us for 262 MB, 4.0 TB/s; about 9 instructions a code, issued in 58% of the cycles.
 // (Without the copies ahead 84 us, with five CTAs on an SM, whose registers spill, 77.)
 constexpr int kUnit = 64;
@@ -392,7 +395,6 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 4) kv8_move_kernel(Kv8 c, int
         const float* const scale = scale_of[y][warp] + token0;
         uint4 r[kLoads];
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) r[i] = lds128(buffer + i * 512);
         // the largest value of each 16 tokens: scale x largest code, exactly the largest product
@@ -411,6 +413,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 4) kv8_move_kernel(Kv8 c, int
             const float m = static_cast<float>(max(hi, lo));
             top[i / kPer16] = max(top[i / kPer16], magnitude(__fmul_rn(scale[i * kTokens], m)));
         }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         if (left > gridDim.x * kMoveWarps) {  // the codes are in registers
             fetch(y ^ 1);
             look(base + 2 * stride);
