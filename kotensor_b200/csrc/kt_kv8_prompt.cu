@@ -230,12 +230,13 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 // the first 16 columns of theirs, the lo terms in the last.  Lane g of the warp has
 // the scales of slots first + 16 g .. in k_scale, v_scale.  The thread with the
 // vector's other 64 slots is in the warp that shares barrier `bar`; their largest
-// scores meet in mine, other.  kEdge: some vector of the warp does not see all of
+// scores meet in mine, other; false if that warp gave up (it left NaN there, as no largest
+// score is).  kEdge: some vector of the warp does not see all of
 // the slots; this one sees those below `limit`.  The loops stay rolled and the scores
 // are read twice: unrolled, the roles' code did not fit the instruction caches, and
 // waiting for instructions was the longest of all stalls.
 template <bool kEdge>
-__device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit, float factor, float k_scale,
+__device__ __forceinline__ bool scores_to_p(uint32_t s_tm, int first, int limit, float factor, float k_scale,
                                             float v_scale, float2* mine, const float2* other, int bar, float& D,
                                             float& l, float& R) {
     // a block the vector does not see has no scale, whatever is there
@@ -273,6 +274,7 @@ __device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit,
     *mine = make_float2(D, R);
     asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
     const float2 there = *other;
+    if (__any_sync(0xffffffffu, there.x != there.x)) return false;
     D = fmaxf(D, there.x);
     R = fmaxf(R, there.y);
     const float ref = D == -INFINITY ? 0.0f : D;
@@ -320,6 +322,7 @@ __device__ __forceinline__ void scores_to_p(uint32_t s_tm, int first, int limit,
     float s0, s1;
     unpair(sum, s0, s1);
     l = s0 + s1;
+    return true;
 }
 
 template <int HDP>
@@ -476,15 +479,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
         for (int i = 0; i < tiles; ++i) {
             const int y = i & 1, first = (from + i) * kSlots + 64 * x, at = first + 16 * (lane % 4);
             const float ks = at < most ? k_scales[at / c.block] : 0.0f, vs = at < most ? v_scales[at / c.block] : 0.0f;
-            if (!wait_all(s_full(y), (i / 2) & 1)) break;
-            tc_after();
-            const uint32_t s_tm = lanes + y * kSlots + 64 * x;
             float2* const mine = meet + (2 * y + x) * kVecTile + row;
             const float2* const other = meet + (2 * y + 1 - x) * kVecTile + row;
             const int bar = 4 + warp % 4;
+            if (!wait_all(s_full(y), (i / 2) & 1)) {  // the other half's warp may have seen it: not left waiting
+                *mine = make_float2(__uint_as_float(0x7fc00000u), 0.0f);
+                asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+                break;
+            }
+            tc_after();
+            const uint32_t s_tm = lanes + y * kSlots + 64 * x;
             float D, l, R;
-            if (__any_sync(0xffffffffu, first + 64 > limit)) scores_to_p<true>(s_tm, first, limit, factor, ks, vs, mine, other, bar, D, l, R);
-            else scores_to_p<false>(s_tm, first, limit, factor, ks, vs, mine, other, bar, D, l, R);
+            if (!(__any_sync(0xffffffffu, first + 64 > limit)
+                      ? scores_to_p<true>(s_tm, first, limit, factor, ks, vs, mine, other, bar, D, l, R)
+                      : scores_to_p<false>(s_tm, first, limit, factor, ks, vs, mine, other, bar, D, l, R)))
+                break;
             float* const to = stats + (i % 4) * 4 * kVecTile + row;
             if (x == 0) to[0] = D, to[kVecTile] = R;
             to[(2 + x) * kVecTile] = l;
