@@ -546,6 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
             __syncwarp();
         } else if (warp == kCopyWarp) {
             if (lane == 0) {
+                int sent[2] = {0, 0};
                 auto copy = [&](int v, int i) {
                     const int y = i & 1;
                     if (i >= 2 && !wait(raw_free(v, y), (i / 2 - 1) & 1)) return;
@@ -555,6 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
                     const int8_t* codes = (v ? c.v_codes : c.k_codes) + (head * c.capacity + slot) * d;
                     dev::mbar_expect_tx(raw_full(v, y), bytes);
                     dev::bulk_load(base + S::kRaw + (2 * v + y) * S::kRawTile, codes, bytes, raw_full(v, y));
+                    sent[v] = i + 1;
                 };
                 copy(0, 0);
                 if (tiles > 1) copy(0, 1);
@@ -562,9 +564,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(Kv8Attention a,
                     copy(1, i);
                     if (ok && i + 2 < tiles) copy(0, i + 2);
                 }
-                // no copy is in flight past this point
-                for (int i = max(0, tiles - 2); ok && i < tiles; ++i)
-                    if (wait(raw_full(0, i & 1), (i / 2) & 1)) wait(raw_full(1, i & 1), (i / 2) & 1);
+                // no copy is in flight past this point, also where a wait has given up
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+                    for (int i = max(0, sent[v] - 2); i < sent[v]; ++i)
+                        if (!wait_counted(raw_full(v, i & 1), (i / 2) & 1)) atomicOr(err, 1);
             }
             __syncwarp();
         }
