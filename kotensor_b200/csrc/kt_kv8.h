@@ -28,17 +28,25 @@ constexpr int kKv8MaxCtas = static_cast<int>(kKv8CounterBytes / sizeof(int32_t))
 // context's device is current inside (the caller's is put back).
 template <typename Body>
 kt_status c_entry(kt_ctx* ctx, Body body) {
+    struct Restore {  // also where the body throws
+        int device = -1;
+        ~Restore() {
+            if (device >= 0) cudaSetDevice(device);
+        }
+    };
     try {
         int before = 0;
+        Restore restore;
         cudaError_t e = cudaGetDevice(&before);
-        if (e == cudaSuccess && before != ctx->device) e = cudaSetDevice(ctx->device);
+        if (e == cudaSuccess && before != ctx->device) {
+            restore.device = before;
+            e = cudaSetDevice(ctx->device);
+        }
         if (e != cudaSuccess) {
             set_error(std::string("cudaSetDevice: ") + cudaGetErrorString(e));
             return KT_ERR_CUDA;
         }
-        const kt_status st = body();
-        if (before != ctx->device) cudaSetDevice(before);
-        return st;
+        return body();
     } catch (const std::bad_alloc&) {
         return KT_ERR_OUT_OF_MEMORY;
     } catch (...) {
