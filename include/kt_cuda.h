@@ -472,7 +472,9 @@ kt_status kt_kv8_store(kt_ctx* ctx, const kt_kv8_cache* cache, const float* k_de
 /* Scratch of kt_kv8_attention and kt_kv8_evict for a cache of these sizes (weights:
  * the cache keeps weights, so attention may accumulate them and tokens may be
  * evicted); its first 4096 bytes must be zero before its first use (they hold counters
- * that every call leaves at zero), and calls that share it must be ordered. */
+ * that every call leaves at zero), and calls that share it must be ordered.  With weights
+ * and few rows a call it is dominated by batch * rows_per_seq * heads * capacity floats,
+ * the scores of one call. */
 size_t kt_kv8_scratch_bytes(int32_t batch, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
                             int32_t capacity, int32_t weights);
 

@@ -326,10 +326,11 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool real)
 // code read before it is read before what others write after it; it comes once the last
 // round's writes, which it also waits for, are long under way (16 sequences x 8 heads
 // with selection: 87 us, ahead of the search for the largest 89, with a relaxed arrival,
-// which promises no order, 85).  Where there are few heads, a cluster of up to 8 CTAs
-// shares each.  16 sequences x 8 heads of 128, 4000 of 8k slots kept:
-// 65 us for 262 MB, 4.0 TB/s; about 9 instructions a code, issued in 58% of the cycles.
-// (Without the copies ahead 84 us, with five CTAs on an SM, whose registers spill, 77.)
+// which promises no order, 85, events around cold calls).  Where there are few heads, a cluster of up to 8 CTAs
+// shares each.  16 sequences x 8 heads of 128, 4000 of 8k slots kept: 68 us for 262 MB,
+// 3.9 TB/s; about 9 instructions a code, issued in 55% of the cycles.  (With the relaxed
+// arrival 65; from there, without the copies ahead 84 us, with five CTAs on an SM, whose
+// registers spill, 77.)
 constexpr int kUnit = 64;
 constexpr int kMoveWarps = 4;
 template <int kPieces>

@@ -611,10 +611,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(Kv8Attention
 }
 
 // The weight of each slot where the rows are few, from the scores and row sums that the
-// attention left: w_j += sum over vectors of 2^(s_j - lse).  Bound by memory, the scores
-// mostly from L2: 16 sequences of 130 to 8190 slots, 32 heads over 8, take 51.7 us with
-// their attention.  (Adding in the attention would need the row sums before they are
-// known.)
+// attention left: w_j += sum over vectors of 2^(s_j - lse).  Bound by latency where the
+// scores are few and in L2: 16 sequences of 130 to 8190 slots, 32 heads over 8 (8.5 MB)
+// 8.5 us beside 43 of their attention; by memory where they are many: 64 sequences of 16k
+// (131 MB, written and read) 118 us beside 371.  (Adding in the attention would need the
+// row sums before they are known.)
 __global__ void __launch_bounds__(256) kv8_add_weights_kernel(Kv8Attention a, const float* __restrict__ scores,
                                                               const float* __restrict__ lse) {
     dev::pdl_wait();
@@ -847,7 +848,9 @@ namespace {
 // head_dim 128 and the codes in L2.  The one on tcgen05 gives 128 vectors to a CTA: 2 us
 // for 128 slots of a wave of 148, or of their part where fewer share the slots out.
 // (30 rows of 32 heads over 8, one sequence of 30000 slots: 171 us here, 55 there; 17
-// rows, 2000 slots: 23 us here, 25 there.)
+// rows, 2000 slots: 23 us here, 25 there.)  Smaller head_dims go by the same numbers, which
+// keep this file's kernel too short there: 1 sequence of 500 slots, 14 heads over 2 of 64,
+// 16 rows: 11.7 us here, 16.1 there, and there it runs.
 // Both grow with the lengths, which only the device knows and which drop out:
 //   sequences x kv_heads x eights x 4 x 1.3 ns  against  waves x 2 us.
 // (The choice must not ask whether weights are accumulated: a context has the same bits

@@ -34,8 +34,8 @@
 //
 // Bound by turns by the products and by the exponentials with the cut of P into terms: a
 // tile takes about 3700 clocks, its products 2048.  2 sequences x 509 rows x 32 heads
-// of 128 over 1500 to 3508 slots: 102 us, 37.6 GFLOP as fp32 counts them, 369 TFLOP/s, or
-// 740 with both terms.  (Sixteen softmax warps and two issuing ones 112 us where these
+// of 128 over 1500 to 3508 slots: 102.5 us, 37.6 GFLOP as fp32 counts them, 367 TFLOP/s, or
+// 734 with both terms.  (Sixteen softmax warps and two issuing ones 112 us where these
 // took 109.)  A CTA spends about 7 us on entering and 3 on leaving.
 #include <cuda_fp16.h>
 
