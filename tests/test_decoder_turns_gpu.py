@@ -151,8 +151,7 @@ def test_penalties_in_the_middle_of_a_text(kt, oracle):
     for q in range(2):
         assert seen(late, q) == seen(early, q)
     late.penalize(presence=1e6, history=4)
-    line = sorted(t for t in late._history[0].tolist() if t >= 0)[-4:]
-    assert len(seen(late)[0]) == 4 and set(seen(late)[0]) <= set(seen(early)[0]) and line is not None
+    assert len(seen(late)[0]) == 4 and set(seen(late)[0]) <= set(seen(early)[0])
     # generate, one sequence: prompt tokens count as prompt
     one = decoder(max_seq=64, kv_bits=8)
     out = one.generate(text[0], 8)
