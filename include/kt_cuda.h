@@ -511,6 +511,77 @@ kt_status kt_kv8_advance(kt_ctx* ctx, int32_t* lengths_dev, int32_t batch, int32
 kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int32_t recent, void* scratch_dev,
                        void* stream);
 
+/* ------------------------------------------------------------ paged key/value cache in 16 bits
+ * (no reference counterpart: KVCache.kt:3-59 holds fp32 in one block a sequence)
+ *   keys, values  [layers][pages][kv_heads][page][head_dim] of bf16 or fp16
+ *   table int32 [batch][width], rows table_stride apart: slot s of sequence b is slot
+ *          s % page of page table[b][s / page] of every layer; sequences may share pages
+ *   lengths int32 [batch]: tokens held, in slots 0..lengths[b]-1
+ * table and lengths are device memory read by the kernels (a captured step replays at any
+ * length and after any change of pages); no call below changes them (kt_kv8_advance moves
+ * lengths on).  An entry outside 0..pages-1 is no page: tokens for it are dropped, no row
+ * sees its slots.  A call's row t of sequence b is the token in slot lengths[b] + t.  Rows
+ * t >= counts[b] (counts_dev NULL: rows_per_seq everywhere) are no tokens, nor are rows past
+ * slot width * page.  head_dim is a multiple of 16 in 64..128, page 16, 32, 64 or 128, batch
+ * at most 32767, width * page at most 2^30, keys and values 16-byte aligned; else
+ * KT_ERR_INVALID_ARGUMENT. */
+enum { KT_FP32 = 0, KT_BF16 = 1, KT_FP16 = 2 };
+typedef struct {
+    void* keys;
+    void* values;
+    const int32_t* table;
+    const int32_t* lengths;
+    int32_t layers, batch, kv_heads, head_dim, pages, page, width, table_stride, dtype;
+} kt_paged_cache;
+
+/* Rotates and stores new tokens of one layer.  Row r = b * rows_per_seq + t of q, k and v
+ * (fp32, `heads`, kv_heads and kv_heads heads of head_dim, rows q_stride, k_stride and
+ * v_stride floats apart) is at position p = lengths[b] + (depths_dev ? depths_dev[r] : t);
+ * the pairs (x, y) = (head[i], head[i + head_dim/2]) of queries and keys become
+ *   (x cos - y sin, x sin + y cos) of the angle p * inv_freq[i], its product exact,
+ * rounded once to the cache's type.  Keys and values go into their slots, queries into
+ * q_out_dev [batch * rows_per_seq][heads * head_dim] of the cache's type (8-byte aligned;
+ * rows that are no tokens get zeros).  q NULL with heads 0: no queries.  A token without a
+ * page sets KT_ERR_INVALID_ARGUMENT in *status_dev (NULL: not reported). */
+kt_status kt_paged_append(kt_ctx* ctx, const kt_paged_cache* cache, int32_t layer, const float* q_dev,
+                          const float* k_dev, const float* v_dev, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                          int32_t heads, const float* inv_freq_dev, int32_t rows_per_seq, const int32_t* counts_dev,
+                          const int32_t* depths_dev, void* q_out_dev, int32_t* status_dev, void* stream);
+
+/* Scratch of kt_paged_attention, the same for every call; its first 4096 bytes must be zero
+ * before its first use (every call leaves them at zero), and calls that share it must be
+ * ordered. */
+size_t kt_paged_scratch_bytes(void);
+
+/* Attention of one layer over what is held and this call's tokens, which kt_paged_append
+ * has stored: row t of sequence b sees slots 0..lengths[b]-1 and, of the new tokens u,
+ * those up to itself or, with visible_dev (int32 words [batch][rows_per_seq][(rows_per_seq
+ * + 31) / 32], at most 1024 rows a sequence), those of bits u % 32 of words u / 32:
+ *   out[row][head] = softmax(scale * q . k) . v,  0 for a row that sees nothing.
+ * q: rows of `heads` heads of the cache's type, rows q_stride elements apart; heads /
+ * kv_heads query heads share a key/value head.  out_dev [batch * rows_per_seq][heads *
+ * head_dim] of the cache's type or fp32 (out_dtype).  Rows that are no tokens give zeros.
+ * Scores and sums are fp32, probabilities are rounded to the cache's type.  What a row does
+ * not see has no part in it, infinities and NaN included; a value that is not finite makes
+ * the rows that see it NaN. */
+kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t layer, const void* q_dev,
+                             int64_t q_stride, void* out_dev, int32_t out_dtype, int32_t rows_per_seq,
+                             const int32_t* counts_dev, const uint32_t* visible_dev, int32_t heads, float scale,
+                             void* scratch_dev, void* stream);
+
+/* The accepted path of drafted trees whose nodes were one call's rows: tokens, parents and
+ * choices int32 [batch][rows_per_seq] (at most 1024) hold each node's token, its parent's
+ * index (smaller than its own; node 0 is the root) and the token chosen after it.  From node
+ * 0 on, the path goes to the lowest child whose token is its parent's choice.  The keys and
+ * values of the path's nodes move to slots lengths[b], lengths[b] + 1, ... in every layer;
+ * taken[b] = nodes of the path (0 where counts[b] is 0), accepted[b][i] = the choice after
+ * its node i, -1 behind its end.  kt_kv8_advance with counts `taken` then moves lengths on.
+ * A node without a page sets KT_ERR_INVALID_ARGUMENT in *status_dev (NULL: not reported). */
+kt_status kt_paged_accept(kt_ctx* ctx, const kt_paged_cache* cache, const int32_t* tokens_dev,
+                          const int32_t* parents_dev, const int32_t* choices_dev, int32_t rows_per_seq,
+                          const int32_t* counts_dev, int32_t* accepted_dev, int32_t* taken_dev, int32_t* status_dev,
+                          void* stream);
+
 /* ------------------------------------------------------------ logits before the choice of a token
  * (no reference counterpart; the choice is argmaxOfLastToken, Transformer.kt:255-266)
  * For each row and token id i, in this order, each step rounded to fp32:

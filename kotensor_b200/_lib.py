@@ -21,6 +21,8 @@ KT_ERR_UNSUPPORTED = 5
 KT_ERR_NCCL = 6
 KT_ERR_IO = 7
 
+KT_FP32, KT_BF16, KT_FP16 = 0, 1, 2
+
 KT_PATH_GEMV, KT_PATH_GENERIC, KT_PATH_TENSOR_CORE, KT_PATH_GEMV_MMA = 0, 1, 2, 3
 
 
@@ -63,6 +65,15 @@ class KtKv8Cache(ctypes.Structure):
         ("weights", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("batch", ctypes.c_int32),
         ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("capacity", ctypes.c_int32),
         ("block", ctypes.c_int32),
+    ]
+
+
+class KtPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+        ("layers", ctypes.c_int32), ("batch", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("pages", ctypes.c_int32), ("page", ctypes.c_int32), ("width", ctypes.c_int32), ("table_stride", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
     ]
 
 
@@ -154,6 +165,10 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "kt_kv8_attention": ([P, ctypes.POINTER(KtKv8Cache), P, I64, P, I32, P, I32, F32, I32, P, P], I32),
     "kt_kv8_advance": ([P, P, I32, I32, P, I32, P], I32),
     "kt_kv8_evict": ([P, ctypes.POINTER(KtKv8Cache), I32, I32, P, P], I32),
+    "kt_paged_append": ([P, ctypes.POINTER(KtPagedCache), I32, P, P, P, I64, I64, I64, I32, P, I32, P, P, P, P, P], I32),
+    "kt_paged_scratch_bytes": ([], SZ),
+    "kt_paged_attention": ([P, ctypes.POINTER(KtPagedCache), I32, P, I64, P, I32, I32, P, P, I32, F32, P, P], I32),
+    "kt_paged_accept": ([P, ctypes.POINTER(KtPagedCache), P, P, P, I32, P, P, P, P, P], I32),
     "kt_logits_process": ([P, ctypes.POINTER(KtLogitsArgs), P], I32),
     "kt_st_open": ([ctypes.c_char_p, PP], I32),
     "kt_st_close": ([P], I32),

@@ -1,0 +1,228 @@
+// kt_paged.h -- the paged 16-bit key/value cache as its kernels see it, the list of
+// tiles that its attention kernels share out, and their launchers (kt_paged.cu,
+// kt_paged_attention.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kt_kv8.h"  // c_entry, launch_dependent, allow_shared
+
+namespace kt {
+
+using Paged = kt_paged_cache;  // passed to kernels by value
+
+// Scratch layout (kt_paged_scratch_bytes): a counter for each CTA, zero between calls, then
+// two parts of an item for each CTA.
+constexpr size_t kPagedCounterBytes = 4096;  // (include/kt_cuda.h and paged.py give this number)
+constexpr int kPagedMostCtas = static_cast<int>(kPagedCounterBytes / sizeof(int32_t));
+
+struct PagedAttention {
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* counts;    // NULL: rows everywhere
+    const uint32_t* visible;  // NULL: row t sees the new tokens 0..t
+    const void* q;
+    void* out;
+    void* scratch;
+    int64_t q_stride;
+    int32_t batch, kv_heads, head_dim, pages, page_shift, table_stride, capacity;
+    int32_t rows, heads, group, words;  // rows of a sequence, words of a row of `visible`
+    float factor;                       // scale * log2(e)
+    int32_t out_f32, aligned;           // aligned: bit 0 pairs of q, bit 1 16 bytes of out
+};
+cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttention& a, int sm_count, int32_t* err,
+                                   cudaStream_t s);
+size_t paged_part_bytes();
+
+#ifdef __CUDACC__
+namespace paged {
+
+// Tokens that sequence b holds, and rows of this call that are tokens, whatever the
+// caller left in the arrays.
+__device__ __forceinline__ int held_of(const int32_t* lengths, int b, int capacity) {
+    return min(max(lengths[b], 0), capacity);
+}
+__device__ __forceinline__ int rows_of(const int32_t* counts, int b, int rows) {
+    return counts == nullptr ? rows : min(max(counts[b], 0), rows);
+}
+
+// An item of the attention's work: kVectors query vectors (rows x heads of a group, in
+// row order) of one sequence and key/value head, over tiles of kTile slots.
+struct Item {
+    int entry;           // sequence * vector tiles + vector tile
+    int b, head, v0, valid;  // first vector, how many there are
+    int held, count;     // tokens held, rows that are tokens
+    int sees, tiles;     // slots the last vector sees
+    int64_t base;        // index of the item's first unit in the list of all
+};
+
+// The list of all tiles, sequences first, then vector tiles, then heads; an item is kStart
+// units, what entering it costs, and one for each tile.  Equal runs of units go to the
+// CTAs: ragged batches, single long sequences and the triangle of a prompt load every SM
+// alike.  Lengths are read here, on the device, so a captured launch fits any.
+template <int kVectors, int kTile, int kStart>
+struct WorkList {
+    const PagedAttention& a;
+    const int vts;
+    int64_t ctas, share, spare, begin, end;
+
+    __device__ WorkList(const PagedAttention& args)
+        : a(args), vts((args.rows * args.group + kVectors - 1) / kVectors), ctas(0), share(0), spare(0), begin(0), end(0) {}
+
+    __device__ void load(Item& it, int entry) const {  // all but head and base
+        it.entry = entry;
+        it.b = entry / vts;
+        it.v0 = (entry - it.b * vts) * kVectors;
+        it.held = held_of(a.lengths, it.b, a.capacity);
+        it.count = min(rows_of(a.counts, it.b, a.rows), a.capacity - it.held);
+        it.valid = min(kVectors, it.count * a.group - it.v0);
+        it.sees = it.valid <= 0 ? 0 : a.visible ? it.held + it.count : it.held + (it.v0 + it.valid - 1) / a.group + 1;
+        it.tiles = (it.sees + kTile - 1) / kTile;
+    }
+    __device__ int64_t run_begin(int64_t cta) const { return cta * share + min(cta, spare); }
+    __device__ int cta_of(int64_t i) const {  // the CTA whose run holds unit i
+        const int64_t longer = spare * (share + 1);
+        return static_cast<int>(i < longer ? i / (share + 1) : spare + (i - longer) / share);
+    }
+    // By all threads of the CTA: shares out the list; false: nothing for this CTA.  `first`:
+    // the item its run begins in.  A CTA gets at least kLeast tiles or an item.
+    template <int kLeast>
+    __device__ bool start(Item& first) {
+        __shared__ int64_t sums[33];
+        __shared__ int64_t counts[33];
+        __shared__ int64_t found[2];
+        const int threads = blockDim.x, warps = threads / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+        const int entries = a.batch * vts, each = (entries + threads - 1) / threads;
+        const int from = min(entries, static_cast<int>(threadIdx.x) * each), to = min(entries, from + each);
+        int64_t units = 0, items = 0;
+        for (int e = from; e < to; ++e) {
+            load(first, e);
+            if (first.tiles > 0) units += first.tiles + kStart, ++items;
+        }
+        units *= a.kv_heads, items *= a.kv_heads;
+        int64_t upto = units;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        int64_t many = items;
+        for (int o = 16; o > 0; o >>= 1) many += __shfl_xor_sync(0xffffffffu, many, o);
+        if (lane == 31) sums[warp] = upto;
+        if (lane == 0) counts[warp] = many;
+        __syncthreads();
+        int64_t before = upto - units, total = 0;
+        items = 0;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+            items += counts[w];
+        }
+        if (items == 0) return false;
+        ctas = min(static_cast<int64_t>(gridDim.x), max(items, (total - items * kStart) / kLeast));
+        share = total / ctas;
+        spare = total - share * ctas;
+        if (blockIdx.x >= ctas) return false;
+        begin = run_begin(blockIdx.x);
+        end = run_begin(blockIdx.x + 1);
+        if (before <= begin && begin < before + units) {  // one thread
+            for (int e = from; e < to; ++e) {
+                load(first, e);
+                const int64_t n = first.tiles > 0 ? static_cast<int64_t>(first.tiles + kStart) * a.kv_heads : 0;
+                if (begin < before + n) {
+                    found[0] = e;
+                    found[1] = before;
+                    break;
+                }
+                before += n;
+            }
+        }
+        __syncthreads();
+        load(first, static_cast<int>(found[0]));
+        first.head = static_cast<int>((begin - found[1]) / (first.tiles + kStart));
+        first.base = found[1] + static_cast<int64_t>(first.head) * (first.tiles + kStart);
+        return true;
+    }
+    // Tiles [from, to) of the item are this CTA's.
+    __device__ int from(const Item& it) const {
+        return static_cast<int>(max(static_cast<int64_t>(0), begin - it.base - kStart));
+    }
+    __device__ int to(const Item& it) const {
+        return static_cast<int>(min(static_cast<int64_t>(it.tiles), max(static_cast<int64_t>(0), end - it.base - kStart)));
+    }
+    // The item after `it`; false: the run ends before it.
+    __device__ bool next(Item& it) const {
+        it.base += it.tiles + kStart;
+        if (it.base >= end) return false;
+        if (++it.head < a.kv_heads) return true;
+        it.head = 0;
+        const int64_t base = it.base;
+        do load(it, it.entry + 1);
+        while (it.tiles == 0);  // (units are left, so a later entry has tiles)
+        it.base = base;
+        return true;
+    }
+};
+
+// Which of `n` (at most 32) slots from `slot` on row t sees: bit i for slot + i.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen_bits(const PagedAttention& a, const Item& it, int t, int slot) {
+    if (a.visible == nullptr) return low_bits(min(it.held + t + 1, it.held + it.count) - slot);
+    uint32_t bits = low_bits(it.held - slot);
+    const int u = slot - it.held;  // the new token in `slot`
+    if (u > -32 && u < it.count) {
+        const uint32_t* row = a.visible + (static_cast<int64_t>(it.b) * a.rows + t) * a.words;
+        uint32_t fresh;
+        if (u < 0) {
+            fresh = row[0] << -u;
+        } else {
+            const int w = u / 32, shift = u % 32;
+            fresh = __funnelshift_r(row[w], w + 1 < a.words ? row[w + 1] : 0u, shift);
+        }
+        bits |= fresh & low_bits(it.count - u) & ~low_bits(-u);
+    }
+    return bits;
+}
+
+__device__ __forceinline__ bool wait_counted(uint32_t bar, uint32_t parity) {  // false after some seconds
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 25); ++i)
+        if (dev::mbar_try_wait(bar, parity)) return true;
+    return false;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16-bit types: pairs, exponents.
+template <typename T>
+struct Half16;
+template <>
+struct Half16<__half> {
+    static constexpr uint32_t kExponent = 0x7c007c00u;
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+template <>
+struct Half16<__nv_bfloat16> {
+    static constexpr uint32_t kExponent = 0x7f807f80u;
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+// Whether one of a word's two values is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    constexpr uint32_t e = Half16<T>::kExponent;
+    return (w & e & 0xffffu) == (e & 0xffffu) || (w & e & 0xffff0000u) == (e & 0xffff0000u);
+}
+
+}  // namespace paged
+#endif
+
+}  // namespace kt

@@ -1,0 +1,433 @@
+// kt_paged_attention.cu -- attention over the paged 16-bit key/value cache, for few query
+// vectors a key/value head (single tokens).
+//
+// Row t of sequence b with n = lengths[b]: for each query head, over the slots j it sees
+// (all j < n, and of this call's tokens those that its mask or the order of rows allows),
+//   s_j = scale * (q . K_j),  out = sum_j softmax(s)_j V_j,   0 where it sees nothing.
+#include <algorithm>
+
+#include "kt_paged.h"
+
+namespace kt {
+namespace {
+
+using namespace paged;
+
+constexpr int kWarps = 4;                        // that compute; one more copies
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kVectors = 16;                     // query vectors of an item (the product's M)
+constexpr int kTile = 64;                        // slots of a tile, 16 to a warp
+constexpr int kStart = 2;                        // tiles that entering an item costs
+constexpr int kLeast = 4;                        // tiles that are worth a CTA
+// Probabilities are kept 2^kLift times larger: in fp16 those down to 2^-36 of the largest
+// stay clear of underflow; the factor cancels in the division by their sum.
+constexpr float kLift = 12.0f;
+
+template <int HDP>
+struct RowsShape {
+    static constexpr int kBlocks = HDP / 64;               // blocks of 64 dims: swizzled rows of 128 bytes
+    static constexpr int kUnit = kBlocks * kTile * 128;    // the keys or the values of a tile
+    static constexpr int kUnits = 80 * 1024 / kUnit;       // in the ring: keys, values, keys, ...
+    static constexpr int kPitch = HDP + 4;
+    static constexpr int kArea = kUnits * kUnit;           // sums of two warps
+    static constexpr int kStats = kArea + 2 * kVectors * kPitch * 4;  // largest score, sum of each warp's vectors
+    static constexpr int kTotals = kStats + 2 * kWarps * kVectors * 4;
+    static constexpr int kBars = kTotals + 2 * kVectors * 4;
+    static constexpr int kValid = kBars + 16 * kUnits;     // boxes of a unit that have a page
+    static constexpr int kSmem = 1024 + kValid + 4 * kUnits;
+    static constexpr int kPart = kVectors * (HDP + 2);     // floats of a part: sums, largest scores, totals
+    static_assert(2 * (kSmem + 1024) <= 233472, "two CTAs on an SM");
+};
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void matrices(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void matrices_turned(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Sums over the parts' own references -> the common one's (0 where nothing was summed).
+__device__ __forceinline__ float weigh(float reference, float sum, float common) {
+    return sum == 0.0f ? 0.0f : ex2(reference - common);
+}
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_constant__ CUtensorMap k_map,
+                                                                 const __grid_constant__ CUtensorMap v_map,
+                                                                 const __grid_constant__ PagedAttention a,
+                                                                 int32_t* __restrict__ err) {
+    using S = RowsShape<HDP>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ int last_cta;
+    const uint32_t raw = dev::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    unsigned char* const smem = smem_raw + (base - raw);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, d = a.head_dim;
+    auto full = [&](int x) { return base + S::kBars + 16 * x; };
+    auto empty = [&](int x) { return base + S::kBars + 16 * x + 8; };
+    volatile uint32_t* const with_page = reinterpret_cast<uint32_t*>(smem + S::kValid);
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < S::kUnits; ++x) {
+            dev::mbar_init(full(x), 1);
+            dev::mbar_init(empty(x), kWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    dev::pdl_wait();
+    dev::pdl_launch_dependents();
+    // rows that are no tokens
+    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * (kWarps + 1) + warp) * 32; r0 < static_cast<int64_t>(a.batch) * a.rows;
+         r0 += static_cast<int64_t>(gridDim.x) * kThreads) {
+        bool token = true;
+        if (r0 + lane < static_cast<int64_t>(a.batch) * a.rows) {
+            const int b = static_cast<int>((r0 + lane) / a.rows), t = static_cast<int>((r0 + lane) % a.rows);
+            token = t < min(rows_of(a.counts, b, a.rows), a.capacity - held_of(a.lengths, b, a.capacity));
+        }
+        for (uint32_t none = __ballot_sync(0xffffffffu, !token); none != 0; none &= none - 1) {
+            const int64_t at = (r0 + __ffs(none) - 1) * a.heads * d;
+            for (int i = lane; i < a.heads * d; i += 32) {
+                if (a.out_f32) static_cast<float*>(a.out)[at + i] = 0.0f;
+                else static_cast<uint16_t*>(a.out)[at + i] = 0;
+            }
+        }
+    }
+    WorkList<kVectors, kTile, kStart> work(a);
+    Item it;
+    if (!work.template start<kLeast>(it)) return;  // (its barriers also publish the mbarriers)
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {  // a lane that has given up goes on without waiting
+        if (ok && !wait_counted(bar, parity)) ok = false;
+    };
+
+    if (warp == kWarps) {
+        // Copies: a lane has a box (64 dims of the slots of a page, at most a tile's) of the keys' or values' unit.
+        const int box = min(kTile, 1 << a.page_shift), boxes = kTile / box;  // 16, 32 or 64 slots; 4, 2 or 1 to a tile
+        const int mine = lane % boxes, block = lane / boxes % S::kBlocks;
+        const bool copies = lane < boxes * S::kBlocks;
+        int64_t unit = 0;
+        do {
+            for (int tile = work.from(it), to = work.to(it); tile < to; ++tile) {
+                const int slot = tile * kTile + mine * box;
+                int page = -1;
+                if (copies && slot < it.sees) page = a.table[static_cast<int64_t>(it.b) * a.table_stride + (slot >> a.page_shift)];
+                const bool here = page >= 0 && page < a.pages;
+                const uint32_t who = __ballot_sync(0xffffffffu, here);
+                const int row = here ? ((page * a.kv_heads + it.head) << a.page_shift) + (slot & ((1 << a.page_shift) - 1)) : 0;
+#pragma unroll
+                for (int v = 0; v < 2; ++v, ++unit) {
+                    const int x = static_cast<int>(unit % S::kUnits);
+                    if (unit >= S::kUnits) wait(empty(x), (unit / S::kUnits - 1) & 1);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    if (lane == 0) {
+                        with_page[x] = who & ((1u << boxes) - 1u);
+                        dev::mbar_expect_tx(full(x), __popc(who) * box * 128);
+                    }
+                    __syncwarp();
+                    if (here)
+                        dev::tma_load_2d(base + x * S::kUnit + block * (kTile * 128) + mine * box * 128, v ? &v_map : &k_map,
+                                         block * 64, row, full(x));
+                }
+                if (!__all_sync(0xffffffffu, ok)) break;
+            }
+        } while (__all_sync(0xffffffffu, ok) && work.next(it));
+        // no copy is in flight past this point, also where a wait has given up
+        for (int64_t u = max(static_cast<int64_t>(0), unit - S::kUnits); u < unit; ++u)
+            if (!wait_counted(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1)) ok = false;
+        if (!ok) atomicOr(err, 1);
+        return;
+    }
+
+    const int r8 = lane / 4, t4 = lane % 4;
+    float* const area = reinterpret_cast<float*>(smem + S::kArea);
+    float* const stats = reinterpret_cast<float*>(smem + S::kStats);    // [warp][vector]: largest scores, then sums
+    float* const totals = reinterpret_cast<float*>(smem + S::kTotals);  // [vector]
+    float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedCounterBytes);
+    int64_t unit = 0;
+    do {
+        const int from = work.from(it), to = work.to(it);
+        if (from >= to) continue;
+        // this thread's vectors, r8 and r8 + 8 of the item, and their queries
+        uint32_t q[HDP / 16][4];
+        int t[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int vec = it.v0 + r8 + 8 * i, row = vec / a.group;
+            const bool real = r8 + 8 * i < it.valid;
+            t[i] = real ? row : -1;
+            const uint16_t* from_q = static_cast<const uint16_t*>(a.q) + (static_cast<int64_t>(it.b) * a.rows + row) * a.q_stride +
+                                     static_cast<int64_t>(it.head * a.group + vec - row * a.group) * d;
+#pragma unroll
+            for (int s = 0; s < HDP / 8; ++s) {
+                const int dim = 8 * s + 2 * t4;
+                uint32_t w = 0;
+                if (real && dim < d)
+                    w = a.aligned & 1 ? *reinterpret_cast<const uint32_t*>(from_q + dim)
+                                      : from_q[dim] | static_cast<uint32_t>(from_q[dim + 1]) << 16;
+                q[s / 2][i + 2 * (s % 2)] = w;
+            }
+        }
+        // slots that all of the item's vectors see
+        const int clear = a.visible ? it.held : min(it.held + it.v0 / a.group + 1, it.sees);
+        float o[HDP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < HDP / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        for (int tile = from; tile < to; ++tile, unit += 2) {
+            const int kx = static_cast<int>(unit % S::kUnits), vx = static_cast<int>((unit + 1) % S::kUnits);
+            const int slot = tile * kTile + warp * 16;
+            float s[2][4] = {};
+            wait(full(kx), (unit / S::kUnits) & 1);
+            __syncwarp();
+            if (slot < it.sees) {
+                const uint32_t k_row = base + kx * S::kUnit + (warp * 16 + lane % 8 + lane / 16 * 8) * 128;
+#pragma unroll
+                for (int i = 0; i < HDP / 16; ++i) {
+                    uint32_t m[4];
+                    matrices(k_row + i / 4 * (kTile * 128) + (((2 * (i % 4) + lane / 8 % 2) ^ (lane % 8)) << 4), m);
+                    mma<T>(s[0], q[i], m[0], m[1]);
+                    mma<T>(s[1], q[i], m[2], m[3]);
+                }
+            }
+            const uint32_t pages = with_page[kx];
+            __syncwarp();
+            if (lane == 0) dev::mbar_arrive(empty(kx));
+            uint32_t p[4] = {0, 0, 0, 0};
+            const bool page = pages >> (warp * 16 / min(kTile, 1 << a.page_shift)) & 1u;
+            const bool edge = slot + 16 > clear || !page;
+            uint32_t seen[2] = {0xffffu, 0xffffu};
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) seen[i] = t[i] >= 0 && page ? seen_bits(a, it, t[i], slot) & 0xffffu : 0u;
+            }
+            if (slot < it.sees) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float z[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {  // slots 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
+                        z[e] = s[e / 2][2 * i + e % 2] * a.factor;
+                        if (edge && !(seen[i] >> (2 * t4 + e % 2 + e / 2 * 8) & 1u)) z[e] = -INFINITY;
+                    }
+                    float high = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                    const float now = fmaxf(top[i], high), less = now == -INFINITY ? 0.0f : now - kLift;
+                    const float fade = top[i] == -INFINITY ? 0.0f : ex2(top[i] - now);
+                    top[i] = now;
+                    if (__any_sync(0xffffffffu, fade != 1.0f)) {
+                        sum[i] = sum[i] == 0.0f ? 0.0f : sum[i] * fade;
+#pragma unroll
+                        for (int j = 0; j < HDP / 8; ++j) o[j][2 * i] *= fade, o[j][2 * i + 1] *= fade;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        z[e] = ex2(z[e] - less);
+                        sum[i] += z[e];
+                    }
+                    p[i] = Half16<T>::pack(z[0], z[1]);
+                    p[i + 2] = Half16<T>::pack(z[2], z[3]);
+                }
+            }
+            wait(full(vx), ((unit + 1) / S::kUnits) & 1);
+            __syncwarp();
+            if (edge && slot < it.sees) {
+                // What no vector sees counts nothing, whatever it is, and a value that is not finite counts for those
+                // that see it alone: such rows of the tile become zeros, the rest is told by the sums.
+                uint32_t any = __reduce_or_sync(0xffffffffu, seen[0] | seen[1]);
+                const int row = lane / 2;
+                uint4* const line = reinterpret_cast<uint4*>(smem + vx * S::kUnit + (warp * 16 + row) * 128);
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < HDP / 16; ++i) {
+                    const int piece = lane % 2 * (HDP / 16) + i;
+                    const uint4 w = line[piece / 8 * (kTile * 128 / 16) + piece % 8];
+                    bad = bad || not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w);
+                }
+                uint32_t told = __ballot_sync(0xffffffffu, bad);
+                told = (told | told >> 1) & 0x55555555u;  // bit 2 * row
+                if (!(any >> row & 1u) || (told >> (2 * row) & 1u)) {
+#pragma unroll
+                    for (int i = 0; i < HDP / 16; ++i) {
+                        const int piece = lane % 2 * (HDP / 16) + i;
+                        line[piece / 8 * (kTile * 128 / 16) + piece % 8] = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                uint32_t rows = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) rows |= (told >> (2 * i) & 1u) << i;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (rows & seen[i]) sum[i] = __uint_as_float(0x7fc00000u);
+                __syncwarp();
+            }
+            if (slot < it.sees) {
+                const uint32_t v_row = base + vx * S::kUnit + (warp * 16 + lane % 16) * 128;
+#pragma unroll
+                for (int j = 0; j < HDP / 16; ++j) {
+                    uint32_t m[4];
+                    matrices_turned(v_row + j / 4 * (kTile * 128) + (((2 * (j % 4) + lane / 16) ^ (lane % 8)) << 4), m);
+                    mma<T>(o[2 * j], p, m[0], m[1]);
+                    mma<T>(o[2 * j + 1], p, m[2], m[3]);
+                }
+            }
+            if (edge) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy to these rows
+            __syncwarp();
+            if (lane == 0) dev::mbar_arrive(empty(vx));
+        }
+        // the warps' sums, brought to a common reference and added in a fixed order
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+            if (t4 == 0) {
+                stats[warp * kVectors + r8 + 8 * i] = top[i];
+                stats[(kWarps + warp) * kVectors + r8 + 8 * i] = sum[i];
+            }
+        }
+        compute_sync();
+        float common[2], by[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int v = r8 + 8 * i;
+            common[i] = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) common[i] = fmaxf(common[i], stats[w * kVectors + v]);
+            by[i] = weigh(top[i], sum[i], common[i]);
+            if (warp == 0 && t4 == 0) {
+                float total = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float m = stats[w * kVectors + v], l = stats[(kWarps + w) * kVectors + v];
+                    total += weigh(m, l, common[i]) * l;
+                }
+                totals[v] = common[i], totals[kVectors + v] = total;
+            }
+        }
+        float* const sums = area + (warp % 2) * (kVectors * S::kPitch);
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+            if (warp / 2 == 1 - step) {
+#pragma unroll
+                for (int j = 0; j < HDP / 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float2* const at = reinterpret_cast<float2*>(sums + (r8 + 8 * i) * S::kPitch + 8 * j + 2 * t4);
+                        const float2 f = step == 0 ? make_float2(0.0f, 0.0f) : *at;
+                        *at = make_float2(f.x + (by[i] == 0.0f ? 0.0f : o[j][2 * i] * by[i]), f.y + (by[i] == 0.0f ? 0.0f : o[j][2 * i + 1] * by[i]));
+                    }
+            }
+            compute_sync();
+        }
+        // dims dim .. dim + 3 of vector `vec`, from their sums and the vector's total
+        auto finish = [&](int vec, int dim, float4 y, float total) {
+            if (dim >= d) return;
+            const int v = it.v0 + vec, row = v / a.group;
+            const int64_t at = ((static_cast<int64_t>(it.b) * a.rows + row) * a.heads + it.head * a.group + v - row * a.group) * d + dim;
+            const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+            y.x *= scale, y.y *= scale, y.z *= scale, y.w *= scale;
+            if (a.out_f32) {
+                float* const to = static_cast<float*>(a.out) + at;
+                if (a.aligned & 2) *reinterpret_cast<float4*>(to) = y;
+                else to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
+            } else {
+                const uint2 w = make_uint2(Half16<T>::pack(y.x, y.y), Half16<T>::pack(y.z, y.w));
+                uint16_t* const to = static_cast<uint16_t*>(a.out) + at;
+                if (a.aligned & 2) *reinterpret_cast<uint2*>(to) = w;
+                else to[0] = w.x & 0xffffu, to[1] = w.x >> 16, to[2] = w.y & 0xffffu, to[3] = w.y >> 16;
+            }
+        };
+        const bool whole = from == 0 && to == it.tiles;
+        // the part of an item that an earlier CTA began is the CTA's part 0, of one that goes on its part 1
+        float* const part = parts + (static_cast<int64_t>(blockIdx.x) * 2 + (from == 0)) * S::kPart;
+        for (int e = threadIdx.x; e < it.valid * (HDP / 4); e += kWarps * 32) {
+            const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
+            float4 y = *reinterpret_cast<const float4*>(area + vec * S::kPitch + dim);
+            const float4 z = *reinterpret_cast<const float4*>(area + (kVectors + vec) * S::kPitch + dim);
+            y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+            if (whole) finish(vec, dim, y, totals[kVectors + vec]);
+            else __stcg(reinterpret_cast<float4*>(part + vec * HDP + dim), y);
+        }
+        if (!whole) {
+            if (threadIdx.x < 2 * kVectors) __stcg(part + kVectors * HDP + threadIdx.x, totals[threadIdx.x]);
+            const int c0 = work.cta_of(it.base + kStart), c1 = work.cta_of(it.base + kStart + it.tiles - 1);
+            int32_t* const counter = static_cast<int32_t*>(a.scratch) + c0;
+            __threadfence();
+            compute_sync();
+            if (threadIdx.x == 0) last_cta = dev::atomic_add_acq_rel(counter, 1) == c1 - c0;
+            compute_sync();
+            if (last_cta) {
+                __threadfence();
+                const int n = c1 - c0 + 1;
+                auto part_of = [&](int x) { return parts + ((static_cast<int64_t>(c0) + x) * 2 + (x == 0)) * S::kPart; };
+                for (int e = threadIdx.x; e < it.valid * (HDP / 4); e += kWarps * 32) {
+                    const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
+                    float m = -INFINITY, total = 0.0f;
+                    for (int x = 0; x < n; ++x) m = fmaxf(m, __ldcg(part_of(x) + kVectors * HDP + vec));
+                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                    for (int x = 0; x < n; ++x) {
+                        const float l = __ldcg(part_of(x) + kVectors * (HDP + 1) + vec);
+                        const float w = weigh(__ldcg(part_of(x) + kVectors * HDP + vec), l, m);
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(part_of(x) + vec * HDP + dim));
+                        total += w * l;
+                        if (w != 0.0f) y.x = fmaf(w, f.x, y.x), y.y = fmaf(w, f.y, y.y), y.z = fmaf(w, f.z, y.z), y.w = fmaf(w, f.w, y.w);
+                    }
+                    finish(vec, dim, y, total);
+                }
+                if (threadIdx.x == 0) *counter = 0;
+            }
+        }
+        compute_sync();  // the areas and last_cta are free again
+    } while (work.next(it));
+    if (!ok) atomicOr(err, 1);
+}
+
+template <typename T, int HDP>
+cudaError_t launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const PagedAttention& a, int sm_count,
+                        int32_t* err, cudaStream_t s) {
+    using S = RowsShape<HDP>;
+    static std::atomic<uint64_t> allowed{0};
+    const auto kernel = paged_rows_kernel<T, HDP>;
+    cudaError_t e = allow_shared(kernel, S::kSmem, allowed);
+    if (e != cudaSuccess) return e;
+    const int64_t items = static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors);
+    const int64_t most = std::max(items, items * ((a.capacity + kTile - 1) / kTile) / kLeast);
+    const int grid = static_cast<int>(std::min<int64_t>(std::min(2 * sm_count, kPagedMostCtas), most));
+    return launch_dependent(kernel, dim3(grid), dim3(kThreads), S::kSmem, s, k_map, v_map, a, err);
+}
+
+}  // namespace
+
+size_t paged_part_bytes() { return static_cast<size_t>(kPagedMostCtas) * 2 * RowsShape<128>::kPart * sizeof(float); }
+
+cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttention& a, int sm_count, int32_t* err,
+                                   cudaStream_t s) {
+    const int64_t rows = static_cast<int64_t>(c.pages) * c.kv_heads * c.page, row_bytes = 2ll * c.head_dim;
+    CUtensorMap maps[2];
+    for (int v = 0; v < 2; ++v)
+        if (!encode_tmap_2d(&maps[v], c.dtype == KT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                            static_cast<const char*>(v ? c.values : c.keys) + layer * rows * row_bytes, c.head_dim, rows, row_bytes,
+                            64, std::min(c.page, kTile), CU_TENSOR_MAP_SWIZZLE_128B))
+            return cudaErrorInvalidValue;
+    const bool bf16 = c.dtype == KT_BF16, wide = c.head_dim > 64;
+    const auto launch = bf16 ? wide ? launch_rows<__nv_bfloat16, 128> : launch_rows<__nv_bfloat16, 64>
+                             : wide ? launch_rows<__half, 128> : launch_rows<__half, 64>;
+    return launch(maps[0], maps[1], a, sm_count, err, s);
+}
+
+}  // namespace kt
