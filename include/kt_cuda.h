@@ -548,10 +548,10 @@ kt_status kt_paged_append(kt_ctx* ctx, const kt_paged_cache* cache, int32_t laye
                           int32_t heads, const float* inv_freq_dev, int32_t rows_per_seq, const int32_t* counts_dev,
                           const int32_t* depths_dev, void* q_out_dev, int32_t* status_dev, void* stream);
 
-/* Scratch of kt_paged_attention, the same for every call; its first 4096 bytes must be zero
+/* Scratch of kt_paged_attention on the context's GPU, the same for every call; its first 4096 bytes must be zero
  * before its first use (every call leaves them at zero), and calls that share it must be
  * ordered. */
-size_t kt_paged_scratch_bytes(void);
+size_t kt_paged_scratch_bytes(kt_ctx* ctx);
 
 /* Attention of one layer over what is held and this call's tokens, which kt_paged_append
  * has stored: row t of sequence b sees slots 0..lengths[b]-1 and, of the new tokens u,

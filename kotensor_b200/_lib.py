@@ -166,7 +166,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "kt_kv8_advance": ([P, P, I32, I32, P, I32, P], I32),
     "kt_kv8_evict": ([P, ctypes.POINTER(KtKv8Cache), I32, I32, P, P], I32),
     "kt_paged_append": ([P, ctypes.POINTER(KtPagedCache), I32, P, P, P, I64, I64, I64, I32, P, I32, P, P, P, P, P], I32),
-    "kt_paged_scratch_bytes": ([], SZ),
+    "kt_paged_scratch_bytes": ([P], SZ),
     "kt_paged_attention": ([P, ctypes.POINTER(KtPagedCache), I32, P, I64, P, I32, I32, P, P, I32, F32, P, P], I32),
     "kt_paged_accept": ([P, ctypes.POINTER(KtPagedCache), P, P, P, I32, P, P, P, P, P], I32),
     "kt_logits_process": ([P, ctypes.POINTER(KtLogitsArgs), P], I32),

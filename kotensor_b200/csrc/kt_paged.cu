@@ -236,7 +236,9 @@ kt_status kt_paged_append(kt_ctx* ctx, const kt_paged_cache* cache, int32_t laye
     });
 }
 
-size_t kt_paged_scratch_bytes(void) { return kPagedCounterBytes + paged_part_bytes(); }
+size_t kt_paged_scratch_bytes(kt_ctx* ctx) {
+    return ctx ? kPagedPartsAt + std::max(paged_rows_bytes(), paged_many_bytes(ctx->sm_count)) : 0;
+}
 
 kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t layer, const void* q, int64_t q_stride,
                              void* out, int32_t out_dtype, int32_t rows_per_seq, const int32_t* counts,
@@ -266,7 +268,8 @@ kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t l
         a.page_shift = cache->page == 16 ? 4 : cache->page == 32 ? 5 : cache->page == 64 ? 6 : 7;
         a.table_stride = cache->table_stride, a.capacity = cache->width * cache->page;
         a.rows = rows_per_seq, a.heads = heads, a.group = heads / cache->kv_heads, a.words = (rows_per_seq + 31) / 32;
-        a.factor = static_cast<float>(scale * 1.4426950408889634);
+        // (with a scale of 0 masked scores still have to be -inf, the others alike)
+        a.factor = scale == 0.0f ? 1e-38f : static_cast<float>(scale * 1.4426950408889634);
         a.out_f32 = out_dtype == KT_FP32;
         a.aligned = (reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 8 == 0 ? 1 : 0) | (aligned16(out) ? 2 : 0);
         return entry_launch(launch_paged_attention(*cache, layer, a, ctx->sm_count, ctx->d_error, static_cast<cudaStream_t>(stream)),

@@ -12,10 +12,13 @@ namespace kt {
 
 using Paged = kt_paged_cache;  // passed to kernels by value
 
-// Scratch layout (kt_paged_scratch_bytes): a counter for each CTA, zero between calls, then
-// two parts of an item for each CTA.
+// Scratch layout (kt_paged_scratch_bytes): a counter for each CTA of the kernel of few
+// vectors, zero between calls; the items that the kernel of many vectors has cut; the parts
+// of cut items, two for each CTA.
 constexpr size_t kPagedCounterBytes = 4096;  // (include/kt_cuda.h and paged.py give this number)
-constexpr int kPagedMostCtas = static_cast<int>(kPagedCounterBytes / sizeof(int32_t));
+constexpr size_t kPagedCutBytes = 8192, kPagedPartsAt = kPagedCounterBytes + kPagedCutBytes;
+constexpr int kPagedRowsCtas = 512, kPagedManyCtas = 256;  // of a launch, at most
+static_assert(kPagedRowsCtas * sizeof(int32_t) <= kPagedCounterBytes, "a counter each");
 
 struct PagedAttention {
     const int32_t* table;
@@ -31,9 +34,16 @@ struct PagedAttention {
     float factor;                       // scale * log2(e)
     int32_t out_f32, aligned;           // aligned: bit 0 pairs of q, bit 1 16 bytes of out
 };
+// Boxes of the tensor maps: 64 dims of the slots of a page, at most 64 of them.
+constexpr int kPagedBox = 64;
+// Which kernel runs, and its launch (kt_paged_attention.cu); the kernel of many vectors
+// (kt_paged_many.cu).
 cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttention& a, int sm_count, int32_t* err,
                                    cudaStream_t s);
-size_t paged_part_bytes();
+cudaError_t launch_paged_many(bool bf16, const CUtensorMap (&maps)[2], const PagedAttention& a, int sm_count, int32_t* err,
+                              cudaStream_t s);
+size_t paged_rows_bytes();
+size_t paged_many_bytes(int sm_count);
 
 #ifdef __CUDACC__
 namespace paged {
@@ -45,6 +55,32 @@ __device__ __forceinline__ int held_of(const int32_t* lengths, int b, int capaci
 }
 __device__ __forceinline__ int rows_of(const int32_t* counts, int b, int rows) {
     return counts == nullptr ? rows : min(max(counts[b], 0), rows);
+}
+
+// Zeros for the rows that are no tokens; by all warps of the grid.
+__device__ __forceinline__ void zero_rows(const PagedAttention& a) {
+    const int warps = blockDim.x / 32, lane = threadIdx.x % 32, width = a.heads * a.head_dim;
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.rows;
+    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / 32) * 32; r0 < rows;
+         r0 += static_cast<int64_t>(gridDim.x) * warps * 32) {
+        bool token = true;
+        if (r0 + lane < rows) {
+            const int b = static_cast<int>((r0 + lane) / a.rows), t = static_cast<int>((r0 + lane) % a.rows);
+            token = t < min(rows_of(a.counts, b, a.rows), a.capacity - held_of(a.lengths, b, a.capacity));
+        }
+        for (uint32_t none = __ballot_sync(0xffffffffu, !token); none != 0; none &= none - 1) {
+            const int64_t at = (r0 + __ffs(none) - 1) * width;
+            for (int i = lane; i < width; i += 32) {
+                if (a.out_f32) static_cast<float*>(a.out)[at + i] = 0.0f;
+                else static_cast<uint16_t*>(a.out)[at + i] = 0;
+            }
+        }
+    }
+}
+// Where the query and the result of an item's vector begin.
+__device__ __forceinline__ int64_t place_of(const PagedAttention& a, int b, int head, int v, int64_t stride) {
+    const int row = v / a.group;
+    return (static_cast<int64_t>(b) * a.rows + row) * stride + static_cast<int64_t>(head * a.group + v - row * a.group) * a.head_dim;
 }
 
 // An item of the attention's work: kVectors query vectors (rows x heads of a group, in
@@ -202,6 +238,7 @@ struct Half16;
 template <>
 struct Half16<__half> {
     static constexpr uint32_t kExponent = 0x7c007c00u;
+    static constexpr uint32_t kUmma = 0;  // the operands' type in tcgen05.mma's descriptor
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __half2 h = __floats2half2_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -210,6 +247,7 @@ struct Half16<__half> {
 template <>
 struct Half16<__nv_bfloat16> {
     static constexpr uint32_t kExponent = 0x7f807f80u;
+    static constexpr uint32_t kUmma = 1u << 7 | 1u << 10;
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -220,6 +258,34 @@ template <typename T>
 __device__ __forceinline__ bool not_finite(uint32_t w) {
     constexpr uint32_t e = Half16<T>::kExponent;
     return (w & e & 0xffffu) == (e & 0xffffu) || (w & e & 0xffff0000u) == (e & 0xffff0000u);
+}
+
+// Four, sixteen dims of a result, `at` elements into out (a multiple of 4, of 16).
+template <typename T>
+__device__ __forceinline__ void put4(const PagedAttention& a, int64_t at, float4 y) {
+    if (a.out_f32) {
+        float* const to = static_cast<float*>(a.out) + at;
+        if (a.aligned & 2) *reinterpret_cast<float4*>(to) = y;
+        else to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
+    } else {
+        const uint2 w = make_uint2(Half16<T>::pack(y.x, y.y), Half16<T>::pack(y.z, y.w));
+        uint16_t* const to = static_cast<uint16_t*>(a.out) + at;
+        if (a.aligned & 2) *reinterpret_cast<uint2*>(to) = w;
+        else to[0] = w.x & 0xffffu, to[1] = w.x >> 16, to[2] = w.y & 0xffffu, to[3] = w.y >> 16;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void put16(const PagedAttention& a, int64_t at, const float (&y)[16]) {
+    if (!a.out_f32 && (a.aligned & 2)) {
+        uint4* const to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            to[i] = make_uint4(Half16<T>::pack(y[8 * i], y[8 * i + 1]), Half16<T>::pack(y[8 * i + 2], y[8 * i + 3]),
+                               Half16<T>::pack(y[8 * i + 4], y[8 * i + 5]), Half16<T>::pack(y[8 * i + 6], y[8 * i + 7]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) put4<T>(a, at + i, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
+    }
 }
 
 }  // namespace paged

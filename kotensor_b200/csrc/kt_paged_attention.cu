@@ -91,22 +91,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
     }
     dev::pdl_wait();
     dev::pdl_launch_dependents();
-    // rows that are no tokens
-    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * (kWarps + 1) + warp) * 32; r0 < static_cast<int64_t>(a.batch) * a.rows;
-         r0 += static_cast<int64_t>(gridDim.x) * kThreads) {
-        bool token = true;
-        if (r0 + lane < static_cast<int64_t>(a.batch) * a.rows) {
-            const int b = static_cast<int>((r0 + lane) / a.rows), t = static_cast<int>((r0 + lane) % a.rows);
-            token = t < min(rows_of(a.counts, b, a.rows), a.capacity - held_of(a.lengths, b, a.capacity));
-        }
-        for (uint32_t none = __ballot_sync(0xffffffffu, !token); none != 0; none &= none - 1) {
-            const int64_t at = (r0 + __ffs(none) - 1) * a.heads * d;
-            for (int i = lane; i < a.heads * d; i += 32) {
-                if (a.out_f32) static_cast<float*>(a.out)[at + i] = 0.0f;
-                else static_cast<uint16_t*>(a.out)[at + i] = 0;
-            }
-        }
-    }
+    zero_rows(a);
     WorkList<kVectors, kTile, kStart> work(a);
     Item it;
     if (!work.template start<kLeast>(it)) return;  // (its barriers also publish the mbarriers)
@@ -117,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
 
     if (warp == kWarps) {
         // Copies: a lane has a box (64 dims of the slots of a page, at most a tile's) of the keys' or values' unit.
-        const int box = min(kTile, 1 << a.page_shift), boxes = kTile / box;  // 16, 32 or 64 slots; 4, 2 or 1 to a tile
+        const int box = min(kPagedBox, 1 << a.page_shift), boxes = kTile / box;  // 16, 32 or 64 slots; 4, 2 or 1 to a tile
         const int mine = lane % boxes, block = lane / boxes % S::kBlocks;
         const bool copies = lane < boxes * S::kBlocks;
         int64_t unit = 0;
@@ -157,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
     float* const area = reinterpret_cast<float*>(smem + S::kArea);
     float* const stats = reinterpret_cast<float*>(smem + S::kStats);    // [warp][vector]: largest scores, then sums
     float* const totals = reinterpret_cast<float*>(smem + S::kTotals);  // [vector]
-    float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedCounterBytes);
+    float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedPartsAt);
     int64_t unit = 0;
     do {
         const int from = work.from(it), to = work.to(it);
@@ -170,8 +155,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
             const int vec = it.v0 + r8 + 8 * i, row = vec / a.group;
             const bool real = r8 + 8 * i < it.valid;
             t[i] = real ? row : -1;
-            const uint16_t* from_q = static_cast<const uint16_t*>(a.q) + (static_cast<int64_t>(it.b) * a.rows + row) * a.q_stride +
-                                     static_cast<int64_t>(it.head * a.group + vec - row * a.group) * d;
+            const uint16_t* from_q = static_cast<const uint16_t*>(a.q) + place_of(a, it.b, it.head, vec, a.q_stride);
 #pragma unroll
             for (int s = 0; s < HDP / 8; ++s) {
                 const int dim = 8 * s + 2 * t4;
@@ -207,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) dev::mbar_arrive(empty(kx));
             uint32_t p[4] = {0, 0, 0, 0};
-            const bool page = pages >> (warp * 16 / min(kTile, 1 << a.page_shift)) & 1u;
+            const bool page = pages >> (warp * 16 / min(kPagedBox, 1 << a.page_shift)) & 1u;
             const bool edge = slot + 16 > clear || !page;
             uint32_t seen[2] = {0xffffu, 0xffffu};
             if (edge) {
@@ -336,20 +320,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
         // dims dim .. dim + 3 of vector `vec`, from their sums and the vector's total
         auto finish = [&](int vec, int dim, float4 y, float total) {
             if (dim >= d) return;
-            const int v = it.v0 + vec, row = v / a.group;
-            const int64_t at = ((static_cast<int64_t>(it.b) * a.rows + row) * a.heads + it.head * a.group + v - row * a.group) * d + dim;
+            const int64_t at = place_of(a, it.b, it.head, it.v0 + vec, static_cast<int64_t>(a.heads) * d) + dim;
             const float scale = total == 0.0f ? 0.0f : 1.0f / total;
             y.x *= scale, y.y *= scale, y.z *= scale, y.w *= scale;
-            if (a.out_f32) {
-                float* const to = static_cast<float*>(a.out) + at;
-                if (a.aligned & 2) *reinterpret_cast<float4*>(to) = y;
-                else to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
-            } else {
-                const uint2 w = make_uint2(Half16<T>::pack(y.x, y.y), Half16<T>::pack(y.z, y.w));
-                uint16_t* const to = static_cast<uint16_t*>(a.out) + at;
-                if (a.aligned & 2) *reinterpret_cast<uint2*>(to) = w;
-                else to[0] = w.x & 0xffffu, to[1] = w.x >> 16, to[2] = w.y & 0xffffu, to[3] = w.y >> 16;
-            }
+            put4<T>(a, at, y);
         };
         const bool whole = from == 0 && to == it.tiles;
         // the part of an item that an earlier CTA began is the CTA's part 0, of one that goes on its part 1
@@ -407,13 +381,13 @@ cudaError_t launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, cons
     if (e != cudaSuccess) return e;
     const int64_t items = static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors);
     const int64_t most = std::max(items, items * ((a.capacity + kTile - 1) / kTile) / kLeast);
-    const int grid = static_cast<int>(std::min<int64_t>(std::min(2 * sm_count, kPagedMostCtas), most));
+    const int grid = static_cast<int>(std::min<int64_t>(std::min(2 * sm_count, kPagedRowsCtas), most));
     return launch_dependent(kernel, dim3(grid), dim3(kThreads), S::kSmem, s, k_map, v_map, a, err);
 }
 
 }  // namespace
 
-size_t paged_part_bytes() { return static_cast<size_t>(kPagedMostCtas) * 2 * RowsShape<128>::kPart * sizeof(float); }
+size_t paged_rows_bytes() { return static_cast<size_t>(kPagedRowsCtas) * 2 * RowsShape<128>::kPart * sizeof(float); }
 
 cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttention& a, int sm_count, int32_t* err,
                                    cudaStream_t s) {
@@ -422,8 +396,9 @@ cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttenti
     for (int v = 0; v < 2; ++v)
         if (!encode_tmap_2d(&maps[v], c.dtype == KT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
                             static_cast<const char*>(v ? c.values : c.keys) + layer * rows * row_bytes, c.head_dim, rows, row_bytes,
-                            64, std::min(c.page, kTile), CU_TENSOR_MAP_SWIZZLE_128B))
+                            64, std::min(c.page, kPagedBox), CU_TENSOR_MAP_SWIZZLE_128B))
             return cudaErrorInvalidValue;
+    if (static_cast<int64_t>(a.rows) * a.group > kVectors) return launch_paged_many(c.dtype == KT_BF16, maps, a, sm_count, err, s);
     const bool bf16 = c.dtype == KT_BF16, wide = c.head_dim > 64;
     const auto launch = bf16 ? wide ? launch_rows<__nv_bfloat16, 128> : launch_rows<__nv_bfloat16, 64>
                              : wide ? launch_rows<__half, 128> : launch_rows<__half, 64>;

@@ -1,0 +1,663 @@
+// kt_paged_many.cu -- attention over the paged 16-bit key/value cache for many query
+// vectors a key/value head (drafted trees, prompts) on the 5th-generation tensor cores.
+#include <algorithm>
+
+#include "kt_paged.h"
+
+namespace kt {
+namespace {
+
+using namespace paged;
+
+constexpr int kLanes = 128;                // vectors of a stream (the MMA's M)
+constexpr int kVectors = 2 * kLanes;       // of an item
+constexpr int kTile = 128;                 // slots of a tile
+constexpr int kStart = 2;                  // tiles that entering an item costs
+constexpr int kLeast = 2;                  // tiles that are worth a CTA
+constexpr int kIssueWarp = 8, kCopyWarp = 9;  // after the softmax warps; the two after them do nothing
+constexpr int kThreads = 384;
+constexpr float kLift = 6.0f;    // probabilities are 2^kLift times larger: fp16 keeps them to 2^-30 of the reference
+constexpr float kSlack = 8.0f;   // the reference moves when a score passes it by this much (2^14 < fp16's largest)
+// Registers of a thread at the launch, and of each role's warps.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 104;
+static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs <= 12 * kLaunchRegs, "registers");
+static_assert(kSoftmaxRegs > kLaunchRegs && kOtherRegs < kLaunchRegs, "one role raises, the other lowers");
+
+template <int HDP>
+struct ManyShape {
+    static constexpr int kBlocks = HDP / 64;             // blocks of 64 dims: swizzled rows of 128 bytes
+    static constexpr int kUnit = kBlocks * kTile * 128;  // queries of a stream; keys or values of a tile
+    static constexpr int kRing = 2 * kUnit, kUnits = 4 * 128 / HDP;  // keys, values, keys, ...
+    static constexpr int kBad = kRing + kUnits * kUnit;  // slots of an edge tile whose values are not finite: [2][3][4] words
+    static constexpr int kStats = kBad + 128;            // of the second stream's vectors
+    static constexpr int kBars = kStats + 2 * kLanes * 4;
+    static constexpr int kSmem = 1024 + kBars + 16 * kUnits + 8 * 8 + 16;
+    static constexpr int kPart = kVectors * (HDP + 2);   // floats of a part: [HDP / 4][vector][4], references, sums
+    static constexpr uint32_t kO = 256;                  // tensor memory: scores (then P) of stream x at 128 x, its O
+    static_assert(kSmem <= 232448 && kO + 2 * HDP <= 512, "memories");
+};
+
+// An item that its CTA begins and later ones go on with, left for the merge.
+struct Cut {
+    int32_t parts, b, head, v0, valid, unused[3];
+};
+static_assert(sizeof(Cut) * kPagedManyCtas <= kPagedCutBytes, "a place each");
+
+__device__ __forceinline__ uint64_t desc_of(uint32_t addr, uint32_t lead) {
+    // 128-byte swizzle, atoms of 8 rows 1024 bytes apart, descriptor version 1
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 128 columns of this warp's 32 lanes, complete on return.  (One statement: between a load
+// and its wait the compiler may copy the registers, which do not hold the values yet.)
+__device__ __forceinline__ void ld128(uint32_t addr, float (&r)[128]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
+          "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
+          "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
+          "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
+          "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63]),
+          "=f"(r[64]), "=f"(r[65]), "=f"(r[66]), "=f"(r[67]), "=f"(r[68]), "=f"(r[69]), "=f"(r[70]), "=f"(r[71]),
+          "=f"(r[72]), "=f"(r[73]), "=f"(r[74]), "=f"(r[75]), "=f"(r[76]), "=f"(r[77]), "=f"(r[78]), "=f"(r[79]),
+          "=f"(r[80]), "=f"(r[81]), "=f"(r[82]), "=f"(r[83]), "=f"(r[84]), "=f"(r[85]), "=f"(r[86]), "=f"(r[87]),
+          "=f"(r[88]), "=f"(r[89]), "=f"(r[90]), "=f"(r[91]), "=f"(r[92]), "=f"(r[93]), "=f"(r[94]), "=f"(r[95]),
+          "=f"(r[96]), "=f"(r[97]), "=f"(r[98]), "=f"(r[99]), "=f"(r[100]), "=f"(r[101]), "=f"(r[102]), "=f"(r[103]),
+          "=f"(r[104]), "=f"(r[105]), "=f"(r[106]), "=f"(r[107]), "=f"(r[108]), "=f"(r[109]), "=f"(r[110]), "=f"(r[111]),
+          "=f"(r[112]), "=f"(r[113]), "=f"(r[114]), "=f"(r[115]), "=f"(r[116]), "=f"(r[117]), "=f"(r[118]), "=f"(r[119]),
+          "=f"(r[120]), "=f"(r[121]), "=f"(r[122]), "=f"(r[123]), "=f"(r[124]), "=f"(r[125]), "=f"(r[126]), "=f"(r[127])
+        : "r"(addr)
+        : "memory");
+}
+// The same for 16 columns, complete on return.
+__device__ __forceinline__ void ld16(uint32_t addr, float (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Two fp32 operations at a time.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all) : "r"(static_cast<uint32_t>(mine)), "r"(id), "r"(threads) : "memory");
+    return all != 0;
+}
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_constant__ CUtensorMap k_map,
+                                                                 const __grid_constant__ CUtensorMap v_map,
+                                                                 const __grid_constant__ PagedAttention a,
+                                                                 int32_t* __restrict__ err) {
+    using S = ManyShape<HDP>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint32_t tmem_slot;
+    const uint32_t raw = dev::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    unsigned char* const smem = smem_raw + (base - raw);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, d = a.head_dim;
+    const uint32_t bars = base + S::kBars;
+    auto full = [&](int x) { return bars + 16 * x; };
+    auto empty = [&](int x) { return bars + 16 * x + 8; };
+    auto s_full = [&](int x) { return bars + 16 * S::kUnits + 8 * x; };
+    auto p_full = [&](int x) { return bars + 16 * S::kUnits + 16 + 8 * x; };
+    auto o_done = [&](int x) { return bars + 16 * S::kUnits + 32 + 8 * x; };
+    const uint32_t q_full = bars + 16 * S::kUnits + 48, finished = q_full + 8;
+    Cut* const cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.scratch) + kPagedCounterBytes);
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < S::kUnits; ++x) {
+            dev::mbar_init(full(x), 1);
+            dev::mbar_init(empty(x), 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            dev::mbar_init(s_full(x), 1);
+            dev::mbar_init(p_full(x), 4);
+            dev::mbar_init(o_done(x), 1);
+        }
+        dev::mbar_init(q_full, 8);
+        dev::mbar_init(finished, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    dev::pdl_wait();
+    if (threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
+    zero_rows(a);
+    WorkList<kVectors, kTile, kStart> work(a);
+    Item it;
+    if (!work.template start<kLeast>(it)) {  // (its barriers also publish the mbarriers)
+        dev::pdl_launch_dependents();
+        return;
+    }
+    if (warp == kIssueWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dev::smem_u32(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = tmem_slot;
+    // only now: a dependent kernel's CTA on this SM must not take the tensor memory first
+    dev::pdl_launch_dependents();
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {  // a lane that has given up goes on without waiting
+        if (ok && !wait_counted(bar, parity)) ok = false;
+    };
+
+    // An item of more than kLanes vectors has two streams over the same tiles, each with its vectors; one of fewer
+    // has two over every other tile, with the same vectors, whose results are added at its end.
+    if (warp < kIssueWarp) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int x = warp / 4, row = threadIdx.x % kLanes;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp % 4) << 21), s_tm = lanes + kLanes * x, o_tm = lanes + S::kO + HDP * x;
+        uint32_t* const bad_words = reinterpret_cast<uint32_t*>(smem + S::kBad);
+        float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedPartsAt);
+        const float factor = fabsf(a.factor);
+        const uint32_t sign = a.factor < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries
+        int64_t unit0 = 0;  // of the run's first tile of this item
+        uint32_t done = 0;  // tiles of this stream
+        do {
+            const int from = work.from(it), to = work.to(it);
+            if (from >= to) continue;
+            const bool twice = it.valid > kLanes;
+            const int step = twice ? 1 : 2, v = (twice ? kLanes * x : 0) + row;  // the vector of this thread, in the item
+            bar_sync(1, 256);  // nobody works on the item before
+            if (threadIdx.x < 24) bad_words[threadIdx.x] = 0;
+            // Queries, rows of this stream's or, with one stream's vectors, half the rows' pieces
+            {
+                unsigned char* const to_q = smem + (twice ? x * S::kUnit : 0) + row * 128;
+                const uint16_t* const q = static_cast<const uint16_t*>(a.q) + (v < it.valid ? place_of(a, it.b, it.head, it.v0 + v, a.q_stride) : 0);
+                for (int piece = twice ? 0 : x; piece < HDP / 8; piece += step) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (v < it.valid && piece * 8 < d) {
+                        if (a.aligned & 1) {
+                            w = *reinterpret_cast<const uint4*>(q + piece * 8);
+                        } else {
+                            uint32_t e[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) e[i] = q[piece * 8 + 2 * i] | static_cast<uint32_t>(q[piece * 8 + 2 * i + 1]) << 16;
+                            w = make_uint4(e[0], e[1], e[2], e[3]);
+                        }
+                        w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
+                    }
+                    *reinterpret_cast<uint4*>(to_q + piece / 8 * (kTile * 128) + ((piece % 8 ^ (row & 7)) << 4)) = w;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bool no_page = false;
+            for (int p = (from * kTile >> a.page_shift) + threadIdx.x; p <= (min(to * kTile, it.sees) - 1) >> a.page_shift; p += 256) {
+                const int page = a.table[static_cast<int64_t>(it.b) * a.table_stride + p];
+                no_page = no_page || page < 0 || page >= a.pages;
+            }
+            no_page = bar_any(1, 256, no_page);
+            if (lane == 0) dev::mbar_arrive(q_full);
+
+            // slots that all of the item's vectors see
+            const int clear = no_page ? 0 : a.visible ? it.held : min(it.held + it.v0 / a.group + 1, it.sees);
+            const int t = v < it.valid ? (it.v0 + v) / a.group : -1;
+            const bool works = it.valid > v - lane;  // some vector of the warp
+            float ref = -INFINITY, sum = 0.0f;
+            int n = 0;  // tiles of this item
+            for (int tile = from + (twice ? 0 : x); tile < to; tile += step, ++n, ++done) {
+                const int slot = tile * kTile;
+                const bool edge = slot + kTile > clear;
+                uint32_t seen[4];
+                wait(s_full(x), done & 1);
+                __syncwarp();
+                tc_after();
+                float s[kTile];
+                if (works) ld128(s_tm, s);
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) seen[i] = t >= 0 ? seen_bits(a, it, t, slot + 32 * i) : 0u;
+                    if (no_page) {
+                        for (int first = 0; first < kTile; first += 16) {
+                            bool page = false;
+                            if (slot + first < it.sees) {
+                                const int p = a.table[static_cast<int64_t>(it.b) * a.table_stride + ((slot + first) >> a.page_shift)];
+                                page = p >= 0 && p < a.pages;
+                            }
+                            if (!page) {
+                                const uint32_t off = ~(0xffffu << (first & 16));
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (first / 32 == i) seen[i] &= off;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(seen[i] >> j & 1u)) s[32 * i + j] = -INFINITY;
+                }
+                if (works) {
+                    float m[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        m[i] = max3(s[i], s[4 + i], s[8 + i]);
+#pragma unroll
+                        for (int j = 12; j < 124; j += 8) m[i] = max3(m[i], s[j + i], s[j + 4 + i]);
+                        m[i] = fmaxf(m[i], s[124 + i]);
+                    }
+                    const float top = fmaxf(max3(m[0], m[1], m[2]), m[3]) * factor;
+                    if (n == 0) {
+                        ref = top;
+                    } else if (__any_sync(0xffffffffu, top > ref + kSlack)) {
+                        // O and the sum go over to a larger reference; rare, as it lags behind by up to kSlack
+                        const bool move = top > ref + kSlack;
+                        const float fade = !move ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
+                        if (move) ref = top;
+                        sum *= fade;
+                        wait(o_done(x), (done - 1) & 1);
+                        __syncwarp();
+                        tc_after();
+#pragma unroll 1
+                        for (int i = 0; i < d; i += 16) {
+                            float o[16];
+                            ld16(o_tm + i, o);
+                            uint32_t w[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * fade);
+                            st16(o_tm + i, w);
+                        }
+                    }
+                    const float less = (ref == -INFINITY ? 0.0f : ref) - kLift;
+                    const uint64_t by = pair(factor, factor), off = pair(-less, -less);
+                    uint64_t total[2] = {0, 0};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float z0, z1;
+                            unpair(fma2(pair(s[32 * i + j], s[32 * i + j + 1]), by, off), z0, z1);
+                            z0 = ex2(z0), z1 = ex2(z1);
+                            total[j / 2 % 2] = add2(total[j / 2 % 2], pair(z0, z1));
+                            p[j / 2] = Half16<T>::pack(z0, z1);
+                        }
+                        st16(s_tm + 16 * i, p);
+                    }
+                    float t0, t1;
+                    unpair(add2(total[0], total[1]), t0, t1);
+                    sum += t0 + t1;
+                }
+                if (edge) {
+                    // Values of slots past the last one seen count nothing, whatever is there, and values that are not
+                    // finite count for the vectors that see them alone: their rows of the tile become zeros, the rest
+                    // is told by the sums.
+                    const int group = twice ? 0 : x, cleaners = twice ? 256 : 128, me = twice ? static_cast<int>(threadIdx.x) : row;
+                    const int64_t vu = unit0 + 2 * (tile - from) + 1;
+                    uint32_t* const words = bad_words + 12 * group + 4 * (n % 3);
+                    wait(full(static_cast<int>(vu % S::kUnits)), (vu / S::kUnits) & 1);
+                    __syncwarp();
+                    for (int e = me; e < kTile * S::kBlocks; e += cleaners) {
+                        const int r = e % kTile;
+                        uint4* const line = reinterpret_cast<uint4*>(smem + S::kRing + (vu % S::kUnits) * S::kUnit + e * 128);
+                        bool clean = slot + r >= it.sees;
+                        if (!clean && no_page) {
+                            const int p = a.table[static_cast<int64_t>(it.b) * a.table_stride + ((slot + r) >> a.page_shift)];
+                            clean = p < 0 || p >= a.pages;
+                        }
+                        if (!clean) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const uint4 w = line[i];
+                                clean = clean || not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w);
+                            }
+                            if (clean) atomicOr(words + r / 32, 1u << (r % 32));
+                        }
+                        if (clean) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    bar_sync(2 + group, cleaners);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (words[i] & seen[i]) sum = __uint_as_float(0x7fc00000u);
+                    if (me < 4) bad_words[12 * group + 4 * ((n + 2) % 3) + me] = 0;  // read two barriers ago, used after the next one
+                }
+                wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) dev::mbar_arrive(p_full(x));
+            }
+            unit0 += 2 * (to - from);
+            if (n > 0) {
+                wait(o_done(x), (done - 1) & 1);
+                __syncwarp();
+                tc_after();
+            }
+            const bool whole = from == 0 && to == it.tiles;
+            // the part of an item that an earlier CTA began is the CTA's part 0, of one that goes on its part 1
+            float* const part = parts + (static_cast<int64_t>(blockIdx.x) * 2 + (from == 0)) * S::kPart;
+            float* const there = reinterpret_cast<float*>(smem + (warp % 4) * (HDP * 128));  // [HDP / 4][32 rows][4], over the queries
+            float* const stats = reinterpret_cast<float*>(smem + S::kStats);                 // [reference, sum][row]
+            float total = sum, by = 1.0f, with = 0.0f, common = ref;
+            if (!twice) {  // the second stream's results go to the first
+                bar_sync(1, 256);  // nothing reads the queries any more
+                if (x == 1) {
+                    stats[row] = ref, stats[kLanes + row] = sum;
+                    if (works && n > 0) {
+#pragma unroll 1
+                        for (int i = 0; i < d; i += 16) {
+                            float o[16];
+                            ld16(o_tm + i, o);
+#pragma unroll
+                            for (int j = 0; j < 16; j += 4)
+                                *reinterpret_cast<float4*>(there + ((i + j) / 4 * 32 + lane) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        }
+                        tc_before();
+                    }
+                }
+                bar_sync(1, 256);
+                if (x == 0) {
+                    const float ref1 = stats[row], sum1 = stats[kLanes + row];
+                    common = fmaxf(ref, ref1);
+                    by = sum == 0.0f ? 0.0f : ex2(ref - common);
+                    with = sum1 == 0.0f ? 0.0f : ex2(ref1 - common);
+                    total = by * sum + with * sum1;
+                }
+            }
+            if (works && (twice || x == 0)) {
+                const float scale = whole ? (total == 0.0f ? 0.0f : by / total) : by;
+                const float scale1 = whole ? (total == 0.0f ? 0.0f : with / total) : with;
+                const int64_t at = v < it.valid ? place_of(a, it.b, it.head, it.v0 + v, static_cast<int64_t>(a.heads) * d) : 0;
+#pragma unroll 1
+                for (int i = 0; i < d; i += 16) {
+                    float o[16];
+                    ld16(o_tm + i, o);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (!twice && with != 0.0f) f = *reinterpret_cast<const float4*>(there + ((i + j) / 4 * 32 + lane) * 4);
+                        o[j] = by == 0.0f ? f.x * scale1 : fmaf(o[j], scale, f.x * scale1);
+                        o[j + 1] = by == 0.0f ? f.y * scale1 : fmaf(o[j + 1], scale, f.y * scale1);
+                        o[j + 2] = by == 0.0f ? f.z * scale1 : fmaf(o[j + 2], scale, f.z * scale1);
+                        o[j + 3] = by == 0.0f ? f.w * scale1 : fmaf(o[j + 3], scale, f.w * scale1);
+                    }
+                    if (v < it.valid && !whole) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            __stcg(reinterpret_cast<float4*>(part + ((i + j) / 4 * kVectors + v) * 4), make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+                    } else if (v < it.valid) {
+                        put16<T>(a, at + i, o);
+                    }
+                    __syncwarp();
+                }
+                if (!whole && v < it.valid) {
+                    __stcg(part + kVectors * HDP + v, common);
+                    __stcg(part + kVectors * (HDP + 1) + v, total);
+                }
+                tc_before();
+            }
+            if (threadIdx.x == 0 && from == 0 && !whole) {
+                const int c1 = work.cta_of(it.base + kStart + it.tiles - 1);
+                cuts[blockIdx.x] = Cut{c1 - static_cast<int>(blockIdx.x) + 1, it.b, it.head, it.v0, it.valid, {}};
+            }
+        } while (work.next(it));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kIssueWarp && lane == 0) {
+            constexpr uint32_t kType = Half16<T>::kUmma;
+            constexpr uint32_t kIdescS = (1u << 4) | kType | (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kLanes >> 4) << 24);
+            // the second product's B is MN-major (bit 16)
+            constexpr uint32_t kIdescO = (1u << 4) | kType | (1u << 16) | (static_cast<uint32_t>(HDP >> 3) << 17) |
+                                         (static_cast<uint32_t>(kLanes >> 4) << 24);
+            int64_t unit0 = 0;
+            uint32_t items = 0, done[2] = {0, 0};
+            do {
+                const int n = work.to(it) - work.from(it);
+                if (n <= 0) continue;
+                const bool twice = it.valid > kLanes;
+                auto landed = [&](int64_t u) { wait(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1); };
+                auto release = [&](int64_t u) { mma_commit(empty(static_cast<int>(u % S::kUnits))); };
+                auto scores = [&](int x, int i) {
+                    const uint64_t kd = desc_of(base + S::kRing + static_cast<uint32_t>((unit0 + 2 * i) % S::kUnits) * S::kUnit, 16);
+                    const uint64_t qd = desc_of(base + (twice ? x * S::kUnit : 0), 16);
+#pragma unroll
+                    for (int k = 0; k < HDP / 16; ++k) {
+                        const uint64_t off = ((k / 4) * (kTile * 128) + (k % 4) * 32) / 16;
+                        mma_ss(tmem + kLanes * x, qd + off, kd + off, kIdescS, k > 0);
+                    }
+                    mma_commit(s_full(x));
+                };
+                auto values = [&](int x, int i, bool first) {
+                    const uint64_t vd = desc_of(base + S::kRing + static_cast<uint32_t>((unit0 + 2 * i + 1) % S::kUnits) * S::kUnit, kTile * 128);
+                    wait(p_full(x), done[x]++ & 1);
+                    tc_after();
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(tmem + S::kO + HDP * x, tmem + kLanes * x + 8 * k, vd + k * 2048 / 16, kIdescO, !(first && k == 0));
+                    mma_commit(o_done(x));
+                };
+                wait(q_full, items++ & 1);
+                tc_after();
+                if (twice) {
+                    landed(unit0);
+                    scores(0, 0);
+                    scores(1, 0);
+                    release(unit0);
+                    for (int i = 0; ok && i < n; ++i) {
+                        const int64_t k1 = unit0 + 2 * (i + 1), v = unit0 + 2 * i + 1;
+                        landed(v);
+                        values(0, i, i == 0);
+                        if (i + 1 < n) {
+                            landed(k1);
+                            scores(0, i + 1);
+                        }
+                        values(1, i, i == 0);
+                        release(v);
+                        if (i + 1 < n) {
+                            scores(1, i + 1);
+                            release(k1);
+                        }
+                    }
+                } else {
+                    for (int i = 0; i < min(2, n); ++i) {
+                        landed(unit0 + 2 * i);
+                        scores(i, i);
+                        release(unit0 + 2 * i);
+                    }
+                    for (int i = 0; ok && i < n; ++i) {
+                        landed(unit0 + 2 * i + 1);
+                        values(i & 1, i, i < 2);
+                        release(unit0 + 2 * i + 1);
+                        if (i + 2 < n) {
+                            landed(unit0 + 2 * (i + 2));
+                            scores(i & 1, i + 2);
+                            release(unit0 + 2 * (i + 2));
+                        }
+                    }
+                }
+                unit0 += 2 * n;
+            } while (ok && work.next(it));
+            // no product is under way past this point, also where a wait has given up
+            mma_commit(finished);
+            if (!wait_counted(finished, 0)) ok = false;
+        } else if (warp == kCopyWarp) {
+            // A lane has a box (64 dims of the slots of a page) of the keys' or values' unit.
+            const int box = min(kPagedBox, 1 << a.page_shift), boxes = kTile / box;
+            const int mine = lane % boxes, block = lane / boxes % S::kBlocks;
+            const bool copies = lane < boxes * S::kBlocks;
+            int64_t unit = 0;
+            do {
+                for (int tile = work.from(it), to = work.to(it); tile < to; ++tile) {
+                    const int slot = tile * kTile + mine * box;
+                    int page = -1;
+                    if (copies && slot < it.sees) page = a.table[static_cast<int64_t>(it.b) * a.table_stride + (slot >> a.page_shift)];
+                    const bool here = page >= 0 && page < a.pages;
+                    const uint32_t who = __ballot_sync(0xffffffffu, here);
+                    const int first = here ? ((page * a.kv_heads + it.head) << a.page_shift) + (slot & ((1 << a.page_shift) - 1)) : 0;
+#pragma unroll
+                    for (int v = 0; v < 2; ++v, ++unit) {
+                        const int x = static_cast<int>(unit % S::kUnits);
+                        if (unit >= S::kUnits) wait(empty(x), (unit / S::kUnits - 1) & 1);
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                        if (lane == 0) dev::mbar_expect_tx(full(x), __popc(who) * box * 128);
+                        __syncwarp();
+                        if (here)
+                            dev::tma_load_2d(base + S::kRing + x * S::kUnit + block * (kTile * 128) + mine * box * 128, v ? &v_map : &k_map,
+                                             block * 64, first, full(x));
+                    }
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                }
+            } while (__all_sync(0xffffffffu, ok) && work.next(it));
+            // no copy is in flight past this point, also where a wait has given up
+            for (int64_t u = max(static_cast<int64_t>(0), unit - S::kUnits); u < unit; ++u)
+                if (!wait_counted(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1)) ok = false;
+        }
+        __syncwarp();
+    }
+    if (!ok) atomicOr(err, 1);
+    tc_before();
+    __syncthreads();
+    if (warp == kIssueWarp) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Items that were cut, from their parts: a thread has four dims of a vector.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedAttention a) {
+    using S = ManyShape<HDP>;
+    dev::pdl_wait();
+    dev::pdl_launch_dependents();
+    const Cut cut = reinterpret_cast<const Cut*>(static_cast<const char*>(a.scratch) + kPagedCounterBytes)[blockIdx.x];
+    const int v = blockIdx.y * 32 + threadIdx.x % 32, d = a.head_dim;
+    if (cut.parts == 0 || v >= cut.valid) return;
+    const float* const parts = reinterpret_cast<const float*>(static_cast<const char*>(a.scratch) + kPagedPartsAt);
+    auto part_of = [&](int i) { return parts + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0)) * S::kPart; };
+    float top = -INFINITY, total = 0.0f;
+    for (int i = 0; i < cut.parts; ++i) top = fmaxf(top, part_of(i)[kVectors * HDP + v]);
+    constexpr int kMine = HDP / 32;
+    float4 y[kMine] = {};
+#pragma unroll 2
+    for (int i = 0; i < cut.parts; ++i) {
+        const float* const part = part_of(i);
+        const float sum = part[kVectors * (HDP + 1) + v], w = sum == 0.0f ? 0.0f : ex2(part[kVectors * HDP + v] - top);
+        total += w * sum;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int quad = threadIdx.x / 32 + 8 * j;
+            if (4 * quad >= d || w == 0.0f) continue;
+            const float4 f = *reinterpret_cast<const float4*>(part + (quad * kVectors + v) * 4);
+            y[j].x = fmaf(w, f.x, y[j].x), y[j].y = fmaf(w, f.y, y[j].y);
+            y[j].z = fmaf(w, f.z, y[j].z), y[j].w = fmaf(w, f.w, y[j].w);
+        }
+    }
+    const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+    const int64_t at = place_of(a, cut.b, cut.head, cut.v0 + v, static_cast<int64_t>(a.heads) * d);
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+        const int dim = 4 * (threadIdx.x / 32 + 8 * j);
+        if (dim < d) put4<T>(a, at + dim, make_float4(y[j].x * scale, y[j].y * scale, y[j].z * scale, y[j].w * scale));
+    }
+}
+
+template <typename T, int HDP>
+cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const PagedAttention& a, int sm_count, int32_t* err,
+                   cudaStream_t s) {
+    using S = ManyShape<HDP>;
+    static std::atomic<uint64_t> allowed{0};
+    const auto kernel = paged_many_kernel<T, HDP>;
+    cudaError_t e = allow_shared(kernel, S::kSmem, allowed);
+    if (e != cudaSuccess) return e;
+    static const int regs = [] {  // what the compiler gave the kernel has to be what the roles share out
+        cudaFuncAttributes f{};
+        return cudaFuncGetAttributes(&f, paged_many_kernel<T, HDP>) == cudaSuccess ? f.numRegs : -1;
+    }();
+    if (regs != kLaunchRegs) return cudaErrorInvalidConfiguration;
+    const int64_t items = static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors);
+    const int64_t most = std::max(items, items * ((a.capacity + kTile - 1) / kTile) / kLeast);
+    const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count, kPagedManyCtas), most));
+    e = launch_dependent(kernel, dim3(grid), dim3(kThreads), S::kSmem, s, k_map, v_map, a, err);
+    if (e == cudaSuccess) e = launch_dependent(paged_merge_kernel<T, HDP>, dim3(grid, kVectors / 32), dim3(256), 0, s, a);
+    return e;
+}
+
+}  // namespace
+
+size_t paged_many_bytes(int sm_count) {
+    return static_cast<size_t>(std::min(sm_count, kPagedManyCtas)) * 2 * ManyShape<128>::kPart * sizeof(float);
+}
+
+cudaError_t launch_paged_many(bool bf16, const CUtensorMap (&maps)[2], const PagedAttention& a, int sm_count, int32_t* err,
+                              cudaStream_t s) {
+    const bool wide = a.head_dim > 64;
+    const auto run = bf16 ? wide ? launch<__nv_bfloat16, 128> : launch<__nv_bfloat16, 64>
+                          : wide ? launch<__half, 128> : launch<__half, 64>;
+    return run(maps[0], maps[1], a, sm_count, err, s);
+}
+
+}  // namespace kt

@@ -101,7 +101,7 @@ class PagedKVCache:
         self._status = self.status.data_ptr()
         self._lib = lib = _lib.load()
         self._append, self._attention, self._accept = lib.kt_paged_append, lib.kt_paged_attention, lib.kt_paged_accept
-        self.scratch = torch.empty(lib.kt_paged_scratch_bytes(), dtype=torch.uint8, device=dev)
+        self.scratch = torch.empty(lib.kt_paged_scratch_bytes(self.ctx.handle), dtype=torch.uint8, device=dev)
         self.scratch[:COUNTER_BYTES].zero_()
         self._scratch = self.scratch.data_ptr()
         self._scale = 1.0 / math.sqrt(head_dim)
