@@ -86,27 +86,35 @@ __device__ __forceinline__ int64_t place_of(const PagedAttention& a, int b, int 
 // An item of the attention's work: kVectors query vectors (rows x heads of a group, in
 // row order) of one sequence and key/value head, over tiles of kTile slots.
 struct Item {
-    int entry;           // sequence * vector tiles + vector tile
+    int64_t base;            // index of the item's first unit in the list of all
+    int entry;               // sequence * vector tiles + vector tile
     int b, head, v0, valid;  // first vector, how many there are
-    int held, count;     // tokens held, rows that are tokens
-    int sees, tiles;     // slots the last vector sees
-    int64_t base;        // index of the item's first unit in the list of all
+    int held, count;         // tokens held, rows that are tokens
+    int sees, tiles;         // slots the last vector sees
+    int from, to;            // tiles of this CTA
+    int last;                // the CTA's last item
+};
+// How the list of all tiles is shared out, and each warp's place in its CTA's run.  In
+// shared memory: the loops over tiles need their registers.
+template <int kWarps>
+struct Plan {
+    int64_t share, spare, begin, end;
+    int64_t sums[kWarps], items[kWarps], base;
+    int entry;
+    Item at[kWarps];
 };
 
 // The list of all tiles, sequences first, then vector tiles, then heads; an item is kStart
 // units, what entering it costs, and one for each tile.  Equal runs of units go to the
 // CTAs: ragged batches, single long sequences and the triangle of a prompt load every SM
 // alike.  Lengths are read here, on the device, so a captured launch fits any.
-template <int kVectors, int kTile, int kStart>
+template <int kWarps, int kVectors, int kTile, int kStart, int kLeast>
 struct WorkList {
     const PagedAttention& a;
-    const int vts;
-    int64_t ctas, share, spare, begin, end;
+    Plan<kWarps>& plan;
 
-    __device__ WorkList(const PagedAttention& args)
-        : a(args), vts((args.rows * args.group + kVectors - 1) / kVectors), ctas(0), share(0), spare(0), begin(0), end(0) {}
-
-    __device__ void load(Item& it, int entry) const {  // all but head and base
+    __device__ __forceinline__ int vector_tiles() const { return (a.rows * a.group + kVectors - 1) / kVectors; }
+    __device__ __forceinline__ void load(Item& it, int entry, int vts) const {  // all but head, base and the tiles
         it.entry = entry;
         it.b = entry / vts;
         it.v0 = (entry - it.b * vts) * kVectors;
@@ -116,25 +124,31 @@ struct WorkList {
         it.sees = it.valid <= 0 ? 0 : a.visible ? it.held + it.count : it.held + (it.v0 + it.valid - 1) / a.group + 1;
         it.tiles = (it.sees + kTile - 1) / kTile;
     }
-    __device__ int64_t run_begin(int64_t cta) const { return cta * share + min(cta, spare); }
-    __device__ int cta_of(int64_t i) const {  // the CTA whose run holds unit i
-        const int64_t longer = spare * (share + 1);
-        return static_cast<int>(i < longer ? i / (share + 1) : spare + (i - longer) / share);
+    __device__ __forceinline__ void cut(Item& it) const {
+        it.from = static_cast<int>(max(static_cast<int64_t>(0), plan.begin - it.base - kStart));
+        it.to = static_cast<int>(min(static_cast<int64_t>(it.tiles), max(static_cast<int64_t>(0), plan.end - it.base - kStart)));
+        it.last = it.base + it.tiles + kStart >= plan.end;
     }
-    // By all threads of the CTA: shares out the list; false: nothing for this CTA.  `first`:
-    // the item its run begins in.  A CTA gets at least kLeast tiles or an item.
-    template <int kLeast>
-    __device__ bool start(Item& first) {
-        __shared__ int64_t sums[33];
-        __shared__ int64_t counts[33];
-        __shared__ int64_t found[2];
-        const int threads = blockDim.x, warps = threads / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-        const int entries = a.batch * vts, each = (entries + threads - 1) / threads;
+    __device__ int cta_of(int64_t unit) const {  // the CTA whose run holds it
+        const int64_t longer = plan.spare * (plan.share + 1);
+        return static_cast<int>(unit < longer ? unit / (plan.share + 1) : plan.spare + (unit - longer) / plan.share);
+    }
+    // The CTAs that share an item's tiles are first_cta .. last_cta.
+    __device__ int first_cta(const Item& it) const { return cta_of(it.base + kStart); }
+    __device__ int last_cta(const Item& it) const { return cta_of(it.base + kStart + it.tiles - 1); }
+
+    // By all threads of the CTA: shares out the list; false: nothing for this CTA.  A CTA gets
+    // at least kLeast tiles or an item.
+    __device__ bool start() const {
+        constexpr int kThreads = kWarps * 32;
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, vts = vector_tiles();
+        const int entries = a.batch * vts, each = (entries + kThreads - 1) / kThreads;
         const int from = min(entries, static_cast<int>(threadIdx.x) * each), to = min(entries, from + each);
+        Item it;
         int64_t units = 0, items = 0;
         for (int e = from; e < to; ++e) {
-            load(first, e);
-            if (first.tiles > 0) units += first.tiles + kStart, ++items;
+            load(it, e, vts);
+            if (it.tiles > 0) units += it.tiles + kStart, ++items;
         }
         units *= a.kv_heads, items *= a.kv_heads;
         int64_t upto = units;
@@ -142,60 +156,69 @@ struct WorkList {
             const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
         }
-        int64_t many = items;
-        for (int o = 16; o > 0; o >>= 1) many += __shfl_xor_sync(0xffffffffu, many, o);
-        if (lane == 31) sums[warp] = upto;
-        if (lane == 0) counts[warp] = many;
+        for (int o = 16; o > 0; o >>= 1) items += __shfl_xor_sync(0xffffffffu, items, o);
+        if (lane == 31) plan.sums[warp] = upto, plan.items[warp] = items;
         __syncthreads();
         int64_t before = upto - units, total = 0;
         items = 0;
-        for (int w = 0; w < warps; ++w) {
-            if (w < warp) before += sums[w];
-            total += sums[w];
-            items += counts[w];
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += plan.sums[w];
+            total += plan.sums[w];
+            items += plan.items[w];
         }
         if (items == 0) return false;
-        ctas = min(static_cast<int64_t>(gridDim.x), max(items, (total - items * kStart) / kLeast));
-        share = total / ctas;
-        spare = total - share * ctas;
+        const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max(items, (total - items * kStart) / kLeast));
         if (blockIdx.x >= ctas) return false;
-        begin = run_begin(blockIdx.x);
-        end = run_begin(blockIdx.x + 1);
+        const int64_t share = total / ctas, spare = total - share * ctas;
+        const int64_t begin = blockIdx.x * share + min(static_cast<int64_t>(blockIdx.x), spare);
+        if (threadIdx.x == 0) {
+            plan.share = share, plan.spare = spare, plan.begin = begin;
+            plan.end = begin + share + (blockIdx.x < spare);
+        }
         if (before <= begin && begin < before + units) {  // one thread
             for (int e = from; e < to; ++e) {
-                load(first, e);
-                const int64_t n = first.tiles > 0 ? static_cast<int64_t>(first.tiles + kStart) * a.kv_heads : 0;
+                load(it, e, vts);
+                const int64_t n = it.tiles > 0 ? static_cast<int64_t>(it.tiles + kStart) * a.kv_heads : 0;
                 if (begin < before + n) {
-                    found[0] = e;
-                    found[1] = before;
+                    plan.entry = e;
+                    plan.base = before;
                     break;
                 }
                 before += n;
             }
         }
         __syncthreads();
-        load(first, static_cast<int>(found[0]));
-        first.head = static_cast<int>((begin - found[1]) / (first.tiles + kStart));
-        first.base = found[1] + static_cast<int64_t>(first.head) * (first.tiles + kStart);
+        if (lane == 0) {
+            Item& mine = plan.at[warp];
+            load(it, plan.entry, vts);
+            it.head = static_cast<int>((begin - plan.base) / (it.tiles + kStart));
+            it.base = plan.base + static_cast<int64_t>(it.head) * (it.tiles + kStart);
+            cut(it);
+            mine = it;
+        }
+        __syncwarp();
         return true;
     }
-    // Tiles [from, to) of the item are this CTA's.
-    __device__ int from(const Item& it) const {
-        return static_cast<int>(max(static_cast<int64_t>(0), begin - it.base - kStart));
-    }
-    __device__ int to(const Item& it) const {
-        return static_cast<int>(min(static_cast<int64_t>(it.tiles), max(static_cast<int64_t>(0), end - it.base - kStart)));
-    }
-    // The item after `it`; false: the run ends before it.
-    __device__ bool next(Item& it) const {
-        it.base += it.tiles + kStart;
-        if (it.base >= end) return false;
-        if (++it.head < a.kv_heads) return true;
-        it.head = 0;
-        const int64_t base = it.base;
-        do load(it, it.entry + 1);
-        while (it.tiles == 0);  // (units are left, so a later entry has tiles)
+    // To the warp's next item; by its lane 0.
+    __device__ void step() const {
+        Item it = plan.at[threadIdx.x / 32];
+        const int64_t base = it.base + it.tiles + kStart;
+        if (++it.head == a.kv_heads) {
+            it.head = 0;
+            const int vts = vector_tiles();
+            do load(it, it.entry + 1, vts);
+            while (it.tiles == 0);  // (units are left, so a later entry has tiles)
+        }
         it.base = base;
+        cut(it);
+        plan.at[threadIdx.x / 32] = it;
+    }
+    // The same by the whole warp; false: the run ends before it.
+    __device__ __forceinline__ bool next() const {
+        if (plan.at[threadIdx.x / 32].last) return false;
+        __syncwarp();
+        if (threadIdx.x % 32 == 0) step();
+        __syncwarp();
         return true;
     }
 };

@@ -92,9 +92,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
     dev::pdl_wait();
     dev::pdl_launch_dependents();
     zero_rows(a);
-    WorkList<kVectors, kTile, kStart> work(a);
-    Item it;
-    if (!work.template start<kLeast>(it)) return;  // (its barriers also publish the mbarriers)
+    __shared__ Plan<kWarps + 1> plan;
+    const WorkList<kWarps + 1, kVectors, kTile, kStart, kLeast> work{a, plan};
+    if (!work.start()) return;  // (its barriers also publish the mbarriers)
+    const Item& it = plan.at[warp];
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {  // a lane that has given up goes on without waiting
         if (ok && !wait_counted(bar, parity)) ok = false;
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
         const bool copies = lane < boxes * S::kBlocks;
         int64_t unit = 0;
         do {
-            for (int tile = work.from(it), to = work.to(it); tile < to; ++tile) {
+            for (int tile = it.from, to = it.to; tile < to; ++tile) {
                 const int slot = tile * kTile + mine * box;
                 int page = -1;
                 if (copies && slot < it.sees) page = a.table[static_cast<int64_t>(it.b) * a.table_stride + (slot >> a.page_shift)];
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
                 }
                 if (!__all_sync(0xffffffffu, ok)) break;
             }
-        } while (__all_sync(0xffffffffu, ok) && work.next(it));
+        } while (__all_sync(0xffffffffu, ok) && work.next());
         // no copy is in flight past this point, also where a wait has given up
         for (int64_t u = max(static_cast<int64_t>(0), unit - S::kUnits); u < unit; ++u)
             if (!wait_counted(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1)) ok = false;
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
     float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedPartsAt);
     int64_t unit = 0;
     do {
-        const int from = work.from(it), to = work.to(it);
+        const int from = it.from, to = it.to;
         if (from >= to) continue;
         // this thread's vectors, r8 and r8 + 8 of the item, and their queries
         uint32_t q[HDP / 16][4];
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
         }
         if (!whole) {
             if (threadIdx.x < 2 * kVectors) __stcg(part + kVectors * HDP + threadIdx.x, totals[threadIdx.x]);
-            const int c0 = work.cta_of(it.base + kStart), c1 = work.cta_of(it.base + kStart + it.tiles - 1);
+            const int c0 = work.first_cta(it), c1 = work.last_cta(it);
             int32_t* const counter = static_cast<int32_t*>(a.scratch) + c0;
             __threadfence();
             compute_sync();
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
             }
         }
         compute_sync();  // the areas and last_cta are free again
-    } while (work.next(it));
+    } while (work.next());
     if (!ok) atomicOr(err, 1);
 }
 

@@ -190,9 +190,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
     dev::pdl_wait();
     if (threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
     zero_rows(a);
-    WorkList<kVectors, kTile, kStart> work(a);
-    Item it;
-    if (!work.template start<kLeast>(it)) {  // (its barriers also publish the mbarriers)
+    __shared__ Plan<kThreads / 32> plan;
+    const WorkList<kThreads / 32, kVectors, kTile, kStart, kLeast> work{a, plan};
+    if (!work.start()) {  // (its barriers also publish the mbarriers)
         dev::pdl_launch_dependents();
         return;
     }
@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_slot;
+    const Item& it = plan.at[warp];
     // only now: a dependent kernel's CTA on this SM must not take the tensor memory first
     dev::pdl_launch_dependents();
     bool ok = true;
@@ -220,42 +221,42 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
         uint32_t* const bad_words = reinterpret_cast<uint32_t*>(smem + S::kBad);
         float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedPartsAt);
         const float factor = fabsf(a.factor);
-        const uint32_t sign = a.factor < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries
         int64_t unit0 = 0;  // of the run's first tile of this item
         uint32_t done = 0;  // tiles of this stream
         do {
-            const int from = work.from(it), to = work.to(it);
+            const int from = it.from, to = it.to;
             if (from >= to) continue;
             const bool twice = it.valid > kLanes;
             const int step = twice ? 1 : 2, v = (twice ? kLanes * x : 0) + row;  // the vector of this thread, in the item
             bar_sync(1, 256);  // nobody works on the item before
             if (threadIdx.x < 24) bad_words[threadIdx.x] = 0;
-            // Queries, rows of this stream's or, with one stream's vectors, half the rows' pieces
+            // Queries: rows of this stream's, or half of the pieces of the rows that both streams work on
             {
-                unsigned char* const to_q = smem + (twice ? x * S::kUnit : 0) + row * 128;
+                const uint32_t to_q = base + (twice ? x * S::kUnit : 0) + row * 128;
                 const uint16_t* const q = static_cast<const uint16_t*>(a.q) + (v < it.valid ? place_of(a, it.b, it.head, it.v0 + v, a.q_stride) : 0);
+#pragma unroll 4
                 for (int piece = twice ? 0 : x; piece < HDP / 8; piece += step) {
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (v < it.valid && piece * 8 < d) {
-                        if (a.aligned & 1) {
-                            w = *reinterpret_cast<const uint4*>(q + piece * 8);
-                        } else {
-                            uint32_t e[4];
+                    const uint32_t at = to_q + piece / 8 * (kTile * 128) + ((piece % 8 ^ (row & 7)) << 4);
+                    const int dim = piece * 8;
+                    if (v >= it.valid || dim >= d) {
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                    } else if (a.aligned & 1) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(q + dim) : "memory");
+                    } else {
+                        uint32_t e[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) e[i] = q[piece * 8 + 2 * i] | static_cast<uint32_t>(q[piece * 8 + 2 * i + 1]) << 16;
-                            w = make_uint4(e[0], e[1], e[2], e[3]);
-                        }
-                        w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
+                        for (int j = 0; j < 4; ++j) e[j] = q[dim + 2 * j] | static_cast<uint32_t>(q[dim + 2 * j + 1]) << 16;
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]) : "memory");
                     }
-                    *reinterpret_cast<uint4*>(to_q + piece / 8 * (kTile * 128) + ((piece % 8 ^ (row & 7)) << 4)) = w;
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             bool no_page = false;
             for (int p = (from * kTile >> a.page_shift) + threadIdx.x; p <= (min(to * kTile, it.sees) - 1) >> a.page_shift; p += 256) {
                 const int page = a.table[static_cast<int64_t>(it.b) * a.table_stride + p];
                 no_page = no_page || page < 0 || page >= a.pages;
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             no_page = bar_any(1, 256, no_page);
             if (lane == 0) dev::mbar_arrive(q_full);
 
@@ -274,6 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 tc_after();
                 float s[kTile];
                 if (works) ld128(s_tm, s);
+                if (a.factor < 0.0f) {
+#pragma unroll
+                    for (int j = 0; j < kTile; ++j) s[j] = -s[j];
+                }
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) seen[i] = t >= 0 ? seen_bits(a, it, t, slot + 32 * i) : 0u;
@@ -361,6 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     for (int e = me; e < kTile * S::kBlocks; e += cleaners) {
                         const int r = e % kTile;
                         uint4* const line = reinterpret_cast<uint4*>(smem + S::kRing + (vu % S::kUnits) * S::kUnit + e * 128);
+                        if (slot + r < clear) continue;  // seen by all
                         bool clean = slot + r >= it.sees;
                         if (!clean && no_page) {
                             const int p = a.table[static_cast<int64_t>(it.b) * a.table_stride + ((slot + r) >> a.page_shift)];
@@ -369,14 +375,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                         if (!clean) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                const uint4 w = line[i];
+                                const uint4 w = line[(i + lane) % 8];
                                 clean = clean || not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w);
                             }
                             if (clean) atomicOr(words + r / 32, 1u << (r % 32));
                         }
                         if (clean) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
+                            for (int i = 0; i < 8; ++i) line[(i + lane) % 8] = make_uint4(0, 0, 0, 0);
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -432,20 +438,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 const float scale = whole ? (total == 0.0f ? 0.0f : by / total) : by;
                 const float scale1 = whole ? (total == 0.0f ? 0.0f : with / total) : with;
                 const int64_t at = v < it.valid ? place_of(a, it.b, it.head, it.v0 + v, static_cast<int64_t>(a.heads) * d) : 0;
+                const bool staged = whole && !a.out_f32 && (a.aligned & 2);
+                // 16-bit results pass through shared memory, [piece of 8 dims][row], and leave it row by row; behind the
+                // second stream's, which are read up to there by then
+                uint4* const stage = twice ? reinterpret_cast<uint4*>(smem + x * S::kUnit + (warp % 4) * (HDP * 64)) : reinterpret_cast<uint4*>(there);
 #pragma unroll 1
                 for (int i = 0; i < d; i += 16) {
                     float o[16];
                     ld16(o_tm + i, o);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (!twice && with != 0.0f) f = *reinterpret_cast<const float4*>(there + ((i + j) / 4 * 32 + lane) * 4);
-                        o[j] = by == 0.0f ? f.x * scale1 : fmaf(o[j], scale, f.x * scale1);
-                        o[j + 1] = by == 0.0f ? f.y * scale1 : fmaf(o[j + 1], scale, f.y * scale1);
-                        o[j + 2] = by == 0.0f ? f.z * scale1 : fmaf(o[j + 2], scale, f.z * scale1);
-                        o[j + 3] = by == 0.0f ? f.w * scale1 : fmaf(o[j + 3], scale, f.w * scale1);
+                    for (int j = 0; j < 16; ++j) o[j] = by == 0.0f ? 0.0f : o[j] * scale;
+                    if (!twice && with != 0.0f) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(there + ((i + j) / 4 * 32 + lane) * 4);
+                            o[j] = fmaf(f.x, scale1, o[j]), o[j + 1] = fmaf(f.y, scale1, o[j + 1]);
+                            o[j + 2] = fmaf(f.z, scale1, o[j + 2]), o[j + 3] = fmaf(f.w, scale1, o[j + 3]);
+                        }
                     }
-                    if (v < it.valid && !whole) {
+                    __syncwarp();
+                    if (staged) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            stage[(i / 8 + j) * 32 + (lane ^ ((i / 8 + j) & 7))] = make_uint4(Half16<T>::pack(o[8 * j], o[8 * j + 1]), Half16<T>::pack(o[8 * j + 2], o[8 * j + 3]),
+                                                          Half16<T>::pack(o[8 * j + 4], o[8 * j + 5]), Half16<T>::pack(o[8 * j + 6], o[8 * j + 7]));
+                    } else if (v < it.valid && !whole) {
 #pragma unroll
                         for (int j = 0; j < 16; j += 4)
                             __stcg(reinterpret_cast<float4*>(part + ((i + j) / 4 * kVectors + v) * 4), make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
@@ -454,6 +471,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     }
                     __syncwarp();
                 }
+                if (staged) {
+                    const int pieces = d / 8;
+#pragma unroll 4
+                    for (int i = 0; i < pieces; ++i) {
+                        const int r = (32 * i + lane) / pieces, c = 32 * i + lane - r * pieces;
+                        const int64_t to_row = __shfl_sync(0xffffffffu, at, r);
+                        if (v - lane + r < it.valid)
+                            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to_row + 8 * c) = stage[c * 32 + (r ^ (c & 7))];
+                    }
+                }
                 if (!whole && v < it.valid) {
                     __stcg(part + kVectors * HDP + v, common);
                     __stcg(part + kVectors * (HDP + 1) + v, total);
@@ -461,10 +488,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 tc_before();
             }
             if (threadIdx.x == 0 && from == 0 && !whole) {
-                const int c1 = work.cta_of(it.base + kStart + it.tiles - 1);
+                const int c1 = work.last_cta(it);
                 cuts[blockIdx.x] = Cut{c1 - static_cast<int>(blockIdx.x) + 1, it.b, it.head, it.v0, it.valid, {}};
             }
-        } while (work.next(it));
+        } while (work.next());
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kIssueWarp && lane == 0) {
@@ -475,9 +502,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                                          (static_cast<uint32_t>(kLanes >> 4) << 24);
             int64_t unit0 = 0;
             uint32_t items = 0, done[2] = {0, 0};
-            do {
-                const int n = work.to(it) - work.from(it);
-                if (n <= 0) continue;
+            while (ok) {
+                const int n = it.to - it.from;
+                if (n <= 0) {
+                    if (it.last) break;
+                    work.step();
+                    continue;
+                }
                 const bool twice = it.valid > kLanes;
                 auto landed = [&](int64_t u) { wait(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1); };
                 auto release = [&](int64_t u) { mma_commit(empty(static_cast<int>(u % S::kUnits))); };
@@ -540,7 +571,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     }
                 }
                 unit0 += 2 * n;
-            } while (ok && work.next(it));
+                if (it.last) break;
+                work.step();
+            }
             // no product is under way past this point, also where a wait has given up
             mma_commit(finished);
             if (!wait_counted(finished, 0)) ok = false;
@@ -551,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             const bool copies = lane < boxes * S::kBlocks;
             int64_t unit = 0;
             do {
-                for (int tile = work.from(it), to = work.to(it); tile < to; ++tile) {
+                for (int tile = it.from, to = it.to; tile < to; ++tile) {
                     const int slot = tile * kTile + mine * box;
                     int page = -1;
                     if (copies && slot < it.sees) page = a.table[static_cast<int64_t>(it.b) * a.table_stride + (slot >> a.page_shift)];
@@ -571,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     }
                     if (!__all_sync(0xffffffffu, ok)) break;
                 }
-            } while (__all_sync(0xffffffffu, ok) && work.next(it));
+            } while (__all_sync(0xffffffffu, ok) && work.next());
             // no copy is in flight past this point, also where a wait has given up
             for (int64_t u = max(static_cast<int64_t>(0), unit - S::kUnits); u < unit; ++u)
                 if (!wait_counted(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1)) ok = false;
