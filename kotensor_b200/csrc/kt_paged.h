@@ -243,11 +243,33 @@ __device__ __forceinline__ uint32_t seen_bits(const PagedAttention& a, const Ite
     return bits;
 }
 
-__device__ __forceinline__ bool wait_counted(uint32_t bar, uint32_t parity) {  // false after some seconds
-#pragma unroll 1
-    for (uint32_t i = 0; i < (1u << 25); ++i)
-        if (dev::mbar_try_wait(bar, parity)) return true;
-    return false;
+__device__ __forceinline__ bool has_page(const PagedAttention& a, int b, int slot) {
+    const int page = a.table[static_cast<int64_t>(b) * a.table_stride + (slot >> a.page_shift)];
+    return page >= 0 && page < a.pages;
+}
+
+// Waits for phase `parity` of `bar`; false after some seconds.  (Four tries to a turn: the turns
+// of warps that wait take issue slots from those that work.)
+__device__ __forceinline__ bool wait_counted(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+        "mov.u32 n, 0;\n\t"
+        "TRY:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@!p mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@!p mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@!p mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra DONE;\n\t"
+        "add.u32 n, n, 1;\n\t"
+        "setp.lt.u32 q, n, 8388608;\n\t"
+        "@q bra TRY;\n\t"
+        "DONE:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -262,6 +284,7 @@ template <>
 struct Half16<__half> {
     static constexpr uint32_t kExponent = 0x7c007c00u;
     static constexpr uint32_t kUmma = 0;  // the operands' type in tcgen05.mma's descriptor
+    static constexpr int kDegree = 4;     // of a polynomial for 2^f that its rounding hides
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __half2 h = __floats2half2_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -271,19 +294,19 @@ template <>
 struct Half16<__nv_bfloat16> {
     static constexpr uint32_t kExponent = 0x7f807f80u;
     static constexpr uint32_t kUmma = 1u << 7 | 1u << 10;
+    static constexpr int kDegree = 3;
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 };
-// Whether one of a word's two values is an infinity or NaN.
+// Not 0 if one of a word's two values is an infinity or NaN: a carry out of the exponent.
 template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-    constexpr uint32_t e = Half16<T>::kExponent;
-    return (w & e & 0xffffu) == (e & 0xffffu) || (w & e & 0xffff0000u) == (e & 0xffff0000u);
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return ((w & 0x7fff7fffu) + (0x80008000u - Half16<T>::kExponent)) & 0x80008000u;
 }
 
-// Four, sixteen dims of a result, `at` elements into out (a multiple of 4, of 16).
+// Four dims of a result, `at` elements into out (a multiple of 4).
 template <typename T>
 __device__ __forceinline__ void put4(const PagedAttention& a, int64_t at, float4 y) {
     if (a.out_f32) {
@@ -297,20 +320,6 @@ __device__ __forceinline__ void put4(const PagedAttention& a, int64_t at, float4
         else to[0] = w.x & 0xffffu, to[1] = w.x >> 16, to[2] = w.y & 0xffffu, to[3] = w.y >> 16;
     }
 }
-template <typename T>
-__device__ __forceinline__ void put16(const PagedAttention& a, int64_t at, const float (&y)[16]) {
-    if (!a.out_f32 && (a.aligned & 2)) {
-        uint4* const to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            to[i] = make_uint4(Half16<T>::pack(y[8 * i], y[8 * i + 1]), Half16<T>::pack(y[8 * i + 2], y[8 * i + 3]),
-                               Half16<T>::pack(y[8 * i + 4], y[8 * i + 5]), Half16<T>::pack(y[8 * i + 6], y[8 * i + 7]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) put4<T>(a, at + i, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
-    }
-}
-
 }  // namespace paged
 #endif
 

@@ -236,14 +236,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
                 uint32_t any = __reduce_or_sync(0xffffffffu, seen[0] | seen[1]);
                 const int row = lane / 2;
                 uint4* const line = reinterpret_cast<uint4*>(smem + vx * S::kUnit + (warp * 16 + row) * 128);
-                bool bad = false;
+                uint32_t over = 0;
 #pragma unroll
                 for (int i = 0; i < HDP / 16; ++i) {
                     const int piece = lane % 2 * (HDP / 16) + i;
                     const uint4 w = line[piece / 8 * (kTile * 128 / 16) + piece % 8];
-                    bad = bad || not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w);
+                    over |= not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w);
                 }
-                uint32_t told = __ballot_sync(0xffffffffu, bad);
+                uint32_t told = __ballot_sync(0xffffffffu, over != 0);
                 told = (told | told >> 1) & 0x55555555u;  // bit 2 * row
                 if (!(any >> row & 1u) || (told >> (2 * row) & 1u)) {
 #pragma unroll

@@ -18,10 +18,7 @@ constexpr int kIssueWarp = 8, kCopyWarp = 9;  // after the softmax warps; the tw
 constexpr int kThreads = 384;
 constexpr float kLift = 6.0f;    // probabilities are 2^kLift times larger: fp16 keeps them to 2^-30 of the reference
 constexpr float kSlack = 8.0f;   // the reference moves when a score passes it by this much (2^14 < fp16's largest)
-// Registers of a thread at the launch, and of each role's warps.
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 104;
-static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs <= 12 * kLaunchRegs, "registers");
-static_assert(kSoftmaxRegs > kLaunchRegs && kOtherRegs < kLaunchRegs, "one role raises, the other lowers");
+constexpr uint32_t kOnUnits = 0x54;  // which of eight pairs of powers of 2 go to the fp32 units
 
 template <int HDP>
 struct ManyShape {
@@ -31,7 +28,7 @@ struct ManyShape {
     static constexpr int kBad = kRing + kUnits * kUnit;  // slots of an edge tile whose values are not finite: [2][3][4] words
     static constexpr int kStats = kBad + 128;            // of the second stream's vectors
     static constexpr int kBars = kStats + 2 * kLanes * 4;
-    static constexpr int kSmem = 1024 + kBars + 16 * kUnits + 8 * 8 + 16;
+    static constexpr int kSmem = 1024 + kBars + 16 * kUnits + 10 * 8 + 16;
     static constexpr int kPart = kVectors * (HDP + 2);   // floats of a part: [HDP / 4][vector][4], references, sums
     static constexpr uint32_t kO = 256;                  // tensor memory: scores (then P) of stream x at 128 x, its O
     static_assert(kSmem <= 232448 && kO + 2 * HDP <= 512, "memories");
@@ -68,19 +65,15 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 128 columns of this warp's 32 lanes, complete on return.  (One statement: between a load
-// and its wait the compiler may copy the registers, which do not hold the values yet.)
-__device__ __forceinline__ void ld128(uint32_t addr, float (&r)[128]) {
+// Columns of this warp's 32 lanes, complete on return.  (One statement: between a load and
+// its wait the compiler may copy the registers, which do not hold the values yet.)
+__device__ __forceinline__ void ld(uint32_t addr, float (&r)[64]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
         "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
         "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
         : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
           "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
@@ -89,15 +82,7 @@ __device__ __forceinline__ void ld128(uint32_t addr, float (&r)[128]) {
           "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
           "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
           "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
-          "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63]),
-          "=f"(r[64]), "=f"(r[65]), "=f"(r[66]), "=f"(r[67]), "=f"(r[68]), "=f"(r[69]), "=f"(r[70]), "=f"(r[71]),
-          "=f"(r[72]), "=f"(r[73]), "=f"(r[74]), "=f"(r[75]), "=f"(r[76]), "=f"(r[77]), "=f"(r[78]), "=f"(r[79]),
-          "=f"(r[80]), "=f"(r[81]), "=f"(r[82]), "=f"(r[83]), "=f"(r[84]), "=f"(r[85]), "=f"(r[86]), "=f"(r[87]),
-          "=f"(r[88]), "=f"(r[89]), "=f"(r[90]), "=f"(r[91]), "=f"(r[92]), "=f"(r[93]), "=f"(r[94]), "=f"(r[95]),
-          "=f"(r[96]), "=f"(r[97]), "=f"(r[98]), "=f"(r[99]), "=f"(r[100]), "=f"(r[101]), "=f"(r[102]), "=f"(r[103]),
-          "=f"(r[104]), "=f"(r[105]), "=f"(r[106]), "=f"(r[107]), "=f"(r[108]), "=f"(r[109]), "=f"(r[110]), "=f"(r[111]),
-          "=f"(r[112]), "=f"(r[113]), "=f"(r[114]), "=f"(r[115]), "=f"(r[116]), "=f"(r[117]), "=f"(r[118]), "=f"(r[119]),
-          "=f"(r[120]), "=f"(r[121]), "=f"(r[122]), "=f"(r[123]), "=f"(r[124]), "=f"(r[125]), "=f"(r[126]), "=f"(r[127])
+          "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
         : "r"(addr)
         : "memory");
 }
@@ -154,6 +139,61 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
     return all != 0;
 }
 
+// 2^z for pairs with -126 <= z on the fp32 units: z = n + f, |f| <= 1/2, a polynomial in f, n into
+// the exponent.  Coefficients by Remez exchange, relative error 7.5e-5 (degree 3, bf16) and
+// 2.6e-6 (degree 4, fp16), of which the rounding to the type that follows is 52 and 94 times.
+template <int kDegree>
+__device__ __forceinline__ uint64_t exp2_of(uint64_t z) {
+    constexpr float kRound = 12582912.0f;  // 1.5 2^23: a sum with it keeps the integer part in its low bits
+    float z0, z1, r0, r1, y0, y1;
+    unpair(z, z0, z1);
+    z = pair(fmaxf(z0, -126.0f), fmaxf(z1, -126.0f));
+    const uint64_t r = add2(z, pair(kRound, kRound)), f = add2(z, fma2(r, pair(-1.0f, -1.0f), pair(kRound, kRound)));
+    uint64_t y;
+    if (kDegree == 3) {
+        y = fma2(pair(0.0551716685f, 0.0551716685f), f, pair(0.242611125f, 0.242611125f));
+        y = fma2(y, f, pair(0.693260968f, 0.693260968f));
+        y = fma2(y, f, pair(0.999928057f, 0.999928057f));
+    } else {
+        y = fma2(pair(0.00957010221f, 0.00957010221f), f, pair(0.0559178591f, 0.0559178591f));
+        y = fma2(y, f, pair(0.240247443f, 0.240247443f));
+        y = fma2(y, f, pair(0.693121791f, 0.693121791f));
+        y = fma2(y, f, pair(0.999999285f, 0.999999285f));
+    }
+    unpair(y, y0, y1);
+    unpair(r, r0, r1);
+    return pair(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(r0) << 23)), __uint_as_float(__float_as_uint(y1) + (__float_as_uint(r1) << 23)));
+}
+// 64 scores of a vector to P in tensor memory; their sum.  kMixed: none is
+// masked, and some of the powers go to the fp32 units.
+template <typename T, bool kMixed>
+__device__ __forceinline__ float probabilities(const float (&s)[64], uint64_t by, uint64_t off, uint32_t p_tm) {
+    uint64_t total[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 64; i += 32) {
+        uint32_t p[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            uint64_t e = fma2(pair(s[i + j], s[i + j + 1]), by, off);
+            float z0, z1;
+            if (kMixed && (kOnUnits >> (j / 2 % 8) & 1)) {
+                e = exp2_of<Half16<T>::kDegree>(e);
+                unpair(e, z0, z1);
+            } else {
+                unpair(e, z0, z1);
+                z0 = ex2(z0), z1 = ex2(z1);
+                e = pair(z0, z1);
+            }
+            total[j / 2 % 2] = add2(total[j / 2 % 2], e);
+            p[j / 2] = Half16<T>::pack(z0, z1);
+        }
+        st16(p_tm + i / 2, p);
+    }
+    float t0, t1;
+    unpair(add2(total[0], total[1]), t0, t1);
+    return t0 + t1;
+}
+
 template <typename T, int HDP>
 __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_constant__ CUtensorMap k_map,
                                                                  const __grid_constant__ CUtensorMap v_map,
@@ -169,9 +209,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
     auto full = [&](int x) { return bars + 16 * x; };
     auto empty = [&](int x) { return bars + 16 * x + 8; };
     auto s_full = [&](int x) { return bars + 16 * S::kUnits + 8 * x; };
-    auto p_full = [&](int x) { return bars + 16 * S::kUnits + 16 + 8 * x; };
-    auto o_done = [&](int x) { return bars + 16 * S::kUnits + 32 + 8 * x; };
-    const uint32_t q_full = bars + 16 * S::kUnits + 48, finished = q_full + 8;
+    auto p_full = [&](int x, int half) { return bars + 16 * S::kUnits + 16 + 16 * x + 8 * half; };
+    auto o_done = [&](int x) { return bars + 16 * S::kUnits + 48 + 8 * x; };
+    const uint32_t q_full = bars + 16 * S::kUnits + 64, finished = q_full + 8;
     Cut* const cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.scratch) + kPagedCounterBytes);
     if (threadIdx.x == 0) {
         for (int x = 0; x < S::kUnits; ++x) {
@@ -180,7 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
         }
         for (int x = 0; x < 2; ++x) {
             dev::mbar_init(s_full(x), 1);
-            dev::mbar_init(p_full(x), 4);
+            dev::mbar_init(p_full(x, 0), 4);
+            dev::mbar_init(p_full(x, 1), 4);
             dev::mbar_init(o_done(x), 1);
         }
         dev::mbar_init(q_full, 8);
@@ -215,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
     // An item of more than kLanes vectors has two streams over the same tiles, each with its vectors; one of fewer
     // has two over every other tile, with the same vectors, whose results are added at its end.
     if (warp < kIssueWarp) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int x = warp / 4, row = threadIdx.x % kLanes;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp % 4) << 21), s_tm = lanes + kLanes * x, o_tm = lanes + S::kO + HDP * x;
         uint32_t* const bad_words = reinterpret_cast<uint32_t*>(smem + S::kBad);
@@ -230,23 +270,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             const int step = twice ? 1 : 2, v = (twice ? kLanes * x : 0) + row;  // the vector of this thread, in the item
             bar_sync(1, 256);  // nobody works on the item before
             if (threadIdx.x < 24) bad_words[threadIdx.x] = 0;
-            // Queries: rows of this stream's, or half of the pieces of the rows that both streams work on
+            // Queries, 32 rows of this stream's, or half of them where both streams work on the same; lanes on neighbouring
+            // pieces of a row
             {
-                const uint32_t to_q = base + (twice ? x * S::kUnit : 0) + row * 128;
-                const uint16_t* const q = static_cast<const uint16_t*>(a.q) + (v < it.valid ? place_of(a, it.b, it.head, it.v0 + v, a.q_stride) : 0);
-#pragma unroll 4
-                for (int piece = twice ? 0 : x; piece < HDP / 8; piece += step) {
-                    const uint32_t at = to_q + piece / 8 * (kTile * 128) + ((piece % 8 ^ (row & 7)) << 4);
-                    const int dim = piece * 8;
-                    if (v >= it.valid || dim >= d) {
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                    } else if (a.aligned & 1) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(q + dim) : "memory");
-                    } else {
-                        uint32_t e[4];
+                constexpr int kPieces = HDP / 8, kRows = 32 / kPieces;  // of 8 dims; rows at a time
+                const int first = v - lane, c = lane % kPieces, valid = it.valid;
+                const uint32_t to_q = base + (twice ? x * S::kUnit : 0) + c / 8 * (kTile * 128);
+                const int64_t mine = v < valid ? place_of(a, it.b, it.head, it.v0 + v, a.q_stride) : 0;
+                const uint16_t* const q = static_cast<const uint16_t*>(a.q);
+                const bool aligned = a.aligned & 1;
+#pragma unroll 1
+                for (int half = twice ? 0 : x; half < (twice ? 2 : x + 1); ++half) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = q[dim + 2 * j] | static_cast<uint32_t>(q[dim + 2 * j + 1]) << 16;
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]) : "memory");
+                    for (int i = 0; i < kPieces / 2; ++i) {
+                        const int r = half * 16 + i * kRows + lane / kPieces, line = row - lane + r;
+                        const int64_t from_q = __shfl_sync(0xffffffffu, mine, r) + 8 * c;
+                        const uint32_t at = to_q + line * 128 + ((c % 8 ^ (line & 7)) << 4);
+                        const bool here = first + r < valid && 8 * c < d;
+                        if (aligned) {
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(q + (here ? from_q : 0)), "r"(here ? 16 : 0));
+                        } else {
+                            uint32_t e[4] = {};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (here) e[j] = q[from_q + 2 * j] | static_cast<uint32_t>(q[from_q + 2 * j + 1]) << 16;
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]));
+                        }
                     }
                 }
             }
@@ -269,48 +318,79 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             for (int tile = from + (twice ? 0 : x); tile < to; tile += step, ++n, ++done) {
                 const int slot = tile * kTile;
                 const bool edge = slot + kTile > clear;
-                uint32_t seen[4];
+                const int group = twice ? 0 : x;
+                uint32_t* const words = bad_words + 12 * group + 4 * (n % 3);
+                if (edge) {
+                    // Values of slots past the last one seen count nothing, whatever is there, and values that are not
+                    // finite count for the vectors that see them alone: their rows of the tile become zeros, the rest
+                    // is told by the sums.
+                    const int cleaners = twice ? 256 : 128, me = twice ? static_cast<int>(threadIdx.x) : row, sees = it.sees;
+                    const int64_t vu = unit0 + 2 * (tile - from) + 1;
+                    wait(full(static_cast<int>(vu % S::kUnits)), (vu / S::kUnits) & 1);
+                    __syncwarp();
+                    for (int e = me; e < kTile * S::kBlocks; e += cleaners) {
+                        const int at = slot + e % kTile;
+                        if (at < clear) continue;  // seen by all
+                        uint4* const line = reinterpret_cast<uint4*>(smem + S::kRing + static_cast<uint32_t>(vu % S::kUnits) * S::kUnit + e * 128);
+                        bool clean = at >= sees || (no_page && !has_page(a, it.b, at));
+                        if (!clean) {
+                            uint32_t over = 0;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const uint4 w = line[i ^ (lane & 7)];
+                                over |= not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w);
+                            }
+                            clean = over != 0;
+                            if (clean) atomicOr(words + e % kTile / 32, 1u << (e % 32));
+                        }
+                        if (clean) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) line[i ^ (lane & 7)] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    bar_sync(2 + group, cleaners);
+                    if (me < 4) bad_words[12 * group + 4 * ((n + 2) % 3) + me] = 0;  // read two barriers ago, used after the next one
+                }
                 wait(s_full(x), done & 1);
                 __syncwarp();
                 tc_after();
-                float s[kTile];
-                if (works) ld128(s_tm, s);
-                if (a.factor < 0.0f) {
-#pragma unroll
-                    for (int j = 0; j < kTile; ++j) s[j] = -s[j];
-                }
-                if (edge) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) seen[i] = t >= 0 ? seen_bits(a, it, t, slot + 32 * i) : 0u;
-                    if (no_page) {
-                        for (int first = 0; first < kTile; first += 16) {
-                            bool page = false;
-                            if (slot + first < it.sees) {
-                                const int p = a.table[static_cast<int64_t>(it.b) * a.table_stride + ((slot + first) >> a.page_shift)];
-                                page = p >= 0 && p < a.pages;
-                            }
-                            if (!page) {
-                                const uint32_t off = ~(0xffffu << (first & 16));
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (first / 32 == i) seen[i] &= off;
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!(seen[i] >> j & 1u)) s[32 * i + j] = -INFINITY;
-                }
                 if (works) {
-                    float m[4];
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        float s[64];
+                        ld(s_tm + 64 * half, s);
+                        if (edge || a.factor < 0.0f) {
+                            uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+                            if (edge) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        m[i] = max3(s[i], s[4 + i], s[8 + i]);
+                                for (int i = 0; i < 2; ++i) {
+                                    const int first = slot + 64 * half + 32 * i;
+                                    seen[i] = t >= 0 ? seen_bits(a, it, t, first) : 0u;
+                                    if (no_page)
+                                        seen[i] &= (first < it.sees && has_page(a, it.b, first) ? 0xffffu : 0u) |
+                                                   (first + 16 < it.sees && has_page(a, it.b, first + 16) ? 0xffff0000u : 0u);
+                                    if (seen[i] & words[2 * half + i]) sum = __uint_as_float(0x7fc00000u);
+                                }
+                            }
+                            const uint32_t sign = a.factor < 0.0f ? 0x80000000u : 0u;
 #pragma unroll
-                        for (int j = 12; j < 124; j += 8) m[i] = max3(m[i], s[j + i], s[j + 4 + i]);
-                        m[i] = fmaxf(m[i], s[124 + i]);
+                            for (int i = 0; i < 64; i += 16) {
+                                uint32_t w[16];
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    s[i + j] = seen[i / 32] >> ((i + j) % 32) & 1u ? __uint_as_float(__float_as_uint(s[i + j]) ^ sign) : -INFINITY;
+                                    w[j] = __float_as_uint(s[i + j]);
+                                }
+                                st16(s_tm + 64 * half + i, w);
+                            }
+                            wait_st();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 64; j += 8)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) m[i] = max3(m[i], s[j + i], s[j + 4 + i]);
                     }
                     const float top = fmaxf(max3(m[0], m[1], m[2]), m[3]) * factor;
                     if (n == 0) {
@@ -334,68 +414,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                             st16(o_tm + i, w);
                         }
                     }
-                    const float less = (ref == -INFINITY ? 0.0f : ref) - kLift;
-                    const uint64_t by = pair(factor, factor), off = pair(-less, -less);
-                    uint64_t total[2] = {0, 0};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            float z0, z1;
-                            unpair(fma2(pair(s[32 * i + j], s[32 * i + j + 1]), by, off), z0, z1);
-                            z0 = ex2(z0), z1 = ex2(z1);
-                            total[j / 2 % 2] = add2(total[j / 2 % 2], pair(z0, z1));
-                            p[j / 2] = Half16<T>::pack(z0, z1);
-                        }
-                        st16(s_tm + 16 * i, p);
-                    }
-                    float t0, t1;
-                    unpair(add2(total[0], total[1]), t0, t1);
-                    sum += t0 + t1;
                 }
-                if (edge) {
-                    // Values of slots past the last one seen count nothing, whatever is there, and values that are not
-                    // finite count for the vectors that see them alone: their rows of the tile become zeros, the rest
-                    // is told by the sums.
-                    const int group = twice ? 0 : x, cleaners = twice ? 256 : 128, me = twice ? static_cast<int>(threadIdx.x) : row;
-                    const int64_t vu = unit0 + 2 * (tile - from) + 1;
-                    uint32_t* const words = bad_words + 12 * group + 4 * (n % 3);
-                    wait(full(static_cast<int>(vu % S::kUnits)), (vu / S::kUnits) & 1);
+                const float less = (ref == -INFINITY ? 0.0f : ref) - kLift;
+                const uint64_t by = pair(factor, factor), off = pair(-less, -less);
+                const bool mixed = !edge && !__any_sync(0xffffffffu, ref == -INFINITY);
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    if (works) {
+                        float s[64];
+                        ld(s_tm + 64 * half, s);
+                        sum += mixed ? probabilities<T, true>(s, by, off, s_tm + 32 * half) : probabilities<T, false>(s, by, off, s_tm + 32 * half);
+                        wait_st();
+                    }
+                    tc_before();
                     __syncwarp();
-                    for (int e = me; e < kTile * S::kBlocks; e += cleaners) {
-                        const int r = e % kTile;
-                        uint4* const line = reinterpret_cast<uint4*>(smem + S::kRing + (vu % S::kUnits) * S::kUnit + e * 128);
-                        if (slot + r < clear) continue;  // seen by all
-                        bool clean = slot + r >= it.sees;
-                        if (!clean && no_page) {
-                            const int p = a.table[static_cast<int64_t>(it.b) * a.table_stride + ((slot + r) >> a.page_shift)];
-                            clean = p < 0 || p >= a.pages;
-                        }
-                        if (!clean) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const uint4 w = line[(i + lane) % 8];
-                                clean = clean || not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w);
-                            }
-                            if (clean) atomicOr(words + r / 32, 1u << (r % 32));
-                        }
-                        if (clean) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) line[(i + lane) % 8] = make_uint4(0, 0, 0, 0);
-                        }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    bar_sync(2 + group, cleaners);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (words[i] & seen[i]) sum = __uint_as_float(0x7fc00000u);
-                    if (me < 4) bad_words[12 * group + 4 * ((n + 2) % 3) + me] = 0;  // read two barriers ago, used after the next one
+                    if (lane == 0) dev::mbar_arrive(p_full(x, half));
                 }
-                wait_st();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) dev::mbar_arrive(p_full(x));
             }
             unit0 += 2 * (to - from);
             if (n > 0) {
@@ -415,11 +449,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     stats[row] = ref, stats[kLanes + row] = sum;
                     if (works && n > 0) {
 #pragma unroll 1
-                        for (int i = 0; i < d; i += 16) {
-                            float o[16];
-                            ld16(o_tm + i, o);
+                        for (int i = 0; i < HDP; i += 64) {
+                            float o[64];
+                            ld(o_tm + i, o);
 #pragma unroll
-                            for (int j = 0; j < 16; j += 4)
+                            for (int j = 0; j < 64; j += 4)
                                 *reinterpret_cast<float4*>(there + ((i + j) / 4 * 32 + lane) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                         }
                         tc_before();
@@ -439,46 +473,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 const float scale1 = whole ? (total == 0.0f ? 0.0f : with / total) : with;
                 const int64_t at = v < it.valid ? place_of(a, it.b, it.head, it.v0 + v, static_cast<int64_t>(a.heads) * d) : 0;
                 const bool staged = whole && !a.out_f32 && (a.aligned & 2);
-                // 16-bit results pass through shared memory, [piece of 8 dims][row], and leave it row by row; behind the
-                // second stream's, which are read up to there by then
+                // 16-bit results pass through shared memory, [piece of 8 dims][row], and leave it row by row
                 uint4* const stage = twice ? reinterpret_cast<uint4*>(smem + x * S::kUnit + (warp % 4) * (HDP * 64)) : reinterpret_cast<uint4*>(there);
 #pragma unroll 1
-                for (int i = 0; i < d; i += 16) {
-                    float o[16];
-                    ld16(o_tm + i, o);
+                for (int i = 0; i < HDP; i += 64) {
+                    float o[64];
+                    ld(o_tm + i, o);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[j] = by == 0.0f ? 0.0f : o[j] * scale;
+                    for (int j = 0; j < 64; ++j) o[j] = by == 0.0f ? 0.0f : o[j] * scale;
                     if (!twice && with != 0.0f) {
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
+                        for (int j = 0; j < 64; j += 4) {
                             const float4 f = *reinterpret_cast<const float4*>(there + ((i + j) / 4 * 32 + lane) * 4);
                             o[j] = fmaf(f.x, scale1, o[j]), o[j + 1] = fmaf(f.y, scale1, o[j + 1]);
                             o[j + 2] = fmaf(f.z, scale1, o[j + 2]), o[j + 3] = fmaf(f.w, scale1, o[j + 3]);
                         }
                     }
                     __syncwarp();
-                    if (staged) {
+                    if (staged) {  // (over the second stream's, which are read as far as this reaches)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            stage[(i / 8 + j) * 32 + (lane ^ ((i / 8 + j) & 7))] = make_uint4(Half16<T>::pack(o[8 * j], o[8 * j + 1]), Half16<T>::pack(o[8 * j + 2], o[8 * j + 3]),
-                                                          Half16<T>::pack(o[8 * j + 4], o[8 * j + 5]), Half16<T>::pack(o[8 * j + 6], o[8 * j + 7]));
+                        for (int j = 0; j < 8; ++j)
+                            stage[(i / 8 + j) * 32 + (lane ^ j)] = make_uint4(Half16<T>::pack(o[8 * j], o[8 * j + 1]), Half16<T>::pack(o[8 * j + 2], o[8 * j + 3]),
+                                                                              Half16<T>::pack(o[8 * j + 4], o[8 * j + 5]), Half16<T>::pack(o[8 * j + 6], o[8 * j + 7]));
                     } else if (v < it.valid && !whole) {
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4)
+                        for (int j = 0; j < 64; j += 4)
                             __stcg(reinterpret_cast<float4*>(part + ((i + j) / 4 * kVectors + v) * 4), make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
                     } else if (v < it.valid) {
-                        put16<T>(a, at + i, o);
+#pragma unroll
+                        for (int j = 0; j < 64; j += 4)
+                            if (i + j < d) put4<T>(a, at + i + j, make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
                     }
                     __syncwarp();
                 }
                 if (staged) {
-                    const int pieces = d / 8;
+                    const int pieces = d / 8, some = 32 / pieces;
+                    int r = lane / pieces, c = lane - r * pieces;
 #pragma unroll 4
                     for (int i = 0; i < pieces; ++i) {
-                        const int r = (32 * i + lane) / pieces, c = 32 * i + lane - r * pieces;
                         const int64_t to_row = __shfl_sync(0xffffffffu, at, r);
                         if (v - lane + r < it.valid)
                             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to_row + 8 * c) = stage[c * 32 + (r ^ (c & 7))];
+                        r += some, c += 32 - some * pieces;
+                        if (c >= pieces) c -= pieces, ++r;
                     }
                 }
                 if (!whole && v < it.valid) {
@@ -493,7 +530,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             }
         } while (work.next());
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kIssueWarp && lane == 0) {
             constexpr uint32_t kType = Half16<T>::kUmma;
             constexpr uint32_t kIdescS = (1u << 4) | kType | (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kLanes >> 4) << 24);
@@ -524,11 +560,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 };
                 auto values = [&](int x, int i, bool first) {
                     const uint64_t vd = desc_of(base + S::kRing + static_cast<uint32_t>((unit0 + 2 * i + 1) % S::kUnits) * S::kUnit, kTile * 128);
-                    wait(p_full(x), done[x]++ & 1);
+                    wait(p_full(x, 0), done[x] & 1);
                     tc_after();
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
+                    for (int k = 0; k < kTile / 32; ++k)
                         mma_ts(tmem + S::kO + HDP * x, tmem + kLanes * x + 8 * k, vd + k * 2048 / 16, kIdescO, !(first && k == 0));
+                    wait(p_full(x, 1), done[x]++ & 1);
+                    tc_after();
+#pragma unroll
+                    for (int k = kTile / 32; k < kTile / 16; ++k)
+                        mma_ts(tmem + S::kO + HDP * x, tmem + kLanes * x + 8 * k, vd + k * 2048 / 16, kIdescO, 1u);
                     mma_commit(o_done(x));
                 };
                 wait(q_full, items++ & 1);
@@ -666,11 +707,6 @@ cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const Pag
     const auto kernel = paged_many_kernel<T, HDP>;
     cudaError_t e = allow_shared(kernel, S::kSmem, allowed);
     if (e != cudaSuccess) return e;
-    static const int regs = [] {  // what the compiler gave the kernel has to be what the roles share out
-        cudaFuncAttributes f{};
-        return cudaFuncGetAttributes(&f, paged_many_kernel<T, HDP>) == cudaSuccess ? f.numRegs : -1;
-    }();
-    if (regs != kLaunchRegs) return cudaErrorInvalidConfiguration;
     const int64_t items = static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors);
     const int64_t most = std::max(items, items * ((a.capacity + kTile - 1) / kTile) / kLeast);
     const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count, kPagedManyCtas), most));
