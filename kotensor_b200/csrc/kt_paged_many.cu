@@ -14,7 +14,7 @@ constexpr int kVectors = 2 * kLanes;       // of an item
 constexpr int kTile = 128;                 // slots of a tile
 constexpr int kStart = 2;                  // tiles that entering an item costs
 constexpr int kLeast = 2;                  // tiles that are worth a CTA
-constexpr int kIssueWarp = 8, kCopyWarp = 9;  // after the softmax warps; the two after them do nothing
+constexpr int kIssueWarp = 8, kCopyWarp = 10;  // after the softmax warps; an issuing warp for each stream; the last does nothing
 constexpr int kThreads = 384;
 constexpr float kLift = 6.0f;    // probabilities are 2^kLift times larger: fp16 keeps them to 2^-30 of the reference
 constexpr float kSlack = 8.0f;   // the reference moves when a score passes it by this much (2^14 < fp16's largest)
@@ -28,7 +28,7 @@ struct ManyShape {
     static constexpr int kBad = kRing + kUnits * kUnit;  // slots of an edge tile whose values are not finite: [2][3][4] words
     static constexpr int kStats = kBad + 128;            // of the second stream's vectors
     static constexpr int kBars = kStats + 2 * kLanes * 4;
-    static constexpr int kSmem = 1024 + kBars + 16 * kUnits + 10 * 8 + 16;
+    static constexpr int kSmem = 1024 + kBars + 16 * kUnits + 14 * 8;
     static constexpr int kPart = kVectors * (HDP + 2);   // floats of a part: [HDP / 4][vector][4], references, sums
     static constexpr uint32_t kO = 256;                  // tensor memory: scores (then P) of stream x at 128 x, its O
     static_assert(kSmem <= 232448 && kO + 2 * HDP <= 512, "memories");
@@ -40,23 +40,24 @@ struct Cut {
 };
 static_assert(sizeof(Cut) * kPagedManyCtas <= kPagedCutBytes, "a place each");
 
-__device__ __forceinline__ uint64_t desc_of(uint32_t addr, uint32_t lead) {
-    // 128-byte swizzle, atoms of 8 rows 1024 bytes apart, descriptor version 1
-    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory descriptors, the low words (the issuing thread adds to 32 bits, not 64):
+// 128-byte swizzle, atoms of 8 rows 1024 bytes apart, descriptor version 1.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_of(uint32_t addr, uint32_t lead) { return (addr & 0x3FFFFu) >> 4 | lead >> 4 << 16; }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
@@ -208,24 +209,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
     const uint32_t bars = base + S::kBars;
     auto full = [&](int x) { return bars + 16 * x; };
     auto empty = [&](int x) { return bars + 16 * x + 8; };
-    auto s_full = [&](int x) { return bars + 16 * S::kUnits + 8 * x; };
-    auto p_full = [&](int x, int half) { return bars + 16 * S::kUnits + 16 + 16 * x + 8 * half; };
-    auto o_done = [&](int x) { return bars + 16 * S::kUnits + 48 + 8 * x; };
-    const uint32_t q_full = bars + 16 * S::kUnits + 64, finished = q_full + 8;
+    // of stream x, for each half of a tile
+    auto s_full = [&](int x, int half) { return bars + 16 * S::kUnits + 16 * x + 8 * half; };
+    auto p_full = [&](int x, int half) { return s_full(x, half) + 32; };
+    auto o_done = [&](int x, int half) { return s_full(x, half) + 64; };
+    const uint32_t q_full = bars + 16 * S::kUnits + 96, finished = q_full + 8;
     Cut* const cuts = reinterpret_cast<Cut*>(static_cast<char*>(a.scratch) + kPagedCounterBytes);
     if (threadIdx.x == 0) {
         for (int x = 0; x < S::kUnits; ++x) {
             dev::mbar_init(full(x), 1);
-            dev::mbar_init(empty(x), 1);
+            dev::mbar_init(empty(x), 2);  // an issuing warp each
         }
-        for (int x = 0; x < 2; ++x) {
-            dev::mbar_init(s_full(x), 1);
-            dev::mbar_init(p_full(x, 0), 4);
-            dev::mbar_init(p_full(x, 1), 4);
-            dev::mbar_init(o_done(x), 1);
+        for (int i = 0; i < 4; ++i) {
+            dev::mbar_init(s_full(i / 2, i % 2), 1);
+            dev::mbar_init(p_full(i / 2, i % 2), 4);
+            dev::mbar_init(o_done(i / 2, i % 2), 1);
         }
         dev::mbar_init(q_full, 8);
-        dev::mbar_init(finished, 1);
+        dev::mbar_init(finished, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     dev::pdl_wait();
@@ -352,78 +353,65 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     bar_sync(2 + group, cleaners);
                     if (me < 4) bad_words[12 * group + 4 * ((n + 2) % 3) + me] = 0;  // read two barriers ago, used after the next one
                 }
-                wait(s_full(x), done & 1);
-                __syncwarp();
-                tc_after();
-                if (works) {
-                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        float s[64];
-                        ld(s_tm + 64 * half, s);
-                        if (edge || a.factor < 0.0f) {
-                            uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-                            if (edge) {
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) {
-                                    const int first = slot + 64 * half + 32 * i;
-                                    seen[i] = t >= 0 ? seen_bits(a, it, t, first) : 0u;
-                                    if (no_page)
-                                        seen[i] &= (first < it.sees && has_page(a, it.b, first) ? 0xffffu : 0u) |
-                                                   (first + 16 < it.sees && has_page(a, it.b, first + 16) ? 0xffff0000u : 0u);
-                                    if (seen[i] & words[2 * half + i]) sum = __uint_as_float(0x7fc00000u);
-                                }
-                            }
-                            const uint32_t sign = a.factor < 0.0f ? 0x80000000u : 0u;
-#pragma unroll
-                            for (int i = 0; i < 64; i += 16) {
-                                uint32_t w[16];
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    s[i + j] = seen[i / 32] >> ((i + j) % 32) & 1u ? __uint_as_float(__float_as_uint(s[i + j]) ^ sign) : -INFINITY;
-                                    w[j] = __float_as_uint(s[i + j]);
-                                }
-                                st16(s_tm + 64 * half + i, w);
-                            }
-                            wait_st();
-                        }
-#pragma unroll
-                        for (int j = 0; j < 64; j += 8)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) m[i] = max3(m[i], s[j + i], s[j + 4 + i]);
-                    }
-                    const float top = fmaxf(max3(m[0], m[1], m[2]), m[3]) * factor;
-                    if (n == 0) {
-                        ref = top;
-                    } else if (__any_sync(0xffffffffu, top > ref + kSlack)) {
-                        // O and the sum go over to a larger reference; rare, as it lags behind by up to kSlack
-                        const bool move = top > ref + kSlack;
-                        const float fade = !move ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
-                        if (move) ref = top;
-                        sum *= fade;
-                        wait(o_done(x), (done - 1) & 1);
-                        __syncwarp();
-                        tc_after();
-#pragma unroll 1
-                        for (int i = 0; i < d; i += 16) {
-                            float o[16];
-                            ld16(o_tm + i, o);
-                            uint32_t w[16];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * fade);
-                            st16(o_tm + i, w);
-                        }
-                    }
-                }
-                const float less = (ref == -INFINITY ? 0.0f : ref) - kLift;
-                const uint64_t by = pair(factor, factor), off = pair(-less, -less);
-                const bool mixed = !edge && !__any_sync(0xffffffffu, ref == -INFINITY);
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
+                    wait(s_full(x, half), done & 1);
+                    __syncwarp();
+                    tc_after();
                     if (works) {
                         float s[64];
                         ld(s_tm + 64 * half, s);
-                        sum += mixed ? probabilities<T, true>(s, by, off, s_tm + 32 * half) : probabilities<T, false>(s, by, off, s_tm + 32 * half);
+                        if (edge) {
+                            const int first = slot + 64 * half;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                uint32_t seen = t >= 0 ? seen_bits(a, it, t, first + 32 * i) : 0u;
+                                if (no_page)
+                                    seen &= (first + 32 * i < it.sees && has_page(a, it.b, first + 32 * i) ? 0xffffu : 0u) |
+                                            (first + 32 * i + 16 < it.sees && has_page(a, it.b, first + 32 * i + 16) ? 0xffff0000u : 0u);
+                                if (seen & words[2 * half + i]) sum = __uint_as_float(0x7fc00000u);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (!(seen >> j & 1u)) s[32 * i + j] = a.factor < 0.0f ? INFINITY : -INFINITY;
+                            }
+                        }
+                        if (a.factor < 0.0f) {  // (a negative scale turns the scores)
+#pragma unroll
+                            for (int j = 0; j < 64; ++j) s[j] = -s[j];
+                        }
+                        float m[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) m[i] = fmaxf(s[i], s[4 + i]);
+#pragma unroll
+                        for (int j = 8; j < 64; j += 8)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) m[i] = max3(m[i], s[j + i], s[j + 4 + i]);
+                        const float top = fmaxf(max3(m[0], m[1], m[2]), m[3]) * factor;
+                        if (n == 0 && half == 0) {
+                            ref = top;
+                        } else if (__any_sync(0xffffffffu, top > ref + kSlack)) {
+                            // O and the sum go over to a larger reference; rare, as it lags behind by up to kSlack
+                            const bool move = top > ref + kSlack;
+                            const float fade = !move ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
+                            if (move) ref = top;
+                            sum *= fade;
+                            wait(o_done(x, 1 - half), (done - 1 + half) & 1);  // of the half before
+                            __syncwarp();
+                            tc_after();
+#pragma unroll 1
+                            for (int i = 0; i < d; i += 16) {
+                                float o[16];
+                                ld16(o_tm + i, o);
+                                uint32_t w[16];
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * fade);
+                                st16(o_tm + i, w);
+                            }
+                        }
+                        const float less = (ref == -INFINITY ? 0.0f : ref) - kLift;
+                        const uint64_t by = pair(factor, factor), off = pair(-less, -less);
+                        const bool mixed = !edge && !__any_sync(0xffffffffu, ref == -INFINITY);
+                        sum += mixed ? probabilities<T, true>(s, by, off, s_tm + 64 * half) : probabilities<T, false>(s, by, off, s_tm + 64 * half);
                         wait_st();
                     }
                     tc_before();
@@ -433,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             }
             unit0 += 2 * (to - from);
             if (n > 0) {
-                wait(o_done(x), (done - 1) & 1);
+                wait(o_done(x, 1), (done - 1) & 1);
                 __syncwarp();
                 tc_after();
             }
@@ -530,92 +518,75 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             }
         } while (work.next());
     } else {
-        if (warp == kIssueWarp && lane == 0) {
+        if (warp < kCopyWarp && lane == 0) {
+            // A stream's products, half a tile at a time: P V, then Q K^T of its next tile's half into the same columns, in the
+            // order of issue.  The other half is with the softmax warps meanwhile.
             constexpr uint32_t kType = Half16<T>::kUmma;
-            constexpr uint32_t kIdescS = (1u << 4) | kType | (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kLanes >> 4) << 24);
+            constexpr uint32_t kIdescS = (1u << 4) | kType | (static_cast<uint32_t>(kTile / 2 >> 3) << 17) | (static_cast<uint32_t>(kLanes >> 4) << 24);
             // the second product's B is MN-major (bit 16)
             constexpr uint32_t kIdescO = (1u << 4) | kType | (1u << 16) | (static_cast<uint32_t>(HDP >> 3) << 17) |
                                          (static_cast<uint32_t>(kLanes >> 4) << 24);
+            const int x = warp - kIssueWarp;
+            const uint32_t s_tm = tmem + kLanes * x, o_tm = tmem + S::kO + HDP * x;
             int64_t unit0 = 0;
-            uint32_t items = 0, done[2] = {0, 0};
+            uint32_t items = 0, done = 0;
             while (ok) {
                 const int n = it.to - it.from;
-                if (n <= 0) {
-                    if (it.last) break;
-                    work.step();
-                    continue;
-                }
-                const bool twice = it.valid > kLanes;
-                auto landed = [&](int64_t u) { wait(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1); };
-                auto release = [&](int64_t u) { mma_commit(empty(static_cast<int>(u % S::kUnits))); };
-                auto scores = [&](int x, int i) {
-                    const uint64_t kd = desc_of(base + S::kRing + static_cast<uint32_t>((unit0 + 2 * i) % S::kUnits) * S::kUnit, 16);
-                    const uint64_t qd = desc_of(base + (twice ? x * S::kUnit : 0), 16);
+                if (n > 0) {
+                    const bool twice = it.valid > kLanes;
+                    const int step = twice ? 1 : 2, first = twice ? 0 : x;
+                    const uint32_t qd = desc_of(base + (twice ? x * S::kUnit : 0), 16);
+                    auto unit_of = [&](int64_t u) { return static_cast<int>(u % S::kUnits); };
+                    auto release = [&](int u) {  // (two arrivals free a unit: one of each stream, or both of the one that uses it)
+                        mma_commit(empty(u));
+                        if (!twice) mma_commit(empty(u));
+                    };
+                    auto scores = [&](int i, int half) {
+                        const int64_t u = unit0 + 2 * i;
+                        const int at = unit_of(u);
+                        const uint32_t kd = desc_of(base + S::kRing + at * S::kUnit + half * (kTile / 2 * 128), 16);
+                        if (half == 0) {
+                            wait(full(at), (u / S::kUnits) & 1);
+                            tc_after();
+                        }
+                        // (all steps, whatever head_dim is: under a condition the later ones lost their descriptors)
 #pragma unroll
-                    for (int k = 0; k < HDP / 16; ++k) {
-                        const uint64_t off = ((k / 4) * (kTile * 128) + (k % 4) * 32) / 16;
-                        mma_ss(tmem + kLanes * x, qd + off, kd + off, kIdescS, k > 0);
-                    }
-                    mma_commit(s_full(x));
-                };
-                auto values = [&](int x, int i, bool first) {
-                    const uint64_t vd = desc_of(base + S::kRing + static_cast<uint32_t>((unit0 + 2 * i + 1) % S::kUnits) * S::kUnit, kTile * 128);
-                    wait(p_full(x, 0), done[x] & 1);
+                        for (int k = 0; k < HDP / 16; ++k) {
+                            const uint32_t off = ((k / 4) * (kTile * 128) + (k % 4) * 32) / 16;
+                            mma_ss(s_tm + 64 * half, qd + off, kd + off, kIdescS, k > 0);
+                        }
+                        mma_commit(s_full(x, half));
+                        if (half == 1) release(at);
+                    };
+                    wait(q_full, items++ & 1);
                     tc_after();
+                    if (first < n) {
+                        scores(first, 0);
+                        scores(first, 1);
+                    }
+                    for (int i = first; ok && i < n; i += step, ++done) {
+                        const int64_t u = unit0 + 2 * i + 1;
+                        const int at = unit_of(u);
+                        wait(full(at), (u / S::kUnits) & 1);
+#pragma unroll 1
+                        for (int half = 0; half < 2; ++half) {
+                            const uint32_t vd = desc_of(base + S::kRing + at * S::kUnit + half * (kTile / 2 * 128), kTile * 128);
+                            wait(p_full(x, half), done & 1);
+                            tc_after();
 #pragma unroll
-                    for (int k = 0; k < kTile / 32; ++k)
-                        mma_ts(tmem + S::kO + HDP * x, tmem + kLanes * x + 8 * k, vd + k * 2048 / 16, kIdescO, !(first && k == 0));
-                    wait(p_full(x, 1), done[x]++ & 1);
-                    tc_after();
-#pragma unroll
-                    for (int k = kTile / 32; k < kTile / 16; ++k)
-                        mma_ts(tmem + S::kO + HDP * x, tmem + kLanes * x + 8 * k, vd + k * 2048 / 16, kIdescO, 1u);
-                    mma_commit(o_done(x));
-                };
-                wait(q_full, items++ & 1);
-                tc_after();
-                if (twice) {
-                    landed(unit0);
-                    scores(0, 0);
-                    scores(1, 0);
-                    release(unit0);
-                    for (int i = 0; ok && i < n; ++i) {
-                        const int64_t k1 = unit0 + 2 * (i + 1), v = unit0 + 2 * i + 1;
-                        landed(v);
-                        values(0, i, i == 0);
-                        if (i + 1 < n) {
-                            landed(k1);
-                            scores(0, i + 1);
-                        }
-                        values(1, i, i == 0);
-                        release(v);
-                        if (i + 1 < n) {
-                            scores(1, i + 1);
-                            release(k1);
+                            for (int k = 0; k < kTile / 32; ++k)
+                                mma_ts(o_tm, s_tm + 64 * half + 8 * k, vd + k * 2048 / 16, kIdescO, i > first || half > 0 || k > 0);
+                            mma_commit(o_done(x, half));
+                            if (half == 1) release(at);
+                            if (i + step < n) scores(i + step, half);
                         }
                     }
-                } else {
-                    for (int i = 0; i < min(2, n); ++i) {
-                        landed(unit0 + 2 * i);
-                        scores(i, i);
-                        release(unit0 + 2 * i);
-                    }
-                    for (int i = 0; ok && i < n; ++i) {
-                        landed(unit0 + 2 * i + 1);
-                        values(i & 1, i, i < 2);
-                        release(unit0 + 2 * i + 1);
-                        if (i + 2 < n) {
-                            landed(unit0 + 2 * (i + 2));
-                            scores(i & 1, i + 2);
-                            release(unit0 + 2 * (i + 2));
-                        }
-                    }
+                    unit0 += 2 * n;
                 }
-                unit0 += 2 * n;
                 if (it.last) break;
                 work.step();
             }
-            // no product is under way past this point, also where a wait has given up
+            // no product of this stream is under way past this point, also where a wait has given up
             mma_commit(finished);
             if (!wait_counted(finished, 0)) ok = false;
         } else if (warp == kCopyWarp) {
