@@ -248,8 +248,7 @@ __device__ __forceinline__ bool has_page(const PagedAttention& a, int b, int slo
     return page >= 0 && page < a.pages;
 }
 
-// Waits for phase `parity` of `bar`; false after some seconds.  (Four tries to a turn: the turns
-// of warps that wait take issue slots from those that work.)
+// Waits for phase `parity` of `bar`; false after some seconds.
 __device__ __forceinline__ bool wait_counted(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -257,12 +256,9 @@ __device__ __forceinline__ bool wait_counted(uint32_t bar, uint32_t parity) {
         "mov.u32 n, 0;\n\t"
         "TRY:\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "@!p mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "@!p mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "@!p mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "@p bra DONE;\n\t"
         "add.u32 n, n, 1;\n\t"
-        "setp.lt.u32 q, n, 8388608;\n\t"
+        "setp.lt.u32 q, n, 33554432;\n\t"
         "@q bra TRY;\n\t"
         "DONE:\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
@@ -284,7 +280,6 @@ template <>
 struct Half16<__half> {
     static constexpr uint32_t kExponent = 0x7c007c00u;
     static constexpr uint32_t kUmma = 0;  // the operands' type in tcgen05.mma's descriptor
-    static constexpr int kDegree = 4;     // of a polynomial for 2^f that its rounding hides
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __half2 h = __floats2half2_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -294,7 +289,6 @@ template <>
 struct Half16<__nv_bfloat16> {
     static constexpr uint32_t kExponent = 0x7f807f80u;
     static constexpr uint32_t kUmma = 1u << 7 | 1u << 10;
-    static constexpr int kDegree = 3;
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);

@@ -12,13 +12,12 @@ using namespace paged;
 constexpr int kLanes = 128;                // vectors of a stream (the MMA's M)
 constexpr int kVectors = 2 * kLanes;       // of an item
 constexpr int kTile = 128;                 // slots of a tile
-constexpr int kStart = 2;                  // tiles that entering an item costs
+constexpr int kStart = 4;                  // tiles that entering an item costs
 constexpr int kLeast = 2;                  // tiles that are worth a CTA
 constexpr int kIssueWarp = 8, kCopyWarp = 10;  // after the softmax warps; an issuing warp for each stream; the last does nothing
 constexpr int kThreads = 384;
 constexpr float kLift = 6.0f;    // probabilities are 2^kLift times larger: fp16 keeps them to 2^-30 of the reference
 constexpr float kSlack = 8.0f;   // the reference moves when a score passes it by this much (2^14 < fp16's largest)
-constexpr uint32_t kOnUnits = 0x54;  // which of eight pairs of powers of 2 go to the fp32 units
 
 template <int HDP>
 struct ManyShape {
@@ -129,6 +128,7 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     return r;
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
     uint32_t all;
     asm volatile(
@@ -140,34 +140,8 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
     return all != 0;
 }
 
-// 2^z for pairs with -126 <= z on the fp32 units: z = n + f, |f| <= 1/2, a polynomial in f, n into
-// the exponent.  Coefficients by Remez exchange, relative error 7.5e-5 (degree 3, bf16) and
-// 2.6e-6 (degree 4, fp16), of which the rounding to the type that follows is 52 and 94 times.
-template <int kDegree>
-__device__ __forceinline__ uint64_t exp2_of(uint64_t z) {
-    constexpr float kRound = 12582912.0f;  // 1.5 2^23: a sum with it keeps the integer part in its low bits
-    float z0, z1, r0, r1, y0, y1;
-    unpair(z, z0, z1);
-    z = pair(fmaxf(z0, -126.0f), fmaxf(z1, -126.0f));
-    const uint64_t r = add2(z, pair(kRound, kRound)), f = add2(z, fma2(r, pair(-1.0f, -1.0f), pair(kRound, kRound)));
-    uint64_t y;
-    if (kDegree == 3) {
-        y = fma2(pair(0.0551716685f, 0.0551716685f), f, pair(0.242611125f, 0.242611125f));
-        y = fma2(y, f, pair(0.693260968f, 0.693260968f));
-        y = fma2(y, f, pair(0.999928057f, 0.999928057f));
-    } else {
-        y = fma2(pair(0.00957010221f, 0.00957010221f), f, pair(0.0559178591f, 0.0559178591f));
-        y = fma2(y, f, pair(0.240247443f, 0.240247443f));
-        y = fma2(y, f, pair(0.693121791f, 0.693121791f));
-        y = fma2(y, f, pair(0.999999285f, 0.999999285f));
-    }
-    unpair(y, y0, y1);
-    unpair(r, r0, r1);
-    return pair(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(r0) << 23)), __uint_as_float(__float_as_uint(y1) + (__float_as_uint(r1) << 23)));
-}
-// 64 scores of a vector to P in tensor memory; their sum.  kMixed: none is
-// masked, and some of the powers go to the fp32 units.
-template <typename T, bool kMixed>
+// 64 scores of a vector to P in tensor memory; their sum.
+template <typename T>
 __device__ __forceinline__ float probabilities(const float (&s)[64], uint64_t by, uint64_t off, uint32_t p_tm) {
     uint64_t total[2] = {0, 0};
 #pragma unroll
@@ -175,17 +149,10 @@ __device__ __forceinline__ float probabilities(const float (&s)[64], uint64_t by
         uint32_t p[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-            uint64_t e = fma2(pair(s[i + j], s[i + j + 1]), by, off);
             float z0, z1;
-            if (kMixed && (kOnUnits >> (j / 2 % 8) & 1)) {
-                e = exp2_of<Half16<T>::kDegree>(e);
-                unpair(e, z0, z1);
-            } else {
-                unpair(e, z0, z1);
-                z0 = ex2(z0), z1 = ex2(z1);
-                e = pair(z0, z1);
-            }
-            total[j / 2 % 2] = add2(total[j / 2 % 2], e);
+            unpair(fma2(pair(s[i + j], s[i + j + 1]), by, off), z0, z1);
+            z0 = ex2(z0), z1 = ex2(z1);
+            total[j / 2 % 2] = add2(total[j / 2 % 2], pair(z0, z1));
             p[j / 2] = Half16<T>::pack(z0, z1);
         }
         st16(p_tm + i / 2, p);
@@ -262,6 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
         uint32_t* const bad_words = reinterpret_cast<uint32_t*>(smem + S::kBad);
         float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedPartsAt);
         const float factor = fabsf(a.factor);
+        if (x == 1) bar_arrive(4, 256);  // the first stream has the first turn
         int64_t unit0 = 0;  // of the run's first tile of this item
         uint32_t done = 0;  // tiles of this stream
         do {
@@ -327,6 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     // is told by the sums.
                     const int cleaners = twice ? 256 : 128, me = twice ? static_cast<int>(threadIdx.x) : row, sees = it.sees;
                     const int64_t vu = unit0 + 2 * (tile - from) + 1;
+                    // (the scores were issued after the values that lay in this place before had landed: the phase is no older one)
+                    wait(s_full(x, 0), done & 1);
                     wait(full(static_cast<int>(vu % S::kUnits)), (vu / S::kUnits) & 1);
                     __syncwarp();
                     for (int e = me; e < kTile * S::kBlocks; e += cleaners) {
@@ -410,9 +380,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                         }
                         const float less = (ref == -INFINITY ? 0.0f : ref) - kLift;
                         const uint64_t by = pair(factor, factor), off = pair(-less, -less);
-                        const bool mixed = !edge && !__any_sync(0xffffffffu, ref == -INFINITY);
-                        sum += mixed ? probabilities<T, true>(s, by, off, s_tm + 64 * half) : probabilities<T, false>(s, by, off, s_tm + 64 * half);
+                        if (twice) bar_sync(4 + x, 256);
+                        sum += probabilities<T>(s, by, off, s_tm + 64 * half);
+                        if (twice) bar_arrive(5 - x, 256);
                         wait_st();
+                    } else if (twice) {
+                        bar_sync(4 + x, 256);
+                        bar_arrive(5 - x, 256);
                     }
                     tc_before();
                     __syncwarp();
@@ -517,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 cuts[blockIdx.x] = Cut{c1 - static_cast<int>(blockIdx.x) + 1, it.b, it.head, it.v0, it.valid, {}};
             }
         } while (work.next());
+        if (x == 0) bar_sync(4, 256);  // the last turn is nobody's
     } else {
         if (warp < kCopyWarp && lane == 0) {
             // A stream's products, half a tile at a time: P V, then Q K^T of its next tile's half into the same columns, in the
@@ -545,10 +520,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                         const int64_t u = unit0 + 2 * i;
                         const int at = unit_of(u);
                         const uint32_t kd = desc_of(base + S::kRing + at * S::kUnit + half * (kTile / 2 * 128), 16);
-                        if (half == 0) {
-                            wait(full(at), (u / S::kUnits) & 1);
-                            tc_after();
-                        }
                         // (all steps, whatever head_dim is: under a condition the later ones lost their descriptors)
 #pragma unroll
                         for (int k = 0; k < HDP / 16; ++k) {
@@ -560,14 +531,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     };
                     wait(q_full, items++ & 1);
                     tc_after();
+                    auto landed = [&](int64_t u) { wait(full(unit_of(u)), (u / S::kUnits) & 1); };
                     if (first < n) {
+                        landed(unit0 + 2 * first);
+                        tc_after();
                         scores(first, 0);
                         scores(first, 1);
                     }
                     for (int i = first; ok && i < n; i += step, ++done) {
                         const int64_t u = unit0 + 2 * i + 1;
                         const int at = unit_of(u);
-                        wait(full(at), (u / S::kUnits) & 1);
+                        // (asked for before P is there: even when a barrier's phase is over, a wait takes two to four hundred clocks)
+                        landed(u);
+                        if (i + step < n) landed(u - 1 + 2 * step);
 #pragma unroll 1
                         for (int half = 0; half < 2; ++half) {
                             const uint32_t vd = desc_of(base + S::kRing + at * S::kUnit + half * (kTile / 2 * 128), kTile * 128);

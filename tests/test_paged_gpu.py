@@ -175,6 +175,16 @@ def test_attention_of_drafted_trees(kt, layout, page, lengths, rows, dtype, ragg
     check_attend(cache, q, layout[0], rows, cache.attend(0, q, layout[0], rows, counts, visible), counts, visible)
 
 
+@pytest.mark.parametrize("tokens", [130, 250, 390, 513, 640])
+@pytest.mark.parametrize("batch,rows", [(3, 7), (20, 9), (41, 18)])
+def test_attention_however_the_work_is_cut(kt, tokens, batch, rows):
+    """Items of one to six tiles, alone in a CTA, several to one or shared by some."""
+    cache = filled((8, 2, 64), 32, BF16, [max(0, tokens - 97 * (i % 4)) for i in range(batch)], rows, poison=True)
+    put(cache, rows)
+    q = queries(cache, 8, rows)
+    check_attend(cache, q, 8, rows, cache.attend(0, q, 8, rows))
+
+
 @pytest.mark.parametrize("layout,rows", [(LLAMA, 1), (QWEN, 70), (WIDE, 30)])
 def test_attention_into_fp32_with_a_scale(kt, layout, rows):
     cache = filled(layout, 32, FP16, [90, 11], rows)
