@@ -100,7 +100,7 @@ template <int kWarps>
 struct Plan {
     int64_t share, spare, begin, end;
     int64_t sums[kWarps], items[kWarps], base;
-    int entry;
+    int entry, dealt;
     Item at[kWarps];
 };
 
@@ -108,7 +108,11 @@ struct Plan {
 // units, what entering it costs, and one for each tile.  Equal runs of units go to the
 // CTAs: ragged batches, single long sequences and the triangle of a prompt load every SM
 // alike.  Lengths are read here, on the device, so a captured launch fits any.
-template <int kWarps, int kVectors, int kTile, int kStart, int kLeast>
+//
+// With kDeal, equal sequences of several vector tiles (a prompt) are not cut where there are
+// kDeal items or more to a CTA: they are dealt out whole, the longest first, every other
+// round backwards, so that the sums are as equal and nothing has to be merged.
+template <int kWarps, int kVectors, int kTile, int kStart, int kLeast, int kDeal>
 struct WorkList {
     const PagedAttention& a;
     Plan<kWarps>& plan;
@@ -123,6 +127,21 @@ struct WorkList {
         it.valid = min(kVectors, it.count * a.group - it.v0);
         it.sees = it.valid <= 0 ? 0 : a.visible ? it.held + it.count : it.held + (it.v0 + it.valid - 1) / a.group + 1;
         it.tiles = (it.sees + kTile - 1) / kTile;
+    }
+    // Item `rank` of those dealt, the last vector tile's first: by the item's round and this CTA.
+    __device__ bool deal(Item& it, int64_t round, int vts) const {
+        const int64_t among = static_cast<int64_t>(a.batch) * a.kv_heads, all = among * vts;
+        const int64_t rank = round * gridDim.x + (round % 2 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (rank >= all) return false;
+        const int vt = vts - 1 - static_cast<int>(rank / among), which = static_cast<int>(rank % among);
+        load(it, which / a.kv_heads * vts + vt, vts);
+        it.head = which % a.kv_heads;
+        it.base = round;
+        it.from = 0, it.to = it.tiles;
+        // (the next round's item of this CTA, if there is one)
+        const int64_t next = (round + 1) * gridDim.x + (round % 2 ? blockIdx.x : gridDim.x - 1 - blockIdx.x);
+        it.last = next >= all;
+        return true;
     }
     __device__ __forceinline__ void cut(Item& it) const {
         it.from = static_cast<int>(max(static_cast<int64_t>(0), plan.begin - it.base - kStart));
@@ -142,6 +161,20 @@ struct WorkList {
     __device__ bool start() const {
         constexpr int kThreads = kWarps * 32;
         const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, vts = vector_tiles();
+        if (kDeal > 0 && vts > 1 && static_cast<int64_t>(a.batch) * a.kv_heads * vts >= static_cast<int64_t>(kDeal) * gridDim.x) {
+            bool equal = true;
+            for (int b = threadIdx.x; b < a.batch; b += kThreads)
+                equal = equal && a.lengths[b] == a.lengths[0] && (a.counts == nullptr || a.counts[b] == a.counts[0]);
+            if (__syncthreads_and(equal)) {
+                if (threadIdx.x == 0) plan.dealt = 1;
+                Item it;
+                const bool any = deal(it, 0, vts);
+                if (lane == 0) plan.at[warp] = it;
+                __syncthreads();
+                return any;
+            }
+        }
+        if (threadIdx.x == 0) plan.dealt = 0;
         const int entries = a.batch * vts, each = (entries + kThreads - 1) / kThreads;
         const int from = min(entries, static_cast<int>(threadIdx.x) * each), to = min(entries, from + each);
         Item it;
@@ -202,6 +235,11 @@ struct WorkList {
     // To the warp's next item; by its lane 0.
     __device__ void step() const {
         Item it = plan.at[threadIdx.x / 32];
+        if (kDeal > 0 && plan.dealt) {
+            deal(it, it.base + 1, vector_tiles());
+            plan.at[threadIdx.x / 32] = it;
+            return;
+        }
         const int64_t base = it.base + it.tiles + kStart;
         if (++it.head == a.kv_heads) {
             it.head = 0;

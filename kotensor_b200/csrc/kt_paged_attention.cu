@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
     dev::pdl_launch_dependents();
     zero_rows(a);
     __shared__ Plan<kWarps + 1> plan;
-    const WorkList<kWarps + 1, kVectors, kTile, kStart, kLeast> work{a, plan};
+    const WorkList<kWarps + 1, kVectors, kTile, kStart, kLeast, 0> work{a, plan};
     if (!work.start()) return;  // (its barriers also publish the mbarriers)
     const Item& it = plan.at[warp];
     bool ok = true;

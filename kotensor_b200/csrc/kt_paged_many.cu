@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
     if (threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
     zero_rows(a);
     __shared__ Plan<kThreads / 32> plan;
-    const WorkList<kThreads / 32, kVectors, kTile, kStart, kLeast> work{a, plan};
+    const WorkList<kThreads / 32, kVectors, kTile, kStart, kLeast, 3> work{a, plan};
     if (!work.start()) {  // (its barriers also publish the mbarriers)
         dev::pdl_launch_dependents();
         return;
@@ -608,42 +608,47 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
     }
 }
 
-// Items that were cut, from their parts: a thread has four dims of a vector.
+// Items that were cut, from their parts: a thread has four dims of a vector, and the loads of
+// four parts under way.
 template <typename T, int HDP>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedAttention a) {
     using S = ManyShape<HDP>;
     dev::pdl_wait();
     dev::pdl_launch_dependents();
     const Cut cut = reinterpret_cast<const Cut*>(static_cast<const char*>(a.scratch) + kPagedCounterBytes)[blockIdx.x];
-    const int v = blockIdx.y * 32 + threadIdx.x % 32, d = a.head_dim;
-    if (cut.parts == 0 || v >= cut.valid) return;
-    const float* const parts = reinterpret_cast<const float*>(static_cast<const char*>(a.scratch) + kPagedPartsAt);
-    auto part_of = [&](int i) { return parts + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0)) * S::kPart; };
+    const int v = blockIdx.y * 32 + threadIdx.x % 32, quad = blockIdx.z * 8 + threadIdx.x / 32;
+    if (cut.parts == 0 || v >= cut.valid || 4 * quad >= a.head_dim) return;
+    const float* const parts = reinterpret_cast<const float*>(static_cast<const char*>(a.scratch) + kPagedPartsAt) +
+                               static_cast<int64_t>(blockIdx.x) * 2 * S::kPart;
     float top = -INFINITY, total = 0.0f;
-    for (int i = 0; i < cut.parts; ++i) top = fmaxf(top, part_of(i)[kVectors * HDP + v]);
-    constexpr int kMine = HDP / 32;
-    float4 y[kMine] = {};
-#pragma unroll 2
-    for (int i = 0; i < cut.parts; ++i) {
-        const float* const part = part_of(i);
-        const float sum = part[kVectors * (HDP + 1) + v], w = sum == 0.0f ? 0.0f : ex2(part[kVectors * HDP + v] - top);
-        total += w * sum;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < cut.parts; i += 4) {
+        float ref[4], sum[4];
+        float4 f[4];
 #pragma unroll
-        for (int j = 0; j < kMine; ++j) {
-            const int quad = threadIdx.x / 32 + 8 * j;
-            if (4 * quad >= d || w == 0.0f) continue;
-            const float4 f = *reinterpret_cast<const float4*>(part + (quad * kVectors + v) * 4);
-            y[j].x = fmaf(w, f.x, y[j].x), y[j].y = fmaf(w, f.y, y[j].y);
-            y[j].z = fmaf(w, f.z, y[j].z), y[j].w = fmaf(w, f.w, y[j].w);
+        for (int j = 0; j < 4; ++j) {
+            // the first is its CTA's part 1, the others are their CTAs' parts 0
+            const float* const part = parts + static_cast<int64_t>(i + j == 0 ? 1 : 2 * min(i + j, cut.parts - 1)) * S::kPart;
+            ref[j] = part[kVectors * HDP + v];
+            sum[j] = i + j < cut.parts ? part[kVectors * (HDP + 1) + v] : 0.0f;
+            f[j] = *reinterpret_cast<const float4*>(part + (quad * kVectors + v) * 4);
+        }
+        float now = top;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) now = fmaxf(now, ref[j]);
+        const float fade = total == 0.0f ? 0.0f : ex2(top - now);
+        top = now;
+        total *= fade, y.x *= fade, y.y *= fade, y.z *= fade, y.w *= fade;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float w = sum[j] == 0.0f ? 0.0f : ex2(ref[j] - top);
+            total += w * sum[j];
+            y.x += w * f[j].x, y.y += w * f[j].y, y.z += w * f[j].z, y.w += w * f[j].w;
         }
     }
     const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-    const int64_t at = place_of(a, cut.b, cut.head, cut.v0 + v, static_cast<int64_t>(a.heads) * d);
-#pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-        const int dim = 4 * (threadIdx.x / 32 + 8 * j);
-        if (dim < d) put4<T>(a, at + dim, make_float4(y[j].x * scale, y[j].y * scale, y[j].z * scale, y[j].w * scale));
-    }
+    put4<T>(a, place_of(a, cut.b, cut.head, cut.v0 + v, static_cast<int64_t>(a.heads) * a.head_dim) + 4 * quad,
+            make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale));
 }
 
 template <typename T, int HDP>
@@ -658,7 +663,7 @@ cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const Pag
     const int64_t most = std::max(items, items * ((a.capacity + kTile - 1) / kTile) / kLeast);
     const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count, kPagedManyCtas), most));
     e = launch_dependent(kernel, dim3(grid), dim3(kThreads), S::kSmem, s, k_map, v_map, a, err);
-    if (e == cudaSuccess) e = launch_dependent(paged_merge_kernel<T, HDP>, dim3(grid, kVectors / 32), dim3(256), 0, s, a);
+    if (e == cudaSuccess) e = launch_dependent(paged_merge_kernel<T, HDP>, dim3(grid, kVectors / 32, HDP / 32), dim3(256), 0, s, a);
     return e;
 }
 
