@@ -57,12 +57,11 @@ __device__ __forceinline__ int rows_of(const int32_t* counts, int b, int rows) {
     return counts == nullptr ? rows : min(max(counts[b], 0), rows);
 }
 
-// Zeros for the rows that are no tokens; by all warps of the grid.
+// Zeros for the rows that are no tokens; by one warp of every CTA.
 __device__ __forceinline__ void zero_rows(const PagedAttention& a) {
-    const int warps = blockDim.x / 32, lane = threadIdx.x % 32, width = a.heads * a.head_dim;
+    const int lane = threadIdx.x % 32, width = a.heads * a.head_dim;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.rows;
-    for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / 32) * 32; r0 < rows;
-         r0 += static_cast<int64_t>(gridDim.x) * warps * 32) {
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 32; r0 < rows; r0 += static_cast<int64_t>(gridDim.x) * 32) {
         bool token = true;
         if (r0 + lane < rows) {
             const int b = static_cast<int>((r0 + lane) / a.rows), t = static_cast<int>((r0 + lane) % a.rows);
@@ -81,6 +80,19 @@ __device__ __forceinline__ void zero_rows(const PagedAttention& a) {
 __device__ __forceinline__ int64_t place_of(const PagedAttention& a, int b, int head, int v, int64_t stride) {
     const int row = v / a.group;
     return (static_cast<int64_t>(b) * a.rows + row) * stride + static_cast<int64_t>(head * a.group + v - row * a.group) * a.head_dim;
+}
+
+// A place in a ring of kUnits, and the phase of its barrier.
+template <int kUnits>
+struct Ring {
+    int at = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == kUnits) at = 0, phase ^= 1;
+    }
+};
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {  // of numbers that are not negative
+    return (x | y) >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y)) : x / y;
 }
 
 // An item of the attention's work: kVectors query vectors (rows x heads of a group, in
@@ -112,7 +124,7 @@ struct Plan {
 // With kDeal, equal sequences of several vector tiles (a prompt) are not cut where there are
 // kDeal items or more to a CTA: they are dealt out whole, the longest first, every other
 // round backwards, so that the sums are as equal and nothing has to be merged.
-template <int kWarps, int kVectors, int kTile, int kStart, int kLeast, int kDeal>
+template <int kWarps, int kVectors, int kTile, int kStart, int kLeast, int kWhole, int kDeal>
 struct WorkList {
     const PagedAttention& a;
     Plan<kWarps>& plan;
@@ -150,14 +162,14 @@ struct WorkList {
     }
     __device__ int cta_of(int64_t unit) const {  // the CTA whose run holds it
         const int64_t longer = plan.spare * (plan.share + 1);
-        return static_cast<int>(unit < longer ? unit / (plan.share + 1) : plan.spare + (unit - longer) / plan.share);
+        return static_cast<int>(unit < longer ? quotient(unit, plan.share + 1) : plan.spare + quotient(unit - longer, plan.share));
     }
     // The CTAs that share an item's tiles are first_cta .. last_cta.
     __device__ int first_cta(const Item& it) const { return cta_of(it.base + kStart); }
     __device__ int last_cta(const Item& it) const { return cta_of(it.base + kStart + it.tiles - 1); }
 
     // By all threads of the CTA: shares out the list; false: nothing for this CTA.  A CTA gets
-    // at least kLeast tiles or an item.
+    // at least kLeast tiles or an item; items of at most kWhole tiles are not cut for more CTAs.
     __device__ bool start() const {
         constexpr int kThreads = kWarps * 32;
         const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, vts = vector_tiles();
@@ -179,9 +191,11 @@ struct WorkList {
         const int from = min(entries, static_cast<int>(threadIdx.x) * each), to = min(entries, from + each);
         Item it;
         int64_t units = 0, items = 0;
+        int longest = 0;
         for (int e = from; e < to; ++e) {
             load(it, e, vts);
             if (it.tiles > 0) units += it.tiles + kStart, ++items;
+            longest = max(longest, it.tiles);
         }
         units *= a.kv_heads, items *= a.kv_heads;
         int64_t upto = units;
@@ -191,7 +205,7 @@ struct WorkList {
         }
         for (int o = 16; o > 0; o >>= 1) items += __shfl_xor_sync(0xffffffffu, items, o);
         if (lane == 31) plan.sums[warp] = upto, plan.items[warp] = items;
-        __syncthreads();
+        const bool whole = !__syncthreads_or(longest > kWhole);
         int64_t before = upto - units, total = 0;
         items = 0;
         for (int w = 0; w < kWarps; ++w) {
@@ -200,9 +214,9 @@ struct WorkList {
             items += plan.items[w];
         }
         if (items == 0) return false;
-        const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max(items, (total - items * kStart) / kLeast));
+        const int64_t ctas = min(static_cast<int64_t>(gridDim.x), whole ? items : max(items, quotient(total - items * kStart, kLeast)));
         if (blockIdx.x >= ctas) return false;
-        const int64_t share = total / ctas, spare = total - share * ctas;
+        const int64_t share = quotient(total, ctas), spare = total - share * ctas;
         const int64_t begin = blockIdx.x * share + min(static_cast<int64_t>(blockIdx.x), spare);
         if (threadIdx.x == 0) {
             plan.share = share, plan.spare = spare, plan.begin = begin;
@@ -224,7 +238,7 @@ struct WorkList {
         if (lane == 0) {
             Item& mine = plan.at[warp];
             load(it, plan.entry, vts);
-            it.head = static_cast<int>((begin - plan.base) / (it.tiles + kStart));
+            it.head = static_cast<int>(quotient(begin - plan.base, it.tiles + kStart));
             it.base = plan.base + static_cast<int64_t>(it.head) * (it.tiles + kStart);
             cut(it);
             mine = it;

@@ -13,12 +13,13 @@ namespace {
 
 using namespace paged;
 
-constexpr int kWarps = 4;                        // that compute; one more copies
+constexpr int kWarps = 8;                        // that compute; one more copies
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kVectors = 16;                     // query vectors of an item (the product's M)
-constexpr int kTile = 64;                        // slots of a tile, 16 to a warp
-constexpr int kStart = 2;                        // tiles that entering an item costs
-constexpr int kLeast = 4;                        // tiles that are worth a CTA
+constexpr int kTile = 128;                       // slots of a tile, 16 to a warp
+constexpr int kStart = 4;                        // tiles that entering an item costs
+constexpr int kLeast = 1;                        // tiles that are worth a CTA
+constexpr int kWhole = 3;                        // tiles of an item that is not worth two
 // Probabilities are kept 2^kLift times larger: in fp16 those down to 2^-36 of the largest
 // stay clear of underflow; the factor cancels in the division by their sum.
 constexpr float kLift = 12.0f;
@@ -27,16 +28,17 @@ template <int HDP>
 struct RowsShape {
     static constexpr int kBlocks = HDP / 64;               // blocks of 64 dims: swizzled rows of 128 bytes
     static constexpr int kUnit = kBlocks * kTile * 128;    // the keys or the values of a tile
-    static constexpr int kUnits = 80 * 1024 / kUnit;       // in the ring: keys, values, keys, ...
+    static constexpr int kUnits = 160 * 1024 / kUnit;      // in the ring: keys, values, keys, ...
     static constexpr int kPitch = HDP + 4;
-    static constexpr int kArea = kUnits * kUnit;           // sums of two warps
-    static constexpr int kStats = kArea + 2 * kVectors * kPitch * 4;  // largest score, sum of each warp's vectors
+    static constexpr int kArea = kUnits * kUnit;           // sums of four pairs of warps; the queries before
+    static constexpr int kQPitch = HDP * 2 + 16;
+    static constexpr int kStats = kArea + 4 * kVectors * kPitch * 4;  // largest score, sum of each warp's vectors
     static constexpr int kTotals = kStats + 2 * kWarps * kVectors * 4;
     static constexpr int kBars = kTotals + 2 * kVectors * 4;
     static constexpr int kValid = kBars + 16 * kUnits;     // boxes of a unit that have a page
     static constexpr int kSmem = 1024 + kValid + 4 * kUnits;
     static constexpr int kPart = kVectors * (HDP + 2);     // floats of a part: sums, largest scores, totals
-    static_assert(2 * (kSmem + 1024) <= 233472, "two CTAs on an SM");
+    static_assert(kSmem <= 232448 && kVectors * kQPitch <= kStats - kArea, "shared memory");
 };
 
 template <typename T>
@@ -61,7 +63,7 @@ __device__ __forceinline__ void matrices_turned(uint32_t addr, uint32_t (&r)[4])
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Sums over the parts' own references -> the common one's (0 where nothing was summed).
 __device__ __forceinline__ float weigh(float reference, float sum, float common) {
@@ -69,7 +71,7 @@ __device__ __forceinline__ float weigh(float reference, float sum, float common)
 }
 
 template <typename T, int HDP>
-__global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_constant__ CUtensorMap k_map,
                                                                  const __grid_constant__ CUtensorMap v_map,
                                                                  const __grid_constant__ PagedAttention a,
                                                                  int32_t* __restrict__ err) {
@@ -89,12 +91,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (threadIdx.x == 32) {
+        dev::prefetch_map(&k_map);
+        dev::prefetch_map(&v_map);
+    }
     dev::pdl_wait();
     dev::pdl_launch_dependents();
-    zero_rows(a);
     __shared__ Plan<kWarps + 1> plan;
-    const WorkList<kWarps + 1, kVectors, kTile, kStart, kLeast, 0> work{a, plan};
-    if (!work.start()) return;  // (its barriers also publish the mbarriers)
+    const WorkList<kWarps + 1, kVectors, kTile, kStart, kLeast, kWhole, 0> work{a, plan};
+    if (!work.start()) {  // (its barriers also publish the mbarriers)
+        if (warp == kWarps) zero_rows(a);
+        return;
+    }
     const Item& it = plan.at[warp];
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {  // a lane that has given up goes on without waiting
@@ -106,7 +114,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
         const int box = min(kPagedBox, 1 << a.page_shift), boxes = kTile / box;  // 16, 32 or 64 slots; 4, 2 or 1 to a tile
         const int mine = lane % boxes, block = lane / boxes % S::kBlocks;
         const bool copies = lane < boxes * S::kBlocks;
-        int64_t unit = 0;
+        Ring<S::kUnits> ring;
+        int units = 0;  // at most kUnits: those that may be in flight
         do {
             for (int tile = it.from, to = it.to; tile < to; ++tile) {
                 const int slot = tile * kTile + mine * box;
@@ -116,10 +125,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
                 const uint32_t who = __ballot_sync(0xffffffffu, here);
                 const int row = here ? ((page * a.kv_heads + it.head) << a.page_shift) + (slot & ((1 << a.page_shift) - 1)) : 0;
 #pragma unroll
-                for (int v = 0; v < 2; ++v, ++unit) {
-                    const int x = static_cast<int>(unit % S::kUnits);
-                    if (unit >= S::kUnits) wait(empty(x), (unit / S::kUnits - 1) & 1);
+                for (int v = 0; v < 2; ++v) {
+                    const int x = ring.at;
+                    if (units == S::kUnits) wait(empty(x), ring.phase ^ 1);
                     if (!__all_sync(0xffffffffu, ok)) break;
+                    units = min(units + 1, S::kUnits);
+                    ring.next();
                     if (lane == 0) {
                         with_page[x] = who & ((1u << boxes) - 1u);
                         dev::mbar_expect_tx(full(x), __popc(who) * box * 128);
@@ -132,9 +143,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
                 if (!__all_sync(0xffffffffu, ok)) break;
             }
         } while (__all_sync(0xffffffffu, ok) && work.next());
+        zero_rows(a);
         // no copy is in flight past this point, also where a wait has given up
-        for (int64_t u = max(static_cast<int64_t>(0), unit - S::kUnits); u < unit; ++u)
-            if (!wait_counted(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1)) ok = false;
+        if (units == S::kUnits) ring.phase ^= 1;  // the oldest one is at the ring's place, of the round before
+        else ring.at = 0;
+        for (; units > 0; --units, ring.next())
+            if (!wait_counted(full(ring.at), ring.phase)) ok = false;
         if (!ok) atomicOr(err, 1);
         return;
     }
@@ -144,39 +158,51 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
     float* const stats = reinterpret_cast<float*>(smem + S::kStats);    // [warp][vector]: largest scores, then sums
     float* const totals = reinterpret_cast<float*>(smem + S::kTotals);  // [vector]
     float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedPartsAt);
-    int64_t unit = 0;
+    Ring<S::kUnits> ring;
     do {
         const int from = it.from, to = it.to;
         if (from >= to) continue;
-        // this thread's vectors, r8 and r8 + 8 of the item, and their queries
-        uint32_t q[HDP / 16][4];
-        int t[2];
+        // the item's queries, through shared memory; this thread's vectors are r8 and r8 + 8
+        {
+            constexpr int kPieces = HDP / 8;
+            const int vec = threadIdx.x / kPieces, dim = threadIdx.x % kPieces * 8;
+            if (vec < kVectors) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (vec < it.valid && dim < d) {
+                    const uint16_t* const from_q = static_cast<const uint16_t*>(a.q) + place_of(a, it.b, it.head, it.v0 + vec, a.q_stride) + dim;
+                    if (a.aligned & 1) {
+                        w = *reinterpret_cast<const uint4*>(from_q);
+                    } else {
+                        uint32_t e[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int vec = it.v0 + r8 + 8 * i, row = vec / a.group;
-            const bool real = r8 + 8 * i < it.valid;
-            t[i] = real ? row : -1;
-            const uint16_t* from_q = static_cast<const uint16_t*>(a.q) + place_of(a, it.b, it.head, vec, a.q_stride);
-#pragma unroll
-            for (int s = 0; s < HDP / 8; ++s) {
-                const int dim = 8 * s + 2 * t4;
-                uint32_t w = 0;
-                if (real && dim < d)
-                    w = a.aligned & 1 ? *reinterpret_cast<const uint32_t*>(from_q + dim)
-                                      : from_q[dim] | static_cast<uint32_t>(from_q[dim + 1]) << 16;
-                q[s / 2][i + 2 * (s % 2)] = w;
+                        for (int j = 0; j < 4; ++j) e[j] = from_q[2 * j] | static_cast<uint32_t>(from_q[2 * j + 1]) << 16;
+                        w = make_uint4(e[0], e[1], e[2], e[3]);
+                    }
+                }
+                *reinterpret_cast<uint4*>(smem + S::kArea + vec * S::kQPitch + dim * 2) = w;
             }
         }
+        const int t[2] = {r8 < it.valid ? (it.v0 + r8) / a.group : -1, r8 + 8 < it.valid ? (it.v0 + r8 + 8) / a.group : -1};
+        compute_sync();
+        uint32_t q[HDP / 16][4];
+#pragma unroll
+        for (int s = 0; s < HDP / 16; ++s)
+            matrices(base + S::kArea + (lane % 16) * S::kQPitch + (16 * s + lane / 16 * 8) * 2, q[s]);
         // slots that all of the item's vectors see
         const int clear = a.visible ? it.held : min(it.held + it.v0 / a.group + 1, it.sees);
         float o[HDP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < HDP / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        for (int tile = from; tile < to; ++tile, unit += 2) {
-            const int kx = static_cast<int>(unit % S::kUnits), vx = static_cast<int>((unit + 1) % S::kUnits);
+        for (int tile = from; tile < to; ++tile) {
+            const int kx = ring.at;
+            const uint32_t k_phase = ring.phase;
+            ring.next();
+            const int vx = ring.at;
+            const uint32_t v_phase = ring.phase;
+            ring.next();
             const int slot = tile * kTile + warp * 16;
             float s[2][4] = {};
-            wait(full(kx), (unit / S::kUnits) & 1);
+            wait(full(kx), k_phase);
             __syncwarp();
             if (slot < it.sees) {
                 const uint32_t k_row = base + kx * S::kUnit + (warp * 16 + lane % 8 + lane / 16 * 8) * 128;
@@ -228,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
                     p[i + 2] = Half16<T>::pack(z[2], z[3]);
                 }
             }
-            wait(full(vx), ((unit + 1) / S::kUnits) & 1);
+            wait(full(vx), v_phase);
             __syncwarp();
             if (edge && slot < it.sees) {
                 // What no vector sees counts nothing, whatever it is, and a value that is not finite counts for those
@@ -303,10 +329,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
                 totals[v] = common[i], totals[kVectors + v] = total;
             }
         }
-        float* const sums = area + (warp % 2) * (kVectors * S::kPitch);
+        float* const sums = area + (warp % 4) * (kVectors * S::kPitch);
 #pragma unroll
         for (int step = 0; step < 2; ++step) {
-            if (warp / 2 == 1 - step) {
+            if (warp / 4 == 1 - step) {
 #pragma unroll
                 for (int j = 0; j < HDP / 8; ++j)
 #pragma unroll
@@ -332,8 +358,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
         for (int e = threadIdx.x; e < it.valid * (HDP / 4); e += kWarps * 32) {
             const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
             float4 y = *reinterpret_cast<const float4*>(area + vec * S::kPitch + dim);
-            const float4 z = *reinterpret_cast<const float4*>(area + (kVectors + vec) * S::kPitch + dim);
-            y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                const float4 z = *reinterpret_cast<const float4*>(area + (i * kVectors + vec) * S::kPitch + dim);
+                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+            }
             if (whole) finish(vec, dim, y, totals[kVectors + vec]);
             else __stcg(reinterpret_cast<float4*>(part + vec * HDP + dim), y);
         }
@@ -348,19 +377,35 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const __grid_co
             if (last_cta) {
                 __threadfence();
                 const int n = c1 - c0 + 1;
-                auto part_of = [&](int x) { return parts + ((static_cast<int64_t>(c0) + x) * 2 + (x == 0)) * S::kPart; };
+                const float* const from_c0 = parts + static_cast<int64_t>(c0) * 2 * S::kPart;
                 for (int e = threadIdx.x; e < it.valid * (HDP / 4); e += kWarps * 32) {
                     const int vec = e / (HDP / 4), dim = e % (HDP / 4) * 4;
-                    float m = -INFINITY, total = 0.0f;
-                    for (int x = 0; x < n; ++x) m = fmaxf(m, __ldcg(part_of(x) + kVectors * HDP + vec));
+                    float top = -INFINITY, total = 0.0f;
                     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int x = 0; x < n; ++x) {
-                        const float l = __ldcg(part_of(x) + kVectors * (HDP + 1) + vec);
-                        const float w = weigh(__ldcg(part_of(x) + kVectors * HDP + vec), l, m);
-                        const float4 f = __ldcg(reinterpret_cast<const float4*>(part_of(x) + vec * HDP + dim));
-                        total += w * l;
-                        if (w != 0.0f) y.x = fmaf(w, f.x, y.x), y.y = fmaf(w, f.y, y.y), y.z = fmaf(w, f.z, y.z), y.w = fmaf(w, f.w, y.w);
+                    constexpr int kBatch = 8;  // parts whose loads are under way together (one by one 37 took 20 us)
+                    for (int i = 0; i < n; i += kBatch) {
+                        float ref[kBatch], sum[kBatch];
+                        float4 f[kBatch];
+#pragma unroll
+                        for (int j = 0; j < kBatch; ++j) {
+                            // the first is its CTA's part 1, the others are their CTAs' parts 0
+                            const float* const p = from_c0 + static_cast<int64_t>(i + j == 0 ? 1 : 2 * min(i + j, n - 1)) * S::kPart;
+                            ref[j] = __ldcg(p + kVectors * HDP + vec);
+                            sum[j] = __ldcg(p + kVectors * (HDP + 1) + vec);
+                            f[j] = __ldcg(reinterpret_cast<const float4*>(p + vec * HDP + dim));
+                        }
+                        float now = top;
+#pragma unroll
+                        for (int j = 0; j < kBatch; ++j) now = fmaxf(now, ref[j]);
+                        const float fade = total == 0.0f ? 0.0f : ex2(top - now);
+                        top = now;
+                        total *= fade, y.x *= fade, y.y *= fade, y.z *= fade, y.w *= fade;
+#pragma unroll
+                        for (int j = 0; j < kBatch; ++j) {
+                            const float l = i + j < n ? sum[j] : 0.0f, w = weigh(ref[j], l, top);
+                            total += w * l;
+                            y.x = fmaf(w, f[j].x, y.x), y.y = fmaf(w, f[j].y, y.y), y.z = fmaf(w, f[j].z, y.z), y.w = fmaf(w, f[j].w, y.w);
+                        }
                     }
                     finish(vec, dim, y, total);
                 }
@@ -382,7 +427,7 @@ cudaError_t launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, cons
     if (e != cudaSuccess) return e;
     const int64_t items = static_cast<int64_t>(a.batch) * a.kv_heads * ((static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors);
     const int64_t most = std::max(items, items * ((a.capacity + kTile - 1) / kTile) / kLeast);
-    const int grid = static_cast<int>(std::min<int64_t>(std::min(2 * sm_count, kPagedRowsCtas), most));
+    const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count, kPagedRowsCtas), most));
     return launch_dependent(kernel, dim3(grid), dim3(kThreads), S::kSmem, s, k_map, v_map, a, err);
 }
 
@@ -399,7 +444,14 @@ cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttenti
                             static_cast<const char*>(v ? c.values : c.keys) + layer * rows * row_bytes, c.head_dim, rows, row_bytes,
                             64, std::min(c.page, kPagedBox), CU_TENSOR_MAP_SWIZZLE_128B))
             return cudaErrorInvalidValue;
-    if (static_cast<int64_t>(a.rows) * a.group > kVectors) return launch_paged_many(c.dtype == KT_BF16, maps, a, sm_count, err, s);
+    // Which kernel is the faster.  This file's reads the cache once for every sixteen vectors, the other one once for
+    // 256, but takes 4 us longer to enter, leave and merge.  So this one runs for sixteen vectors or fewer; for up to 32
+    // while its items leave no SM two (20 vectors of 32 heads over 8 of 128, 1 / 8 / 64 sequences of 300 tokens: 10.1 /
+    // 10.4 / 58 us here, 14.6 / 18.0 / 56 there; 8 sequences of 4000: 46, 56); and for more where they are very few (112
+    // vectors of 14 heads over 2 of 64, 1 / 8 sequences: 300 tokens 8.2 / 8.5 us here, 12.5 / 12.9 there, 20000 and 4000 tokens
+    // 23 / 33 here, 28 / 18 there).
+    const int64_t sixteens = (static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors, items = sixteens * a.batch * a.kv_heads;
+    if (sixteens > 1 && items > (sixteens == 2 ? sm_count : 16)) return launch_paged_many(c.dtype == KT_BF16, maps, a, sm_count, err, s);
     const bool bf16 = c.dtype == KT_BF16, wide = c.head_dim > 64;
     const auto launch = bf16 ? wide ? launch_rows<__nv_bfloat16, 128> : launch_rows<__nv_bfloat16, 64>
                              : wide ? launch_rows<__half, 128> : launch_rows<__half, 64>;

@@ -14,6 +14,8 @@ constexpr int kVectors = 2 * kLanes;       // of an item
 constexpr int kTile = 128;                 // slots of a tile
 constexpr int kStart = 4;                  // tiles that entering an item costs
 constexpr int kLeast = 2;                  // tiles that are worth a CTA
+constexpr int kWhole = 4;                  // tiles of an item that is not worth two
+constexpr int kDeal = 3;                   // items to a CTA from which they are dealt whole
 constexpr int kIssueWarp = 8, kCopyWarp = 10;  // after the softmax warps; an issuing warp for each stream; the last does nothing
 constexpr int kThreads = 384;
 constexpr float kLift = 6.0f;    // probabilities are 2^kLift times larger: fp16 keeps them to 2^-30 of the reference
@@ -196,13 +198,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
         dev::mbar_init(finished, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (threadIdx.x == 32) {
+        dev::prefetch_map(&k_map);
+        dev::prefetch_map(&v_map);
+    }
     dev::pdl_wait();
     if (threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
-    zero_rows(a);
     __shared__ Plan<kThreads / 32> plan;
-    const WorkList<kThreads / 32, kVectors, kTile, kStart, kLeast, 3> work{a, plan};
+    const WorkList<kThreads / 32, kVectors, kTile, kStart, kLeast, kWhole, kDeal> work{a, plan};
     if (!work.start()) {  // (its barriers also publish the mbarriers)
         dev::pdl_launch_dependents();
+        if (warp == kCopyWarp) zero_rows(a);
         return;
     }
     if (warp == kIssueWarp) {
@@ -593,6 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     if (!__all_sync(0xffffffffu, ok)) break;
                 }
             } while (__all_sync(0xffffffffu, ok) && work.next());
+            zero_rows(a);
             // no copy is in flight past this point, also where a wait has given up
             for (int64_t u = max(static_cast<int64_t>(0), unit - S::kUnits); u < unit; ++u)
                 if (!wait_counted(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1)) ok = false;
