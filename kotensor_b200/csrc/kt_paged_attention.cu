@@ -1,9 +1,26 @@
 // kt_paged_attention.cu -- attention over the paged 16-bit key/value cache, for few query
-// vectors a key/value head (single tokens).
+// vectors a key/value head (single tokens), and the choice of the kernel.
 //
 // Row t of sequence b with n = lengths[b]: for each query head, over the slots j it sees
 // (all j < n, and of this call's tokens those that its mask or the order of rows allows),
 //   s_j = scale * (q . K_j),  out = sum_j softmax(s)_j V_j,   0 where it sees nothing.
+//
+// Sixteen query vectors that share a key/value head (rows x heads of a group) are an item,
+// over tiles of 128 slots.  A warp has 16 slots of each tile, which one m16n8k16 product
+// after the other takes as they lie: keys as the first product's B, values, transposed by
+// the load, as the second's; scores leave the first in the layout in which the second reads
+// probabilities.  Every warp keeps its own largest scores and sums, in fp32; an item's end
+// brings them together.  Probabilities are rounded to the cache's type, half a step of each
+// (2^-8 of it in bfloat16, 2^-11 in fp16) as the result itself is at the end: the products
+// take no wider ones, and two terms each would double the second product.
+//
+// A ninth warp copies: the pages of a tile as swizzled boxes of 64 dims by TMA, keys and
+// values in turn through a ring of 160 KB, so that some 100 KB are on their way to an SM at
+// any time and across the ends of items.  (Two CTAs of four warps with rings of 80 KB: 231 us
+// where this takes 224, and 37 parts to merge where this leaves 18, 93 where this takes 84.)
+// Bound by memory: 64 sequences of 3001 to 8190 tokens, 8 heads of 128, 226 us, 6.5 TB/s; one of
+// 120001 84 us, 5.9 TB/s, of which about 5 go into the merge.  By latency when short: 301
+// tokens 7.9 us, of which a tile's chain of copy, product, exponentials and product is 1.5.
 #include <algorithm>
 
 #include "kt_paged.h"
@@ -17,9 +34,10 @@ constexpr int kWarps = 8;                        // that compute; one more copie
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kVectors = 16;                     // query vectors of an item (the product's M)
 constexpr int kTile = 128;                       // slots of a tile, 16 to a warp
-constexpr int kStart = 4;                        // tiles that entering an item costs
-constexpr int kLeast = 1;                        // tiles that are worth a CTA
-constexpr int kWhole = 3;                        // tiles of an item that is not worth two
+// What entering an item costs, in tiles (8 sequences of 5000 tokens, 8 heads of 128: 35.0 us, counted as two tiles
+// 36.6), and up to how many an item is not cut (300 tokens 9.4 us, cut into single tiles 10.4; 1000 tokens cut so
+// 10.8, into fours 13.7).
+constexpr int kStart = 4, kLeast = 1, kWhole = 3;
 // Probabilities are kept 2^kLift times larger: in fp16 those down to 2^-36 of the largest
 // stay clear of underflow; the factor cancels in the division by their sum.
 constexpr float kLift = 12.0f;

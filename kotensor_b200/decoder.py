@@ -136,6 +136,11 @@ class DeviceDecoder:
     peer memory, else NCCL), after which every rank holds the whole residual
     stream.
 
+    ``kv_bits`` 16: keys and values in a PagedKVCache (``cache``) of ``kv_dtype`` (bfloat16
+    unless given), half the fp32 cache's memory: ``kv_pages`` pages (enough for every
+    sequence unless given) of ``kv_page`` positions, which sequences receive as they grow.
+    ``generate_drafted`` then checks several drafted tokens in one pass.
+
     ``kv_bits`` 8: keys and values in a KVCache8 (``cache``) with a scale for every
     ``kv_block`` positions of a head, a quarter of the fp32 cache's memory and of the
     bytes a step's attention reads.  ``kv_weights`` also accumulates the attention
@@ -146,9 +151,10 @@ class DeviceDecoder:
     max_block_rows = 65535
 
     def __init__(self, cfg: DecoderConfig, weights, max_seq: int, device: Optional[int] = None, batch: int = 1,
-                 comm=None, kv_bits: int = 32, kv_block: int = 64, kv_weights: bool = False):
-        if kv_bits not in (8, 32):
-            raise ValueError(f"kv_bits must be 8 or 32, got {kv_bits}")
+                 comm=None, kv_bits: int = 32, kv_block: int = 64, kv_weights: bool = False, kv_page: int = 64,
+                 kv_pages: Optional[int] = None, kv_dtype=None):
+        if kv_bits not in (8, 16, 32):
+            raise ValueError(f"kv_bits must be 8, 16 or 32, got {kv_bits}")
         if kv_weights and kv_bits != 8:
             raise ValueError("attention weights are kept by the 8-bit cache only")
         self.cfg = cfg
@@ -207,10 +213,17 @@ class DeviceDecoder:
         # one KV cache per sequence, each in the reference's layout [L][kvH][maxSeq][hd]
         # (this rank's key/value heads under tensor parallelism)
         self.cache = self.keys = self.values = None
+        self.paged = kv_bits == 16
         if kv_bits == 8:
             from .kv8 import KVCache8
             self.cache = KVCache8(cfg.layers, batch, self.kv_local, cfg.head_dim, max_seq, kv_block, kv_weights, self.ctx.device)
             self.cache._scratch_of(1, self.heads_local)  # what a captured step needs
+        elif kv_bits == 16:
+            from .paged import PagedKVCache
+            if kv_pages is None:
+                kv_pages = batch * -(-max_seq // kv_page)
+            self.cache = PagedKVCache(cfg.layers, batch, self.kv_local, cfg.head_dim, kv_pages, max_seq, kv_page, kv_dtype,
+                                      self.ctx.device)
         else:
             self.keys = torch.zeros((batch, cfg.layers, self.kv_local, max_seq, cfg.head_dim), **f32)
             self.values = torch.zeros_like(self.keys)
@@ -232,6 +245,8 @@ class DeviceDecoder:
         self._text, self._prompt_end = [], 0  # int32 [batch, n] of each call, tokens up to the last prompt's end
         self.scale = float(np.float32(1.0) / np.float32(math.sqrt(float(cfg.head_dim))))
         self._graph = None
+        self._drafts = None  # buffers and graph of generate_drafted's passes
+        self.passes = 0      # of its last call
         g_ = self.heads_local // self.kv_local
         self._fused_attention = g_ <= 8 and cfg.head_dim in (64, 128) and max_seq <= 16384
         if P > 1:
@@ -272,6 +287,8 @@ class DeviceDecoder:
         b.ctx = torch.empty((rows, self.q_width), **f32)
         b.gu = torch.empty((rows, 2 * self.hidden_local), **f32)
         b.act = torch.empty((rows, self.hidden_local), **f32)
+        # rotated queries in the paged cache's type
+        b.q16 = torch.empty((rows, self.q_width), dtype=self.cache.dtype, device=dev) if self.paged else None
         b.tokens = tokens if tokens is not None else torch.empty(rows, dtype=torch.int32, device=dev)
         # attention scratch; zero-filled: its tail holds the fused kernel's merge counters
         # (the 8-bit cache has its own)
@@ -321,7 +338,13 @@ class DeviceDecoder:
         allgather_columns(self.comm, self.logits, full, self.batch)
         return full
 
-    def _layers(self, b: "_Rows", rows: int, rows_per_seq: int, seq0: int = 0) -> None:
+    def _reserve(self, positions: int) -> None:
+        """Pages of the paged cache for so many positions of every sequence."""
+        if self.paged:
+            for q in range(self.batch):
+                self.cache.reserve(q, min(positions, self.cache.capacity))
+
+    def _layers(self, b: "_Rows", rows: int, rows_per_seq: int, seq0: int = 0, counts=None, depths=None, visible=None) -> None:
         """Embedding lookup of b.tokens[:rows] through every block; leaves the
         residual rows in b.x (the head applies the final norm).  Row r is
         sequence seq0 + r / rows_per_seq at position *position + r %
@@ -330,7 +353,8 @@ class DeviceDecoder:
         output projection added to the residual, norm2 + gate|up + SiLU * up,
         the down projection added to the residual -- five launches at batch 1,
         where the GEMV applies each norm while staging its input row and forms
-        silu(gate) * up in its epilogue."""
+        silu(gate) * up in its epilogue.  With a paged cache the rows of a sequence may be a
+        drafted tree (``counts``, ``depths``, ``visible`` as PagedKVCache takes them)."""
         L_ = _lib.load()
         cfg, h = self.cfg, self.ctx.handle
         s, p = self._stream(), self._p
@@ -350,7 +374,11 @@ class DeviceDecoder:
         for l, L in enumerate(self.layers):
             _lib.check(L_.kt_rmsnorm_qmatmul(h, L["wqkv"].handle, p(b.x), p(L["norm1"]), cfg.eps, p(b.normed),
                                              p(b.qkv), rows, 0, p(L["bqkv"]), s))
-            if self.cache is not None:
+            if self.paged:
+                q, k, v = b.qkv[:rows].split([self.q_width, kv, kv], 1)
+                q = cache.append(l, q, k, v, self.inv_freq, rows_per_seq, counts, depths, out=b.q16[:rows])
+                cache.attend(l, q, self.heads_local, rows_per_seq, counts, visible, self.scale, out=b.ctx[:rows])
+            elif self.cache is not None:
                 _lib.check(L_.kt_rope_seqs(h, p(b.qkv), rows, self.q_width, kvh, hd, p(self.inv_freq), p(self.position),
                                            rows_per_seq, s))
                 q, k, v = b.qkv[:rows].split([self.q_width, kv, kv], 1)
@@ -436,6 +464,7 @@ class DeviceDecoder:
             raise ValueError(f"KV cache full: {self.held} + {T} positions exceed maxSequenceLength {self.max_seq}")
         if T > self.max_block_rows:
             raise ValueError(f"{T} prompt tokens exceed {self.max_block_rows} rows of one prefill block")
+        self._reserve(self.held + T)
         # whole sequences per block: a block holds at most max_block_rows rows (the
         # kernels' grid rows); larger batches are prefilled in several blocks
         per = min(self.batch, self.max_block_rows // T)
@@ -480,6 +509,7 @@ class DeviceDecoder:
                 raise ValueError(f"{t} out of vocab bounds {self.cfg.vocab}")
         if self.held >= self.max_seq:
             raise ValueError(f"KV cache full: maxSequenceLength {self.max_seq}")
+        self._reserve(self.held + 1)
         self.token.copy_(torch.tensor(tokens, dtype=torch.int32))
         self._launch_step(remember)
         self.length += 1
@@ -501,9 +531,10 @@ class DeviceDecoder:
         if self.held + prompt + max_tokens - 1 > self.max_seq:
             raise ValueError(f"KV cache full: {self.held} + {prompt} + {max_tokens - 1} positions exceed maxSequenceLength "
                              f"{self.max_seq}")
+        self._reserve(self.held + prompt + max_tokens - 1)
 
     def _check_dropped(self) -> None:
-        """An error if the 8-bit cache, until ``reset``, had no room for a token it was given."""
+        """An error if the 8-bit or paged cache, until ``reset``, had no room for a token it was given."""
         if self.cache is not None and int(self.cache.status.item()) != 0:
             raise ValueError("KV cache full: tokens were dropped")
 
@@ -559,9 +590,132 @@ class DeviceDecoder:
         self._check_dropped()
         return [[row[q] for row in out] for q in range(self.batch)]
 
+    def generate_drafted(self, prompts, max_tokens: int, nodes: int = 16, draft=None) -> list:
+        """Greedy continuation of every sequence, several tokens a pass (``kv_bits`` 16): the
+        tokens that may follow each text are drafted as a tree of at most ``nodes`` nodes,
+        its first the text's last token; one pass over the model gives the choice after each
+        node, and the path that the choices confirm is kept (PagedKVCache.accept).  The
+        choices are those of the model on the tokens before them, so drafts change how
+        many passes a text takes and not what it says, but for choices within the
+        difference of the matmul kernels (m = batch x nodes instead of m = batch).
+
+        ``draft``: a function of a text (a list of token ids) that returns lists of tokens
+        that may follow it, the likeliest first; drafts.look_up unless given.  ``passes``
+        counts the passes of the last call."""
+        from .drafts import grow, look_up
+        from .paged import MOST_NODES
+        if not self.paged:
+            raise ValueError("drafted tokens need kv_bits 16")
+        if self.comm is not None or self._penal is not None:
+            raise ValueError("drafted tokens need the whole logits and the plain choice: no tensor parallelism, no penalties")
+        if len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray)):
+            prompts = [prompts]
+        if not 1 <= nodes <= MOST_NODES or self.batch * nodes > self.max_block_rows:
+            raise ValueError(f"nodes must be in 1..{MOST_NODES} with at most {self.max_block_rows} rows in all, got {nodes}")
+        if max_tokens < 1:
+            raise ValueError(f"max_tokens must be positive, got {max_tokens}")
+        draft = draft or look_up
+        begin = self.length
+        self._check_room(len(prompts[0]), max_tokens)
+        self.prefill(prompts)
+        known = np.concatenate(self._text, 1)
+        texts = [known[q].tolist() for q in range(self.batch)]
+        out = [[t] for t in self.next_token.tolist()]
+        end = begin + len(prompts[0]) + max_tokens - 1  # positions held by every sequence at the end
+        if self._drafts is None or self._drafts.rows_per_seq != nodes:
+            self._drafts = self._draft_buffers(nodes)
+        d = self._drafts
+        self.passes = 0
+        try:
+            while any(len(o) < max_tokens for o in out):
+                trees = []
+                for text, o in zip(texts, out):
+                    room = min(nodes, max_tokens - len(o))  # every node may be accepted; its position is within `end`
+                    trees.append(grow(o[-1] if room > 0 else 0, draft(text + o) if room > 1 else [], room, self.cfg.vocab))
+                accepted, taken = self._pass(d, trees)
+                self.passes += 1
+                for o, tokens, n in zip(out, accepted, taken):
+                    o += tokens[:n]
+        except BaseException:
+            self.cache.lengths.fill_(self.length)  # as the prompts left it
+            raise
+        self._check_dropped()
+        # the sequences go on together: what the longer ones hold beyond `end` is given up
+        self.cache.lengths.fill_(end)
+        self.position.fill_(end)
+        self.length = end
+        chosen = np.array([o[:max_tokens] for o in out], dtype=np.int32)
+        self._text.append(chosen[:, :-1])
+        self.next_token.copy_(torch.from_numpy(chosen[:, -1].copy()))
+        self.token.copy_(self.next_token)
+        return chosen.tolist()
+
+    def _draft_buffers(self, nodes: int) -> "_Rows":
+        dev, batch, rows = self.position.device, self.batch, self.batch * nodes
+        d = _Rows()
+        d.rows_per_seq, d.graph, d.warm = nodes, None, False
+        words = (nodes + 31) // 32
+        # tokens, parents, depths, visible words and counts of a pass, copied in one piece
+        sizes = [rows, rows, rows, rows * words, batch]
+        d.host = torch.zeros(sum(sizes), dtype=torch.int32, pin_memory=True)
+        d.device = torch.zeros(sum(sizes), dtype=torch.int32, device=dev)
+        d.fields, d.given = (x.split(sizes) for x in (d.host, d.device))
+        tokens, parents, depths, visible, d.counts = d.given
+        d.parents, d.depths = parents.view(batch, nodes), depths.view(batch, nodes)
+        d.visible = visible.view(batch, nodes, words)
+        d.tokens = tokens.view(batch, nodes)
+        d.b = self._buffers(rows, tokens=tokens)
+        f32 = dict(dtype=torch.float32, device=dev)
+        d.normed, d.logits = torch.empty((rows, self.cfg.dim), **f32), torch.empty((rows, self.cfg.vocab), **f32)
+        d.choices = torch.zeros((batch, nodes), dtype=torch.int32, device=dev)
+        d.result = torch.zeros(rows + batch, dtype=torch.int32, device=dev)
+        d.accepted, d.taken = d.result[:rows].view(batch, nodes), d.result[rows:]
+        return d
+
+    def _pass(self, d: "_Rows", trees):
+        """One pass over drafted trees ((tokens, parents) of each sequence): accepted tokens and
+        how many, as lists."""
+        from .paged import draft_tree
+        nodes, words = d.rows_per_seq, (d.rows_per_seq + 31) // 32
+        tokens, parents, depths, visible, counts = (x.numpy() for x in d.fields)
+        shape = (self.batch, nodes)
+        tokens, parents, depths = tokens.reshape(shape), parents.reshape(shape), depths.reshape(shape)
+        tokens[:], parents[:], depths[:], visible[:] = 0, -1, 0, 0
+        visible = visible.reshape(*shape, words)
+        for q, (t, p) in enumerate(trees):
+            n = counts[q] = len(t)
+            if n > 0:
+                tokens[q, :n], parents[q, :n] = t, p
+                depths[q, :n], seen = draft_tree(p)
+                visible[q, :n, :seen.shape[1]] = seen
+        d.device.copy_(d.host, non_blocking=True)
+        if not d.warm:  # (a graph is captured when it is about to be replayed: its first replay zeroes workspaces)
+            self._launch_pass(d)
+            d.warm = True
+        else:
+            if d.graph is None:
+                torch.cuda.synchronize()
+                d.graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(d.graph):
+                    self._launch_pass(d)
+            d.graph.replay()
+        result = d.result.tolist()
+        accepted = result[:self.batch * nodes]
+        return [accepted[q * nodes:(q + 1) * nodes] for q in range(self.batch)], result[self.batch * nodes:]
+
+    def _launch_pass(self, d: "_Rows") -> None:
+        L_ = _lib.load()
+        h, s, p, rows = self.ctx.handle, self._stream(), self._p, self.batch * d.rows_per_seq
+        self._layers(d.b, rows, d.rows_per_seq, counts=d.counts, depths=d.depths, visible=d.visible)
+        _lib.check(L_.kt_rmsnorm_qmatmul(h, self.head.handle, p(d.b.x), p(self.final_norm), self.cfg.eps, p(d.normed),
+                                         p(d.logits), rows, 0, p(self.head_bias), s))
+        _lib.check(L_.kt_argmax(h, p(d.logits), rows, self.cfg.vocab, p(d.choices), s))
+        self.cache.accept(d.tokens, d.parents, d.choices, d.counts, d.accepted, d.taken)
+        self.cache.advance(d.rows_per_seq, counts=d.taken)
+
     # -- the 8-bit cache and the choice of tokens
     def _check_evict(self, keep: int, recent: int) -> None:
-        if self.cache is None or self.cache.weights is None:
+        if self.cache is None or self.paged or self.cache.weights is None:
             raise ValueError("eviction needs kv_bits 8 and kv_weights")
         if keep < 1 or not 0 <= recent <= keep:
             raise ValueError(f"eviction needs 0 <= recent <= keep and 1 <= keep, got {recent} and {keep}")

@@ -109,6 +109,7 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))
         self._own = [[] for _ in range(batch)]
         self._first = 0  # of the whole cache's sequences, for a view
+        self._results = {}  # of accept, by rows
         self._describe()
 
     def _describe(self) -> None:
@@ -124,7 +125,7 @@ class PagedKVCache:
             raise ValueError(f"sequences {begin}..{end} of {self.batch}")
         view = copy.copy(self)
         view.batch, view._first = end - begin, self._first + begin
-        view.table, view.lengths = self.table[begin:end], self.lengths[begin:end]
+        view.table, view.lengths, view._results = self.table[begin:end], self.lengths[begin:end], {}
         view._describe()
         return view
 
@@ -247,17 +248,22 @@ class PagedKVCache:
         [batch, rows], the rows of the last ``append``; ``counts``: nodes of each tree).  Moves
         the path's keys and values of every layer to the slots behind the text and returns
         ``accepted`` (int32 [batch, rows]: the choices along the path, then -1) and ``taken``
-        (int32 [batch]: the path's nodes), by which ``advance(rows, counts=taken)`` moves on."""
+        (int32 [batch]: the path's nodes), by which ``advance(rows, counts=taken)`` moves on:
+        those given, or buffers of this object that its next call with as many rows overwrites."""
         rows = tokens.shape[1] if tokens.dim() == 2 else 0
         shape = (self.batch, rows)
-        if accepted is None:
-            accepted = torch.empty(shape, dtype=torch.int32, device=self.device)
-        if taken is None:
-            taken = torch.empty(self.batch, dtype=torch.int32, device=self.device)
-        _lib.check(self._accept(self.ctx.handle, self._ref, self._ints("tokens", tokens, shape), self._ints("parents", parents, shape),
-                                self._ints("choices", choices, shape), rows, self._ints("counts", counts, (self.batch,)),
-                                self._ints("accepted", accepted, shape), self._ints("taken", taken, (self.batch,)),
-                                self._status, raw_stream(self.ctx.device)))
+        given = (self._ints("tokens", tokens, shape), self._ints("parents", parents, shape), self._ints("choices", choices, shape),
+                 rows, self._ints("counts", counts, (self.batch,)))
+        if rows < 1:
+            raise ValueError("a drafted tree has a node at least")
+        if accepted is None or taken is None:
+            mine = self._results.get(rows)
+            if mine is None:
+                mine = self._results[rows] = (torch.empty(shape, dtype=torch.int32, device=self.device),
+                                              torch.empty(self.batch, dtype=torch.int32, device=self.device))
+            accepted, taken = mine[0] if accepted is None else accepted, mine[1] if taken is None else taken
+        _lib.check(self._accept(self.ctx.handle, self._ref, *given, self._ints("accepted", accepted, shape),
+                                self._ints("taken", taken, (self.batch,)), self._status, raw_stream(self.ctx.device)))
         return accepted, taken
 
     def advance(self, rows: int = 1, counts=None) -> None:

@@ -115,7 +115,7 @@ def cache(monkeypatch):
     c._ref, c._status, c._scratch, c._scale, c.made = None, 0, 0, 0.125, []
     c._append = c._attention = c._accept = lambda *args: c.made.append(args) or 0
     c._lib = SimpleNamespace(kt_kv8_advance=c._append)
-    c.lengths = Tensor([2], torch.int32)
+    c.lengths, c._results = Tensor([2], torch.int32), {}
     return c
 
 
