@@ -282,8 +282,9 @@ kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t l
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "out_dtype must be the cache's or KT_FP32");
     if (!aligned16(scratch)) return entry_fail(KT_ERR_INVALID_ARGUMENT, "scratch must be 16-byte aligned");
     if (visible && rows_per_seq > kMostNodes) return entry_fail(KT_ERR_INVALID_ARGUMENT, "visible needs at most 1024 rows a sequence");
+    // (vectors of a sequence, and items of all, are counted in 32 bits)
     if (static_cast<int64_t>(rows_per_seq) * heads > (1 << 30) ||
-        static_cast<int64_t>(cache->batch) * rows_per_seq > (1 << 30))
+        static_cast<int64_t>(rows_per_seq) * heads / cache->kv_heads * cache->batch > (1ll << 31) - 1)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "too many rows");
     return c_entry(ctx, [&] {
         PagedAttention a{};

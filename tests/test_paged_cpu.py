@@ -55,7 +55,7 @@ def test_caches_that_are_refused(kt, change, message):
     ("attend", dict(layer=2), "layer"), ("attend", dict(rows=-1), "Negative"), ("attend", dict(q=None), "NULL"), ("attend", dict(heads=3), "multiple"),
     ("attend", dict(heads=0), "multiple"), ("attend", dict(q_stride=100), "shorter"), ("attend", dict(out_dtype=2), "out_dtype"),
     ("attend", dict(scratch=4100), "scratch"), ("attend", dict(scratch=None), "NULL"), ("attend", dict(rows=1025, visible=4096), "1024"),
-    ("attend", dict(rows=1 << 29), "too many rows"),
+    ("attend", dict(rows=1 << 29), "too many rows"), ("attend", dict(rows=1 << 28, heads=12, q_stride=768), "too many rows"),
     ("accept", dict(rows=0), "1..1024"), ("accept", dict(rows=1025), "1..1024"),
 ])
 def test_calls_that_are_refused(kt, name, change, message):

@@ -185,6 +185,45 @@ def test_attention_however_the_work_is_cut(kt, tokens, batch, rows):
     check_attend(cache, q, 8, rows, cache.attend(0, q, 8, rows))
 
 
+@pytest.mark.parametrize("layout,rows,dtype", [(MQA, 1, BF16), (MQA, 33, BF16), (QWEN, 1, FP16), (QWEN, 45, FP16), (LLAMA, 3, BF16)])
+def test_a_long_context(kt, layout, rows, dtype):
+    """50021 tokens against 64 bits on the GPU; the tolerance of check_attend."""
+    heads, kv, d = layout
+    held, n = 50021, 50021 + rows
+    cache = filled(layout, 64, dtype, [held], rows)
+    put(cache, rows)
+    q = queries(cache, heads, rows)
+    got = cache.attend(0, q, heads, rows).reshape(rows, kv, -1, d).double()
+    slot = torch.arange(n, device="cuda")
+    page = cache.table[0, slot // 64].long()
+    half = torch.finfo(dtype).eps / 2
+    hidden = slot > held + torch.arange(rows, device="cuda")[:, None]
+    for h in range(kv):
+        k, v = (x[0, page, h, slot % 64].double() for x in (cache.keys, cache.values))
+        z = q.reshape(rows, kv, -1, d)[:, h].double()
+        p = torch.softmax((z @ k.T / d ** 0.5).masked_fill(hidden[:, None], -float("inf")), -1)
+        want, size = p @ v, p @ v.abs()
+        spread = (z.abs() @ k.abs().T).amax(-1, keepdim=True) / d ** 0.5
+        bound = (size * (half * 1.01 + 2 * d * 2.0 ** -23 * spread + n * 2.0 ** -26 + 2.0 ** -20) + 2.0 ** -24) * (1 + half)
+        assert ((got[:, h] - want).abs() <= bound + half * want.abs()).all()
+
+
+def test_sequences_share_pages(kt):
+    """Two sequences with the first pages in common, and tails of their own, give what copies give."""
+    heads, kv, d = LLAMA
+    for rows in (1, 30):
+        apart = filled(LLAMA, 32, BF16, [96, 96], rows)
+        shared = filled(LLAMA, 32, BF16, [96, 96], rows)
+        for x in (apart, shared):
+            for pool in (x.keys, x.values):
+                pool[0, x.table[1, :3].long()] = pool[0, x.table[0, :3].long()]
+        shared.table[1, :3] = shared.table[0, :3]
+        put(apart, rows)
+        put(shared, rows)
+        q = queries(apart, heads, rows)
+        assert torch.equal(apart.attend(0, q, heads, rows), shared.attend(0, q, heads, rows))
+
+
 @pytest.mark.parametrize("layout,rows", [(LLAMA, 1), (QWEN, 70), (WIDE, 30)])
 def test_attention_into_fp32_with_a_scale(kt, layout, rows):
     cache = filled(layout, 32, FP16, [90, 11], rows)
