@@ -699,7 +699,9 @@ cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const Pag
     const int64_t most = std::max(items, items * ((a.capacity + kTile - 1) / kTile) / kLeast);
     const int grid = static_cast<int>(std::min<int64_t>(std::min(sm_count, kPagedManyCtas), most));
     e = launch_dependent(kernel, dim3(grid), dim3(kThreads), S::kSmem, s, k_map, v_map, a, err);
-    if (e == cudaSuccess) e = launch_dependent(paged_merge_kernel<T, HDP>, dim3(grid, kVectors / 32, HDP / 32), dim3(256), 0, s, a);
+    // (one sequence's items are dealt or not by numbers known here; dealt ones have no parts)
+    const bool dealt = a.batch == 1 && items > a.kv_heads && items >= static_cast<int64_t>(kDeal) * grid;
+    if (e == cudaSuccess && !dealt) e = launch_dependent(paged_merge_kernel<T, HDP>, dim3(grid, kVectors / 32, HDP / 32), dim3(256), 0, s, a);
     return e;
 }
 
