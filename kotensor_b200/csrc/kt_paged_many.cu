@@ -27,8 +27,9 @@
 // Bound by turns by the products (2560 clocks of a tile's 3700: scores of 64 slots read the
 // queries again, 48 clocks a step where 128 slots would take 64), and by what an item
 // costs: about 4500 clocks to enter, 5500 to leave, and twice a tile for one with masks.  A
-// prompt of 4093 rows of 32 heads over 8 of 128: 160 us, 860 TFLOP/s; 4 trees of 63 rows over
-// 6001 tokens 41 us.
+// prompt of 4093 rows of 32 heads over 8 of 128: 166 us, 827 TFLOP/s; 2 x 509 rows over 1000 to
+// 2999 tokens 68 us; 4 trees of 63 rows over 2500 to 6001 tokens 41 us, about 6 of them the merge.
+// (Some of the powers as polynomials on the fp32 units: 0 to 7 % slower.)
 #include <algorithm>
 
 #include "kt_paged.h"
