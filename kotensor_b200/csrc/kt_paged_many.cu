@@ -46,7 +46,7 @@ constexpr int kTile = 128;                 // slots of a tile
 // tiles that are worth a CTA, and up to how many an item is not cut (a tree of 20 rows over 300 tokens of each of 8
 // sequences: 18.1 us, cut 19.8); from how many items to a CTA a prompt's are dealt whole (170 us cut, 160 dealt).
 constexpr int kStart = 4, kLeast = 2, kWhole = 4, kDeal = 3;
-constexpr int kIssueWarp = 8, kCopyWarp = 10;  // after the softmax warps; an issuing warp for each stream; the last does nothing
+constexpr int kIssueWarp = 8, kCopyWarp = 10, kLandWarp = 11;  // after the softmax warps; an issuing warp for each stream
 constexpr int kThreads = 384;
 constexpr float kLift = 6.0f;   // probabilities are 2^kLift times larger: fp16 keeps them to 2^-30 of the reference
 constexpr float kSlack = 8.0f;   // the reference moves when a score passes it by this much (2^14 < fp16's largest)
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
         }
         for (int i = 0; i < 4; ++i) {
             dev::mbar_init(s_full(i / 2, i % 2), 1);
-            dev::mbar_init(p_full(i / 2, i % 2), 4);
+            dev::mbar_init(p_full(i / 2, i % 2), i % 2 ? 4 : 5);  // the softmax warps, and the landing one before a tile
             dev::mbar_init(o_done(i / 2, i % 2), 1);
         }
         dev::mbar_init(q_full, 8);
@@ -567,19 +567,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     };
                     wait(q_full, items++ & 1);
                     tc_after();
-                    auto landed = [&](int64_t u) { wait(full(unit_of(u)), (u / S::kUnits) & 1); };
                     if (first < n) {
-                        landed(unit0 + 2 * first);
+                        wait(full(unit_of(unit0 + 2 * first)), ((unit0 + 2 * first) / S::kUnits) & 1);
                         tc_after();
                         scores(first, 0);
                         scores(first, 1);
                     }
                     for (int i = first; ok && i < n; i += step, ++done) {
-                        const int64_t u = unit0 + 2 * i + 1;
-                        const int at = unit_of(u);
-                        // (asked for before P is there: even when a barrier's phase is over, a wait takes two to four hundred clocks)
-                        landed(u);
-                        if (i + step < n) landed(u - 1 + 2 * step);
+                        const int at = unit_of(unit0 + 2 * i + 1);  // whose values have landed, and the next tile's keys, once P is there
 #pragma unroll 1
                         for (int half = 0; half < 2; ++half) {
                             const uint32_t vd = desc_of(base + S::kRing + at * S::kUnit + half * (kTile / 2 * 128), kTile * 128);
@@ -601,6 +596,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             // no product of this stream is under way past this point, also where a wait has given up
             mma_commit(finished);
             if (!wait_counted(finished, 0)) ok = false;
+        } else if (warp == kLandWarp && lane == 0) {
+            // Waits for the values of a tile and the keys of the stream's next, in place of the issuing warps (a wait
+            // takes them 300 clocks even when the phase is over: a prompt of 4093 rows 150 us, with this 141), and joins the softmax
+            // warps in telling them of the tile's first P.
+            int64_t unit0 = 0;
+            uint32_t done[2] = {0, 0};
+            while (ok) {
+                const int n = it.to - it.from;
+                if (n > 0) {
+                    const bool twice = it.valid > kLanes;
+                    auto landed = [&](int64_t u) { wait(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1); };
+                    for (int i = 0; ok && i < n; ++i) {
+                        const int next = i + (twice ? 1 : 2);
+                        landed(unit0 + 2 * i + 1);
+                        if (next < n) landed(unit0 + 2 * next);
+                        for (int x = twice ? 0 : i & 1; x <= (twice ? 1 : i & 1); ++x) {
+                            if (done[x] > 0) wait(p_full(x, 0), (done[x] - 1) & 1);  // (one arrival a phase)
+                            ++done[x];
+                            dev::mbar_arrive(p_full(x, 0));
+                        }
+                    }
+                    unit0 += 2 * n;
+                }
+                if (it.last) break;
+                work.step();
+            }
         } else if (warp == kCopyWarp) {
             // A lane has a box (64 dims of the slots of a page) of the keys' or values' unit.
             const int box = min(kPagedBox, 1 << a.page_shift), boxes = kTile / box;
