@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             dev::mbar_init(p_full(i / 2, i % 2), i % 2 ? 4 : 5);  // the softmax warps, and the landing one before a tile
             dev::mbar_init(o_done(i / 2, i % 2), 1);
         }
-        dev::mbar_init(q_full, 8);
+        dev::mbar_init(q_full, 9);  // the softmax warps, and the landing one
         dev::mbar_init(finished, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -567,9 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                     };
                     wait(q_full, items++ & 1);
                     tc_after();
-                    if (first < n) {
-                        wait(full(unit_of(unit0 + 2 * first)), ((unit0 + 2 * first) / S::kUnits) & 1);
-                        tc_after();
+                    if (first < n) {  // (the first keys have landed too)
                         scores(first, 0);
                         scores(first, 1);
                     }
@@ -597,16 +595,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             mma_commit(finished);
             if (!wait_counted(finished, 0)) ok = false;
         } else if (warp == kLandWarp && lane == 0) {
-            // Waits for the values of a tile and the keys of the stream's next, in place of the issuing warps (a wait
-            // takes them 300 clocks even when the phase is over: a prompt of 4093 rows 150 us, with this 141), and joins the softmax
-            // warps in telling them of the tile's first P.
+            // Waits for keys and values in place of the issuing warps (a wait takes them 300 clocks even when the phase is
+            // over: a prompt of 4093 rows 150 us, with this 141): for an item's first keys, when it joins the softmax warps in
+            // telling them of the queries, and for the values of a tile and the keys of the stream's next, when it joins
+            // them in telling of the tile's first P.  It sees every unit, in the ring's order at each place, and before
+            // any product that frees it: no phase is mistaken for the one before or after.
             int64_t unit0 = 0;
-            uint32_t done[2] = {0, 0};
+            uint32_t items = 0, done[2] = {0, 0};
             while (ok) {
                 const int n = it.to - it.from;
                 if (n > 0) {
                     const bool twice = it.valid > kLanes;
                     auto landed = [&](int64_t u) { wait(full(static_cast<int>(u % S::kUnits)), (u / S::kUnits) & 1); };
+                    landed(unit0);
+                    if (!twice && n > 1) landed(unit0 + 2);
+                    dev::mbar_arrive(q_full);
+                    wait(q_full, items++ & 1);  // (one arrival a phase)
                     for (int i = 0; ok && i < n; ++i) {
                         const int next = i + (twice ? 1 : 2);
                         landed(unit0 + 2 * i + 1);
