@@ -11,7 +11,7 @@
 //   O += P V        tcgen05.mma, P and O in tensor memory
 // and while its softmax has one half, its issuing warp has the products of the other: P V of
 // a half, then Q K^T of the same half of the next tile.  (Whole tiles, one set of scores a
-// stream: products and softmax took turns, 4700 clocks a tile where this takes 3700.)  The
+// stream: products and softmax took turns, 4700 clocks a tile where this takes 3000.)  The
 // streams take turns with their powers of two, which one unit serves: left alone they fell
 // into step and both waited for it, then both for the tensor cores.
 //
@@ -24,12 +24,13 @@
 // last slot and rows that are not finite become zeros, and vectors that see one of the
 // latter get NaN through their sums; so nothing that is not seen reaches a result.
 //
-// Bound by turns by the products (2560 clocks of a tile's 3700: scores of 64 slots read the
-// queries again, 48 clocks a step where 128 slots would take 64), and by what an item
-// costs: about 4500 clocks to enter, 5500 to leave, and twice a tile for one with masks.  A
-// prompt of 4093 rows of 32 heads over 8 of 128: 166 us, 827 TFLOP/s; 2 x 509 rows over 1000 to
-// 2999 tokens 68 us; 4 trees of 63 rows over 2500 to 6001 tokens 41 us, about 6 of them the merge.
-// (Some of the powers as polynomials on the fp32 units: 0 to 7 % slower.)
+// Bound by the streams' turns with their powers of two, 750 clocks a half (512 of the unit),
+// which the products just follow (2560 clocks of a tile's 3000: scores of 64 slots read the
+// queries again, 48 clocks a step where 128 slots would take 64); and by what an item costs:
+// about 5000 clocks to enter, 5500 to leave, and twice a tile for one with masks.  A prompt
+// of 4093 rows of 32 heads over 8 of 128: 163 us, 844 TFLOP/s (141 back to back); 2 x 509 rows over 1000 to
+// 2999 tokens 67 us; 4 trees of 63 rows over 2500 to 6001 tokens 41 us, about 6 of them the merge.
+// (Some of the powers as polynomials on the fp32 units: 1 % faster with one in eight, 5 % slower with three.)
 #include <algorithm>
 
 #include "kt_paged.h"
