@@ -159,6 +159,39 @@ def test_attention_in_order(kt, layout, page, lengths, rows, dtype):
     check_attend(cache, q, layout[0], rows, cache.attend(0, q, layout[0], rows))
 
 
+@pytest.mark.parametrize("layout,page,dtype", [((6, 2, 112), 16, BF16), ((40, 1, 64), 64, FP16), ((130, 1, 64), 32, BF16),
+                                               ((3, 3, 96), 128, FP16), ((9, 3, 80), 16, BF16)])
+@pytest.mark.parametrize("rows", [1, 9, 65, 300])
+def test_padded_batches_in_order(kt, layout, page, dtype, rows):
+    """Prompts of unlike lengths in one call: rows behind a sequence's own give zeros and are not seen."""
+    heads, kv, d = layout
+    counts = torch.tensor([rows, 0, max(1, rows // 2), rows + 5, -3], dtype=torch.int32).cuda()
+    cache = filled(layout, page, dtype, [7, 40, 0, 129, 64], rows, poison=True)
+    put(cache, rows, counts)
+    q = queries(cache, heads, rows)
+    out = torch.full_like(q, float("nan"))
+    cache.attend(0, q, heads, rows, counts, out=out)
+    lines = out.view(5, rows, -1)
+    assert not lines[1].any() and not lines[2, max(1, rows // 2):].any() and not lines[4].any()
+    check_attend(cache, q, heads, rows, out, counts)
+
+
+def test_rows_past_the_last_slot_are_no_tokens(kt):
+    heads, kv, d = QWEN
+    for rows in (5, 60):
+        cache = filled(QWEN, 16, BF16, [30, 5], 2, poison=True)  # 32 slots each
+        assert cache.capacity == 32
+        put(cache, rows)
+        assert int(cache.status) != 0
+        q = queries(cache, heads, rows)
+        out = cache.attend(0, q, heads, rows)
+        assert not out.view(2, rows, -1)[0, 2:].any() and not out.view(2, rows, -1)[1, 27:].any()
+        check_attend(cache, q, heads, rows, out)
+        cache.advance(rows)
+        assert cache.lengths.tolist() == [32, min(32, 5 + rows)]
+        assert not cache.attend(0, q, heads, rows).view(2, rows, -1)[0].any()  # a full sequence has no room for tokens
+
+
 @pytest.mark.parametrize("layout,page,lengths,rows,dtype", [
     (LLAMA, 64, [100, 0, 513], 33, BF16), (QWEN, 16, [64, 7], 2, FP16), (QWEN, 32, [500], 64, BF16), (MHA, 128, [20, 21], 31, FP16),
     (MQA, 64, [0], 100, BF16), (WIDE, 16, [250, 3], 61, BF16), (ODD, 32, [31, 32, 33], 40, FP16), (LLAMA, 128, [1000], 130, FP16),
