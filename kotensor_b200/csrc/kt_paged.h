@@ -186,8 +186,38 @@ struct WorkList {
                 return any;
             }
         }
-        if (threadIdx.x == 0) plan.dealt = 0;
         const int entries = a.batch * vts, each = (entries + kThreads - 1) / kThreads;
+        if (entries <= 32) {  // an entry to a lane, every warp for itself (the sums of all threads took 1 us longer)
+            Item it;
+            it.tiles = 0;
+            if (lane < entries) load(it, lane, vts);
+            const int64_t units = it.tiles > 0 ? static_cast<int64_t>(it.tiles + kStart) * a.kv_heads : 0;
+            const int64_t items = static_cast<int64_t>(__popc(__ballot_sync(0xffffffffu, it.tiles > 0))) * a.kv_heads;
+            const bool whole = !__any_sync(0xffffffffu, it.tiles > kWhole);
+            int64_t upto = units;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+            if (items == 0) return false;
+            const int64_t ctas = min(static_cast<int64_t>(gridDim.x), whole ? items : max(items, quotient(total - items * kStart, kLeast)));
+            if (blockIdx.x >= ctas) return false;
+            const int64_t share = quotient(total, ctas), spare = total - share * ctas;
+            const int64_t begin = blockIdx.x * share + min(static_cast<int64_t>(blockIdx.x), spare);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, upto > begin)) - 1) {  // (equal numbers from every warp)
+                plan.share = share, plan.spare = spare, plan.begin = begin;
+                plan.end = begin + share + (blockIdx.x < spare);
+                plan.dealt = 0;
+                it.head = static_cast<int>(quotient(begin - (upto - units), it.tiles + kStart));
+                it.base = upto - units + static_cast<int64_t>(it.head) * (it.tiles + kStart);
+                cut(it);
+                plan.at[warp] = it;
+            }
+            __syncthreads();
+            return true;
+        }
+        if (threadIdx.x == 0) plan.dealt = 0;
         const int from = min(entries, static_cast<int>(threadIdx.x) * each), to = min(entries, from + each);
         Item it;
         int64_t units = 0, items = 0;
