@@ -9,6 +9,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kMostNodes = 1024;  // of a drafted tree
+constexpr int kMostPairs = 64;    // of a head
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -19,10 +20,11 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 //   x' = x cos - y sin,   y' = x sin + y cos.
 // The angle's product is taken in 64 bits and brought into [-pi, pi] there: rounded to
 // fp32, as the reference does, the product at position 100,000 would be off by up to 4e-3,
-// twice what bf16 keeps.  A thread owns four pairs of a row, whose sines it forms once,
-// and goes over heads.
-// Bound by memory for prompts: 4 x 1021 rows of 32 + 8 + 8 heads of 128 27.4 us, 5.5 TB/s (one
-// head's loads at a time 28.9); by latency for steps: a token of 64 sequences 3.1 us.
+// twice what bf16 keeps.  A CTA has a row, whose sines it forms once; a thread four pairs of
+// it, for which it goes over heads.  (A thread forming its own four for every head: 28.7 us
+// where this takes 26.0, and a token of 64 sequences 3.1 where this takes 2.5.)
+// Bound by memory for prompts: 4 x 1021 rows of 32 + 8 + 8 heads of 128 26.0 us, 5.8 TB/s; by
+// latency for steps.
 
 struct Append {
     const float *q, *k, *v, *inv_freq;
@@ -49,37 +51,45 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(Paged c, Append 
     dev::pdl_launch_dependents();
     const int d = c.head_dim, half = d / 2, quads = half / 4;
     const int64_t r = blockIdx.x;
-    const int b = static_cast<int>(r / a.rows), t = static_cast<int>(r - static_cast<int64_t>(b) * a.rows);
+    const int b = static_cast<int>(blockIdx.x / static_cast<uint32_t>(a.rows)), t = static_cast<int>(blockIdx.x) - b * a.rows;
     const int at_once = kThreads / quads, quad = threadIdx.x % quads, first = threadIdx.x / quads;
-    if (first >= at_once) return;
     const int all = a.heads + 2 * c.kv_heads;
     const int begin = blockIdx.y * at_once * a.each + first, end = min(all, (static_cast<int>(blockIdx.y) + 1) * at_once * a.each);
     T* const q_out = static_cast<T*>(a.q_out) + r * a.heads * d + 4 * quad;
     if (t >= paged::rows_of(a.counts, b, a.rows)) {  // not a token
+        if (first >= at_once) return;
         for (int h = begin; h < min(end, a.heads); h += at_once) {
             *reinterpret_cast<uint2*>(q_out + static_cast<int64_t>(h) * d) = make_uint2(0u, 0u);
             *reinterpret_cast<uint2*>(q_out + static_cast<int64_t>(h) * d + half) = make_uint2(0u, 0u);
         }
         return;
     }
-    const int64_t slot = static_cast<int64_t>(max(c.lengths[b], 0)) + t;
-    int page = -1;
-    if (slot < static_cast<int64_t>(c.width) * c.page) page = c.table[static_cast<int64_t>(b) * c.table_stride + slot / c.page];
+    __shared__ float2 turn[kMostPairs];  // cosines and sines of the row's angles
+    const int held = max(c.lengths[b], 0), shift = __ffs(c.page) - 1;
+    const bool fits = static_cast<int64_t>(held) + t < static_cast<int64_t>(c.width) << shift;
+    const int slot = fits ? held + t : 0;
+    const int page = fits ? c.table[static_cast<int64_t>(b) * c.table_stride + (slot >> shift)] : -1;
     const bool stored = page >= 0 && page < c.pages;
     if (!stored && a.status != nullptr && threadIdx.x == 0 && blockIdx.y == 0) *a.status = KT_ERR_INVALID_ARGUMENT;
-    float sn[4], cs[4];
-    if (begin < a.heads + c.kv_heads) {
-        const double p = static_cast<double>(max(c.lengths[b], 0)) +
-                         static_cast<double>(a.depths ? a.depths[static_cast<int64_t>(b) * a.rows + t] : t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double angle = p * static_cast<double>(a.inv_freq[4 * quad + i]);
+    if (begin - first < a.heads + c.kv_heads) {  // as for the whole CTA
+        if (threadIdx.x < half) {
+            const double p = static_cast<double>(held) + static_cast<double>(a.depths ? a.depths[r] : t);
+            const double angle = p * static_cast<double>(a.inv_freq[threadIdx.x]);
             const double turns = rint(angle * 0.15915494309189535);
-            sincosf(static_cast<float>(fma(-turns, 6.283185307179586, angle)), &sn[i], &cs[i]);
+            float sn, cs;
+            sincosf(static_cast<float>(fma(-turns, 6.283185307179586, angle)), &sn, &cs);
+            turn[threadIdx.x] = make_float2(cs, sn);
         }
+        __syncthreads();
+    }
+    if (first >= at_once) return;
+    float sn[4] = {}, cs[4] = {};
+    if (begin < a.heads + c.kv_heads) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[i] = turn[4 * quad + i].x, sn[i] = turn[4 * quad + i].y;
     }
     const int64_t layer = static_cast<int64_t>(a.layer) * c.pages;
-    const int64_t row = ((layer + page) * c.kv_heads) * c.page + slot % c.page;  // of head 0
+    const int64_t row = ((layer + page) * c.kv_heads << shift) + (slot & (c.page - 1));  // of head 0
     // two heads at a time, so that the loads of one do not wait for the other's
     for (int h0 = begin; h0 < end; h0 += 2 * at_once) {
         float u[2][4], w[2][4];

@@ -18,9 +18,9 @@
 // values in turn through a ring of 160 KB, so that some 100 KB are on their way to an SM at
 // any time and across the ends of items.  (Two CTAs of four warps with rings of 80 KB: 231 us
 // where this takes 224, and 37 parts to merge where this leaves 18, 93 where this takes 84.)
-// Bound by memory: 64 sequences of 3001 to 8190 tokens, 8 heads of 128, 226 us, 6.5 TB/s; one of
-// 120001 84 us, 5.9 TB/s, of which about 5 go into the merge.  By latency when short: 301
-// tokens 7.9 us, of which a tile's chain of copy, product, exponentials and product is 1.5.
+// Bound by memory: 64 sequences of 3001 to 8190 tokens, 8 heads of 128, 222 us, 6.6 TB/s; one of
+// 120001 82 us, 6.0 TB/s, of which about 5 go into the merge.  By latency when short: 301
+// tokens 7.3 us, of which a tile's chain of copy, product, exponentials and product is 1.5.
 #include <algorithm>
 
 #include "kt_paged.h"
@@ -34,9 +34,9 @@ constexpr int kWarps = 8;                        // that compute; one more copie
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kVectors = 16;                     // query vectors of an item (the product's M)
 constexpr int kTile = 128;                       // slots of a tile, 16 to a warp
-// What entering an item costs, in tiles (8 sequences of 5000 tokens, 8 heads of 128: 35.0 us, counted as two tiles
-// 36.6), and up to how many an item is not cut (300 tokens 9.4 us, cut into single tiles 10.4; 1000 tokens cut so
-// 10.8, into fours 13.7).
+// What entering an item costs, in tiles (8 sequences of 5000 tokens, 8 heads of 128: 33.2 us, counted as two tiles
+// 34.6), and up to how many an item is not cut (300 tokens 8.2 us, cut into single tiles 9.7; 1000 tokens cut so
+// 9.6, into fours 13.5).
 constexpr int kStart = 4, kLeast = 1, kWhole = 3;
 // Probabilities are kept 2^kLift times larger: in fp16 those down to 2^-36 of the largest
 // stay clear of underflow; the factor cancels in the division by their sum.
@@ -464,10 +464,10 @@ cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttenti
             return cudaErrorInvalidValue;
     // Which kernel is the faster.  This file's reads the cache once for every sixteen vectors, the other one once for
     // 256, but takes 4 us longer to enter, leave and merge.  So this one runs for sixteen vectors or fewer; for up to 32
-    // while its items leave no SM two (20 vectors of 32 heads over 8 of 128, 1 / 8 / 64 sequences of 300 tokens: 10.1 /
-    // 10.4 / 58 us here, 14.6 / 18.0 / 56 there; 8 sequences of 4000: 46, 56); and for more where they are very few (112
-    // vectors of 14 heads over 2 of 64, 1 / 8 sequences: 300 tokens 8.2 / 8.5 us here, 12.5 / 12.9 there, 20000 and 4000 tokens
-    // 23 / 33 here, 28 / 18 there).
+    // while its items leave no SM two (20 vectors of 32 heads over 8 of 128, 1 / 8 / 64 sequences of 300 tokens: 9.2 /
+    // 9.4 / 57 us here, 14.7 / 17.6 / 57 there; 8 sequences of 4000: 43, 56); and for more where they are very few (112
+    // vectors of 14 heads over 2 of 64, 1 / 8 sequences: 300 tokens 7.6 / 8.6 us here, 12.6 / 12.6 there, 20000 and 4000 tokens
+    // 22 / 33 here, 27 / 17 there).
     const int64_t sixteens = (static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors, items = sixteens * a.batch * a.kv_heads;
     if (sixteens > 1 && items > (sixteens == 2 ? sm_count : 16)) return launch_paged_many(c.dtype == KT_BF16, maps, a, sm_count, err, s);
     const bool bf16 = c.dtype == KT_BF16, wide = c.head_dim > 64;

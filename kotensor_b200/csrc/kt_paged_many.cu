@@ -28,8 +28,8 @@
 // which the products just follow (2560 clocks of a tile's 3000: scores of 64 slots read the
 // queries again, 48 clocks a step where 128 slots would take 64); and by what an item costs:
 // about 5000 clocks to enter, 5500 to leave, and twice a tile for one with masks.  A prompt
-// of 4093 rows of 32 heads over 8 of 128: 163 us, 844 TFLOP/s (141 back to back); 2 x 509 rows over 1000 to
-// 2999 tokens 67 us; 4 trees of 63 rows over 2500 to 6001 tokens 41 us, about 6 of them the merge.
+// of 4093 rows of 32 heads over 8 of 128: 162 us, 849 TFLOP/s (141 back to back); 2 x 509 rows over 1000 to
+// 2999 tokens 65 us; 4 trees of 63 rows over 2500 to 6001 tokens 39 us, about 6 of them the merge.
 // (Some of the powers as polynomials on the fp32 units: 1 % faster with one in eight, 5 % slower with three.)
 #include <algorithm>
 
@@ -43,9 +43,9 @@ using namespace paged;
 constexpr int kLanes = 128;                // vectors of a stream (the MMA's M)
 constexpr int kVectors = 2 * kLanes;       // of an item
 constexpr int kTile = 128;                 // slots of a tile
-// What entering an item costs, in tiles (a prompt of 4093 rows: 177 us, counted as two 214, as six 183), the
+// What entering an item costs, in tiles (a prompt of 4093 rows, cut: 157 us, counted as two 212, as six 162), the
 // tiles that are worth a CTA, and up to how many an item is not cut (a tree of 20 rows over 300 tokens of each of 8
-// sequences: 18.1 us, cut 19.8); from how many items to a CTA a prompt's are dealt whole (170 us cut, 160 dealt).
+// sequences: 17.9 us, cut 19.3); from how many items to a CTA a prompt's are dealt whole (157 us cut, 141 dealt).
 constexpr int kStart = 4, kLeast = 2, kWhole = 4, kDeal = 3;
 constexpr int kIssueWarp = 8, kCopyWarp = 10, kLandWarp = 11;  // after the softmax warps; an issuing warp for each stream
 constexpr int kThreads = 384;
