@@ -561,8 +561,8 @@ size_t kt_paged_scratch_bytes(kt_ctx* ctx);
  * q: rows of `heads` heads of the cache's type, rows q_stride elements apart; heads /
  * kv_heads query heads share a key/value head.  out_dev [batch * rows_per_seq][heads *
  * head_dim] of the cache's type or fp32 (out_dtype).  Rows that are no tokens give zeros.
- * At most 2^30 query vectors a sequence (rows times heads), 2^31 - 1 of all sequences'
- * rows times heads / kv_heads.
+ * At most 65535 heads, 2^30 query vectors a sequence (rows times heads), 2^31 - 1 of all sequences'
+ * rows times heads / kv_heads; scale and scale * log2(e) are finite.
  * Scores and sums are fp32, probabilities are rounded to the cache's type.  What a row does
  * not see has no part in it, infinities and NaN included; a value that is not finite makes
  * the rows that see it NaN. */

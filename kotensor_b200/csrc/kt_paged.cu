@@ -1,6 +1,7 @@
 // kt_paged.cu -- the paged 16-bit key/value cache: new tokens, rotated by their
 // positions, into their pages; the accepted path of a drafted tree; the C entries.
 #include <algorithm>
+#include <cmath>
 
 #include "kt_paged.h"
 
@@ -284,12 +285,14 @@ kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t l
     if (rows_per_seq < 0) return entry_fail(KT_ERR_INVALID_ARGUMENT, "Negative row count");
     if (rows_per_seq == 0) return KT_OK;
     if (!q || !out || !scratch) return entry_fail(KT_ERR_INVALID_ARGUMENT, "NULL argument");
-    if (heads < 1 || heads % cache->kv_heads != 0)
-        return entry_fail(KT_ERR_INVALID_ARGUMENT, "heads must be a positive multiple of kv_heads");
+    if (heads < 1 || heads > 65535 || heads % cache->kv_heads != 0)
+        return entry_fail(KT_ERR_INVALID_ARGUMENT, "heads must be a positive multiple of kv_heads, at most 65535");
     if (q_stride < static_cast<int64_t>(heads) * cache->head_dim)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "rows of q are shorter than heads * head_dim");
     if (out_dtype != cache->dtype && out_dtype != KT_FP32)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "out_dtype must be the cache's or KT_FP32");
+    const float factor = static_cast<float>(scale * 1.4426950408889634);
+    if (!std::isfinite(factor)) return entry_fail(KT_ERR_INVALID_ARGUMENT, "scale must be finite, in powers of two as well");
     if (!aligned16(scratch)) return entry_fail(KT_ERR_INVALID_ARGUMENT, "scratch must be 16-byte aligned");
     if (visible && rows_per_seq > kMostNodes) return entry_fail(KT_ERR_INVALID_ARGUMENT, "visible needs at most 1024 rows a sequence");
     // (vectors of a sequence, and items of all, are counted in 32 bits)
@@ -305,7 +308,7 @@ kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t l
         a.table_stride = cache->table_stride, a.capacity = cache->width * cache->page;
         a.rows = rows_per_seq, a.heads = heads, a.group = heads / cache->kv_heads, a.words = (rows_per_seq + 31) / 32;
         // (with a scale of 0 masked scores still have to be -inf, the others alike)
-        a.factor = scale == 0.0f ? 1e-38f : static_cast<float>(scale * 1.4426950408889634);
+        a.factor = scale == 0.0f ? 1e-38f : factor;
         a.out_f32 = out_dtype == KT_FP32;
         a.aligned = (reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 8 == 0 ? 1 : 0) | (aligned16(out) ? 2 : 0);
         return entry_launch(launch_paged_attention(*cache, layer, a, ctx->sm_count, ctx->d_error, static_cast<cudaStream_t>(stream)),

@@ -64,6 +64,19 @@ def test_calls_that_are_refused(kt, name, change, message):
     assert message in lib.kt_last_error().decode()
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])  # (3e38 * log2(e) is past fp32)
+def test_scales_that_are_refused(kt, scale):
+    lib = kt.load_library()
+    assert lib.kt_paged_attention(ctypes.c_void_p(4096), ctypes.byref(good()), 0, 4096, 256, 4096, 1, 1, None, None, 4, scale, 4096, None) == 1
+    assert "scale" in lib.kt_last_error().decode()
+
+
+def test_more_heads_than_a_launch_counts(kt):
+    lib = kt.load_library()
+    assert calls(lib, ctypes.c_void_p(4096), good(), heads=65536, q_stride=1 << 22)["attend"]() == 1
+    assert "65535" in lib.kt_last_error().decode()
+
+
 def test_no_context_and_no_rows(kt):
     lib = kt.load_library()
     for call in calls(lib, None, good()).values():
