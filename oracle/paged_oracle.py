@@ -1,6 +1,6 @@
 """The paged 16-bit key/value cache in plain torch on the CPU, in 64 bits: rotation and
-store, attention with its masks, and the accepted path of a drafted tree.  The checker of
-tests/test_paged_gpu.py; the definitions are those of include/kt_cuda.h."""
+store, attention with its masks, and the accepted path of a drafted tree.  What
+tests/test_paged_gpu.py compares with; the definitions are those of include/kt_cuda.h."""
 import math
 
 import torch
@@ -33,7 +33,7 @@ def rotate(x, positions, inv_freq):
 def attend(keys, values, table, lengths, q, heads, rows, counts=None, visible=None, scale=None):
     """(out, magnitude) float64 [batch * rows, heads, d] of one layer's keys and values
     [pages, kv_heads, page, d]: the attention, and the same with |values|, by which
-    roundings are judged.  Slots without a page are seen by no row."""
+    roundings are counted.  Slots without a page are seen by no row."""
     pages, kv, page, d = keys.shape
     batch, capacity = table.shape[0], table.shape[1] * page
     scale = 1.0 / math.sqrt(d) if scale is None else scale
