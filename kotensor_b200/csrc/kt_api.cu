@@ -103,6 +103,17 @@ void free_weight(kt_qweight* w) {
     delete w;
 }
 
+// Zeroes device memory outside any capture, done on return.
+cudaError_t zero_now(void* p, size_t bytes) {
+    cudaStream_t aside = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&aside, cudaStreamNonBlocking);
+    if (e != cudaSuccess) return e;
+    e = cudaMemsetAsync(p, 0, bytes, aside);
+    const cudaError_t done = cudaStreamSynchronize(aside);
+    cudaStreamDestroy(aside);
+    return e != cudaSuccess ? e : done;
+}
+
 }  // namespace
 
 cudaError_t stream_workspace(kt_ctx* ctx, cudaStream_t s, size_t bytes, void** out) {
@@ -114,21 +125,23 @@ cudaError_t stream_workspace(kt_ctx* ctx, cudaStream_t s, size_t bytes, void** o
         *out = hit->ptr;
         return cudaSuccess;
     }
-    // Grow to at least 1 MiB at a time.  cudaMalloc is not a stream operation;
-    // while `s` is being captured into a CUDA graph it is allowed in relaxed
-    // capture mode, and the zeroing below then becomes a node of that graph.
+    // Grow to at least 1 MiB at a time.  cudaMalloc is not a stream operation; while
+    // `s` is being captured into a CUDA graph it is allowed in relaxed capture mode.  The
+    // zeros must not become a node of that graph then: the graph may never be replayed, and
+    // another one captured on `s`, or a launch on it, would find the memory as it was.
     const size_t cap = std::max(bytes, static_cast<size_t>(1) << 20);
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     cudaThreadExchangeStreamCaptureMode(&mode);
     void* p = nullptr;
     cudaError_t e = cudaMalloc(&p, cap);
+    if (e == cudaSuccess) {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        e = cudaStreamIsCapturing(s, &status);
+        if (e == cudaSuccess) e = status == cudaStreamCaptureStatusNone ? cudaMemsetAsync(p, 0, cap, s) : zero_now(p, cap);
+        if (e != cudaSuccess) cudaFree(p);
+    }
     cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) return e;
-    e = cudaMemsetAsync(p, 0, cap, s);
-    if (e != cudaSuccess) {
-        cudaFree(p);
-        return e;
-    }
     if (hit != nullptr) {
         ctx->retired.push_back(hit->ptr);  // queued launches may still use it
         hit->ptr = p;

@@ -689,7 +689,7 @@ class DeviceDecoder:
                 depths[q, :n], seen = draft_tree(p)
                 visible[q, :n, :seen.shape[1]] = seen
         d.device.copy_(d.host, non_blocking=True)
-        if not d.warm:  # (a graph is captured when it is about to be replayed: its first replay zeroes workspaces)
+        if not d.warm:  # (a text of one pass is not worth a graph)
             self._launch_pass(d)
             d.warm = True
         else:
