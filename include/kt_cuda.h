@@ -578,7 +578,8 @@ kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t l
  * values of the path's nodes move to slots lengths[b], lengths[b] + 1, ... in every layer;
  * taken[b] = nodes of the path (0 where counts[b] is 0), accepted[b][i] = the choice after
  * its node i, -1 behind its end.  kt_kv8_advance with counts `taken` then moves lengths on.
- * A node without a page sets KT_ERR_INVALID_ARGUMENT in *status_dev (NULL: not reported). */
+ * A node without a page sets KT_ERR_INVALID_ARGUMENT in *status_dev (NULL: not reported).
+ * accepted, taken and status may not overlap one another, the other arrays, table or lengths. */
 kt_status kt_paged_accept(kt_ctx* ctx, const kt_paged_cache* cache, const int32_t* tokens_dev,
                           const int32_t* parents_dev, const int32_t* choices_dev, int32_t rows_per_seq,
                           const int32_t* counts_dev, int32_t* accepted_dev, int32_t* taken_dev, int32_t* status_dev,

@@ -234,6 +234,19 @@ const char* check(const Paged* c) {
     return nullptr;
 }
 
+// Whether the output (of `bytes`) shares memory with an input: `rows` of row_bytes, `stride`
+// bytes apart.
+bool overlaps(const void* out, int64_t bytes, const void* in, int64_t row_bytes, int64_t rows = 1, int64_t stride = 1) {
+    if (out == nullptr || in == nullptr || bytes <= 0 || row_bytes <= 0 || rows <= 0) return false;
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in), end = i + row_bytes;
+    const int64_t first = o < end ? 0 : static_cast<int64_t>((o - end) / stride) + 1;  // the first row that ends behind o
+    return first < rows && i + first * stride < o + bytes;
+}
+// The same for what every call reads of the cache's table and lengths.
+bool overlaps_places(const void* out, int64_t bytes, const Paged& c) {
+    return overlaps(out, bytes, c.lengths, 4ll * c.batch) || overlaps(out, bytes, c.table, 4ll * c.width, c.batch, 4ll * c.table_stride);
+}
+
 }  // namespace
 }  // namespace kt
 
@@ -324,6 +337,15 @@ kt_status kt_paged_accept(kt_ctx* ctx, const kt_paged_cache* cache, const int32_
     if (!tokens || !parents || !choices || !accepted || !taken) return entry_fail(KT_ERR_INVALID_ARGUMENT, "NULL argument");
     if (rows_per_seq < 1 || rows_per_seq > kMostNodes)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "a drafted tree has 1..1024 nodes");
+    // (every CTA walks the trees for itself, while one already writes what it found)
+    const int64_t nodes = 4ll * cache->batch * rows_per_seq, each = 4ll * cache->batch;
+    const auto read = [&](const void* out, int64_t bytes) {
+        return overlaps(out, bytes, tokens, nodes) || overlaps(out, bytes, parents, nodes) || overlaps(out, bytes, choices, nodes) ||
+               overlaps(out, bytes, counts, each) || overlaps_places(out, bytes, *cache);
+    };
+    if (read(accepted, nodes) || read(taken, each) || read(status, 4) || overlaps(accepted, nodes, taken, each) ||
+        overlaps(status, 4, accepted, nodes) || overlaps(status, 4, taken, each))
+        return entry_fail(KT_ERR_INVALID_ARGUMENT, "accepted, taken and status must not overlap each other or what the call reads");
     return c_entry(ctx, [&] {
         const Accept a{tokens, parents, choices, counts, accepted, taken, status, rows_per_seq};
         return entry_launch(launch_dependent(paged_accept_kernel, dim3(2 * cache->layers, cache->batch), dim3(kThreads), 0,

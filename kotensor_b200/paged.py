@@ -249,7 +249,8 @@ class PagedKVCache:
         the path's keys and values of every layer to the slots behind the text and returns
         ``accepted`` (int32 [batch, rows]: the choices along the path, then -1) and ``taken``
         (int32 [batch]: the path's nodes), by which ``advance(rows, counts=taken)`` moves on:
-        those given, or buffers of this object that its next call with as many rows overwrites."""
+        those given (no memory that the call reads), or buffers of this object that its next call
+        with as many rows overwrites."""
         rows = tokens.shape[1] if tokens.dim() == 2 else 0
         shape = (self.batch, rows)
         given = (self._ints("tokens", tokens, shape), self._ints("parents", parents, shape), self._ints("choices", choices, shape),

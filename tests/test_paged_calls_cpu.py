@@ -1,0 +1,36 @@
+"""Paged cache without a GPU: calls whose outputs share memory with what they read, and pages for all sequences or none."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+# one array after the other: a cache of 2 layers and 3 sequences, 5 rows a sequence
+PLACES = {name: (i + 1) << 20 for i, name in enumerate(
+    ["keys", "values", "table", "lengths", "tokens", "parents", "choices", "counts", "accepted", "taken", "status", "q", "k", "v", "inv_freq",
+     "depths", "visible", "out", "scratch"])}
+
+
+def cache():
+    from kotensor_b200 import _lib
+    at = {n: PLACES[n] for n in ("keys", "values", "table", "lengths")}
+    return _lib.KtPagedCache(**at, layers=2, batch=3, kv_heads=2, head_dim=64, pages=5, page=16, width=4, table_stride=6, dtype=_lib.KT_BF16)
+
+
+def refused(lib, status):
+    return status == 1 and "overlap" in lib.kt_last_error().decode()
+
+
+@pytest.mark.parametrize("change", [
+    dict(accepted="choices"), dict(accepted="tokens"), dict(accepted="parents"), dict(accepted=("choices", 56)), dict(accepted=("choices", -56)),
+    dict(accepted="counts"), dict(accepted=("lengths", 8)), dict(accepted="table"), dict(accepted=("table", 5 * 6 * 4 - 60 - 8)), dict(taken="counts"), dict(taken="lengths"),
+    dict(taken=("tokens", 59)), dict(taken=("parents", -8)), dict(taken=("table", 24 * 2 + 12)), dict(taken="accepted"), dict(taken=("accepted", 56)),
+    dict(status="lengths"), dict(status=("accepted", 4)), dict(status=("taken", 8)), dict(status=("choices", 56)), dict(status="counts"),
+])
+def test_accepted_paths_over_what_is_read(kt, change):
+    lib = kt.load_library()
+    at = dict(PLACES)
+    for name, place in change.items():
+        at[name] = PLACES[place] if isinstance(place, str) else PLACES[place[0]] + place[1]
+    assert refused(lib, lib.kt_paged_accept(ctypes.c_void_p(4096), ctypes.byref(cache()), at["tokens"], at["parents"], at["choices"], 5, at["counts"],
+                                            at["accepted"], at["taken"], at["status"], None))
