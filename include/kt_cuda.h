@@ -542,7 +542,8 @@ typedef struct {
  * rounded once to the cache's type.  Keys and values go into their slots, queries into
  * q_out_dev [batch * rows_per_seq][heads * head_dim] of the cache's type (8-byte aligned;
  * rows that are no tokens get zeros).  q NULL with heads 0: no queries.  A token without a
- * page sets KT_ERR_INVALID_ARGUMENT in *status_dev (NULL: not reported). */
+ * page sets KT_ERR_INVALID_ARGUMENT in *status_dev (NULL: not reported).  q_out and status
+ * may not overlap each other or what the call reads. */
 kt_status kt_paged_append(kt_ctx* ctx, const kt_paged_cache* cache, int32_t layer, const float* q_dev,
                           const float* k_dev, const float* v_dev, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                           int32_t heads, const float* inv_freq_dev, int32_t rows_per_seq, const int32_t* counts_dev,
@@ -560,7 +561,9 @@ size_t kt_paged_scratch_bytes(kt_ctx* ctx);
  *   out[row][head] = softmax(scale * q . k) . v,  0 for a row that sees nothing.
  * q: rows of `heads` heads of the cache's type, rows q_stride elements apart; heads /
  * kv_heads query heads share a key/value head.  out_dev [batch * rows_per_seq][heads *
- * head_dim] of the cache's type or fp32 (out_dtype).  Rows that are no tokens give zeros.
+ * head_dim] of the cache's type or fp32 (out_dtype); it may not overlap what the call reads,
+ * but for q itself, where that has rows without gaps and the same type.  Rows that are no
+ * tokens give zeros.
  * At most 65535 heads, 2^30 query vectors a sequence (rows times heads), 2^31 - 1 of all sequences'
  * rows times heads / kv_heads; scale and scale * log2(e) are finite.
  * Scores and sums are fp32, probabilities are rounded to the cache's type.  What a row does

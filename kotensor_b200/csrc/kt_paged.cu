@@ -270,6 +270,15 @@ kt_status kt_paged_append(kt_ctx* ctx, const kt_paged_cache* cache, int32_t laye
     if (q && reinterpret_cast<uintptr_t>(q_out) % 8 != 0) return entry_fail(KT_ERR_INVALID_ARGUMENT, "q_out must be 8-byte aligned");
     const int64_t rows = static_cast<int64_t>(cache->batch) * rows_per_seq;
     if (rows > (1ll << 31) - 1) return entry_fail(KT_ERR_INVALID_ARGUMENT, "too many rows");
+    // (CTAs have parts of a row each, in no order)
+    const auto read = [&](const void* out, int64_t bytes) {
+        return overlaps(out, bytes, q, 4ll * heads * cache->head_dim, rows, 4 * q_stride) || overlaps(out, bytes, k, 4 * width, rows, 4 * k_stride) ||
+               overlaps(out, bytes, v, 4 * width, rows, 4 * v_stride) || overlaps(out, bytes, inv_freq, 2ll * cache->head_dim) ||
+               overlaps(out, bytes, counts, 4ll * cache->batch) || overlaps(out, bytes, depths, 4 * rows) || overlaps_places(out, bytes, *cache);
+    };
+    const int64_t q_bytes = q ? 2 * rows * heads * cache->head_dim : 0;
+    if (read(q_out, q_bytes) || read(status, 4) || overlaps(status, 4, q_out, q_bytes))
+        return entry_fail(KT_ERR_INVALID_ARGUMENT, "q_out and status must not overlap each other or what the call reads");
     return c_entry(ctx, [&] {
         const auto quads = [](const float* p, int64_t stride) { return aligned16(p) && stride % 4 == 0; };
         const int aligned = (quads(q, q_stride) ? 1 : 0) | (quads(k, k_stride) ? 2 : 0) | (quads(v, v_stride) ? 4 : 0);
@@ -312,6 +321,13 @@ kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t l
     if (static_cast<int64_t>(rows_per_seq) * heads > (1 << 30) ||
         static_cast<int64_t>(rows_per_seq) * heads / cache->kv_heads * cache->batch > (1ll << 31) - 1)
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "too many rows");
+    // (a CTA writes the results of the queries that it has read, or that all who share them have: they may take their place)
+    const int64_t rows = static_cast<int64_t>(cache->batch) * rows_per_seq, width = static_cast<int64_t>(heads) * cache->head_dim;
+    const int64_t bytes = rows * width * (out_dtype == KT_FP32 ? 4 : 2);
+    const bool in_place = out == q && q_stride == width && out_dtype == cache->dtype;
+    if ((!in_place && overlaps(out, bytes, q, 2 * width, rows, 2 * q_stride)) || overlaps(out, bytes, counts, 4ll * cache->batch) ||
+        overlaps(out, bytes, visible, 4 * rows * ((rows_per_seq + 31) / 32)) || overlaps_places(out, bytes, *cache))
+        return entry_fail(KT_ERR_INVALID_ARGUMENT, "out must not overlap what the call reads, but for the queries it takes the place of");
     return c_entry(ctx, [&] {
         PagedAttention a{};
         a.table = cache->table, a.lengths = cache->lengths, a.counts = counts, a.visible = visible;

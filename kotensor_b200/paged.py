@@ -224,8 +224,9 @@ class PagedKVCache:
         (``append`` of the same rows comes first) up to itself, or those whose bits are set in
         ``visible`` (int32 [batch, rows_per_seq, (rows_per_seq + 31) // 32], ``draft_tree``).  ``q``
         [batch * rows_per_seq, heads * head_dim] of the cache's type; the result has its
-        type, or ``out``'s (the cache's or float32).  ``scale`` is 1 / sqrt(head_dim) unless
-        given.  Rows that see nothing, or are no tokens by ``counts``, give zeros."""
+        type, or ``out``'s (the cache's or float32; ``q`` itself where its rows have no gaps).
+        ``scale`` is 1 / sqrt(head_dim) unless given.  Rows that see nothing, or are no tokens
+        by ``counts``, give zeros."""
         rows, width, device = self.batch * rows_per_seq, heads * self.head_dim, self.ctx.device
         if q.dtype is not self.dtype or q.get_device() != device or q.shape != (rows, width):
             raise ValueError(f"q must be a {str(self.dtype).replace('torch.', '')} tensor of shape [{rows}, {width}] on "

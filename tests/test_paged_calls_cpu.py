@@ -34,3 +34,32 @@ def test_accepted_paths_over_what_is_read(kt, change):
         at[name] = PLACES[place] if isinstance(place, str) else PLACES[place[0]] + place[1]
     assert refused(lib, lib.kt_paged_accept(ctypes.c_void_p(4096), ctypes.byref(cache()), at["tokens"], at["parents"], at["choices"], 5, at["counts"],
                                             at["accepted"], at["taken"], at["status"], None))
+
+
+@pytest.mark.parametrize("change", [
+    dict(out="q"), dict(out=("q", 104)), dict(out="k"), dict(out=("v", 14 * 1024 + 504)), dict(out=("v", -7672)), dict(out="inv_freq"), dict(out=("counts", 8)),
+    dict(out=("depths", 56)), dict(out="lengths"), dict(out=("table", 64 - 8)), dict(status="counts"), dict(status=("q", 14 * 1024 + 1020)),
+    dict(status=("depths", 56)), dict(status=("out", 7676)), dict(status=("table", 12)), dict(status="lengths"), dict(status=("inv_freq", 124)),
+])
+def test_appended_queries_over_what_is_read(kt, change):
+    """15 rows of 4 + 2 + 2 heads of 64; rows of q, k and v lie 1024 bytes apart."""
+    lib = kt.load_library()
+    at = dict(PLACES)
+    for name, place in change.items():
+        at[name] = PLACES[place] if isinstance(place, str) else PLACES[place[0]] + place[1]
+    assert refused(lib, lib.kt_paged_append(ctypes.c_void_p(4096), ctypes.byref(cache()), 0, at["q"], at["k"], at["v"], 256, 256, 256, 4,
+                                            at["inv_freq"], 5, at["counts"], at["depths"], at["out"], at["status"], None))
+
+
+@pytest.mark.parametrize("change,stride,dtype", [
+    (dict(out="q"), 264, 1), (dict(out="q"), 256, 0), (dict(out=("q", 2)), 256, 1), (dict(out=("q", -7678)), 256, 1),
+    (dict(out=("q", 14 * 1024 + 510)), 512, 1), (dict(out=("counts", 8)), 256, 1), (dict(out="visible"), 256, 1), (dict(out=("visible", 56)), 256, 1),
+    (dict(out=("lengths", 8)), 256, 1), (dict(out=("table", 60)), 256, 0),
+])
+def test_attention_over_what_it_reads(kt, change, stride, dtype):
+    lib = kt.load_library()
+    at = dict(PLACES)
+    for name, place in change.items():
+        at[name] = PLACES[place] if isinstance(place, str) else PLACES[place[0]] + place[1]
+    assert refused(lib, lib.kt_paged_attention(ctypes.c_void_p(4096), ctypes.byref(cache()), 0, at["q"], stride, at["out"], dtype, 5, at["counts"],
+                                               at["visible"], 4, 1.0, at["scratch"], None))
