@@ -568,7 +568,8 @@ size_t kt_paged_scratch_bytes(kt_ctx* ctx);
  * rows times heads / kv_heads; scale and scale * log2(e) are finite.
  * Scores and sums are fp32, probabilities are rounded to the cache's type.  What a row does
  * not see has no part in it, infinities and NaN included; a value that is not finite makes
- * the rows that see it NaN. */
+ * the rows that see it NaN in its dim, and in no other; a score that is NaN or +infinity its
+ * row and head in all. */
 kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t layer, const void* q_dev,
                              int64_t q_stride, void* out_dev, int32_t out_dtype, int32_t rows_per_seq,
                              const int32_t* counts_dev, const uint32_t* visible_dev, int32_t heads, float scale,

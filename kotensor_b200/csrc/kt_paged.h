@@ -376,11 +376,18 @@ struct Half16<__nv_bfloat16> {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 };
-// Not 0 if one of a word's two values is an infinity or NaN: a carry out of the exponent.
+// Bits 15 and 31 where one of a word's two values is an infinity or NaN: a carry out of the
+// exponent.
 template <typename T>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return ((w & 0x7fff7fffu) + (0x80008000u - Half16<T>::kExponent)) & 0x80008000u;
 }
+template <typename T>
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {  // 0 in place of such values
+    return w & ~((not_finite<T>(w) >> 15) * 0xffffu);
+}
+// A result that an infinite value has reached is NaN like one that a NaN has.
+__device__ __forceinline__ float nan_if_infinite(float y) { return fmaf(y, 0.0f, y); }
 
 // Four dims of a result, `at` elements into out (a multiple of 4).
 template <typename T>

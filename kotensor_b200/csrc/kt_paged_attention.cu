@@ -275,11 +275,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             wait(full(vx), v_phase);
             __syncwarp();
             if (edge && slot < it.sees) {
-                // What no vector sees counts nothing, whatever it is, and a value that is not finite counts for those
-                // that see it alone: such rows of the tile become zeros, the rest is told by the sums.
-                uint32_t any = __reduce_or_sync(0xffffffffu, seen[0] | seen[1]);
+                // What no vector sees counts nothing, whatever it is: its rows of the tile become zeros.  A value that is
+                // not finite counts for those that see it alone, who get NaN in its dim; a zero takes its place.
+                const uint32_t any = __reduce_or_sync(0xffffffffu, seen[0] | seen[1]);
                 const int row = lane / 2;
-                uint4* const line = reinterpret_cast<uint4*>(smem + vx * S::kUnit + (warp * 16 + row) * 128);
+                unsigned char* const rows = smem + vx * S::kUnit + warp * 16 * 128;
+                uint4* const line = reinterpret_cast<uint4*>(rows + row * 128);
                 uint32_t over = 0;
 #pragma unroll
                 for (int i = 0; i < HDP / 16; ++i) {
@@ -287,21 +288,34 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     const uint4 w = line[piece / 8 * (kTile * 128 / 16) + piece % 8];
                     over |= not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w);
                 }
-                uint32_t told = __ballot_sync(0xffffffffu, over != 0);
-                told = (told | told >> 1) & 0x55555555u;  // bit 2 * row
-                if (!(any >> row & 1u) || (told >> (2 * row) & 1u)) {
+                const bool hidden = !(any >> row & 1u);
+                for (uint32_t told = __ballot_sync(0xffffffffu, over != 0 && !hidden); told != 0;) {
+                    const int r = (__ffs(told) - 1) / 2;
+                    told &= ~(3u << (2 * r));
+#pragma unroll
+                    for (int j = 0; j < HDP / 8; ++j) {
+                        const uint32_t bad = not_finite<T>(
+                            *reinterpret_cast<const uint32_t*>(rows + j / 8 * (kTile * 128) + r * 128 + ((j % 8 ^ (r & 7)) << 4) + 4 * t4));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if ((e % 2 ? bad >> 31 : bad & 0x8000u) && (seen[e / 2] >> r & 1u)) o[j][e] = __uint_as_float(0x7fc00000u);
+                    }
+                }
+                __syncwarp();
+                if (hidden) {
 #pragma unroll
                     for (int i = 0; i < HDP / 16; ++i) {
                         const int piece = lane % 2 * (HDP / 16) + i;
                         line[piece / 8 * (kTile * 128 / 16) + piece % 8] = make_uint4(0, 0, 0, 0);
                     }
+                } else if (over != 0) [[unlikely]] {
+#pragma unroll 1
+                    for (int i = 0; i < HDP / 16; ++i) {
+                        const int piece = lane % 2 * (HDP / 16) + i;
+                        uint4& w = line[piece / 8 * (kTile * 128 / 16) + piece % 8];
+                        w = make_uint4(finite_part<T>(w.x), finite_part<T>(w.y), finite_part<T>(w.z), finite_part<T>(w.w));
+                    }
                 }
-                uint32_t rows = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) rows |= (told >> (2 * i) & 1u) << i;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (rows & seen[i]) sum[i] = __uint_as_float(0x7fc00000u);
                 __syncwarp();
             }
             if (slot < it.sees) {
@@ -357,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     for (int i = 0; i < 2; ++i) {
                         float2* const at = reinterpret_cast<float2*>(sums + (r8 + 8 * i) * S::kPitch + 8 * j + 2 * t4);
                         const float2 f = step == 0 ? make_float2(0.0f, 0.0f) : *at;
-                        *at = make_float2(f.x + (by[i] == 0.0f ? 0.0f : o[j][2 * i] * by[i]), f.y + (by[i] == 0.0f ? 0.0f : o[j][2 * i + 1] * by[i]));
+                        *at = make_float2(f.x + o[j][2 * i] * by[i], f.y + o[j][2 * i + 1] * by[i]);
                     }
             }
             compute_sync();
@@ -367,8 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             if (dim >= d) return;
             const int64_t at = place_of(a, it.b, it.head, it.v0 + vec, static_cast<int64_t>(a.heads) * d) + dim;
             const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-            y.x *= scale, y.y *= scale, y.z *= scale, y.w *= scale;
-            put4<T>(a, at, y);
+            put4<T>(a, at, make_float4(nan_if_infinite(y.x * scale), nan_if_infinite(y.y * scale), nan_if_infinite(y.z * scale), nan_if_infinite(y.w * scale)));
         };
         const bool whole = from == 0 && to == it.tiles;
         // the part of an item that an earlier CTA began is the CTA's part 0, of one that goes on its part 1

@@ -21,8 +21,8 @@
 //
 // Masks.  Only tiles that some vector does not see in full (the last ones, and all that hold
 // new tokens of a tree) look at them.  There values are read first: rows of the tile past the
-// last slot and rows that are not finite become zeros, and vectors that see one of the
-// latter get NaN through their sums; so nothing that is not seen reaches a result.
+// last slot and values that are not finite become zeros, and vectors that see one of the
+// latter get NaN in its dim at their item's end; so nothing that is not seen reaches a result.
 //
 // Bound by the streams' turns with their powers of two, 750 clocks a half (512 of the unit),
 // which the products just follow (2560 clocks of a tile's 3000: scores of 64 slots read the
@@ -59,7 +59,10 @@ struct ManyShape {
     static constexpr int kRing = 2 * kUnit, kUnits = 4 * 128 / HDP;  // keys, values, keys, ...
     static constexpr int kBad = kRing + kUnits * kUnit;  // slots of an edge tile whose values are not finite: [2][3][4] words
     static constexpr int kStats = kBad + 128;            // of the second stream's vectors
-    static constexpr int kBars = kStats + 2 * kLanes * 4;
+    static constexpr int kWords = HDP / 32;              // of a bit for each dim
+    static constexpr int kMap = kStats + 2 * kLanes * 4; // which dims of those slots: [2][2][slot][word]
+    static constexpr int kMarks = kMap + 4 * kTile * kWords * 4;  // dims in which a vector gets NaN: [word][thread]
+    static constexpr int kBars = kMarks + kWords * 256 * 4;
     static constexpr int kSmem = 1024 + kBars + 16 * kUnits + 14 * 8;
     static constexpr int kPart = kVectors * (HDP + 2);   // floats of a part: [HDP / 4][vector][4], references, sums
     static constexpr uint32_t kO = 256;                  // tensor memory: scores (then P) of stream x at 128 x, its O
@@ -264,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
         const int x = warp / 4, row = threadIdx.x % kLanes;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp % 4) << 21), s_tm = lanes + kLanes * x, o_tm = lanes + S::kO + HDP * x;
         uint32_t* const bad_words = reinterpret_cast<uint32_t*>(smem + S::kBad);
+        uint32_t* const marks = reinterpret_cast<uint32_t*>(smem + S::kMarks) + threadIdx.x;
         float* const parts = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kPagedPartsAt);
         const float factor = fabsf(a.factor);
         if (x == 1) bar_arrive(4, 256);  // the first stream has the first turn
@@ -276,6 +280,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             const int step = twice ? 1 : 2, v = (twice ? kLanes * x : 0) + row;  // the vector of this thread, in the item
             bar_sync(1, 256);  // nobody works on the item before
             if (threadIdx.x < 24) bad_words[threadIdx.x] = 0;
+#pragma unroll
+            for (int w = 0; w < S::kWords; ++w) marks[256 * w] = 0;
             // Queries, 32 rows of this stream's, or half of them where both streams work on the same; lanes on neighbouring
             // pieces of a row
             {
@@ -326,10 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 const bool edge = slot + kTile > clear;
                 const int group = twice ? 0 : x;
                 uint32_t* const words = bad_words + 12 * group + 4 * (n % 3);
+                uint32_t* const map = reinterpret_cast<uint32_t*>(smem + S::kMap) + (2 * group + n % 2) * (kTile * S::kWords);
                 if (edge) {
                     // Values of slots past the last one seen count nothing, whatever is there, and values that are not
-                    // finite count for the vectors that see them alone: their rows of the tile become zeros, the rest
-                    // is told by the sums.
+                    // finite count for the vectors that see them alone, who get NaN in their dims: zeros take their place.
                     const int cleaners = twice ? 256 : 128, me = twice ? static_cast<int>(threadIdx.x) : row, sees = it.sees;
                     const int64_t vu = unit0 + 2 * (tile - from) + 1;
                     // (the scores were issued after the values that lay in this place before had landed: the phase is no older one)
@@ -340,21 +346,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                         const int at = slot + e % kTile;
                         if (at < clear) continue;  // seen by all
                         uint4* const line = reinterpret_cast<uint4*>(smem + S::kRing + static_cast<uint32_t>(vu % S::kUnits) * S::kUnit + e * 128);
-                        bool clean = at >= sees || (no_page && !has_page(a, it.b, at));
-                        if (!clean) {
-                            uint32_t over = 0;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const uint4 w = line[i ^ (lane & 7)];
-                                over |= not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w);
-                            }
-                            clean = over != 0;
-                            if (clean) atomicOr(words + e % kTile / 32, 1u << (e % 32));
-                        }
-                        if (clean) {
+                        if (at >= sees || (no_page && !has_page(a, it.b, at))) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) line[i ^ (lane & 7)] = make_uint4(0, 0, 0, 0);
+                            continue;
                         }
+                        uint32_t over = 0, low = 0, high = 0;  // bits of the dims
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 w = line[i ^ (lane & 7)];
+                            over |= not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w);
+                        }
+                        if (over != 0) [[unlikely]] {
+                            atomicOr(words + e % kTile / 32, 1u << (e % 32));
+#pragma unroll 1
+                            for (int i = 0; i < 32; ++i) {  // pairs of dims
+                                uint32_t& w = reinterpret_cast<uint32_t*>(line + (i / 4 ^ (lane & 7)))[i % 4];
+                                const uint32_t bad = not_finite<T>(w);
+                                const uint32_t two = (bad >> 15 & 1u) | bad >> 30;
+                                if (i < 16) low |= two << 2 * i;
+                                else high |= two << (2 * i - 32);
+                                w = finite_part<T>(w);
+                            }
+                        }
+                        // (of all: the other 64 dims of the slot may hold one)
+                        *reinterpret_cast<uint2*>(map + e % kTile * S::kWords + e / kTile * 2) = make_uint2(low, high);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     bar_sync(2 + group, cleaners);
@@ -376,7 +392,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                                 if (no_page)
                                     seen &= (first + 32 * i < it.sees && has_page(a, it.b, first + 32 * i) ? 0xffffu : 0u) |
                                             (first + 32 * i + 16 < it.sees && has_page(a, it.b, first + 32 * i + 16) ? 0xffff0000u : 0u);
-                                if (seen & words[2 * half + i]) sum = __uint_as_float(0x7fc00000u);
+#pragma unroll 1
+                                for (uint32_t bad = seen & words[2 * half + i]; bad != 0; bad &= bad - 1) {
+#pragma unroll
+                                    for (int w = 0; w < S::kWords; ++w) marks[256 * w] |= map[(64 * half + 32 * i + __ffs(bad) - 1) * S::kWords + w];
+                                }
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)
                                     if (!(seen >> j & 1u)) s[32 * i + j] = a.factor < 0.0f ? INFINITY : -INFINITY;
@@ -442,6 +462,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             float* const there = reinterpret_cast<float*>(smem + (warp % 4) * (HDP * 128));  // [HDP / 4][32 rows][4], over the queries
             float* const stats = reinterpret_cast<float*>(smem + S::kStats);                 // [reference, sum][row]
             float total = sum, by = 1.0f, with = 0.0f, common = ref;
+            auto mark = [&](float (&o)[64], int i) {  // NaN in the vector's marked dims, of 64 from i
+                const uint32_t low = marks[256 * (i / 32)], high = marks[256 * (i / 32 + 1)];
+                if (__any_sync(0xffffffffu, (low | high) != 0)) [[unlikely]] {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if ((j < 32 ? low : high) >> (j % 32) & 1u) o[j] = __uint_as_float(0x7fc00000u);
+                }
+            };
             if (!twice) {  // the second stream's results go to the first
                 bar_sync(1, 256);  // nothing reads the queries any more
                 if (x == 1) {
@@ -451,6 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                         for (int i = 0; i < HDP; i += 64) {
                             float o[64];
                             ld(o_tm + i, o);
+                            mark(o, i);
 #pragma unroll
                             for (int j = 0; j < 64; j += 4)
                                 *reinterpret_cast<float4*>(there + ((i + j) / 4 * 32 + lane) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
@@ -478,14 +507,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                 for (int i = 0; i < HDP; i += 64) {
                     float o[64];
                     ld(o_tm + i, o);
+                    mark(o, i);
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) o[j] = by == 0.0f ? 0.0f : o[j] * scale;
-                    if (!twice && with != 0.0f) {
+                    for (int j = 0; j < 64; ++j) o[j] *= scale;
+                    if (!twice && to - from > 1) {  // (the second stream had a tile)
 #pragma unroll
                         for (int j = 0; j < 64; j += 4) {
                             const float4 f = *reinterpret_cast<const float4*>(there + ((i + j) / 4 * 32 + lane) * 4);
                             o[j] = fmaf(f.x, scale1, o[j]), o[j + 1] = fmaf(f.y, scale1, o[j + 1]);
                             o[j + 2] = fmaf(f.z, scale1, o[j + 2]), o[j + 3] = fmaf(f.w, scale1, o[j + 3]);
+                        }
+                    }
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < 64; j += 2) {  // (nan_if_infinite)
+                            const uint64_t y = pair(o[j], o[j + 1]);
+                            unpair(fma2(y, pair(0.0f, 0.0f), y), o[j], o[j + 1]);
                         }
                     }
                     __syncwarp();
@@ -711,7 +748,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
     }
     const float scale = total == 0.0f ? 0.0f : 1.0f / total;
     put4<T>(a, place_of(a, cut.b, cut.head, cut.v0 + v, static_cast<int64_t>(a.heads) * a.head_dim) + 4 * quad,
-            make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale));
+            make_float4(nan_if_infinite(y.x * scale), nan_if_infinite(y.y * scale), nan_if_infinite(y.z * scale), nan_if_infinite(y.w * scale)));
 }
 
 template <typename T, int HDP>

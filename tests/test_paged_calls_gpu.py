@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_paged_gpu import BF16, FP16, LLAMA, MQA, QWEN, check_attend, filled, no_wait_ran_out, put, queries, trees  # noqa: E402,F401
+from test_paged_gpu import BF16, FP16, LLAMA, MQA, ODD, QWEN, WIDE, filled, no_wait_ran_out, put, queries, trees  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,94 @@ def test_results_in_the_queries_place(kt, layout, rows, lengths):
     with pytest.raises(ValueError, match="overlap"):
         cache.attend(0, beside, layout[0], rows, out=room[:-8].view(q.shape))
     assert torch.equal(beside, q)
+
+
+def poke(cache, which, slot, dim, value, b=0):
+    """One value of every head in a slot."""
+    page = int(cache.table[b, slot // cache.page])
+    getattr(cache, which)[0, page, :, slot % cache.page, dim] = value
+
+
+@pytest.mark.parametrize("layout,dtype,rows,held", [
+    (LLAMA, BF16, 1, 700), (QWEN, FP16, 1, 301), (QWEN, BF16, 3, 5000), (ODD, FP16, 2, 400), (LLAMA, BF16, 70, 700), (QWEN, FP16, 30, 700),
+    (QWEN, BF16, 300, 130), (MQA, FP16, 16, 900), (MQA, BF16, 130, 5000), (ODD, BF16, 100, 400), (WIDE, FP16, 24, 600),
+])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_a_value_that_is_not_finite_reaches_its_dim_alone(kt, layout, dtype, rows, held, bad):
+    """Wherever its slot lies in a tile and however the work is cut: NaN in the value's dim for the rows that see it,
+    and every other bit as with a 0 in its place."""
+    heads, kv, d = layout
+    cache = filled(layout, 32, dtype, [held, held // 2], rows, poison=True)
+    put(cache, rows)
+    q = queries(cache, heads, rows)
+    new = min(rows - 1, 5)
+    for slot, dim in ((3, 5), (held // 2, d - 1), (held - 1, 0), (held + new, 33)):
+        poke(cache, "values", slot, dim, 0.0)
+        want = cache.attend(0, q, heads, rows).view(2, rows, heads, d).clone()
+        assert torch.isfinite(want).all()
+        sees = torch.arange(rows, device="cuda") >= slot - held
+        want[0, sees, :, dim] = float("nan")
+        poke(cache, "values", slot, dim, bad)
+        for out in (None, torch.empty(2 * rows, heads * d, device="cuda")):
+            got = cache.attend(0, q, heads, rows, out=out).view(want.shape).to(dtype)
+            assert torch.equal(got.isnan(), want.isnan())
+            assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+        poke(cache, "values", slot, dim, 0.25)
+
+
+@pytest.mark.parametrize("layout,dtype,rows", [(LLAMA, BF16, 1), (QWEN, FP16, 2), (MQA, BF16, 16), (MQA, FP16, 40), (LLAMA, BF16, 65)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_value_of_no_weight_that_is_not_finite(kt, layout, dtype, rows, bad):
+    """Scores of the first 400 slots lie so far below the others that their powers are 0; what is there is seen all the same."""
+    heads, kv, d = layout
+    cache = filled(layout, 64, dtype, [1200], rows)
+    put(cache, rows)
+    q = torch.ones(rows, heads * d, dtype=dtype, device="cuda")
+    slot = torch.arange(400)
+    cache.keys[0, cache.table[0].cpu()[slot // 64].long(), :, slot % 64] = -60.0
+    for at in (7, 390):
+        poke(cache, "values", at, 9, bad)
+        got = cache.attend(0, q, heads, rows).view(rows, heads, d)
+        poke(cache, "values", at, 9, 0.0)
+        want = cache.attend(0, q, heads, rows).view(rows, heads, d)
+        assert torch.isnan(got[..., 9]).all() and torch.equal(got[..., :9], want[..., :9]) and torch.equal(got[..., 10:], want[..., 10:])
+
+
+@pytest.mark.parametrize("layout,dtype,rows", [(LLAMA, BF16, 5), (QWEN, FP16, 60)])
+def test_a_key_that_is_not_a_number_reaches_all_dims_of_its_head(kt, layout, dtype, rows):
+    heads, kv, d = layout
+    cache = filled(layout, 64, dtype, [300], rows)
+    put(cache, rows)
+    q = queries(cache, heads, rows)
+    want = cache.attend(0, q, heads, rows).view(rows, kv, heads // kv, d)
+    for slot in (10, 299, 302):
+        page = int(cache.table[0, slot // 64])
+        was = cache.keys[0, page, 1, slot % 64, 3].clone()
+        cache.keys[0, page, 1, slot % 64, 3] = float("nan")
+        got = cache.attend(0, q, heads, rows).view(want.shape)
+        sees = torch.arange(rows, device="cuda") >= slot - 300
+        assert torch.isnan(got[sees][:, 1]).all() and torch.equal(got[~sees], want[~sees])
+        assert torch.equal(got[:, [h for h in range(kv) if h != 1]], want[:, [h for h in range(kv) if h != 1]])
+        cache.keys[0, page, 1, slot % 64, 3] = was
+
+
+@pytest.mark.parametrize("rows", [6, 70])
+def test_drafted_values_that_are_not_finite(kt, rows):
+    """Some of a tree's nodes see them and some do not, in several dims and slots of a tile."""
+    from kotensor_b200.paged import draft_tree
+    heads, kv, d = LLAMA
+    _, visible = draft_tree(trees(1, rows, seed=5))
+    seen = torch.from_numpy(visible).cuda()
+    cache = filled(LLAMA, 64, BF16, [100], rows, poison=True)
+    put(cache, rows)
+    spots = [(1, 5, float("inf")), (1, 70, float("nan")), (3, 6, -float("inf")), (4, 127, float("nan")), (rows - 1, 0, float("inf"))]
+    for u, dim, _ in spots:
+        poke(cache, "values", 100 + u, dim, 0.0)
+    q = queries(cache, heads, rows)
+    want = cache.attend(0, q, heads, rows, visible=seen).view(rows, heads, d).clone()
+    for u, dim, bad in spots:
+        poke(cache, "values", 100 + u, dim, bad)
+        sees = (seen[0, :, u // 32] >> (u % 32) & 1).bool()
+        want[sees, :, dim] = float("nan")
+    got = cache.attend(0, q, heads, rows, visible=seen).view(want.shape)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
