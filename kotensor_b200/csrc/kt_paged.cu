@@ -57,7 +57,11 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(Paged c, Append 
     const int all = a.heads + 2 * c.kv_heads;
     const int begin = blockIdx.y * at_once * a.each + first, end = min(all, (static_cast<int>(blockIdx.y) + 1) * at_once * a.each);
     T* const q_out = static_cast<T*>(a.q_out) + r * a.heads * d + 4 * quad;
-    if (t >= paged::rows_of(a.counts, b, a.rows)) {  // not a token
+    const bool token = t < paged::rows_of(a.counts, b, a.rows);
+    const int held = max(c.lengths[b], 0), shift = __ffs(c.page) - 1;
+    const bool fits = static_cast<int64_t>(held) + t < static_cast<int64_t>(c.width) << shift;
+    if (!token || !fits) {  // (past the last slot: dropped, and no token either)
+        if (token && a.status != nullptr && threadIdx.x == 0 && blockIdx.y == 0) *a.status = KT_ERR_INVALID_ARGUMENT;
         if (first >= at_once) return;
         for (int h = begin; h < min(end, a.heads); h += at_once) {
             *reinterpret_cast<uint2*>(q_out + static_cast<int64_t>(h) * d) = make_uint2(0u, 0u);
@@ -66,10 +70,8 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(Paged c, Append 
         return;
     }
     __shared__ float2 turn[kMostPairs];  // cosines and sines of the row's angles
-    const int held = max(c.lengths[b], 0), shift = __ffs(c.page) - 1;
-    const bool fits = static_cast<int64_t>(held) + t < static_cast<int64_t>(c.width) << shift;
-    const int slot = fits ? held + t : 0;
-    const int page = fits ? c.table[static_cast<int64_t>(b) * c.table_stride + (slot >> shift)] : -1;
+    const int slot = held + t;
+    const int page = c.table[static_cast<int64_t>(b) * c.table_stride + (slot >> shift)];
     const bool stored = page >= 0 && page < c.pages;
     if (!stored && a.status != nullptr && threadIdx.x == 0 && blockIdx.y == 0) *a.status = KT_ERR_INVALID_ARGUMENT;
     if (begin - first < a.heads + c.kv_heads) {  // as for the whole CTA

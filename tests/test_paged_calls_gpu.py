@@ -116,3 +116,18 @@ def test_drafted_values_that_are_not_finite(kt, rows):
         want[sees, :, dim] = float("nan")
     got = cache.attend(0, q, heads, rows, visible=seen).view(want.shape)
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+@pytest.mark.parametrize("rows", [1, 5, 60])
+def test_queries_of_rows_past_the_last_slot_are_zeros(kt, rows):
+    heads, kv, d = QWEN
+    cache = filled(QWEN, 16, BF16, [46, 5, 48], 0)
+    assert cache.capacity == 48
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(3 * rows, n * d, generator=gen).cuda() for n in (heads, kv, kv))
+    out = torch.full((3 * rows, heads * d), float("nan"), dtype=BF16, device="cuda")
+    cache.append(0, q, k, v, torch.ones(d // 2, device="cuda"), rows, out=out)
+    lines = out.view(3, rows, -1)
+    for b, room in enumerate((2, 43, 0)):
+        assert (lines[b, :room].abs().sum(-1) > 0).all() and not lines[b, room:].any()
+    assert int(cache.status) != 0
