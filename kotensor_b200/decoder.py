@@ -339,10 +339,9 @@ class DeviceDecoder:
         return full
 
     def _reserve(self, positions: int) -> None:
-        """Pages of the paged cache for so many positions of every sequence."""
+        """Pages of the paged cache for so many positions of every sequence, or of none."""
         if self.paged:
-            for q in range(self.batch):
-                self.cache.reserve(q, min(positions, self.cache.capacity))
+            self.cache.reserve(range(self.batch), min(positions, self.cache.capacity))
 
     def _layers(self, b: "_Rows", rows: int, rows_per_seq: int, seq0: int = 0, counts=None, depths=None, visible=None) -> None:
         """Embedding lookup of b.tokens[:rows] through every block; leaves the

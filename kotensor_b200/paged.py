@@ -135,18 +135,24 @@ class PagedKVCache:
         """Pages that ``reserve`` can still hand out."""
         return len(self._free)
 
-    def reserve(self, sequence: int, tokens: int) -> None:
-        """Pages for the first ``tokens`` slots of a sequence (those it has stay)."""
-        own = self._pages_of(sequence)
+    def reserve(self, sequence, tokens: int) -> None:
+        """Pages for the first ``tokens`` slots of a sequence, or of each of several (those they
+        have stay).  Where the pool has too few, nobody gets any."""
+        sequences = [sequence] if isinstance(sequence, (int, np.integer)) else list(dict.fromkeys(sequence))
+        owns = [self._pages_of(q) for q in sequences]
         if not 0 <= tokens <= self.capacity:
             raise ValueError(f"{tokens} tokens do not fit a sequence of {self.capacity}")
-        n = -(-tokens // self.page) - len(own)
+        pages = -(-tokens // self.page)
+        n = sum(max(0, pages - len(own)) for own in owns)
         if n > len(self._free):
             raise ValueError(f"{n} pages wanted, {len(self._free)} are free")
-        if n > 0:
-            new = [self._free.pop() for _ in range(n)]
-            self.table[sequence, len(own):len(own) + n] = torch.tensor(new, dtype=torch.int32, device=self.device)
-            own += new
+        for q, own in zip(sequences, owns):
+            more = pages - len(own)
+            if more > 0:
+                new = self._free[:-more - 1:-1]
+                self.table[q, len(own):pages] = torch.tensor(new, dtype=torch.int32, device=self.device)
+                del self._free[-more:]
+                own += new
 
     def release(self, sequence: int) -> None:
         """Empties a sequence; its pages may be handed out again to calls that come after

@@ -63,3 +63,43 @@ def test_attention_over_what_it_reads(kt, change, stride, dtype):
         at[name] = PLACES[place] if isinstance(place, str) else PLACES[place[0]] + place[1]
     assert refused(lib, lib.kt_paged_attention(ctypes.c_void_p(4096), ctypes.byref(cache()), 0, at["q"], stride, at["out"], dtype, 5, at["counts"],
                                                at["visible"], 4, 1.0, at["scratch"], None))
+
+
+def pool(batch, pages):
+    """A cache's table and pool on the CPU: pages of 16 slots, 8 to a sequence."""
+    from kotensor_b200.paged import PagedKVCache
+    c = object.__new__(PagedKVCache)
+    c.batch, c.page, c.capacity, c._first, c.device = batch, 16, 128, 0, torch.device("cpu")
+    c._free, c._own = list(range(pages - 1, -1, -1)), [[] for _ in range(batch)]
+    c.table, c.lengths = torch.full((batch, 8), -1, dtype=torch.int32), torch.zeros(batch, dtype=torch.int32)
+    return c
+
+
+def test_pages_for_all_sequences_or_none():
+    c = pool(3, 10)
+    with pytest.raises(ValueError, match="12 pages wanted, 10 are free"):
+        c.reserve(range(3), 50)
+    assert c.free_pages == 10 and (c.table == -1).all()
+    c.reserve([0, 0, 2], 20)  # (a sequence twice is one)
+    assert c.free_pages == 6 and [len(o) for o in c._own] == [2, 0, 2]
+    c.reserve(range(3), 48)
+    assert c.free_pages == 1 and (c.table >= 0).sum(1).tolist() == [3, 3, 3]
+    assert len(set(c.table[c.table >= 0].tolist())) == 9 and [c.table[b, :3].tolist() for b in range(3)] == c._own
+    with pytest.raises(ValueError, match="3 pages wanted, 1 are free"):
+        c.reserve(range(3), 49)
+    with pytest.raises(ValueError, match="sequence 3 of 3"):
+        c.reserve([0, 3], 64)
+    with pytest.raises(ValueError, match="do not fit"):
+        c.reserve(range(3), 129)
+    assert c.free_pages == 1
+    c.reserve(1, 64)
+    c.release(0)
+    assert c.free_pages == 3
+
+
+def test_pages_that_could_not_be_written_down_stay_free(monkeypatch):
+    c = pool(2, 6)
+    monkeypatch.setattr(torch, "tensor", lambda *a, **k: 1 / 0)
+    with pytest.raises(ZeroDivisionError):
+        c.reserve(0, 40)
+    assert c.free_pages == 6 and c._own == [[], []]

@@ -131,3 +131,17 @@ def test_queries_of_rows_past_the_last_slot_are_zeros(kt, rows):
     for b, room in enumerate((2, 43, 0)):
         assert (lines[b, :room].abs().sum(-1) > 0).all() and not lines[b, room:].any()
     assert int(cache.status) != 0
+
+
+def test_a_batch_that_the_pool_cannot_hold_takes_no_pages(kt, oracle):
+    from test_decoder_paged_gpu import decoder
+    prompts = np.random.default_rng(3).integers(0, 700, (2, 50)).tolist()
+    d = decoder("int4_gqa", max_seq=128, batch=2, kv_bits=16, kv_page=16, kv_pages=7)
+    with pytest.raises(ValueError, match="8 pages wanted, 7 are free"):
+        d.prefill(prompts)
+    with pytest.raises(ValueError, match="pages wanted"):
+        d.generate_batch(prompts, 20)
+    assert d.cache.free_pages == 7 and d.length == 0
+    got = d.prefill([p[:40] for p in prompts])  # three pages each
+    assert d.cache.free_pages == 1 and torch.equal(got, decoder("int4_gqa", max_seq=128, batch=2, kv_bits=16, kv_page=16).prefill(
+        [p[:40] for p in prompts]))
