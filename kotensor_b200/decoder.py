@@ -635,15 +635,13 @@ class DeviceDecoder:
                 self.passes += 1
                 for o, tokens, n in zip(out, accepted, taken):
                     o += tokens[:n]
+            self._check_dropped()
         except BaseException:
             self.cache.lengths.fill_(self.length)  # as the prompts left it
             raise
-        self._check_dropped()
-        # the sequences go on together: what the longer ones hold beyond `end` is given up
-        self.cache.lengths.fill_(end)
-        self.position.fill_(end)
+        self.position.fill_(end)  # (as the lengths are: no tree had more nodes than tokens to come)
         self.length = end
-        chosen = np.array([o[:max_tokens] for o in out], dtype=np.int32)
+        chosen = np.array(out, dtype=np.int32)
         self._text.append(chosen[:, :-1])
         self.next_token.copy_(torch.from_numpy(chosen[:, -1].copy()))
         self.token.copy_(self.next_token)

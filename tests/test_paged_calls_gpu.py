@@ -145,3 +145,15 @@ def test_a_batch_that_the_pool_cannot_hold_takes_no_pages(kt, oracle):
     got = d.prefill([p[:40] for p in prompts])  # three pages each
     assert d.cache.free_pages == 1 and torch.equal(got, decoder("int4_gqa", max_seq=128, batch=2, kv_bits=16, kv_page=16).prefill(
         [p[:40] for p in prompts]))
+
+
+def test_a_drafted_text_that_lost_tokens_leaves_the_prompt(kt, oracle):
+    from test_decoder_paged_gpu import decoder
+    prompts = np.random.default_rng(13).integers(0, 700, (2, 12)).tolist()
+    d, e = (decoder("int4_gqa", max_seq=96, batch=2, kv_bits=16) for _ in range(2))
+    d.cache.status.fill_(1)  # as a token without a page would
+    with pytest.raises(ValueError, match="dropped"):
+        d.generate_drafted(prompts, 30)
+    e.prefill(prompts)
+    assert d.length == 12 == int(d.position) and d.cache.lengths.tolist() == [12, 12]
+    assert torch.equal(d.step([5, 6]), e.step([5, 6])) and d.cache.lengths.tolist() == [13, 13]
