@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
             dev::mbar_init(p_full(i / 2, i % 2), i % 2 ? 4 : 5);  // the softmax warps, and the landing one before a tile
             dev::mbar_init(o_done(i / 2, i % 2), 1);
         }
-        dev::mbar_init(q_full, 9);  // the softmax warps, and the landing one
+        dev::mbar_init(q_full, 11);  // the softmax warps, the landing one, and the issuing ones, which see every phase that way
         dev::mbar_init(finished, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -603,6 +603,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_many_kernel(const __grid_co
                         mma_commit(s_full(x, half));
                         if (half == 1) release(at);
                     };
+                    // (a stream without a tile of this item has nothing else that would keep it from missing a phase)
+                    dev::mbar_arrive(q_full);
                     wait(q_full, items++ & 1);
                     tc_after();
                     if (first < n) {  // (the first keys have landed too)

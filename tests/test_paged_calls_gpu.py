@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_paged_gpu import BF16, FP16, LLAMA, MQA, ODD, QWEN, WIDE, filled, no_wait_ran_out, put, queries, trees  # noqa: E402,F401
+from test_paged_gpu import BF16, FP16, LLAMA, MQA, ODD, QWEN, WIDE, check_attend, filled, no_wait_ran_out, put, queries, trees  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +157,15 @@ def test_a_drafted_text_that_lost_tokens_leaves_the_prompt(kt, oracle):
     e.prefill(prompts)
     assert d.length == 12 == int(d.position) and d.cache.lengths.tolist() == [12, 12]
     assert torch.equal(d.step([5, 6]), e.step([5, 6])) and d.cache.lengths.tolist() == [13, 13]
+
+
+def test_many_items_of_one_tile(kt):
+    """Items of 72 vectors over one tile, several to a CTA: the second stream has no tile in any of them."""
+    heads, rows = MQA[0], 9
+    cache = filled(MQA, 32, BF16, [(37 * i) % 119 for i in range(450)], rows, poison=True)
+    counts = torch.tensor([rows - i % 3 for i in range(450)], dtype=torch.int32).cuda()
+    put(cache, rows, counts)
+    q = queries(cache, heads, rows)
+    got = cache.attend(0, q, heads, rows, counts)
+    assert all(torch.equal(cache.attend(0, q, heads, rows, counts), got) for _ in range(20))
+    check_attend(cache, q, heads, rows, got, counts)
