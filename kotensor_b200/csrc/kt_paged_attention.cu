@@ -11,8 +11,9 @@
 // the load, as the second's; scores leave the first in the layout in which the second reads
 // probabilities.  Every warp keeps its own largest scores and sums, in fp32; an item's end
 // brings them together.  Probabilities are rounded to the cache's type, half a step of each
-// (2^-8 of it in bfloat16, 2^-11 in fp16) as the result itself is at the end: the products
-// take no wider ones, and two terms each would double the second product.
+// (2^-8 of it in bfloat16, 2^-11 in fp16) as a 16-bit result itself is at the end; they are
+// all of an fp32 result's error, 8e-4 of its size in bfloat16.  The products take no wider ones,
+// and two terms each would double the second product.
 //
 // A ninth warp copies: the pages of a tile as swizzled boxes of 64 dims by TMA, keys and
 // values in turn through a ring of 160 KB, so that some 100 KB are on their way to an SM at

@@ -17,7 +17,13 @@
 //
 // The reference of a vector is its largest score so far, less up to 2^8: only when a score
 // passes it by more do O and the sum go over to a new one, which needs the products under
-// way to end.  Sums, references and O are fp32.
+// way to end.  So the largest probability is rounded like the others.  Where few count, as in
+// the cases below, results are off by 2.2e-3 of their size in bfloat16 and 2.7e-4 in fp16;
+// always at the largest score by 1.8e-3 and 2.2e-4 (of which 1.7e-3 and 2.1e-4 are the result's
+// own rounding), but then the prompt takes 189 us, the chunk 80, the trees 46.  The sum is of
+// the probabilities before their rounding: a result is off by at most half a step of its sum
+// of |p v|, of rounded ones by up to a whole step, though the 2.2e-3 would be 2.0e-3.  Sums,
+// references and O are fp32.
 //
 // Masks.  Only tiles that some vector does not see in full (the last ones, and all that hold
 // new tokens of a tree) look at them.  There values are read first: rows of the tile past the
