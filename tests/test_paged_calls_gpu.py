@@ -169,3 +169,63 @@ def test_many_items_of_one_tile(kt):
     got = cache.attend(0, q, heads, rows, counts)
     assert all(torch.equal(cache.attend(0, q, heads, rows, counts), got) for _ in range(20))
     check_attend(cache, q, heads, rows, got, counts)
+
+
+@pytest.mark.parametrize("layout,rows,held", [((8, 2, 64), 10, 1300), ((8, 1, 128), 12, 1200), ((14, 2, 64), 40, 900), ((8, 2, 128), 48, 1000),
+                                              (MQA, 1, 2000), (QWEN, 6, 1100)])
+@pytest.mark.parametrize("dtype,rising", [(BF16, True), (FP16, True), (FP16, False)])
+def test_largest_scores_late_in_a_text(kt, layout, rows, held, dtype, rising):
+    """Scores that rise by more than 2^8 every few hundred slots, for some rows and not for others (with rows of both
+    signs some fall): references move in the middle of a run, in some vectors of a warp, in one stream or both."""
+    heads, kv, d = layout
+    batch = 60 if rows == 10 else 9 if rows == 12 else 2  # enough of the small ones for the kernel of many vectors
+    cache = filled(layout, 32, dtype, [held - 7 * b for b in range(batch)], rows, poison=True)
+    for b in range(batch):
+        slot = torch.arange(held - 7 * b)
+        level = (slot // 200 if rising else (held - slot) // 150).float() - 3.0
+        page = cache.table[b].cpu()[slot // 32].long()
+        noise = cache.keys[0, page, :, slot % 32].float() * 0.1
+        cache.keys[0, page, :, slot % 32] = (level.cuda()[:, None, None] + noise).to(dtype)
+    put(cache, rows)
+    gen = torch.Generator().manual_seed(9)
+    slope = torch.tensor([1.0, -0.5, 0.0, 2.0, 1.5])[torch.randint(0, 5, (batch * rows, heads, 1), generator=gen)]
+    q = (slope + 0.1 * torch.randn(batch * rows, heads, d, generator=gen)).reshape(batch * rows, -1).to(dtype).cuda()
+    for scale in (None, -0.1):
+        got = cache.attend(0, q, heads, rows, scale=scale, out=torch.empty(q.shape, device="cuda"))
+        assert torch.equal(got, cache.attend(0, q, heads, rows, scale=scale, out=torch.empty_like(got)))
+        some = cache.sequences(0, 2)  # (the oracle's time)
+        check_attend(some, q[:2 * rows], heads, rows, got[:2 * rows], scale=scale)
+
+
+@pytest.mark.parametrize("layout,rows", [(QWEN, 1), (LLAMA, 5), (LLAMA, 40), (MQA, 20)])
+def test_a_scale_of_zero_weighs_all_alike(kt, layout, rows):
+    heads, kv, d = layout
+    cache = filled(layout, 32, FP16, [90, 300], rows, poison=True)
+    put(cache, rows)
+    q = queries(cache, heads, rows)
+    for scale in (0.0, -0.0, 1e-44):
+        check_attend(cache, q, heads, rows, cache.attend(0, q, heads, rows, scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("name,batch", [("int4_gqa", 2), ("int8_tied_mha", 1)])
+def test_true_drafts_are_accepted(kt, oracle, name, batch):
+    """A text told in full is accepted seven drafts at a time behind a wrong branch; a text told wrong takes one pass a
+    token.  Both say the same.  Of 47 tokens after the first, five passes give 8 each; the sixth may have 7 nodes, one of
+    which the wrong branch takes, and gives 6; the seventh gives the last."""
+    from test_decoder_paged_gpu import decoder
+    prompts = np.random.default_rng(14).integers(0, 700, (batch, 12)).tolist()
+    options = dict(max_seq=160, batch=batch, kv_bits=16, kv_page=16)
+    wrong = decoder(name, **options)
+    truth = wrong.generate_drafted(prompts, 48, nodes=12, draft=lambda text: [[700, 701, 702], [703]])
+    assert wrong.passes == 47 and not any(t in (700, 703) for text in truth for t in text)
+
+    def told(text):
+        for p, t in zip(prompts, truth):
+            if text[:12] == p and text[12:] == t[:len(text) - 12]:
+                after = t[len(text) - 12:][:7]
+                return [after[:2] + [700], after]
+        raise AssertionError("another text")
+
+    d = decoder(name, **options)
+    assert d.generate_drafted(prompts, 48, nodes=12, draft=told) == truth
+    assert d.passes == 7
