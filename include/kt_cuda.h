@@ -519,12 +519,13 @@ kt_status kt_kv8_evict(kt_ctx* ctx, const kt_kv8_cache* cache, int32_t keep, int
  *   lengths int32 [batch]: tokens held, in slots 0..lengths[b]-1
  * table and lengths are device memory read by the kernels (a captured step replays at any
  * length and after any change of pages); no call below changes them (kt_kv8_advance moves
- * lengths on).  An entry outside 0..pages-1 is no page: tokens for it are dropped, no row
- * sees its slots.  A call's row t of sequence b is the token in slot lengths[b] + t.  Rows
- * t >= counts[b] (counts_dev NULL: rows_per_seq everywhere) are no tokens, nor are rows past
- * slot width * page.  head_dim is a multiple of 16 in 64..128, page 16, 32, 64 or 128, batch
- * at most 32767, width * page at most 2^30, keys and values 16-byte aligned; else
- * KT_ERR_INVALID_ARGUMENT. */
+ * lengths on).  A slot that a call writes must be one sequence's alone, and there once: shared
+ * pages hold tokens that all who share them keep.  An entry outside 0..pages-1 is no page:
+ * tokens for it are dropped, no row sees its slots.  A call's row t of sequence b is the token
+ * in slot lengths[b] + t.  Rows t >= counts[b] (counts_dev NULL: rows_per_seq everywhere) are
+ * no tokens, nor are rows past slot width * page.  head_dim is a multiple of 16 in 64..128,
+ * page 16, 32, 64 or 128, batch at most 32767, width * page at most 2^30, keys and values
+ * 16-byte aligned; else KT_ERR_INVALID_ARGUMENT. */
 enum { KT_FP32 = 0, KT_BF16 = 1, KT_FP16 = 2 };
 typedef struct {
     void* keys;
@@ -569,7 +570,7 @@ size_t kt_paged_scratch_bytes(kt_ctx* ctx);
  * Scores and sums are fp32, probabilities are rounded to the cache's type.  What a row does
  * not see has no part in it, infinities and NaN included; a value that is not finite makes
  * the rows that see it NaN in its dim, and in no other; a score that is NaN or +infinity its
- * row and head in all. */
+ * row and head in all, and one of -infinity has no weight. */
 kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t layer, const void* q_dev,
                              int64_t q_stride, void* out_dev, int32_t out_dtype, int32_t rows_per_seq,
                              const int32_t* counts_dev, const uint32_t* visible_dev, int32_t heads, float scale,

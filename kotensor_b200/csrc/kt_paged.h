@@ -32,7 +32,7 @@ struct PagedAttention {
     int32_t batch, kv_heads, head_dim, pages, page_shift, table_stride, capacity;
     int32_t rows, heads, group, words;  // rows of a sequence, words of a row of `visible`
     float factor;                       // scale * log2(e)
-    int32_t out_f32, aligned;           // aligned: bit 0 pairs of q, bit 1 16 bytes of out
+    int32_t out_f32, aligned;           // aligned to 16 bytes: bit 0 the rows of q, bit 1 out
 };
 // Boxes of the tensor maps: 64 dims of the slots of a page, at most 64 of them.
 constexpr int kPagedBox = 64;

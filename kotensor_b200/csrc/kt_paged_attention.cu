@@ -19,8 +19,8 @@
 // values in turn through a ring of 160 KB, so that some 100 KB are on their way to an SM at
 // any time and across the ends of items.  (Two CTAs of four warps with rings of 80 KB: 231 us
 // where this takes 224, and 37 parts to merge where this leaves 18, 93 where this takes 84.)
-// Bound by memory: 64 sequences of 3001 to 8190 tokens, 8 heads of 128, 222 us, 6.6 TB/s; one of
-// 120001 82 us, 6.0 TB/s, of which about 5 go into the merge.  By latency when short: 301
+// Bound by memory: 64 sequences of 3001 to 8190 tokens, 8 heads of 128, 225 us, 6.5 TB/s; one of
+// 120001 84 us, 5.9 TB/s, of which about 5 go into the merge.  By latency when short: 301
 // tokens 7.3 us, of which a tile's chain of copy, product, exponentials and product is 1.5.
 #include <algorithm>
 
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 
     if (warp == kWarps) {
         // Copies: a lane has a box (64 dims of the slots of a page, at most a tile's) of the keys' or values' unit.
-        const int box = min(kPagedBox, 1 << a.page_shift), boxes = kTile / box;  // 16, 32 or 64 slots; 4, 2 or 1 to a tile
+        const int box = min(kPagedBox, 1 << a.page_shift), boxes = kTile / box;  // 16, 32 or 64 slots; 8, 4 or 2 to a tile
         const int mine = lane % boxes, block = lane / boxes % S::kBlocks;
         const bool copies = lane < boxes * S::kBlocks;
         Ring<S::kUnits> ring;
@@ -481,7 +481,9 @@ cudaError_t launch_paged_attention(const Paged& c, int layer, const PagedAttenti
     // while its items leave no SM two (20 vectors of 32 heads over 8 of 128, 1 / 8 / 64 sequences of 300 tokens: 9.2 /
     // 9.4 / 57 us here, 14.7 / 17.6 / 57 there; 8 sequences of 4000: 43, 56); and for more where they are very few (112
     // vectors of 14 heads over 2 of 64, 1 / 8 sequences: 300 tokens 7.6 / 8.6 us here, 12.6 / 12.6 there, 20000 and 4000 tokens
-    // 22 / 33 here, 27 / 17 there).
+    // 22 / 33 here, 27 / 17 there).  Sequences past some 20000 slots are not told apart, which costs the most vectors that
+    // stay here: 100000 slots of one head of 128, 64 / 128 / 256 vectors 41 / 61 / 104 us here, 53 / 55 / 55 there (20000 slots
+    // 21 / 23 / 31 and 28 / 30 / 31); of two of 64, 56 / 112 vectors 46 / 72 us here, 36 / 37 there.
     const int64_t sixteens = (static_cast<int64_t>(a.rows) * a.group + kVectors - 1) / kVectors, items = sixteens * a.batch * a.kv_heads;
     if (sixteens > 1 && items > (sixteens == 2 ? sm_count : 16)) return launch_paged_many(c.dtype == KT_BF16, maps, a, sm_count, err, s);
     const bool bf16 = c.dtype == KT_BF16, wide = c.head_dim > 64;

@@ -11,8 +11,9 @@
 //   O += P V        tcgen05.mma, P and O in tensor memory
 // and while its softmax has one half, its issuing warp has the products of the other: P V of
 // a half, then Q K^T of the same half of the next tile.  (Whole tiles, one set of scores a
-// stream: products and softmax took turns, 4700 clocks a tile where this takes 3000.)  The
-// streams take turns with their powers of two, which one unit serves: left alone they fell
+// stream: products and softmax took turns, 4700 clocks a tile where halves took 3700, before a
+// warp of its own waited for copies, with which halves take 3000 and whole tiles were not
+// tried.)  The streams take turns with their powers of two, which one unit serves: left alone they fell
 // into step and both waited for it, then both for the tensor cores.
 //
 // The reference of a vector is its largest score so far, less up to 2^8: only when a score

@@ -69,7 +69,9 @@ class PagedKVCache:
     page numbers of its own instead (shared prefixes).  ``append`` and ``attend`` of every
     layer work at the same ``lengths``; ``advance`` moves on after the last layer.  Calls
     run on the current stream of the cache's device and share one scratch buffer: order
-    them on one stream.
+    them on one stream.  A slot that a call writes must be one sequence's alone, and there
+    once (shared pages hold tokens that all who share them keep).  A cache, or a view, whose
+    calls were captured has to outlive the graph.
     """
 
     def __init__(self, layers: int, batch: int, kv_heads: int, head_dim: int, pages: int, max_tokens: int, page: int = 64,
