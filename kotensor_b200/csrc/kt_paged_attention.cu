@@ -19,9 +19,9 @@
 // values in turn through a ring of 160 KB, so that some 100 KB are on their way to an SM at
 // any time and across the ends of items.  (Two CTAs of four warps with rings of 80 KB: 231 us
 // where this takes 224, and 37 parts to merge where this leaves 18, 93 where this takes 84.)
-// Bound by memory: 64 sequences of 3001 to 8190 tokens, 8 heads of 128, 225 us, 6.5 TB/s; one of
-// 120001 84 us, 5.9 TB/s, of which about 5 go into the merge.  By latency when short: 301
-// tokens 7.3 us, of which a tile's chain of copy, product, exponentials and product is 1.5.
+// Bound by memory: 64 sequences of 3001 to 8190 tokens, 8 heads of 128, 222 to 225 us, 6.5 to 6.6
+// TB/s; one of 120001 82 to 84 us, 5.9 TB/s, of which about 5 go into the merge.  By latency when short: 301
+// tokens 7.4 us, of which a tile's chain of copy, product, exponentials and product is 1.5.
 #include <algorithm>
 
 #include "kt_paged.h"

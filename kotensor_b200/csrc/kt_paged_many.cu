@@ -35,8 +35,8 @@
 // which the products just follow (2560 clocks of a tile's 3000: scores of 64 slots read the
 // queries again, 48 clocks a step where 128 slots would take 64); and by what an item costs:
 // about 5000 clocks to enter, 5500 to leave, and twice a tile for one with masks.  A prompt
-// of 4093 rows of 32 heads over 8 of 128: 162 us, 849 TFLOP/s (141 back to back); 2 x 509 rows over 1000 to
-// 2999 tokens 65 us; 4 trees of 63 rows over 2500 to 6001 tokens 39 us, about 6 of them the merge.
+// of 4093 rows of 32 heads over 8 of 128: 162 us, 847 TFLOP/s (141 back to back); 2 x 509 rows over 1000 to
+// 2999 tokens 65 us; 4 trees of 63 rows over 2500 to 6001 tokens 40 us, about 6 of them the merge.
 // (Some of the powers as polynomials on the fp32 units: 1 % faster with one in eight, 5 % slower with three.)
 #include <algorithm>
 
