@@ -326,7 +326,7 @@ kt_status kt_paged_attention(kt_ctx* ctx, const kt_paged_cache* cache, int32_t l
     // (a CTA writes the results of the queries that it has read, or that all who share them have: they may take their place)
     const int64_t rows = static_cast<int64_t>(cache->batch) * rows_per_seq, width = static_cast<int64_t>(heads) * cache->head_dim;
     const int64_t bytes = rows * width * (out_dtype == KT_FP32 ? 4 : 2);
-    const bool in_place = out == q && q_stride == width && out_dtype == cache->dtype;
+    const bool in_place = out == q && (q_stride == width || rows == 1) && out_dtype == cache->dtype;
     if ((!in_place && overlaps(out, bytes, q, 2 * width, rows, 2 * q_stride)) || overlaps(out, bytes, counts, 4ll * cache->batch) ||
         overlaps(out, bytes, visible, 4 * rows * ((rows_per_seq + 31) / 32)) || overlaps_places(out, bytes, *cache))
         return entry_fail(KT_ERR_INVALID_ARGUMENT, "out must not overlap what the call reads, but for the queries it takes the place of");
