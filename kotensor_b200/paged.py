@@ -13,6 +13,7 @@ from __future__ import annotations
 import copy
 import ctypes
 import math
+import operator
 from typing import Optional
 
 import numpy as np
@@ -140,7 +141,10 @@ class PagedKVCache:
     def reserve(self, sequence, tokens: int) -> None:
         """Pages for the first ``tokens`` slots of a sequence, or of each of several (those they
         have stay).  Where the pool has too few, nobody gets any."""
-        sequences = [sequence] if isinstance(sequence, (int, np.integer)) else list(dict.fromkeys(sequence))
+        try:
+            sequences = [operator.index(sequence)]
+        except TypeError:
+            sequences = list(dict.fromkeys(sequence))
         owns = [self._pages_of(q) for q in sequences]
         if not 0 <= tokens <= self.capacity:
             raise ValueError(f"{tokens} tokens do not fit a sequence of {self.capacity}")

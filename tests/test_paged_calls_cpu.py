@@ -92,7 +92,7 @@ def test_pages_for_all_sequences_or_none():
     with pytest.raises(ValueError, match="do not fit"):
         c.reserve(range(3), 129)
     assert c.free_pages == 1
-    c.reserve(1, 64)
+    c.reserve(torch.tensor(1), 64)
     c.release(0)
     assert c.free_pages == 3
 
